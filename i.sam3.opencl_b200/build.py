@@ -22,9 +22,9 @@ NVCC = os.path.join(CUDA, "bin", "nvcc")
 
 CU = ["gemm_tc.cu", "attn_tc.cu", "attn_simt.cu", "attn_decoder.cu", "elementwise.cu", "attn_noalloc.cu",
       "decoder.cu", "neck.cu", "input.cu",
-      "detector.cu"]
+      "detector.cu", "rotary.cu", "attn_cross.cu", "groupnorm.cu"]
 C = ["cuda_backend.c", "sam3_ops.c", "sam3_encoder.c", "sam3_decoder.c", "sam3_neck.c", "sam3_input.c",
-     "synth.c"]
+     "sam3_prompt.c", "synth.c"]
 HEADERS = ["tc_ptx.cuh", "tmap.cuh", "pdl.cuh", "kernels.h", "backend_internal.h"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -1,0 +1,698 @@
+// SPDX-License-Identifier: Unlicense
+// Cross attention of query rows over an encoder's states of another length
+// (the detector's queries and image tokens over padded prompts and over
+// the image; attend, sam3_text.c:305-343, for batches of sequences with
+// their own key counts, a key mask and shared key heads): per sequence b and
+// head h
+//   O = softmax_j(scale q . k_j over visible j) V,
+// key j visible when j < klen[b] and kmask[b][j] == 0; a row without a
+// visible key gets zeros. Masked and absent keys never reach the arithmetic
+// (their rows are filled with zeros instead of being read), so what they
+// hold, NaN included, does not matter.
+//
+// This file holds the form for few rows or few keys (bandwidth and latency
+// bound) on warp-level tensor instructions, in one launch without a
+// workspace. The rows of a tile are the (query, head) pairs of one key head,
+// so that the heads sharing it read its keys once. Four warps of 16 rows
+// each take 64-key steps through a ring of cp.async stages; with 16 rows or
+// fewer (single tokens) the four warps split a step's keys instead. When
+// the tiles are fewer than the CTA slots, a cluster of up to 16 CTAs shares a
+// tile's keys: each CTA leaves (max, sum, output) in its shared memory and
+// the CTAs merge rows of it through distributed shared memory.
+//
+// bf16 / f16: products on mma.m16n8k16 with fp32 accumulation, P rounded to
+// the operands' type (half a unit in the last place of at most 2^-8 / 2^-11 of
+// a weight, the operands' own precision). fp32: each operand is split into
+// two tf32 parts and x y taken as hi hi + hi lo + lo hi on mma.m16n8k8, off by
+// about 2^-21 of a product; the dropped lo lo is of that size.
+#include "kernels.h"
+#include "pdl.cuh"
+#include "tc_ptx.cuh"
+#include "tmap.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+namespace sam3 {
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kMaxCluster = 16;
+
+struct XaArgs {
+    const void *q, *k, *v;
+    void *o;
+    long qld, qs0, qs1, kld, ks0, ks1, vld, vs0, vs1, old, os0, os1;
+    const int *klen;
+    const uint8_t *kmask;
+    int Nq, Nk, heads, kvheads, g, hd;
+    long rows;    // Nq * g rows of one key head
+    int nqt, cs;  // tiles of rows, CTAs sharing a tile's keys
+    int kvec, qvec, ovec;  // 16-byte accesses allowed
+    float scale_log2;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+                 "r"(live ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_commit()
+{
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4],
+                                                     uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+                 "{%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                              uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+                 "{%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+                 "{%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi)
+{
+    return pack_bf16x2(lo, hi);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// x = hi + lo: hi rounded to tf32's 11 significand bits, lo the rest rounded
+// the same way.
+__device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo)
+{
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
+__device__ __forceinline__ float ld_dsmem(uint32_t a)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ T out_of(float v);
+template <>
+__device__ __forceinline__ float out_of<float>(float v)
+{
+    return v;
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 out_of<__nv_bfloat16>(float v)
+{
+    return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half out_of<__half>(float v)
+{
+    return __float2half_rn(v);
+}
+
+// Shared memory of a tile in 16-byte chunks. 16-bit types: rows of HDP * 2
+// bytes with the chunk index XORed by the row (no conflicts for ldmatrix);
+// fp32: rows padded by 16 bytes (fragment loads of 4 rows x 8 columns hit 32
+// banks).
+template <typename T, int HDP>
+struct Tile {
+    static constexpr int CPR = HDP * (int)sizeof(T) / 16;  // chunks of a row
+    static constexpr int PITCH = sizeof(T) == 4 ? HDP * 4 + 16 : HDP * 2;
+    static __device__ __forceinline__ uint32_t at(int row, int chunk)
+    {
+        if (sizeof(T) == 4)
+            return (uint32_t)(row * PITCH + chunk * 16);
+        const int x = CPR >= 8 ? (row & 7) : ((row >> 1) & 3);
+        return (uint32_t)(row * PITCH + ((chunk ^ x) << 4));
+    }
+};
+
+template <typename T, int HDP>
+struct Cfg {
+    static constexpr int BK = sizeof(T) == 4 && HDP == 128 ? 32 : 64;  // keys per step
+    static constexpr int STAGES = sizeof(T) == 4 ? 2 : (HDP == 128 ? 3 : 4);
+    static constexpr int KV_BYTES = BK * Tile<T, HDP>::PITCH;
+    static constexpr int STAGE_BYTES = 2 * KV_BYTES;
+    static constexpr int VIS_BYTES = STAGES * BK;
+};
+
+// Rows of a tile (16 WM), partial outputs (fp32) of its WK = 4 / WM key parts:
+// (max, sum) then HDP columns per row, over the stages' memory.
+template <typename T, int HDP, int WM>
+constexpr int smem_bytes()
+{
+    const int q = 16 * WM * Tile<T, HDP>::PITCH;
+    const int ring = Cfg<T, HDP>::STAGES * Cfg<T, HDP>::STAGE_BYTES;
+    const int part = (4 / WM) * 16 * WM * (HDP + 4) * 4;
+    return q + (ring > part ? ring : part) + Cfg<T, HDP>::VIS_BYTES + 16;
+}
+
+template <typename T, int HDP, int WM>
+__global__ void __launch_bounds__(kThreads) attn_cross_kernel(const __grid_constant__ XaArgs a)
+{
+    using TL = Tile<T, HDP>;
+    using CF = Cfg<T, HDP>;
+    constexpr int WK = 4 / WM, BM = 16 * WM, BK = CF::BK, KW = BK / WK;
+    constexpr int CPR = TL::CPR, EPC = 16 / (int)sizeof(T);  // elements per chunk
+    constexpr int STAGES = CF::STAGES;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int NT = KW / 8, DT = HDP / 8;  // score and output tiles of a warp
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint8_t *ring = smem + BM * TL::PITCH;
+    constexpr int RING = STAGES * CF::STAGE_BYTES;
+    constexpr int PART = WK * BM * (HDP + 4) * 4;
+    uint8_t *vis = ring + (RING > PART ? RING : PART);
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const int wm = warp % WM, wk = warp / WM;
+    const int g4 = lane >> 2, t4 = lane & 3;
+
+    const int rank = (int)(blockIdx.x % a.cs);
+    const long item = blockIdx.x / a.cs;
+    const int qt = (int)(item % a.nqt);
+    const long bh = item / a.nqt;
+    const int b = (int)(bh / a.kvheads), kh = (int)(bh - (long)b * a.kvheads);
+    const long r0 = (long)qt * BM;
+
+    griddep_wait();
+    griddep_launch();
+
+    int len = a.Nk;
+    if (a.klen)
+        len = min(max(__ldg(a.klen + b), 0), a.Nk);
+    const uint8_t *mask = a.kmask ? a.kmask + (long)b * a.Nk : nullptr;
+    const int steps_all = (len + BK - 1) / BK;
+    const int s0 = (int)((long)steps_all * rank / a.cs);
+    const int nsteps = (int)((long)steps_all * (rank + 1) / a.cs) - s0;
+    const T *kb = reinterpret_cast<const T *>(a.k) + b * a.ks0 + kh * a.ks1;
+    const T *vb = reinterpret_cast<const T *>(a.v) + b * a.vs0 + kh * a.vs1;
+    const int hdc = (a.hd + EPC - 1) / EPC;  // chunks of a row that hold columns
+
+    // ---- query rows
+    {
+        const T *qb = reinterpret_cast<const T *>(a.q) + b * a.qs0 + (long)kh * a.g * a.qs1;
+        for (int i = t; i < BM * CPR; i += kThreads) {
+            const int r = i / CPR, c = i % CPR;
+            const long gr = r0 + r, qi = gr / a.g;
+            const T *src = qb + qi * a.qld + (gr - qi * a.g) * a.qs1 + c * EPC;
+            const bool live = gr < a.rows && c < hdc;
+            const uint32_t dst = smem_addr(smem + TL::at(r, c));
+            if (a.qvec)
+                cp16(dst, live ? src : a.q, live);
+            else {
+                T w[EPC];
+#pragma unroll
+                for (int e = 0; e < EPC; e++)
+                    w[e] = live && c * EPC + e < a.hd ? src[e] : out_of<T>(0.0f);
+                *reinterpret_cast<uint4 *>(smem + TL::at(r, c)) = *reinterpret_cast<const uint4 *>(w);
+            }
+        }
+        cp_commit();
+    }
+    // ---- ring of key / value steps; each thread's chunks are fixed
+    constexpr int PER = (BK * CPR + kThreads - 1) / kThreads;
+    auto load = [&](int s, const bool (&see)[PER]) {
+        const int st = s % STAGES;
+        uint8_t *kd = ring + st * CF::STAGE_BYTES, *vd = kd + CF::KV_BYTES;
+        const int j0 = (s0 + s) * BK;
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            const int i = t + p * kThreads;
+            if (BK * CPR % kThreads && i >= BK * CPR)
+                break;
+            const int r = i / CPR, c = i % CPR;
+            const bool live = see[p] && c < hdc;
+            const T *ks = kb + (long)(j0 + r) * a.kld + c * EPC, *vs = vb + (long)(j0 + r) * a.vld + c * EPC;
+            const uint32_t off = TL::at(r, c);
+            if (a.kvec) {
+                cp16(smem_addr(kd + off), live ? ks : kb, live);
+                cp16(smem_addr(vd + off), live ? vs : vb, live);
+            }
+            else {
+                T w[EPC], x[EPC];
+#pragma unroll
+                for (int e = 0; e < EPC; e++) {
+                    const bool in = live && c * EPC + e < a.hd;
+                    w[e] = in ? ks[e] : out_of<T>(0.0f);
+                    x[e] = in ? vs[e] : out_of<T>(0.0f);
+                }
+                *reinterpret_cast<uint4 *>(kd + off) = *reinterpret_cast<const uint4 *>(w);
+                *reinterpret_cast<uint4 *>(vd + off) = *reinterpret_cast<const uint4 *>(x);
+            }
+            if (mask && c == 0)
+                vis[st * BK + r] = see[p];
+        }
+    };
+    // which of this thread's rows of step s are visible (the mask bytes are
+    // read one step before the rows they guard)
+    auto look = [&](int s, bool (&see)[PER]) {
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            const int i = t + p * kThreads, j = (s0 + s) * BK + i / CPR;
+            see[p] = s < nsteps && j < len;
+            if (mask && see[p])
+                see[p] = __ldg(mask + j) == 0;
+        }
+    };
+    bool see[PER];
+#pragma unroll 1
+    for (int s = 0; s < STAGES - 1; s++) {
+        look(s, see);
+        if (s < nsteps)
+            load(s, see);
+        cp_commit();
+    }
+    look(STAGES - 1, see);
+
+    float o[DT][4];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            o[d][e] = 0.0f;
+    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+    uint32_t qf[F32 ? 1 : HDP / 16][4];
+
+    for (int s = 0; s < nsteps; s++) {
+        cp_wait<STAGES - 2>();
+        __syncthreads();
+        if (s + STAGES - 1 < nsteps)
+            load(s + STAGES - 1, see);
+        cp_commit();
+        look(s + STAGES, see);
+        const int st = s % STAGES;
+        const uint8_t *ks = ring + st * CF::STAGE_BYTES, *vs = ks + CF::KV_BYTES;
+        const uint32_t ka = smem_addr(ks), va = smem_addr(vs);
+        const int jw = wk * KW;  // this warp's first key of the step
+
+        float sc[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                sc[n][e] = 0.0f;
+        if constexpr (!F32) {
+            if (s == 0) {
+#pragma unroll
+                for (int kk = 0; kk < HDP / 16; kk++)
+                    ldsm4(smem_addr(smem) + TL::at(wm * 16 + (lane & 15), kk * 2 + (lane >> 4)), qf[kk]);
+            }
+#pragma unroll
+            for (int kk = 0; kk < HDP / 16; kk++) {
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+                    // keys n*8 .. n*8+15, columns kk*16 .. kk*16+15
+                    uint32_t kf[4];
+                    ldsm4(ka + TL::at(jw + n * 8 + (lane & 7) + ((lane >> 4) << 3),
+                                      kk * 2 + ((lane >> 3) & 1)),
+                          kf);
+                    mma16<T>(sc[n], qf[kk], kf[0], kf[1]);
+                    mma16<T>(sc[n + 1], qf[kk], kf[2], kf[3]);
+                }
+            }
+        }
+        else {
+            const float *qs = reinterpret_cast<const float *>(smem) + (wm * 16 + g4) * (TL::PITCH / 4) + t4;
+            const float *kf = reinterpret_cast<const float *>(ks) + (jw + g4) * (TL::PITCH / 4) + t4;
+#pragma unroll 2
+            for (int kk = 0; kk < HDP / 8; kk++) {
+                uint32_t ah[4], al[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    split_tf32(qs[(e & 1) * 8 * (TL::PITCH / 4) + kk * 8 + (e >> 1) * 4], ah[e], al[e]);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    uint32_t bh0, bl0, bh1, bl1;
+                    split_tf32(kf[n * 8 * (TL::PITCH / 4) + kk * 8], bh0, bl0);
+                    split_tf32(kf[n * 8 * (TL::PITCH / 4) + kk * 8 + 4], bh1, bl1);
+                    mma8(sc[n], al, bh0, bh1);
+                    mma8(sc[n], ah, bl0, bl1);
+                    mma8(sc[n], ah, bh0, bh1);
+                }
+            }
+        }
+        // ---- online softmax of rows g4 and g4 + 8
+        const int j0 = (s0 + s) * BK + jw;
+        if (mask) {
+            const uint8_t *vw = vis + st * BK + jw;
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const uint16_t two = *reinterpret_cast<const uint16_t *>(vw + n * 8 + t4 * 2);
+                if (!(two & 0xff))
+                    sc[n][0] = sc[n][2] = -INFINITY;
+                if (!(two >> 8))
+                    sc[n][1] = sc[n][3] = -INFINITY;
+            }
+        }
+        else if (j0 + KW > len) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (j0 + n * 8 + t4 * 2 + (e & 1) >= len)
+                        sc[n][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float m = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+                m = max3f(m, sc[n][2 * h], sc[n][2 * h + 1]);
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const float mn = fmaxf(mx[h], m * a.scale_log2);
+            const float base = mn == -INFINITY ? 0.0f : mn;
+            const float corr = exp2f(mx[h] - base);
+            mx[h] = mn;
+            float add = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                sc[n][2 * h] = F32 ? exp2f(fmaf(sc[n][2 * h], a.scale_log2, -base))
+                                   : ex2_approx(fmaf(sc[n][2 * h], a.scale_log2, -base));
+                sc[n][2 * h + 1] = F32 ? exp2f(fmaf(sc[n][2 * h + 1], a.scale_log2, -base))
+                                       : ex2_approx(fmaf(sc[n][2 * h + 1], a.scale_log2, -base));
+                add += sc[n][2 * h] + sc[n][2 * h + 1];
+            }
+            sum[h] = fmaf(sum[h], corr, add);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                o[d][2 * h] *= corr;
+                o[d][2 * h + 1] *= corr;
+            }
+        }
+        // ---- O += P V
+        if constexpr (!F32) {
+#pragma unroll
+            for (int n = 0; n < NT; n += 2) {
+                const uint32_t pf[4] = {pack2<T>(sc[n][0], sc[n][1]), pack2<T>(sc[n][2], sc[n][3]),
+                                        pack2<T>(sc[n + 1][0], sc[n + 1][1]),
+                                        pack2<T>(sc[n + 1][2], sc[n + 1][3])};
+#pragma unroll
+                for (int d = 0; d < DT; d += 2) {
+                    uint32_t vf[4];
+                    ldsm4t(va + TL::at(jw + n * 8 + (lane & 15), d + (lane >> 4)), vf);
+                    mma16<T>(o[d], pf, vf[0], vf[1]);
+                    mma16<T>(o[d + 1], pf, vf[2], vf[3]);
+                }
+            }
+        }
+        else {
+            // The product's k index runs over keys in any order as long as both
+            // operands agree: index t4 is key 2 t4, t4 + 4 is key 2 t4 + 1, as
+            // the scores already lie.
+            const float *vf = reinterpret_cast<const float *>(vs) + (jw + 2 * t4) * (TL::PITCH / 4) + g4;
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                uint32_t ph[4], pl[4];
+                split_tf32(sc[n][0], ph[0], pl[0]);
+                split_tf32(sc[n][2], ph[1], pl[1]);
+                split_tf32(sc[n][1], ph[2], pl[2]);
+                split_tf32(sc[n][3], ph[3], pl[3]);
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    uint32_t bh0, bl0, bh1, bl1;
+                    split_tf32(vf[n * 8 * (TL::PITCH / 4) + d * 8], bh0, bl0);
+                    split_tf32(vf[(n * 8 + 1) * (TL::PITCH / 4) + d * 8], bh1, bl1);
+                    mma8(o[d], pl, bh0, bh1);
+                    mma8(o[d], ph, bl0, bl1);
+                    mma8(o[d], ph, bh0, bh1);
+                }
+            }
+        }
+    }
+    cp_wait<0>();
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+    }
+    T *ob = reinterpret_cast<T *>(a.o) + b * a.os0 + (long)kh * a.g * a.os1;
+
+    if (WK == 1 && a.cs == 1) {  // the tile is whole: straight from registers
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const long gr = r0 + wm * 16 + g4 + 8 * h, qi = gr / a.g;
+            if (gr >= a.rows)
+                continue;
+            T *dst = ob + qi * a.old + (gr - qi * a.g) * a.os1;
+            const float inv = sum[h] > 0.0f || sum[h] != sum[h] ? 1.0f / sum[h] : 0.0f;
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const int c = d * 8 + t4 * 2;
+                if (c >= a.hd)
+                    continue;
+                const float x = o[d][2 * h] * inv, y = o[d][2 * h + 1] * inv;
+                if (a.ovec) {
+                    if constexpr (F32)
+                        *reinterpret_cast<float2 *>(dst + c) = make_float2(x, y);
+                    else
+                        *reinterpret_cast<uint32_t *>(dst + c) = pack2<T>(x, y);
+                }
+                else {
+                    dst[c] = out_of<T>(x);
+                    dst[c + 1] = out_of<T>(y);
+                }
+            }
+        }
+        return;
+    }
+    // ---- partial results: [wk][row][HDP + 4] fp32, (max, sum) at HDP
+    __syncthreads();
+    float *part = reinterpret_cast<float *>(ring);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        float *pr = part + (long)(wk * BM + wm * 16 + g4 + 8 * h) * (HDP + 4);
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+            *reinterpret_cast<float2 *>(pr + d * 8 + t4 * 2) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
+        if (t4 == 0) {
+            pr[HDP] = mx[h];
+            pr[HDP + 1] = sum[h];
+        }
+    }
+    if (a.cs > 1)
+        cluster_sync_all();
+    else
+        __syncthreads();
+    // Row r belongs to CTA r % cs, a warp per row: weights 2^(max_p - max) of
+    // the cs * WK parts first, then the columns.
+    const int live_rows = (int)min((long)BM, a.rows - r0);
+    const int nparts = a.cs * WK;
+    const uint32_t base = smem_addr(part);
+    for (int r = rank + a.cs * warp; r < live_rows; r += a.cs * 4) {
+        float w[kMaxCluster * WK / 32 + 1];
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kMaxCluster * WK / 32 + 1; i++) {
+            const int p = lane + 32 * i;
+            w[i] = -INFINITY;
+            if (p < nparts) {
+                const uint32_t at = base + (uint32_t)(((p % WK) * BM + r) * (HDP + 4) + HDP) * 4;
+                w[i] = ld_dsmem(a.cs > 1 ? mapa_shared(at, p / WK) : at);
+            }
+            m = fmaxf(m, w[i]);
+        }
+#pragma unroll
+        for (int x = 16; x; x >>= 1)
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+        float l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kMaxCluster * WK / 32 + 1; i++) {
+            const int p = lane + 32 * i;
+            w[i] = w[i] == -INFINITY ? 0.0f : exp2f(w[i] - m);
+            if (p < nparts) {
+                const uint32_t at = base + (uint32_t)(((p % WK) * BM + r) * (HDP + 4) + HDP + 1) * 4;
+                l = fmaf(ld_dsmem(a.cs > 1 ? mapa_shared(at, p / WK) : at), w[i], l);
+            }
+        }
+#pragma unroll
+        for (int x = 16; x; x >>= 1)
+            l += __shfl_xor_sync(0xffffffffu, l, x);
+        constexpr int NC = HDP / 32;  // columns of a lane: lane + 32 i
+        float acc[NC];
+#pragma unroll
+        for (int i = 0; i < NC; i++)
+            acc[i] = 0.0f;
+#pragma unroll 2
+        for (int p = 0; p < nparts; p++) {
+            float wp = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kMaxCluster * WK / 32 + 1; i++)
+                if (p / 32 == i)
+                    wp = __shfl_sync(0xffffffffu, w[i], p & 31);
+            const uint32_t at = base + (uint32_t)(((p % WK) * BM + r) * (HDP + 4) + lane) * 4;
+            const uint32_t src = a.cs > 1 ? mapa_shared(at, p / WK) : at;
+#pragma unroll
+            for (int i = 0; i < NC; i++)
+                acc[i] = fmaf(ld_dsmem(src + 128 * i), wp, acc[i]);
+        }
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        const long gr = r0 + r, qi = gr / a.g;
+        T *dst = ob + qi * a.old + (gr - qi * a.g) * a.os1;
+#pragma unroll
+        for (int i = 0; i < NC; i++)
+            if (lane + 32 * i < a.hd)
+                dst[lane + 32 * i] = out_of<T>(acc[i] * inv);
+    }
+    if (a.cs > 1)
+        cluster_sync_all();  // peers read this CTA's part until here
+}
+
+template <auto Kern>
+cudaError_t prepare_once(int smem)
+{
+    static int done[64];
+    int dev = 0;
+    const bool known = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
+    if (known && done[dev])
+        return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(Kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && known)
+        done[dev] = 1;
+    return e;
+}
+
+template <typename T, int HDP, int WM>
+int launch(XaArgs &a, int nb, cudaStream_t s)
+{
+    constexpr int smem = smem_bytes<T, HDP, WM>();
+    const cudaError_t pe = prepare_once<attn_cross_kernel<T, HDP, WM>>(smem);
+    if (pe != cudaSuccess)
+        return (int)pe;
+    constexpr int BM = 16 * WM;
+    const long nqt = (a.rows + BM - 1) / BM;
+    if (nqt > 0x7fffffffL)
+        return K_EARG;
+    a.nqt = (int)nqt;
+    const long items = (long)nb * a.kvheads * nqt;
+    // CTAs sharing a tile's keys: until two CTAs per SM are busy, each with
+    // at least two steps.
+    const long slots = 2L * device_sms(), steps = (a.Nk + Cfg<T, HDP>::BK - 1) / Cfg<T, HDP>::BK;
+    a.cs = 1;
+    while (a.cs < kMaxCluster && items * a.cs * 2 <= slots && steps >= a.cs * 4)
+        a.cs *= 2;
+    if (items > 0x7fffffffL / a.cs)
+        return K_EARG;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.cs;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(items * a.cs));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&cfg, attn_cross_kernel<T, HDP, WM>, (const XaArgs)a);
+}
+
+template <typename T>
+int launch_t(XaArgs &a, int nb, cudaStream_t s)
+{
+    const bool few = a.rows <= 16;
+    if (a.hd <= 32)
+        return few ? launch<T, 32, 1>(a, nb, s) : launch<T, 32, 4>(a, nb, s);
+    if (a.hd <= 64)
+        return few ? launch<T, 64, 1>(a, nb, s) : launch<T, 64, 4>(a, nb, s);
+    return few ? launch<T, 128, 1>(a, nb, s) : launch<T, 128, 4>(a, nb, s);
+}
+
+}  // namespace
+}  // namespace sam3
+
+extern "C" int k_cross_attend(const struct k_rows *Q, const struct k_rows *K, const struct k_rows *V,
+                              const struct k_rows *O, int nb, int Nq, int Nk, int heads, int kvheads,
+                              int hd, const int *klen, const unsigned char *kmask, float scale,
+                              k_stream s)
+{
+    using namespace sam3;
+    if (nb <= 0 || Nq <= 0 || Nk <= 0 || heads <= 0 || kvheads <= 0 || heads % kvheads || hd <= 0 ||
+        hd > 128 || hd % 8)
+        return K_EARG;
+    const int es = Q->dt == K_F32 ? 4 : 2;
+    auto vec = [&](const struct k_rows *x) {
+        const long m = 16 / es;
+        return !(reinterpret_cast<uintptr_t>(x->p) & 15) && x->ld % m == 0 && x->s0 % m == 0 && x->s1 % m == 0;
+    };
+    auto pairs = [&](const struct k_rows *x) {
+        return !(reinterpret_cast<uintptr_t>(x->p) & (2 * es - 1)) && x->ld % 2 == 0 && x->s0 % 2 == 0 &&
+               x->s1 % 2 == 0;
+    };
+    XaArgs a = {};
+    a.q = Q->p;
+    a.k = K->p;
+    a.v = V->p;
+    a.o = O->p;
+    a.qld = Q->ld, a.qs0 = Q->s0, a.qs1 = Q->s1;
+    a.kld = K->ld, a.ks0 = K->s0, a.ks1 = K->s1;
+    a.vld = V->ld, a.vs0 = V->s0, a.vs1 = V->s1;
+    a.old = O->ld, a.os0 = O->s0, a.os1 = O->s1;
+    a.klen = klen;
+    a.kmask = kmask;
+    a.Nq = Nq;
+    a.Nk = Nk;
+    a.heads = heads;
+    a.kvheads = kvheads;
+    a.g = heads / kvheads;
+    a.hd = hd;
+    a.rows = (long)Nq * a.g;
+    a.qvec = vec(Q);
+    a.kvec = vec(K) && vec(V);
+    a.ovec = pairs(O);
+    a.scale_log2 = (float)(scale * 1.4426950408889634);
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(s);
+    if (Q->dt == K_F32)
+        return launch_t<float>(a, nb, st);
+    if (Q->dt == K_BF16)
+        return launch_t<__nv_bfloat16>(a, nb, st);
+    return launch_t<__half>(a, nb, st);
+}

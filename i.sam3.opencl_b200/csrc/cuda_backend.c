@@ -13,6 +13,7 @@ size_t cbi_dtype_size(int dtype)
 {
     switch (dtype) {
     case CB_F32:
+    case CB_I32:
         return 4;
     case CB_BF16:
     case CB_F16:

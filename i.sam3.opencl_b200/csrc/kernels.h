@@ -268,6 +268,41 @@ int k_attend_simt(int Nq, int Nk, int heads, int hd, const float *Q, int ldq,
                   int ldo, int causal, const float *dy, const float *dx,
                   int W, void *ws, size_t ws_bytes, int num_sms, k_stream s);
 
+/* ---- rotary positions, cross attention over padded states, group norm
+ * (sam3_prompt.c checks the arguments) */
+#define K_F32 0
+#define K_BF16 1
+#define K_F16 2
+#define K_ROPE_HALVES 1 /* pair j = columns (j, rot / 2 + j); 0: (2j, 2j + 1) */
+#define K_ROPE_MAX 256  /* rotated columns of a table */
+
+/* Rows of an operand: element (b, n, h, d) at p[b * s0 + n * ld + h * s1 + d]. */
+struct k_rows {
+    void *p;
+    int dt; /* K_F32, K_BF16, K_F16 */
+    long ld, s0, s1;
+};
+
+/* cs[p * rot / 2 + j] = amp (cos, sin) of (first + p) * turns[j] turns. */
+int k_rope_table(long npos, int rot, long first, const double *turns, float amp,
+                 float *cs, k_stream s);
+/* Y = X with the first rot columns of every head rotated by table row pos[b *
+ * N + n] (pos NULL: pos0 + n), rows outside the table copied; X may be Y. */
+int k_rope_rotate(const struct k_rows *X, const struct k_rows *Y, int nb, int N,
+                  int heads, int hd, int rot, int layout, const int *pos, int pos0,
+                  int npos, const float *cs, k_stream s);
+/* Attention of Nq query rows over the visible ones of Nk key rows, heads /
+ * kvheads query heads per key head; all operands of one type. */
+int k_cross_attend(const struct k_rows *Q, const struct k_rows *K,
+                   const struct k_rows *V, const struct k_rows *O, int nb, int Nq,
+                   int Nk, int heads, int kvheads, int hd, const int *klen,
+                   const unsigned char *kmask, float scale, k_stream s);
+/* Group norm and activation of [nb, npix, C] maps; Y has X's type, or X is
+ * fp32. */
+int k_groupnorm(const void *X, int xt, long ldx, long sx, void *Y, int yt, long ldy,
+                long sy, const float *g, const float *b, int nb, long npix, int C,
+                int groups, float eps, int act, k_stream s);
+
 /* uint8 HWC tiles -> bf16 patch rows in window-major token order:
  * out[ntile * grid^2, kpad], column c*ps*ps + ky*ps + kx (the Conv2d weight
  * order), value (u/255 - 0.5)/0.5 (image.c:360-366), zero for columns >= 3

@@ -14,9 +14,11 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libsam3cuda.so")
 
-F32, BF16, F16, U8 = 0, 1, 2, 3
+F32, BF16, F16, U8, I32 = 0, 1, 2, 3, 4
 ACT_NONE, ACT_GELU, ACT_RELU = 0, 1, 2
 ATTN_TC, ATTN_F32 = 0, 1
+ROPE_PAIRS, ROPE_HALVES = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_BASE, ROPE_SCALE_RAMP = 0, 1, 2, 3
 
 STATUS = {0: "CB_OK", 1: "CB_ENODEV", 2: "CB_EALLOC", 3: "CB_EARG",
           4: "CB_ECUDA", 5: "CB_ETIMEOUT", 6: "CB_EDTYPE"}
@@ -39,7 +41,7 @@ EXPORTS = [
     "cb_decoder_init_random", "cb_decoder_set_weight", "cb_decoder_set_image",
     "cb_decode", "cb_neck_create", "cb_neck_free", "cb_neck_init_random",
     "cb_neck_set_weight", "cb_neck_run", "cb_image_encoder_input",
-    "cb_attend",
+    "cb_attend", "cb_rope_table", "cb_rope_rotate", "cb_cross_attend", "cb_groupnorm",
     "sam3_synth_normal", "sam3_synth_u8", "sam3_synth_rope_axial",
 ]
 
@@ -86,6 +88,17 @@ class EncoderConfig(C.Structure):
                 ("mlp", C.c_int), ("grid", C.c_int), ("patch", C.c_int),
                 ("window", C.c_int), ("max_tiles", C.c_int),
                 ("global_mask", C.c_uint64)]
+
+
+class RopeScaling(C.Structure):
+    """struct cb_rope_scaling: the frequencies of a rotary table."""
+    _fields_ = [("theta", C.c_double), ("kind", C.c_int), ("factor", C.c_double),
+                ("orig_len", C.c_double), ("turns_fast", C.c_double),
+                ("turns_slow", C.c_double), ("amplitude", C.c_double)]
+
+    def __init__(self, theta=10000.0, kind=0, factor=1.0, orig_len=0.0, turns_fast=32.0,
+                 turns_slow=1.0, amplitude=1.0):
+        super().__init__(theta, kind, factor, orig_len, turns_fast, turns_slow, amplitude)
 
 
 class CBError(RuntimeError):
@@ -175,6 +188,11 @@ def lib():
                                          vp]),
         "cb_attend": (i32, [vp, i32, i32, i32, i32, vp, i32, vp, i32, vp, i32, vp, i32, i32,
                             vp, vp, i32, i32]),
+        "cb_rope_table": (i32, [vp, i32, i32, i64, C.POINTER(RopeScaling), vp]),
+        "cb_rope_rotate": (i32, [vp, i32, i32, i32, i32, i32, i32, Opnd, Opnd, vp, i32, vp, i32]),
+        "cb_cross_attend": (i32, [vp, i32, i32, i32, i32, i32, i32, Opnd, Opnd, Opnd, Opnd, vp,
+                                  vp, f32]),
+        "cb_groupnorm": (i32, [vp, i32, i64, i32, i32, Opnd, Opnd, vp, vp, f32, i32]),
         "sam3_synth_normal": (None, [C.c_uint64, C.c_uint64, sz, f32, f32, vp]),
         "sam3_synth_u8": (None, [C.c_uint64, C.c_uint64, sz, vp]),
         "sam3_synth_rope_axial": (None, [i32, i32, C.c_double, vp]),
@@ -286,7 +304,7 @@ class Backend:
         import torch
         dt = dtype if dtype is not None else {
             torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16,
-            torch.uint8: U8}[tensor.dtype]
+            torch.uint8: U8, torch.int32: I32}[tensor.dtype]
         m = C.c_void_p()
         self.check(lib().cb_wrap(self.h, C.c_void_p(tensor.data_ptr()),
                                  tensor.numel() * tensor.element_size(), dt,
@@ -381,6 +399,32 @@ class Backend:
         self.check(lib().cb_attend(self.h, Nq, Nk, heads, hd, Q.h, ldq, K.h, ldk, V.h, ldv,
                                    O.h, ldo, causal, dy.h if dy else None,
                                    dx.h if dx else None, W, mode))
+
+    # ---- prompt path: operands are bmat() descriptors
+    @staticmethod
+    def bmat(mem, off, ld, s0=0, s1=0):
+        """A strided operand (cb_bmat); keeps its Mem alive."""
+        o = Opnd(mem.h.value, off, ld, s0, s1)
+        o.mem = mem
+        return o
+
+    def rope_table(self, npos, rot, first, scaling, cs):
+        self.check(lib().cb_rope_table(self.h, npos, rot, first,
+                                       C.byref(scaling) if scaling is not None else None, cs.h))
+
+    def rope_rotate(self, nb, N, heads, hd, rot, layout, X, Y, cs, npos, pos=None, pos0=0):
+        self.check(lib().cb_rope_rotate(self.h, nb, N, heads, hd, rot, layout, X, Y, cs.h, npos,
+                                        pos.h if pos else None, pos0))
+
+    def cross_attend(self, nb, Nq, Nk, heads, kvheads, hd, Q, K, V, O, klen=None, kmask=None,
+                     scale=None):
+        """scale: hd ** -0.5 when None."""
+        self.check(lib().cb_cross_attend(self.h, nb, Nq, Nk, heads, kvheads, hd, Q, K, V, O,
+                                         klen.h if klen else None, kmask.h if kmask else None,
+                                         hd ** -0.5 if scale is None else scale))
+
+    def groupnorm(self, nb, npix, Cn, groups, X, Y, g, b, eps=1e-5, act=ACT_NONE):
+        self.check(lib().cb_groupnorm(self.h, nb, npix, Cn, groups, X, Y, g.h, b.h, eps, act))
 
     def mask_logits(self, U, hyper, out, P, npix):
         self.check(lib().cb_mask_logits(self.h, U.h, hyper.h, out.h, P, npix))

@@ -34,6 +34,7 @@ extern "C" {
 #define CB_BF16 1
 #define CB_F16 2
 #define CB_U8 3
+#define CB_I32 4 /* positions and lengths */
 
 /* Activations, as sam3_ops.h:11-13. */
 #define CB_ACT_NONE 0
@@ -418,6 +419,86 @@ int cb_neck_run(cb_neck *n, cb_mem x, int ntile, cb_mem emb, cb_mem feat_s0,
 int cb_attend(cb_backend *b, int Nq, int Nk, int heads, int hd, cb_mem Q,
               int ldq, cb_mem K, int ldk, cb_mem V, int ldv, cb_mem O, int ldo,
               int causal, cb_mem dy, cb_mem dx, int W, int mode);
+
+/* ------------------------------------------------------------ prompt path
+ * Operators of the prompt-conditioned path for batches of sequences: rotary
+ * positions on rows of any layout, attention over an encoder's states of
+ * another length, group norm. Operands are cb_bmat() descriptors: element (b,
+ * n, h, d) of a [nb, rows, heads, hd] operand lies at off + b * s0 + n * ld + h
+ * * s1 + d; strides are not negative (0 repeats an input), and no two elements
+ * of an output share an address. Any alignment of the element type is taken;
+ * 16-byte aligned starts and strides run fastest. Each call enqueues one
+ * kernel on the backend's stream, allocates nothing and uses no scratch
+ * buffer, so it may be captured into a graph and several captured calls may
+ * replay at once on their own buffers. An output may not overlap an input,
+ * except where in-place use is named. */
+
+/* Frequencies of a table: pair j of rot columns turns by w_j per position,
+ *   NONE:   w_j = theta^(-2j / rot);
+ *   LINEAR: w_j / factor (positions interpolated);
+ *   BASE:   theta replaced by theta * factor^(rot / (rot - 2));
+ *   RAMP:   w_j for pairs that make at least turns_fast turns over orig_len
+ *           positions, w_j / factor for those that make at most turns_slow, a
+ *           linear ramp over the pair index between (YaRN, Peng et al. 2023).
+ * theta > 1; factor >= 1 except with NONE; amplitude > 0 multiplies cos and
+ * sin. */
+#define CB_ROPE_SCALE_NONE 0
+#define CB_ROPE_SCALE_LINEAR 1
+#define CB_ROPE_SCALE_BASE 2
+#define CB_ROPE_SCALE_RAMP 3
+struct cb_rope_scaling {
+    double theta;
+    int kind;
+    double factor;
+    double orig_len, turns_fast, turns_slow; /* RAMP */
+    double amplitude;
+};
+
+/* cs F32 [npos, rot / 2] (cos, sin) of positions first .. first + npos - 1
+ * (within +-2^31; angles are reduced in 64 bits), the table of cb_rope_apply,
+ * cb_attention and cb_rope_rotate. rot even, at most 256. scaling NULL: theta
+ * 10000, none. */
+int cb_rope_table(cb_backend *b, int npos, int rot, int64_t first,
+                  const struct cb_rope_scaling *scaling, cb_mem cs);
+
+/* Y = X with the first rot (even) of every head's hd columns rotated, the
+ * others copied: (x0, x1) -> (x0 cos - x1 sin, x0 sin + x1 cos) for the pairs
+ * (2j, 2j + 1) (CB_ROPE_PAIRS, as cb_rope_apply) or (j, rot / 2 + j)
+ * (CB_ROPE_HALVES). Row (b, n) takes table row pos[b * N + n] (CB_I32; pos0
+ * 0), or pos0 + n when pos is NULL (pos0 + N <= npos). A position outside [0,
+ * npos) leaves its row as it is. X and Y of one type, or X F32 and Y BF16 /
+ * F16; rotated in 32 bits and rounded once. Y may be X (same layout). Queries
+ * and keys of one fused row are rotated by one call over their heads. */
+#define CB_ROPE_PAIRS 0
+#define CB_ROPE_HALVES 1
+int cb_rope_rotate(cb_backend *b, int nb, int N, int heads, int hd, int rot,
+                   int layout, struct cb_opnd X, struct cb_opnd Y, cb_mem cs,
+                   int npos, cb_mem pos, int pos0);
+
+/* O[b, i, h] = softmax over visible j of (scale Q[b, i, h] . K[b, j, h']) V[b,
+ * j, h'], h' = h / (heads / kvheads): Q, O [nb, Nq, heads, hd], K, V [nb, Nk,
+ * kvheads, hd], one type (F32, BF16, F16), hd a multiple of 8 up to 128, scale
+ * > 0. Key j of sequence b is visible when j < klen[b] (CB_I32 [nb], clamped
+ * to [0, Nk]; NULL: all) and kmask[b * Nk + j] is 0 (CB_U8 [nb, Nk], nonzero
+ * marks padding; NULL: none). What masked and absent rows of K and V hold does
+ * not enter the result; a row without a visible key, or whose visible scores
+ * are all -inf, gets zeros. Softmax and sums in 32 bits; F32 operands keep
+ * about 21 bits of each product (finite values), BF16 / F16 weights are
+ * rounded to the operands' type before the product with V. */
+int cb_cross_attend(cb_backend *b, int nb, int Nq, int Nk, int heads,
+                    int kvheads, int hd, struct cb_opnd Q, struct cb_opnd K,
+                    struct cb_opnd V, struct cb_opnd O, cb_mem klen,
+                    cb_mem kmask, float scale);
+
+/* Group norm and activation (CB_ACT_*) of channels-last maps (groupnorm_relu,
+ * sam3_kernels.cl:926-953): Y[b, p, c] = act((X - mean) / sqrt(var + eps) g[c]
+ * + bias[c]), mean and variance over the npix pixels and C / groups adjacent
+ * channels of (b, group), in 32 bits. X, Y: [nb, npix, C] with pixel stride ld
+ * and sample stride s0 (s1 0); one type, or X F32 and Y BF16 / F16; g, bias
+ * F32 [C]. Y may be X (same layout). */
+int cb_groupnorm(cb_backend *b, int nb, int64_t npix, int C, int groups,
+                 struct cb_opnd X, struct cb_opnd Y, cb_mem g, cb_mem bias,
+                 float eps, int act);
 
 /* ------------------------------------------------------------ input path
  * image_encoder_input (image.c:346-371) on the device: the crop (x0, y0, w,
