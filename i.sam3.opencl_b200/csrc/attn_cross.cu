@@ -25,6 +25,7 @@
 // a weight, the operands' own precision). fp32: each operand is split into
 // two tf32 parts and x y taken as hi hi + hi lo + lo hi on mma.m16n8k8, off by
 // about 2^-21 of a product; the dropped lo lo is of that size.
+#include "attn_cross.cuh"
 #include "kernels.h"
 #include "pdl.cuh"
 #include "tc_ptx.cuh"
@@ -39,19 +40,6 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kMaxCluster = 16;
-
-struct XaArgs {
-    const void *q, *k, *v;
-    void *o;
-    long qld, qs0, qs1, kld, ks0, ks1, vld, vs0, vs1, old, os0, os1;
-    const int *klen;
-    const uint8_t *kmask;
-    int Nq, Nk, heads, kvheads, g, hd;
-    long rows;    // Nq * g rows of one key head
-    int nqt, cs;  // tiles of rows, CTAs sharing a tile's keys
-    int kvec, qvec, ovec;  // 16-byte accesses allowed
-    float scale_log2;
-};
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live)
 {
@@ -109,20 +97,6 @@ __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi)
-{
-    return pack_bf16x2(lo, hi);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
-{
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 // x = hi + lo: hi rounded to tf32's 11 significand bits, lo the rest rounded
 // the same way.
 __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo)
@@ -130,30 +104,6 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo)
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
 }
-__device__ __forceinline__ float ld_dsmem(uint32_t a)
-{
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-    return v;
-}
-template <typename T>
-__device__ __forceinline__ T out_of(float v);
-template <>
-__device__ __forceinline__ float out_of<float>(float v)
-{
-    return v;
-}
-template <>
-__device__ __forceinline__ __nv_bfloat16 out_of<__nv_bfloat16>(float v)
-{
-    return __float2bfloat16_rn(v);
-}
-template <>
-__device__ __forceinline__ __half out_of<__half>(float v)
-{
-    return __float2half_rn(v);
-}
-
 // Shared memory of a tile in 16-byte chunks. 16-bit types: rows of HDP * 2
 // bytes with the chunk index XORed by the row (no conflicts for ldmatrix);
 // fp32: rows padded by 16 bytes (fragment loads of 4 rows x 8 columns hit 32
@@ -443,23 +393,33 @@ __global__ void __launch_bounds__(kThreads) attn_cross_kernel(const __grid_const
             // The product's k index runs over keys in any order as long as both
             // operands agree: index t4 is key 2 t4, t4 + 4 is key 2 t4 + 1, as
             // the scores already lie.
+            // Each step's sum starts from zero and is added to O outside the
+            // matrix unit, whose own additions truncate (5184 keys in one chain
+            // were 8e-6 off).
             const float *vf = reinterpret_cast<const float *>(vs) + (jw + 2 * t4) * (TL::PITCH / 4) + g4;
+            uint32_t ph[NT][4], pl[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                uint32_t ph[4], pl[4];
-                split_tf32(sc[n][0], ph[0], pl[0]);
-                split_tf32(sc[n][2], ph[1], pl[1]);
-                split_tf32(sc[n][1], ph[2], pl[2]);
-                split_tf32(sc[n][3], ph[3], pl[3]);
+                split_tf32(sc[n][0], ph[n][0], pl[n][0]);
+                split_tf32(sc[n][2], ph[n][1], pl[n][1]);
+                split_tf32(sc[n][1], ph[n][2], pl[n][2]);
+                split_tf32(sc[n][3], ph[n][3], pl[n][3]);
+            }
 #pragma unroll
-                for (int d = 0; d < DT; d++) {
+            for (int d = 0; d < DT; d++) {
+                float hi[4] = {0.0f, 0.0f, 0.0f, 0.0f}, lo[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
                     uint32_t bh0, bl0, bh1, bl1;
                     split_tf32(vf[n * 8 * (TL::PITCH / 4) + d * 8], bh0, bl0);
                     split_tf32(vf[(n * 8 + 1) * (TL::PITCH / 4) + d * 8], bh1, bl1);
-                    mma8(o[d], pl, bh0, bh1);
-                    mma8(o[d], ph, bl0, bl1);
-                    mma8(o[d], ph, bh0, bh1);
+                    mma8(lo, pl[n], bh0, bh1);
+                    mma8(lo, ph[n], bl0, bl1);
+                    mma8(hi, ph[n], bh0, bh1);
                 }
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    o[d][e] += hi[e] + lo[e];
             }
         }
     }
@@ -652,7 +612,7 @@ int launch_t(XaArgs &a, int nb, cudaStream_t s)
 extern "C" int k_cross_attend(const struct k_rows *Q, const struct k_rows *K, const struct k_rows *V,
                               const struct k_rows *O, int nb, int Nq, int Nk, int heads, int kvheads,
                               int hd, const int *klen, const unsigned char *kmask, float scale,
-                              k_stream s)
+                              int *err, k_stream s)
 {
     using namespace sam3;
     if (nb <= 0 || Nq <= 0 || Nk <= 0 || heads <= 0 || kvheads <= 0 || heads % kvheads || hd <= 0 ||
@@ -689,7 +649,16 @@ extern "C" int k_cross_attend(const struct k_rows *Q, const struct k_rows *K, co
     a.kvec = vec(K) && vec(V);
     a.ovec = pairs(O);
     a.scale_log2 = (float)(scale * 1.4426950408889634);
+    a.err = err;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(s);
+    // many rows over many keys: tcgen05
+    if (Nq >= 96 && Nk >= 192 && attn_cross_tc_takes(a, nb, Q->dt)) {
+        a.ovec = vec(O);
+        const int rc = attn_cross_tc(a, nb, Q->dt, st);
+        if (rc != K_ETMAP)
+            return rc;
+        a.ovec = pairs(O);
+    }
     if (Q->dt == K_F32)
         return launch_t<float>(a, nb, st);
     if (Q->dt == K_BF16)

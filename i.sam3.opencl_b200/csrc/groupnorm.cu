@@ -5,20 +5,25 @@
 // of each sample's group of channels over all pixels.
 //
 // One launch, no workspace. A unit is (sample, slab), a slab the fewest
-// whole groups whose channels fill kSlabBytes of a pixel's row, so that a
-// warp reads whole 32-byte sectors although it reads part of each row. A
-// cluster of 1 to 16 CTAs shares a unit's pixels: each CTA reads its share
-// once, keeping what fits of it in shared memory, the CTAs exchange
-// (count, mean, M2) per group through distributed shared memory, and the
-// second pass takes the kept part from shared memory and re-reads the rest,
-// latest first (L2 still holds it when the map in flight is not far larger).
+// whole groups whose channels fill kSlabBytes of a pixel's row in whole
+// 16-byte vectors, so that a warp reads whole sectors although it reads part
+// of each row. A cluster of 1 to 16 CTAs shares a unit's pixels. Each CTA
+// streams its share once through a ring of cp.async slots in shared memory
+// (each thread its own slots, so no barrier), which ends holding the last
+// steps; the CTAs exchange (count, mean, M2) per group through distributed
+// shared memory; the second pass walks back from the last step, out of the
+// ring and then re-reading earlier steps into the freed slots (from L2, when
+// the maps in flight are not far larger than it).
 //
-// Statistics in fp32 without the cancellation of E[x^2] - E[x]^2: a thread
-// reduces kUnroll vectors at a time to their own mean and M2 = sum (x -
-// mean)^2 and merges these into its running pair (mean += d f, M2 += M2' + d^2
-// n f, d = mean' - mean, f = n' / (n + n'); Chan, Golub and LeVeque 1979);
-// threads and CTAs are merged by sum n_i mean_i / n and sum M2_i + n_i
-// (mean_i - mean)^2 in a fixed order, so a result does not depend on timing.
+// A thread owns a vector of channels and steps over pixels. Statistics in
+// fp32 without the cancellation of E[x^2] - E[x]^2: per channel, kUnroll
+// pixels at a time are reduced to their own mean and M2 = sum (x - mean)^2 and
+// merged into the running pair (mean += d f, M2 += M2' + d^2 n f, d = mean' -
+// mean, f = n' / (n + n'); Chan, Golub and LeVeque 1979), two channels to an
+// instruction; channels, threads and CTAs are merged by sum n_i mean_i / n and
+// sum M2_i + n_i (mean_i - mean)^2 in a fixed order, so a result does not depend
+// on timing. Per-channel pairs cost about as many instructions as one pair per
+// vector and let a vector span groups of any width.
 #include "kernels.h"
 #include "pdl.cuh"
 #include "tc_ptx.cuh"
@@ -36,19 +41,22 @@ constexpr int kUnroll = 4;
 constexpr int kSlabBytes = 64;
 constexpr int kMaxSlabGroups = 128;
 constexpr int kMaxCluster = 16;
-constexpr int kCacheBytes = 96 * 1024;  // per CTA; two CTAs share an SM
+constexpr int kRing = 24;  // slots of 16-byte vectors, 6 batches
+constexpr int kRingBytes = kThreads * kRing * 16;  // per CTA, one per SM
 
 struct GnArgs {
     const void *x;
     void *y;
     const float *g, *b;
     long ldx, sx, ldy, sy;  // elements: pixel and sample strides
-    long npix;
+    long per, extra;        // pixels of a CTA; the first `extra` ranks have one more
+    int steps, srem;        // per / rows, per % rows
     int cg, gps, S, nslab;  // group width, groups and channels per slab, slabs
     int lpp;                // vectors per pixel of a slab
-    int rows, nk;           // pixels per step, steps per pixel (lpp > kThreads)
+    int rows, nk;           // pixels per step, blocks of vectors per pixel (lpp > kThreads)
     int cs;                 // cluster size
-    int ncache;             // steps kept in shared memory
+    int bpk, nring;         // batches of kUnroll steps per block of vectors, of the ring
+    int span;               // a vector may hold channels of several groups
     float eps;
     int act;
 };
@@ -93,13 +101,67 @@ struct alignas(sizeof(T) * V) Vec {
     T v[V];
 };
 
-__device__ __forceinline__ float gn_act(float v, int act)
+// Values 2 e and 2 e + 1 of a vector (one value and 0 when V is 1).
+template <typename T, int V>
+__device__ __forceinline__ uint64_t pair(const Vec<T, V> &v, int e)
 {
-    if (act == K_ACT_GELU)
-        return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-    if (act == K_ACT_RELU)
-        return v > 0.0f ? v : (v != v ? v : 0.0f);
-    return v;
+    return f2_make(to_f(v.v[2 * e]), V > 1 ? to_f(v.v[V > 1 ? 2 * e + 1 : 0]) : 0.0f);
+}
+
+// Activation of two values: GELU of a 32-bit output through erff, of 16-bit
+// ones through the shorter form (off by 4.2e-7 of the value at most); else
+// max(x, lowest), NaN kept (lowest 0 is ReLU, -inf none).
+template <typename TO, bool GELU>
+__device__ __forceinline__ void gn_act(float &x, float &y, float lowest)
+{
+    if constexpr (GELU && sizeof(TO) == 2)
+        gelu_pair(x, y);
+    else if constexpr (GELU) {
+        x = 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
+        y = 0.5f * y * (1.0f + erff(y * 0.70710678118654752f));
+    }
+    else {
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(lowest));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(lowest));
+    }
+}
+
+// Two results side by side, rounded to nearest.
+__device__ __forceinline__ void put2(float *dst, float x, float y)
+{
+    dst[0] = x;
+    dst[1] = y;
+}
+__device__ __forceinline__ void put2(__nv_bfloat16 *dst, float x, float y)
+{
+    *reinterpret_cast<__nv_bfloat162 *>(dst) = __floats2bfloat162_rn(x, y);
+}
+__device__ __forceinline__ void put2(__half *dst, float x, float y)
+{
+    *reinterpret_cast<__half2 *>(dst) = __floats2half2_rn(x, y);
+}
+
+// A vector from global memory into a thread's own slot: cp.async where it has
+// a size for it.
+template <int BYTES>
+__device__ __forceinline__ void fetch(uint8_t *slot, const void *src)
+{
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(slot)), "l"(src) : "memory");
+    else if constexpr (BYTES >= 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_addr(slot)), "l"(src), "n"(BYTES)
+                     : "memory");
+    else
+        *reinterpret_cast<uint16_t *>(slot) = *reinterpret_cast<const uint16_t *>(src);
+}
+__device__ __forceinline__ void fetch_commit()
+{
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void fetch_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ float ld_cluster(uint32_t addr)
@@ -109,210 +171,344 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr)
     return v;
 }
 
-template <typename TI, typename TO, int V>
-__global__ void __launch_bounds__(kThreads, 2) groupnorm_kernel(const GnArgs a)
+template <typename TI, typename TO, int V, bool GELU>
+__global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_constant__ GnArgs a)
 {
     using VI = Vec<TI, V>;
     using VO = Vec<TO, V>;
-    extern __shared__ __align__(16) uint8_t cache_raw[];
-    VI *cache = reinterpret_cast<VI *>(cache_raw);
-    __shared__ float sn[kThreads], sm[kThreads], sq[kThreads];
-    __shared__ float pub[kMaxSlabGroups][3];       // this CTA's (n, mean, M2), read by the cluster
-    __shared__ float gmean[kMaxSlabGroups], grstd[kMaxSlabGroups];
+    constexpr int NP = (V + 1) / 2;
+    // ring of slots, then the threads' statistics: (mean, M2) per thread, or per channel of it
+    extern __shared__ __align__(16) uint8_t dyn[];
+    constexpr int VB = (int)sizeof(VI);
+    constexpr int kAhead = 2;  // batches in flight; the ring has at least one more
+    uint8_t *ring = dyn + threadIdx.x * VB;
+    float2 *red = reinterpret_cast<float2 *>(dyn + (size_t)a.nring * kUnroll * kThreads * VB);
+    __shared__ float pub[kMaxSlabGroups][3];  // this CTA's (n, mean, M2), read by the cluster
+    __shared__ float2 gstat[kMaxSlabGroups];  // mean, 1 / sqrt(var + eps)
     const int t = threadIdx.x;
     const int rank = (int)(blockIdx.x % a.cs), unit = (int)(blockIdx.x / a.cs);
     const int sample = unit / a.nslab, slab = unit - sample * a.nslab;
     const int c0 = slab * a.S;
-    const TI *x = reinterpret_cast<const TI *>(a.x) + sample * a.sx + c0;
-    TO *y = reinterpret_cast<TO *>(a.y) + sample * a.sy + c0;
     // this CTA's pixels [p0, p0 + np)
-    const long per = a.npix / a.cs, extra = a.npix - per * a.cs;
-    const long p0 = rank * per + (rank < extra ? rank : extra);
-    const long np = per + (rank < extra ? 1 : 0);
-    // A step covers `rows` pixels (nk == 1: thread = (row, vector)), or one
-    // nk-th of a pixel (nk > 1, a group wider than the block).
+    const bool more = rank < a.extra;
+    const long p0 = rank * a.per + (more ? rank : a.extra);
+    const long np = a.per + more;
+    const bool roll = a.srem + more == a.rows;  // the extra pixel fills a step
+    const int q = a.steps + roll, rem = roll ? 0 : a.srem + more;
+    // thread = (row, vector); with nk > 1 (a group wider than the block) the
+    // block walks over all pixels once per block of vectors
     const int row = a.nk == 1 ? t / a.lpp : 0;
     const int lane0 = a.nk == 1 ? t - row * a.lpp : t;
-    const bool in_row = a.nk > 1 || row < a.rows;
-    const long steps = a.nk == 1 ? (np + a.rows - 1) / a.rows : np * a.nk;
-    auto where = [&](long it, long &pix, int &lane) {
-        if (a.nk == 1) {
-            pix = it * a.rows + row;
-            lane = lane0;
-            return in_row && pix < np;
-        }
-        pix = it / a.nk;
-        lane = t + (int)(it - pix * a.nk) * kThreads;
-        return lane < a.lpp;
-    };
+    auto count = [&](int r) { return r < a.rows ? q + (r < rem) : 0; };
+    const int mine = count(row);
+    const TI *x = reinterpret_cast<const TI *>(a.x) + sample * a.sx + (p0 + row) * a.ldx + c0;
+    TO *y = reinterpret_cast<TO *>(a.y) + sample * a.sy + (p0 + row) * a.ldy + c0;
+    const long dx = a.rows * a.ldx, dy = a.rows * a.ldy;
 
     griddep_wait();
     griddep_launch();
 
-    float n = 0.0f, mean = 0.0f, m2 = 0.0f;
-    for (long it = 0; it < steps; it += kUnroll) {
-        VI v[kUnroll];
-        bool ok[kUnroll];
-        int cnt = 0;
+    // Batches of kUnroll steps, bpk per block of vectors, in order: this thread's
+    // vectors of the next one into its slots of the ring. All ring indexes
+    // step round by one, without divisions.
+    const int batches = a.nk * a.bpk;
+    constexpr int SLOT = kUnroll * kThreads * VB;  // bytes of a batch in the ring
+    auto fetch4 = [&](uint8_t *slot, const TI *src, int left) {
+        if (left >= kUnroll) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; u++) {
-            long pix;
-            int lane;
-            ok[u] = it + u < steps && where(it + u, pix, lane);
-            if (ok[u]) {
-                v[u] = *reinterpret_cast<const VI *>(x + (p0 + pix) * a.ldx + lane * V);
-                cnt += V;
-            }
+            for (int u = 0; u < kUnroll; u++)
+                fetch<VB>(slot + u * kThreads * VB, src + u * dx);
         }
-        if (!cnt)
-            continue;
-        float s = 0.0f;
+        else {
+            for (int u = 0; u < left; u++)
+                fetch<VB>(slot + u * kThreads * VB, src + u * dx);
+        }
+    };
+    auto live = [&](int k) { return lane0 + k * kThreads < a.lpp ? mine : 0; };
+    int lk = 0, lb = 0, lslot = 0;  // next batch to load: block, batch of it, slot
+    const TI *lsrc = x + lane0 * V;
+    auto load_next = [&]() {
+        fetch4(ring + lslot * SLOT, lsrc, live(lk) - lb * kUnroll);
+        lsrc += kUnroll * dx;
+        lslot = lslot + 1 == a.nring ? 0 : lslot + 1;
+        if (++lb == a.bpk) {
+            lb = 0;
+            lk++;
+            lsrc = x + (lane0 + lk * kThreads) * V;
+        }
+    };
+    for (int i = 0; i < kAhead; i++) {
+        if (i < batches)
+            load_next();
+        fetch_commit();
+    }
+    int i = 0, islot = 0;  // batch at hand
+    float tn = 0.0f, tmean = 0.0f, tm2 = 0.0f;  // the thread's, over its vectors (not span)
+    for (int k = 0; k < a.nk; k++) {
+        const int lane = lane0 + k * kThreads;
+        const int n = lane < a.lpp ? mine : 0;
+        uint64_t mean[NP], m2[NP];
 #pragma unroll
-        for (int u = 0; u < kUnroll; u++)
-            if (ok[u]) {
+        for (int e = 0; e < NP; e++)
+            mean[e] = m2[e] = 0;
+        for (int bi = 0; bi < a.bpk; bi++) {
+            const int it = bi * kUnroll;
+            if (i + kAhead < batches)
+                load_next();
+            fetch_commit();
+            fetch_wait<kAhead>();
+            const VI *slot = reinterpret_cast<const VI *>(ring + islot * SLOT);
+            i++;
+            islot = islot + 1 == a.nring ? 0 : islot + 1;
+            if (it + kUnroll <= n) {
+                VI v[kUnroll];
 #pragma unroll
-                for (int e = 0; e < V; e++)
-                    s += to_f(v[u].v[e]);
-                if (it + u < a.ncache)
-                    cache[(it + u) * kThreads + t] = v[u];
-            }
-        const float c = (float)cnt, mu = s / c;
-        float q = 0.0f;
+                for (int u = 0; u < kUnroll; u++)
+                    v[u] = slot[u * kThreads];
+                const float f = rcp_approx((float)(bi + 1)), w = kUnroll * (1.0f - f);
+                const uint64_t f2 = f2_make(f, f), w2 = f2_make(w, w);
 #pragma unroll
-        for (int u = 0; u < kUnroll; u++)
-            if (ok[u]) {
+                for (int e = 0; e < NP; e++) {
+                    static_assert(kUnroll == 4, "mean of a batch");
+                    uint64_t fv[kUnroll];
 #pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const float d = to_f(v[u].v[e]) - mu;
-                    q = fmaf(d, d, q);
+                    for (int u = 0; u < kUnroll; u++)
+                        fv[u] = pair<TI, V>(v[u], e);
+                    const uint64_t mu = mul2(add2(add2(fv[0], fv[1]), add2(fv[2], fv[3])),
+                                             f2_make(0.25f, 0.25f));
+                    const uint64_t neg = f2_make(-1.0f, -1.0f);
+                    uint64_t q = 0;
+#pragma unroll
+                    for (int u = 0; u < kUnroll; u++) {
+                        const uint64_t d = fma2(mu, neg, fv[u]);
+                        q = fma2(d, d, q);
+                    }
+                    const uint64_t d = fma2(mean[e], neg, mu);
+                    mean[e] = fma2(d, f2, mean[e]);
+                    m2[e] = add2(m2[e], fma2(mul2(d, d), w2, q));
                 }
             }
-        const float n1 = n + c, f = c / n1, d = mu - mean;
-        mean = fmaf(d, f, mean);
-        m2 += fmaf(d * d, n * f, q);
-        n = n1;
+            else {
+                for (int j = it; j < n; j++) {
+                    const VI v = slot[(j - it) * kThreads];
+                    const float f = 1.0f / (float)(j + 1), w = (float)j * f;
+                    const uint64_t f2 = f2_make(f, f), w2 = f2_make(w, w);
+#pragma unroll
+                    for (int e = 0; e < NP; e++) {
+                        const uint64_t d = fma2(mean[e], f2_make(-1.0f, -1.0f), pair<TI, V>(v, e));
+                        mean[e] = fma2(d, f2, mean[e]);
+                        m2[e] = fma2(mul2(d, d), w2, m2[e]);
+                    }
+                }
+            }
+        }
+        float me[2 * NP], qe[2 * NP];
+#pragma unroll
+        for (int e = 0; e < NP; e++) {
+            f2_split(mean[e], me[2 * e], me[2 * e + 1]);
+            f2_split(m2[e], qe[2 * e], qe[2 * e + 1]);
+        }
+        if (a.span) {  // nk is 1: channel statistics [row][channel]
+            if (row < a.rows) {
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    red[row * a.S + lane * V + e] = make_float2(me[e], qe[e]);
+            }
+        }
+        else if (n > 0) {  // one group: merge the channels
+            float s = 0.0f, q = 0.0f;
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                s += me[e];
+            const float mu = s * (1.0f / V), c = (float)n;
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                q += fmaf((me[e] - mu) * (me[e] - mu), c, qe[e]);
+            const float nn = c * V, n1 = tn + nn, f = nn / n1, d = mu - tmean;
+            tmean = fmaf(d, f, tmean);
+            tm2 += fmaf(d * d, tn * f, q);
+            tn = n1;
+        }
     }
-    sn[t] = n;
-    sm[t] = mean;
-    sq[t] = m2;
+    if (!a.span)
+        red[t] = make_float2(tmean, tm2);
     __syncthreads();
-    // a warp per group: the threads of the group's vectors (all when nk > 1)
+    // The members of a group are the threads of its vectors, or its (row,
+    // channel) pairs; nparts warps share a group: means first, then sum
+    // n_i (mean_i - mean)^2.
+    constexpr int NW = kThreads / 32;
+    __shared__ float psum[kMaxSlabGroups], psq[kMaxSlabGroups];
     const int warp = t >> 5, lane32 = t & 31;
-    const int vpg = a.nk == 1 ? a.cg / V : kThreads;  // threads of a row in a group
-    const int members = a.nk == 1 ? a.rows * vpg : kThreads;
-    for (int gi = warp; gi < a.gps; gi += kThreads / 32) {
-        float tn = 0.0f, ts = 0.0f, tq = 0.0f;
-        for (int m = lane32; m < members; m += 32) {
-            const int r = m / vpg, i = r * a.lpp + gi * vpg + (m - r * vpg);
-            const int idx = a.nk == 1 ? i : m;
-            tn += sn[idx];
-            ts = fmaf(sn[idx], sm[idx], ts);
-        }
+    const int nparts = a.gps >= NW ? 1 : NW / a.gps;
+    const int width = a.span ? a.cg : (a.nk == 1 ? a.cg / V : kThreads);
+    const int pitch = a.span ? a.S : a.lpp;
+    const int members = a.rows * width;
+    const float sn = (float)np * (float)a.cg;
+    const int dr = nparts * 32 / width, di = nparts * 32 - dr * width;  // to a lane's next member
+    auto size = [&](int r, int i) {  // values behind member i of row r
+        if (a.nk == 1)
+            return (float)count(r) * (a.span ? 1 : V);
+        return (float)np * V * (float)(i < a.lpp ? (a.lpp - 1 - i) / kThreads + 1 : 0);
+    };
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            tn += __shfl_xor_sync(0xffffffffu, tn, o);
-            ts += __shfl_xor_sync(0xffffffffu, ts, o);
-        }
-        const float mu = tn > 0.0f ? ts / tn : 0.0f;
-        for (int m = lane32; m < members; m += 32) {
-            const int r = m / vpg, i = r * a.lpp + gi * vpg + (m - r * vpg);
-            const int idx = a.nk == 1 ? i : m;
-            const float d = sm[idx] - mu;
-            if (sn[idx] > 0.0f)
-                tq += fmaf(d * d, sn[idx], sq[idx]);
-        }
+    for (int pass = 0; pass < 2; pass++) {
+        for (int w = warp; w < a.gps * nparts; w += NW) {
+            const int gi = w / nparts, part = w - gi * nparts;
+            float mu = 0.0f, s = 0.0f;
+            if (pass == 1) {
+                for (int i = 0; i < nparts; i++)
+                    mu += psum[gi * nparts + i];
+                mu /= sn;
+            }
+            int r = (part * 32 + lane32) / width, i = part * 32 + lane32 - r * width;
+            for (int m = part * 32 + lane32; m < members; m += nparts * 32) {
+                const float c = size(r, i);
+                if (c > 0.0f) {
+                    const float2 st = red[r * pitch + gi * width + i];
+                    s += pass == 0 ? c * st.x : fmaf((st.x - mu) * (st.x - mu), c, st.y);
+                }
+                i += di;
+                r += dr;
+                if (i >= width) {
+                    i -= width;
+                    r++;
+                }
+            }
 #pragma unroll
-        for (int o = 16; o; o >>= 1)
-            tq += __shfl_xor_sync(0xffffffffu, tq, o);
-        if (lane32 == 0) {
-            pub[gi][0] = tn;
-            pub[gi][1] = mu;
-            pub[gi][2] = tq;
+            for (int o = 16; o; o >>= 1)
+                s += __shfl_xor_sync(0xffffffffu, s, o);
+            if (lane32 == 0) {
+                if (pass == 0)
+                    psum[w] = s;
+                else {
+                    psq[w] = s;
+                    if (part == 0) {
+                        pub[gi][0] = sn;
+                        pub[gi][1] = mu;
+                    }
+                }
+            }
         }
+        __syncthreads();
+    }
+    if (t < a.gps) {
+        float s = 0.0f;
+        for (int i = 0; i < nparts; i++)
+            s += psq[t * nparts + i];
+        pub[t][2] = s;
     }
     if (a.cs > 1)
         cluster_sync_all();
     else
         __syncthreads();
-    for (int gi = t; gi < a.gps; gi += kThreads) {
-        const uint32_t mine = smem_addr(&pub[gi][0]);
-        float tn = 0.0f, ts = 0.0f, tq = 0.0f;
-        for (int r = 0; r < a.cs; r++) {
-            const uint32_t p = a.cs > 1 ? mapa_shared(mine, r) : mine;
-            const float pn = ld_cluster(p);
-            tn += pn;
-            ts = fmaf(pn, ld_cluster(p + 4), ts);
+    // a half warp per group, lane = CTA of the cluster
+    for (int g0 = 0; g0 < a.gps; g0 += kThreads / 16) {
+        const int gi = g0 + (t >> 4), r = t & 15;
+        float pn = 0.0f, pm = 0.0f, pq = 0.0f;
+        if (gi < a.gps && r < a.cs) {
+            const uint32_t own = smem_addr(&pub[gi][0]);
+            const uint32_t p = a.cs > 1 ? mapa_shared(own, r) : own;
+            pn = ld_cluster(p);
+            pm = ld_cluster(p + 4);
+            pq = ld_cluster(p + 8);
         }
-        const float mu = ts / tn;
-        for (int r = 0; r < a.cs; r++) {
-            const uint32_t p = a.cs > 1 ? mapa_shared(mine, r) : mine;
-            const float pn = ld_cluster(p);
-            if (pn > 0.0f) {
-                const float d = ld_cluster(p + 4) - mu;
-                tq += fmaf(d * d, pn, ld_cluster(p + 8));
-            }
+        float sn = pn, ss = pn > 0.0f ? pn * pm : 0.0f;
+#pragma unroll
+        for (int o = 8; o; o >>= 1) {
+            sn += __shfl_xor_sync(0xffffffffu, sn, o);
+            ss += __shfl_xor_sync(0xffffffffu, ss, o);
         }
-        gmean[gi] = mu;
-        grstd[gi] = 1.0f / sqrtf(tq / tn + a.eps);
+        const float mu = ss / sn;
+        float sq = pn > 0.0f ? fmaf((pm - mu) * (pm - mu), pn, pq) : 0.0f;
+#pragma unroll
+        for (int o = 8; o; o >>= 1)
+            sq += __shfl_xor_sync(0xffffffffu, sq, o);
+        if (r == 0 && gi < a.gps)
+            gstat[gi] = make_float2(mu, 1.0f / sqrtf(sq / sn + a.eps));
     }
     __syncthreads();
     // no CTA may exit while another still reads its published statistics
     if (a.cs > 1)
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
-    const bool fixed = a.nk == 1;
-    float ga[V], be[V], mu = 0.0f, rs = 0.0f;
-    if (fixed && in_row) {
-        const int gi = lane0 * V / a.cg;
-        mu = gmean[gi];
-        rs = grstd[gi];
+    // Back from the last batch; those before the ring's are re-read as its slots
+    // come free.
+    const float lowest = a.act == K_ACT_RELU ? 0.0f : -INFINITY;
+    int ri = batches - 1 - a.nring;  // next batch to re-read
+    int rk = ri >= 0 ? ri / a.bpk : 0, rb = ri - rk * a.bpk;
+    const TI *rsrc = x + (lane0 + rk * kThreads) * V + (long)rb * kUnroll * dx;
+    for (int k = a.nk - 1; k >= 0; k--) {
+        const int lane = lane0 + k * kThreads;
+        const int n = lane < a.lpp ? mine : 0;
+        uint64_t nm[NP], ga[NP], be[NP];  // -mean, gamma rstd, beta
+        {
+            float sm[2 * NP], sg[2 * NP], sb[2 * NP];
 #pragma unroll
-        for (int e = 0; e < V; e++) {
-            ga[e] = __ldg(a.g + c0 + lane0 * V + e) * rs;
-            be[e] = __ldg(a.b + c0 + lane0 * V + e);
-        }
-    }
-    else {
-        mu = gmean[0];
-        rs = grstd[0];
-    }
-    for (long top = steps; top > 0; top -= kUnroll) {
-        VI v[kUnroll];
-        bool ok[kUnroll];
-        long pix[kUnroll];
-        int lane[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; u++) {
-            const long it = top - 1 - u;
-            ok[u] = it >= 0 && where(it, pix[u], lane[u]);
-            if (ok[u])
-                v[u] = it < a.ncache ? cache[it * kThreads + t]
-                                     : *reinterpret_cast<const VI *>(x + (p0 + pix[u]) * a.ldx +
-                                                                     lane[u] * V);
-        }
-#pragma unroll
-        for (int u = 0; u < kUnroll; u++)
-            if (ok[u]) {
-                if (!fixed) {
-#pragma unroll
-                    for (int e = 0; e < V; e++) {
-                        ga[e] = __ldg(a.g + c0 + lane[u] * V + e) * rs;
-                        be[e] = __ldg(a.b + c0 + lane[u] * V + e);
-                    }
-                }
-                VO w;
-#pragma unroll
-                for (int e = 0; e < V; e++)
-                    w.v[e] = from_f<TO>(gn_act(fmaf(to_f(v[u].v[e]) - mu, ga[e], be[e]), a.act));
-                *reinterpret_cast<VO *>(y + (p0 + pix[u]) * a.ldy + lane[u] * V) = w;
+            for (int e = 0; e < 2 * NP; e++) {
+                const int ch = (lane < a.lpp ? lane : 0) * V + (e < V ? e : 0);
+                const float2 st = gstat[ch / a.cg];
+                sm[e] = -st.x;
+                sg[e] = __ldg(a.g + c0 + ch) * st.y;
+                sb[e] = __ldg(a.b + c0 + ch);
             }
+#pragma unroll
+            for (int e = 0; e < NP; e++) {
+                nm[e] = f2_make(sm[2 * e], sm[2 * e + 1]);
+                ga[e] = f2_make(sg[2 * e], sg[2 * e + 1]);
+                be[e] = f2_make(sb[2 * e], sb[2 * e + 1]);
+            }
+        }
+        auto one = [&](const VI &v, TO *dst) {
+            VO w;
+#pragma unroll
+            for (int e = 0; e < NP; e++) {
+                float z0, z1;
+                f2_split(fma2(add2(pair<TI, V>(v, e), nm[e]), ga[e], be[e]), z0, z1);
+                gn_act<TO, GELU>(z0, z1, lowest);
+                if constexpr (V > 1)
+                    put2(w.v + 2 * e, z0, z1);
+                else
+                    w.v[0] = from_f<TO>(z0);
+            }
+            *reinterpret_cast<VO *>(dst) = w;
+        };
+        TO *py = y + lane * V + (long)a.bpk * kUnroll * dy;
+        for (int bi = a.bpk - 1; bi >= 0; bi--) {
+            const int left = n - bi * kUnroll;
+            py -= kUnroll * dy;
+            islot = islot == 0 ? a.nring - 1 : islot - 1;
+            // a re-read batch has kAhead newer groups behind it at least
+            if (--i + a.nring < batches)
+                fetch_wait<kAhead>();
+            const VI *slot = reinterpret_cast<const VI *>(ring + islot * SLOT);
+            if (left >= kUnroll) {
+#pragma unroll
+                for (int u = 0; u < kUnroll; u++)
+                    one(slot[u * kThreads], py + u * dy);
+            }
+            else {
+                for (int u = 0; u < left; u++)
+                    one(slot[u * kThreads], py + u * dy);
+            }
+            if (ri >= 0) {
+                fetch4(ring + islot * SLOT, rsrc, live(rk) - rb * kUnroll);
+                ri--;
+                rsrc -= kUnroll * dx;
+                if (--rb < 0) {
+                    rb = a.bpk - 1;
+                    rk--;
+                    rsrc = x + (lane0 + rk * kThreads) * V + (long)rb * kUnroll * dx;
+                }
+            }
+            fetch_commit();
+        }
     }
     if (a.cs > 1)
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Shared-memory limit and clusters above 8 CTAs, once per kernel and device.
-template <auto Kern>
+template <auto Kern, int V>
 cudaError_t prepare_once()
 {
     static int done[64];
@@ -321,7 +517,7 @@ cudaError_t prepare_once()
     if (known && done[dev])
         return cudaSuccess;
     cudaError_t e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kCacheBytes);
+                                         kRingBytes + kThreads * (int)sizeof(float2));
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(Kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess && known)
@@ -329,38 +525,71 @@ cudaError_t prepare_once()
     return e;
 }
 
-template <typename TI, typename TO, int V>
-int launch(GnArgs &a, int nb, int C, int groups, cudaStream_t s)
+// Clusters of c CTAs (with the whole ring) that run at the same time, asked
+// once per device.
+template <typename TI, typename TO, int V, bool GELU>
+long clusters_at_once(int c)
 {
-    const cudaError_t pe = prepare_once<groupnorm_kernel<TI, TO, V>>();
+    static int known[64][kMaxCluster + 1];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
+        return 0;
+    if (!known[dev][c]) {
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = c;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(c);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = kRingBytes;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, groupnorm_kernel<TI, TO, V, GELU>, &cfg) != cudaSuccess) {
+            (void)cudaGetLastError();
+            return 0;
+        }
+        known[dev][c] = n + 1;
+    }
+    return known[dev][c] - 1;
+}
+
+template <typename TI, typename TO, int V, bool GELU>
+int launch_a(GnArgs &a, int nb, long npix, int C, cudaStream_t s)
+{
+    const cudaError_t pe = prepare_once<groupnorm_kernel<TI, TO, V, GELU>, V>();
     if (pe != cudaSuccess)
         return (int)pe;
-    // the fewest whole groups of kSlabBytes
-    a.gps = 1;
-    for (int d = 1; d <= groups && d <= kMaxSlabGroups && d * (a.cg / V) <= kThreads; d++)
-        if (groups % d == 0) {
-            a.gps = d;
-            if ((long)d * a.cg * (long)sizeof(TI) >= kSlabBytes)
-                break;
-        }
-    a.S = a.gps * a.cg;
     a.nslab = C / a.S;
     a.lpp = a.S / V;
     a.nk = a.lpp > kThreads ? (a.lpp + kThreads - 1) / kThreads : 1;
     a.rows = a.nk == 1 ? kThreads / a.lpp : 1;
+    a.span = a.cg % V != 0;
     const long units = (long)nb * a.nslab;
-    // CTAs per unit: enough to fill two CTAs per SM, none with less than a step
-    const long slots = 2L * device_sms();
-    const long steps = a.nk == 1 ? (a.npix + a.rows - 1) / a.rows : a.npix * a.nk;
+    // CTAs per unit: the largest cluster of which all units' run at once (a
+    // second wave of clusters costs more than the idle SMs: 24 units of 6
+    // CTAs, 22 clusters fit, 24.6 us; of 4 CTAs, 33 fit, 15.6 us), none with less
+    // than a step
+    const long steps = (npix + a.rows - 1) / a.rows;
     a.cs = 1;
-    while (a.cs < kMaxCluster && units * a.cs * 2 <= slots && a.cs * 2 <= steps && a.cs * 2 <= a.npix)
-        a.cs *= 2;
-    if (units * a.cs > 0x7fffffffL)
+    for (int c = 2; c <= kMaxCluster; c *= 2)
+        if (units <= clusters_at_once<TI, TO, V, GELU>(c) && c <= steps)
+            a.cs = c;
+    a.per = npix / a.cs;
+    a.extra = npix - a.per * a.cs;
+    // batches of a CTA: the ring holds them all, or as many as fit
+    const long msteps = (a.per + (a.extra > 0) + a.rows - 1) / a.rows;
+    if (units > 0x7fffffffL / a.cs || msteps > (0x7fffffffL - kUnroll) / a.nk)
         return K_EARG;
-    const long mine = (a.npix + a.cs - 1) / a.cs;
-    const long msteps = a.nk == 1 ? (mine + a.rows - 1) / a.rows : mine * a.nk;
-    const long room = kCacheBytes / (long)(kThreads * V * sizeof(TI));
-    a.ncache = (int)(msteps < room ? msteps : room);
+    a.bpk = (int)((msteps + kUnroll - 1) / kUnroll);
+    const size_t red = (size_t)kThreads * (a.span ? V : 1) * sizeof(float2);
+    constexpr long batch = (long)kUnroll * kThreads * V * (long)sizeof(TI);
+    const long room = (kRingBytes - (a.span ? (long)red : 0)) / batch, all = (long)a.bpk * a.nk;
+    a.nring = (int)(all < room ? all : room);
+    a.steps = (int)(a.per / a.rows);
+    a.srem = (int)(a.per - (long)a.steps * a.rows);
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -371,29 +600,54 @@ int launch(GnArgs &a, int nb, int C, int groups, cudaStream_t s)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(units * a.cs));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = (size_t)a.ncache * kThreads * V * sizeof(TI);
+    cfg.dynamicSmemBytes = (size_t)a.nring * batch + red;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, groupnorm_kernel<TI, TO, V>, (const GnArgs)a);
+    return (int)cudaLaunchKernelEx(&cfg, groupnorm_kernel<TI, TO, V, GELU>, (const GnArgs)a);
+}
+
+template <typename TI, typename TO, int V>
+int launch(GnArgs &a, int nb, long npix, int C, cudaStream_t s)
+{
+    return a.act == K_ACT_GELU ? launch_a<TI, TO, V, true>(a, nb, npix, C, s)
+                               : launch_a<TI, TO, V, false>(a, nb, npix, C, s);
 }
 
 template <typename TI, typename TO>
-int launch_v(GnArgs &a, int nb, int C, int groups, cudaStream_t s)
+int launch_v(GnArgs &a, int nb, long npix, int C, int groups, cudaStream_t s)
 {
-    // widest vector that divides a group and every row start
+    // the fewest whole groups that are whole 16-byte vectors and kSlabBytes
+    // long, else the fewest that are that long, else what a block can hold
+    auto whole = [&](int d) { return (long)d * a.cg * (long)sizeof(TI); };
+    int plain = 0, vec = 0;
+    for (int d = 1; d <= groups && d <= kMaxSlabGroups && (long)d * a.cg <= kThreads; d++)
+        if (groups % d == 0 && whole(d) >= kSlabBytes) {
+            if (!plain)
+                plain = d;
+            if (!vec && whole(d) % 16 == 0)
+                vec = d;
+        }
+    a.gps = vec ? vec : (plain ? plain : 1);
+    if (!plain && !vec)  // few channels in all, or one group wider than a block
+        for (int d = 1; d <= groups && d <= kMaxSlabGroups && (long)d * a.cg <= kThreads; d++)
+            if (groups % d == 0)
+                a.gps = d;
+    a.S = a.gps * a.cg;
+    // widest vector that divides a slab and every row start
     auto fits = [&](int v) {
-        return a.cg % v == 0 && a.ldx % v == 0 && a.ldy % v == 0 && a.sx % v == 0 && a.sy % v == 0 &&
+        return a.S % v == 0 && a.ldx % v == 0 && a.ldy % v == 0 && a.sx % v == 0 && a.sy % v == 0 &&
                reinterpret_cast<uintptr_t>(a.x) % (v * sizeof(TI)) == 0 &&
-               reinterpret_cast<uintptr_t>(a.y) % (v * sizeof(TO)) == 0;
+               reinterpret_cast<uintptr_t>(a.y) % (v * sizeof(TO)) == 0 &&
+               (a.S / v <= kThreads || a.cg % v == 0);
     };
     if (sizeof(TI) == 2 && fits(8))
-        return launch<TI, TO, sizeof(TI) == 2 ? 8 : 4>(a, nb, C, groups, s);
+        return launch<TI, TO, sizeof(TI) == 2 ? 8 : 4>(a, nb, npix, C, s);
     if (fits(4))
-        return launch<TI, TO, 4>(a, nb, C, groups, s);
+        return launch<TI, TO, 4>(a, nb, npix, C, s);
     if (fits(2))
-        return launch<TI, TO, 2>(a, nb, C, groups, s);
-    return launch<TI, TO, 1>(a, nb, C, groups, s);
+        return launch<TI, TO, 2>(a, nb, npix, C, s);
+    return launch<TI, TO, 1>(a, nb, npix, C, s);
 }
 
 }  // namespace
@@ -415,20 +669,19 @@ extern "C" int k_groupnorm(const void *X, int xt, long ldx, long sx, void *Y, in
     a.sx = sx;
     a.ldy = ldy;
     a.sy = sy;
-    a.npix = npix;
     a.cg = C / groups;
     a.eps = eps;
     a.act = act;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(s);
     if (xt == K_F32 && yt == K_F32)
-        return launch_v<float, float>(a, nb, C, groups, st);
+        return launch_v<float, float>(a, nb, npix, C, groups, st);
     if (xt == K_F32 && yt == K_BF16)
-        return launch_v<float, __nv_bfloat16>(a, nb, C, groups, st);
+        return launch_v<float, __nv_bfloat16>(a, nb, npix, C, groups, st);
     if (xt == K_F32 && yt == K_F16)
-        return launch_v<float, __half>(a, nb, C, groups, st);
+        return launch_v<float, __half>(a, nb, npix, C, groups, st);
     if (xt == K_BF16 && yt == K_BF16)
-        return launch_v<__nv_bfloat16, __nv_bfloat16>(a, nb, C, groups, st);
+        return launch_v<__nv_bfloat16, __nv_bfloat16>(a, nb, npix, C, groups, st);
     if (xt == K_F16 && yt == K_F16)
-        return launch_v<__half, __half>(a, nb, C, groups, st);
+        return launch_v<__half, __half>(a, nb, npix, C, groups, st);
     return K_EARG;
 }

@@ -296,7 +296,7 @@ int k_rope_rotate(const struct k_rows *X, const struct k_rows *Y, int nb, int N,
 int k_cross_attend(const struct k_rows *Q, const struct k_rows *K,
                    const struct k_rows *V, const struct k_rows *O, int nb, int Nq,
                    int Nk, int heads, int kvheads, int hd, const int *klen,
-                   const unsigned char *kmask, float scale, k_stream s);
+                   const unsigned char *kmask, float scale, int *err, k_stream s);
 /* Group norm and activation of [nb, npix, C] maps; Y has X's type, or X is
  * fp32. */
 int k_groupnorm(const void *X, int xt, long ldx, long sx, void *Y, int yt, long ldy,

@@ -241,7 +241,7 @@ int cb_cross_attend(cb_backend *b, int nb, int Nq, int Nk, int heads, int kvhead
                      k_cross_attend(&q.k, &k.k, &v.k, &o.k, nb, Nq, Nk, heads, kvheads, hd,
                                     klen ? (const int *)klen->ptr : NULL,
                                     kmask ? (const unsigned char *)kmask->ptr : NULL, scale,
-                                    (k_stream)b->stream),
+                                    b->d_err, (k_stream)b->stream),
                      "cross_attend");
     cbi_prof_end(b);
     return rc;

@@ -624,6 +624,37 @@ __device__ __forceinline__ void exp2_poly2(float x0, float x1, float &y0, float 
     y1 = __uint_as_float(__float_as_uint(j1) * 8388608u + __float_as_uint(p1));
 }
 
+// GELU(x) = 0.5 x (1 + erf(x / sqrt 2)) (sam3_kernels.cl:43-46) on a pair of
+// values, with erf from Abramowitz & Stegun 7.1.26 (Hastings):
+//   erf(z) = 1 - t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) e^(-z^2),
+//   t = 1 / (1 + p z), z >= 0, |error| <= 1.5e-7,
+// so with h = erfc(|x| / sqrt 2) / 2 = t (...) 2^(-x^2 log2(e) / 2 - 1),
+// GELU(x) = x (1 - h) for x >= 0 and x h for x < 0, i.e. max(x, 0) - |x| h
+// for every x. Two MUFU operations per value (reciprocal, 2^x); the
+// polynomial and products run in packed fp32. The result differs from the
+// erf form by at most 4.2e-7 |x|-relative, far below the bf16 rounding of
+// the output it feeds.
+__device__ __forceinline__ void gelu_pair(float &x0, float &x1)
+{
+    const float kP = 0.3275911f * 0.70710678118654752f;
+    const float kE = -0.72134752044448170f;  // -log2(e) / 2
+    const float t0 = rcp_approx(fmaf(kP, fabsf(x0), 1.0f));
+    const float t1 = rcp_approx(fmaf(kP, fabsf(x1), 1.0f));
+    const uint64_t x = f2_make(x0, x1);
+    const uint64_t t = f2_make(t0, t1);
+    uint64_t q = fma2(f2_make(1.061405429f, 1.061405429f), t, f2_make(-1.453152027f, -1.453152027f));
+    q = fma2(q, t, f2_make(1.421413741f, 1.421413741f));
+    q = fma2(q, t, f2_make(-0.284496736f, -0.284496736f));
+    q = fma2(q, t, f2_make(0.254829592f, 0.254829592f));
+    float g0, g1;
+    f2_split(fma2(mul2(x, f2_make(kE, kE)), x, f2_make(-1.0f, -1.0f)), g0, g1);
+    q = mul2(mul2(q, t), f2_make(ex2_approx(g0), ex2_approx(g1)));
+    float h0, h1;
+    f2_split(q, h0, h1);
+    x0 = fmaf(-fabsf(x0), h0, fmaxf(x0, 0.0f));
+    x1 = fmaf(-fabsf(x1), h1, fmaxf(x1, 0.0f));
+}
+
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
                                              uint32_t d)
 {
