@@ -70,12 +70,14 @@ __host__ __device__ constexpr uint32_t idesc(int M, int N, int b_mn_major)
            ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// 2^x of two values as exp2_poly2 (tc_ptx.cuh), but a NaN stays one or
-// becomes huge instead of 2^-125, so that the tile's sum shows it.
+// 2^x of two values as exp2_poly2 (tc_ptx.cuh), but a NaN becomes NaN or huge
+// instead of 2^-125, so that the tile's sum shows it: the clamp at -125 is a
+// minimum of the bit patterns, which grow with the magnitude of a negative
+// number and are smaller for positive ones and for the NaN of an fma.
 __device__ __forceinline__ void exp2_poly2_nan(float x0, float x1, float &y0, float &y1)
 {
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-125.0f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-125.0f));
+    x0 = __uint_as_float(min(__float_as_uint(x0), 0xc2fa0000u));
+    x1 = __uint_as_float(min(__float_as_uint(x1), 0xc2fa0000u));
     const float kMagic = 12582912.0f;
     const uint64_t x = f2_make(x0, x1);
     const uint64_t j = add2(x, f2_make(kMagic, kMagic));
@@ -235,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             const uint64_t dK = sw128_desc(smem_addr(smem + G::OFF_K), 16, 1024);
             const uint64_t dV = sw128_desc(smem_addr(smem + G::OFF_V), BKV * 128, 1024);
             struct Cur {
-                int u, n, j, g, qn;
+                int u, n, j, g, qn, st, ph;
             };
             auto settle = [&](Cur &c) {  // to the next item with tiles
                 while (c.u < ta.nitems) {
@@ -247,6 +249,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             };
             auto adv = [&](Cur &c) {
                 c.g++;
+                if (++c.st == KST) {
+                    c.st = 0;
+                    c.ph ^= 1;
+                }
                 if (++c.j == c.n) {
                     c.j = 0;
                     c.qn++;
@@ -255,19 +261,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 }
             };
             auto issue_s = [&](const Cur &c) -> bool {
-                const int st = c.g % KST, qb = c.qn % NQ;
-                if (!mbar_wait(&k_full[st], (c.g / KST) & 1, a.err, abort_flag))
+                const int st = c.st, qb = c.qn & (NQ - 1);
+                if (!mbar_wait(&k_full[st], c.ph, a.err, abort_flag))
                     return false;
                 if (c.j == 0 && !mbar_wait(&q_full[qb], (c.qn / NQ) & 1, a.err, abort_flag))
                     return false;
                 tc_fence_after();
                 const uint32_t dS = tmem_base + (c.g & 1) * BKV;
+                const uint64_t qd = dQ + (uint64_t)((qb * G::Q_BYTES) >> 4);
+                const uint64_t kd = dK + (uint64_t)((st * G::KV_BYTES) >> 4);
 #pragma unroll
-                for (int kq = 0; kq < HDP / 16; kq++) {
-                    const uint64_t qd = dQ + (uint64_t)((qb * G::Q_BYTES + (kq / 4) * BQ * 128 + (kq % 4) * 32) >> 4);
-                    const uint64_t kd = dK + (uint64_t)((st * G::KV_BYTES + (kq / 4) * BKV * 128 + (kq % 4) * 32) >> 4);
-                    tc_mma(dS, qd, kd, idS, kq != 0);
-                }
+                for (int kq = 0; kq < HDP / 16; kq++)
+                    tc_mma(dS, qd + (((kq / 4) * BQ * 128 + (kq % 4) * 32) >> 4),
+                           kd + (((kq / 4) * BKV * 128 + (kq % 4) * 32) >> 4), idS, kq != 0);
                 tc_commit(&s_full[c.g & 1]);
                 tc_commit(&k_empty[st]);
                 if (c.j == c.n - 1)
@@ -275,22 +281,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 return true;
             };
             auto issue_pv = [&](const Cur &c) -> bool {
-                const int st = c.g % KST;
-                if (!mbar_wait(&v_full[st], (c.g / KST) & 1, a.err, abort_flag))
+                const int st = c.st;
+                if (!mbar_wait(&v_full[st], c.ph, a.err, abort_flag))
                     return false;
                 if (!mbar_wait(&p_ready[c.g & 1], (c.g >> 1) & 1, a.err, abort_flag))
                     return false;
                 tc_fence_after();
                 const uint32_t aP = tmem_base + (c.g & 1) * BKV;
+                const uint64_t vd = dV + (uint64_t)((st * G::KV_BYTES) >> 4);
 #pragma unroll
                 for (int kk = 0; kk < BKV / 16; kk++)
-                    tc_mma_ts(tmem_base + G::TM_O, aP + kk * 8,
-                              dV + (uint64_t)((st * G::KV_BYTES + kk * 16 * 128) >> 4), idPV, (c.j | kk) != 0);
+                    tc_mma_ts(tmem_base + G::TM_O, aP + kk * 8, vd + 128 * kk, idPV, (c.j | kk) != 0);
                 tc_commit(&pv_full[c.g & 1]);
                 tc_commit(&v_empty[st]);
                 return true;
             };
-            Cur ahead = {first, 0, 0, 0, 0};
+            Cur ahead = {first, 0, 0, 0, 0, 0, 0};
             settle(ahead);
             Cur cur = ahead;
             bool ok = true;
@@ -341,15 +347,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 uint32_t vis[NW];
                 bool whole = true;
 #pragma unroll
-                for (int w = 0; w < NW; w++) {
-                    const int left = it.len - (it.j0 + j) * BKV - w * 32;
-                    vis[w] = left >= 32 ? 0xffffffffu : (left > 0 ? (1u << left) - 1 : 0u);
+                for (int w = 0; w < NW; w++)
+                    vis[w] = 0xffffffffu;
+                if (mask || j == it.n - 1) {
+#pragma unroll
+                    for (int w = 0; w < NW; w++) {
+                        const int left = it.len - (it.j0 + j) * BKV - w * 32;
+                        vis[w] = left >= 32 ? 0xffffffffu : (left > 0 ? (1u << left) - 1 : 0u);
+                        if (mask)
+                            vis[w] &= __ballot_sync(0xffffffffu, ahead[w] == 0);
+                        whole = whole && vis[w] == 0xffffffffu;
+                    }
                     if (mask)
-                        vis[w] &= __ballot_sync(0xffffffffu, ahead[w] == 0);
-                    whole = whole && vis[w] == 0xffffffffu;
+                        look(j + 1);
                 }
-                if (mask)
-                    look(j + 1);
                 if (!whole) {
                     const int st = g % KST;
                     ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (g / KST) & 1, a.err, abort_flag));
@@ -379,92 +390,108 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 bool resc = false;
                 float factor = 1.0f;
                 if (rows_live) {
-                    uint32_t s[BKV];
-                    auto fetch = [&]() {
+                    uint64_t t0 = 0, t1 = 0;
+                    bool over = true;
+                    if (whole) {
+                        uint32_t s[BKV];
 #pragma unroll
                         for (int c = 0; c < NW; c++)
                             tmem_ld32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
                         tmem_wait_ld();
-                        if (!whole) {
-#pragma unroll
-                            for (int e = 0; e < BKV; e++)
-                                if (!((vis[e / 32] >> (e % 32)) & 1))
-                                    s[e] = __float_as_uint(-INFINITY);
-                        }
-                    };
-                    fetch();
-                    uint64_t t0, t1;
-#pragma unroll 1
-                    for (int pass = 0;; pass++) {
-                        if (m_used == -INFINITY || pass == 1) {
+                        if (m_used == -INFINITY) {
                             float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
                             for (int e = 0; e < BKV; e += 4) {
                                 mx0 = max3f(mx0, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
                                 mx1 = max3f(mx1, __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
                             }
-                            const float m_tile = fmaxf(mx0, mx1) * a.scale_log2;
-                            if (m_used == -INFINITY)
-                                m_used = m_tile;
-                            else if (m_tile > m_used) {
-                                resc = true;
-                                factor = ex2_approx(m_used - m_tile);
-                                m_used = m_tile;
-                                lsum0 = mul2(lsum0, f2_make(factor, factor));
-                                lsum1 = mul2(lsum1, f2_make(factor, factor));
-                            }
+                            m_used = fmaxf(mx0, mx1) * a.scale_log2;
                         }
                         const float base = m_used == -INFINITY ? 0.0f : -m_used;
                         const uint64_t negm = f2_make(base, base);
-                        t0 = 0;
-                        t1 = 0;
-                        if (pass == 0) {
 #pragma unroll
-                            for (int e = 0; e < BKV; e += 2) {
-                                const uint64_t x2 = fma2(f2_make(__uint_as_float(s[e]),
-                                                                 __uint_as_float(s[e + 1])),
-                                                         sl2x2, negm);
-                                float x0, x1, p0, p1;
-                                f2_split(x2, x0, x1);
-                                if (((e >> 1) & 7) >= 8 - kPolyPairsPer8)
-                                    exp2_poly2_nan(x0, x1, p0, p1);
-                                else {
-                                    p0 = ex2_approx(x0);
-                                    p1 = ex2_approx(x1);
-                                }
-                                if ((e >> 1) & 1)
-                                    t1 = add2(t1, f2_make(p0, p1));
-                                else
-                                    t0 = add2(t0, f2_make(p0, p1));
-                                s[e >> 1] = pack2<T>(p0, p1);
+                        for (int e = 0; e < BKV; e += 2) {
+                            const uint64_t x2 = fma2(f2_make(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
+                                                     sl2x2, negm);
+                            float x0, x1, p0, p1;
+                            f2_split(x2, x0, x1);
+                            if (((e >> 1) & 7) >= 8 - kPolyPairsPer8)
+                                exp2_poly2_nan(x0, x1, p0, p1);
+                            else {
+                                p0 = ex2_approx(x0);
+                                p1 = ex2_approx(x1);
                             }
-                        }
-                        else {
-#pragma unroll
-                            for (int e = 0; e < BKV; e += 2) {
-                                const uint64_t x2 = fma2(f2_make(__uint_as_float(s[e]),
-                                                                 __uint_as_float(s[e + 1])),
-                                                         sl2x2, negm);
-                                float x0, x1;
-                                f2_split(x2, x0, x1);
-                                const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                            if ((e >> 1) & 1)
+                                t1 = add2(t1, f2_make(p0, p1));
+                            else
                                 t0 = add2(t0, f2_make(p0, p1));
-                                s[e >> 1] = pack2<T>(p0, p1);
-                            }
+                            s[e >> 1] = pack2<T>(p0, p1);
                         }
                         float u0, u1, u2, u3;
                         f2_split(t0, u0, u1);
                         f2_split(t1, u2, u3);
-                        const bool over = !(((u0 + u1) + (u2 + u3)) < kOverflowSum);
-                        if (pass == 1 || !__any_sync(0xffffffffu, over))
-                            break;
-                        fetch();
+                        over = __any_sync(0xffffffffu, !(((u0 + u1) + (u2 + u3)) < kOverflowSum));
+                        if (!over) {
+                            tmem_st32(tS, *reinterpret_cast<const uint32_t(*)[32]>(s));
+                            if constexpr (BKV == 96)
+                                tmem_st16(tS + 32, *reinterpret_cast<const uint32_t(*)[16]>(s + 32));
+                        }
+                    }
+                    if (over) {
+                        // A tile with hidden keys, or one to take again: 32 columns
+                        // at a time in rolled loops (the unrolled code above has to
+                        // stay in the instruction cache), its maximum, then the
+                        // exponentials, P of a chunk written below the scores not
+                        // yet read.
+                        auto chunk = [&](int c, uint32_t (&s)[32]) {
+                            tmem_ld32(tS + 32 * c, s);
+                            tmem_wait_ld();
+                            uint32_t seen = vis[0];
+#pragma unroll
+                            for (int w = 1; w < NW; w++)
+                                seen = c == w ? vis[w] : seen;
+#pragma unroll
+                            for (int e = 0; e < 32; e++)
+                                if (!((seen >> e) & 1))
+                                    s[e] = __float_as_uint(-INFINITY);
+                        };
+                        float mx = -INFINITY;
+#pragma unroll 1
+                        for (int c = 0; c < NW; c++) {
+                            uint32_t s[32];
+                            chunk(c, s);
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2)
+                                mx = max3f(mx, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+                        }
+                        const float m_tile = mx * a.scale_log2;
+                        if (m_used == -INFINITY)
+                            m_used = m_tile;
+                        else if (m_tile > m_used) {
+                            resc = true;
+                            factor = ex2_approx(m_used - m_tile);
+                            m_used = m_tile;
+                            lsum0 = mul2(lsum0, f2_make(factor, factor));
+                            lsum1 = mul2(lsum1, f2_make(factor, factor));
+                        }
+                        const float base = m_used == -INFINITY ? 0.0f : -m_used;
+                        t0 = t1 = 0;
+#pragma unroll 1
+                        for (int c = 0; c < NW; c++) {
+                            uint32_t s[32], p[16];
+                            chunk(c, s);
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) {
+                                const float p0 = ex2_approx(fmaf(__uint_as_float(s[e]), a.scale_log2, base));
+                                const float p1 = ex2_approx(fmaf(__uint_as_float(s[e + 1]), a.scale_log2, base));
+                                t0 = add2(t0, f2_make(p0, p1));
+                                p[e >> 1] = pack2<T>(p0, p1);
+                            }
+                            tmem_st16(tS + 16 * c, p);
+                        }
                     }
                     lsum0 = add2(lsum0, t0);
                     lsum1 = add2(lsum1, t1);
-                    tmem_st32(tS, *reinterpret_cast<const uint32_t(*)[32]>(s));
-                    if constexpr (BKV == 96)
-                        tmem_st16(tS + 32, *reinterpret_cast<const uint32_t(*)[16]>(s + 32));
                 }
                 if (__any_sync(0xffffffffu, resc)) {
                     const int gp = g - 1;
