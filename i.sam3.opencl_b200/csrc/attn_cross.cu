@@ -461,84 +461,355 @@ __global__ void __launch_bounds__(kThreads) attn_cross_kernel(const __grid_const
     }
     // ---- partial results: [wk][row][HDP + 4] fp32, (max, sum) at HDP
     __syncthreads();
+    constexpr int PR = HDP + 4;
     float *part = reinterpret_cast<float *>(ring);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        float *pr = part + (long)(wk * BM + wm * 16 + g4 + 8 * h) * (HDP + 4);
+        float *pr = part + (long)(wk * BM + wm * 16 + g4 + 8 * h) * PR;
 #pragma unroll
         for (int d = 0; d < DT; d++)
             *reinterpret_cast<float2 *>(pr + d * 8 + t4 * 2) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
-        if (t4 == 0) {
-            pr[HDP] = mx[h];
-            pr[HDP + 1] = sum[h];
-        }
+        if (t4 == 0)
+            *reinterpret_cast<float2 *>(pr + HDP) = make_float2(mx[h], sum[h]);
     }
-    if (a.cs > 1)
-        cluster_sync_all();
-    else
+    const int live = (int)min((long)BM, a.rows - r0);
+    auto store = [&](int row, int col, float v, float l) {
+        const long gr = r0 + row, qi = gr / a.g;
+        if (col < a.hd)
+            ob[qi * a.old + (gr - qi * a.g) * a.os1 + col] =
+                out_of<T>(v * (l > 0.0f || l != l ? 1.0f / l : 0.0f));
+    };
+    __syncthreads();
+    // The warps' parts of an element: O = sum_p O_p 2^(max_p - max), the same
+    // for the sums; kept in the first part (or written, without a cluster).
+    if constexpr (WK > 1) {
+        constexpr int NE = BM * HDP / kThreads;  // elements of a thread
+        float v[NE];
+        float2 ml[NE];
+#pragma unroll
+        for (int i = 0; i < NE; i++) {
+            const int idx = t + i * kThreads, row = idx / HDP, col = idx % HDP;
+            float2 q[WK];
+            float m = -INFINITY;
+#pragma unroll
+            for (int p = 0; p < WK; p++) {
+                q[p] = *reinterpret_cast<const float2 *>(part + (p * BM + row) * PR + HDP);
+                m = fmaxf(m, q[p].x);
+            }
+            ml[i] = make_float2(m, 0.0f);
+            v[i] = 0.0f;
+#pragma unroll
+            for (int p = 0; p < WK; p++) {
+                const float w = q[p].x == -INFINITY ? 0.0f : exp2f(q[p].x - m);
+                v[i] = fmaf(part[(p * BM + row) * PR + col], w, v[i]);
+                ml[i].y = fmaf(q[p].y, w, ml[i].y);
+            }
+        }
         __syncthreads();
-    // Row r belongs to CTA r % cs, a warp per row: weights 2^(max_p - max) of
-    // the cs * WK parts first, then the columns.
-    const int live_rows = (int)min((long)BM, a.rows - r0);
-    const int nparts = a.cs * WK;
+#pragma unroll
+        for (int i = 0; i < NE; i++) {
+            const int idx = t + i * kThreads, row = idx / HDP, col = idx % HDP;
+            if (a.cs > 1) {
+                part[row * PR + col] = v[i];
+                if (col == 0)
+                    *reinterpret_cast<float2 *>(part + row * PR + HDP) = ml[i];
+            }
+            else if (row < live)
+                store(row, col, v[i], ml[i].y);
+        }
+        if (a.cs == 1)
+            return;
+    }
+    // The CTAs' parts: the tile's elements are dealt out to the cluster, every
+    // load of an element in flight at once.
+    cluster_sync_all();
     const uint32_t base = smem_addr(part);
-    for (int r = rank + a.cs * warp; r < live_rows; r += a.cs * 4) {
-        float w[kMaxCluster * WK / 32 + 1];
+    for (int idx = rank * kThreads + t; idx < live * HDP; idx += a.cs * kThreads) {
+        const int row = idx / HDP, col = idx % HDP;
+        const uint32_t at = base + (uint32_t)(row * PR) * 4;
+        float pm[kMaxCluster], pl[kMaxCluster], po[kMaxCluster];
         float m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kMaxCluster * WK / 32 + 1; i++) {
-            const int p = lane + 32 * i;
-            w[i] = -INFINITY;
-            if (p < nparts) {
-                const uint32_t at = base + (uint32_t)(((p % WK) * BM + r) * (HDP + 4) + HDP) * 4;
-                w[i] = ld_dsmem(a.cs > 1 ? mapa_shared(at, p / WK) : at);
-            }
-            m = fmaxf(m, w[i]);
-        }
-#pragma unroll
-        for (int x = 16; x; x >>= 1)
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-        float l = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kMaxCluster * WK / 32 + 1; i++) {
-            const int p = lane + 32 * i;
-            w[i] = w[i] == -INFINITY ? 0.0f : exp2f(w[i] - m);
-            if (p < nparts) {
-                const uint32_t at = base + (uint32_t)(((p % WK) * BM + r) * (HDP + 4) + HDP + 1) * 4;
-                l = fmaf(ld_dsmem(a.cs > 1 ? mapa_shared(at, p / WK) : at), w[i], l);
+        for (int p = 0; p < kMaxCluster; p++) {
+            pm[p] = -INFINITY;
+            pl[p] = po[p] = 0.0f;
+            if (p < a.cs) {
+                const uint32_t src = mapa_shared(at, p);
+                pm[p] = ld_dsmem(src + HDP * 4);
+                pl[p] = ld_dsmem(src + HDP * 4 + 4);
+                po[p] = ld_dsmem(src + col * 4);
             }
         }
 #pragma unroll
-        for (int x = 16; x; x >>= 1)
-            l += __shfl_xor_sync(0xffffffffu, l, x);
-        constexpr int NC = HDP / 32;  // columns of a lane: lane + 32 i
-        float acc[NC];
+        for (int p = 0; p < kMaxCluster; p++)
+            m = fmaxf(m, pm[p]);
+        float v = 0.0f, l = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NC; i++)
-            acc[i] = 0.0f;
-#pragma unroll 2
-        for (int p = 0; p < nparts; p++) {
-            float wp = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kMaxCluster * WK / 32 + 1; i++)
-                if (p / 32 == i)
-                    wp = __shfl_sync(0xffffffffu, w[i], p & 31);
-            const uint32_t at = base + (uint32_t)(((p % WK) * BM + r) * (HDP + 4) + lane) * 4;
-            const uint32_t src = a.cs > 1 ? mapa_shared(at, p / WK) : at;
-#pragma unroll
-            for (int i = 0; i < NC; i++)
-                acc[i] = fmaf(ld_dsmem(src + 128 * i), wp, acc[i]);
+        for (int p = 0; p < kMaxCluster; p++) {
+            const float w = pm[p] == -INFINITY ? 0.0f : exp2f(pm[p] - m);
+            v = fmaf(po[p], w, v);
+            l = fmaf(pl[p], w, l);
         }
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        const long gr = r0 + r, qi = gr / a.g;
-        T *dst = ob + qi * a.old + (gr - qi * a.g) * a.os1;
-#pragma unroll
-        for (int i = 0; i < NC; i++)
-            if (lane + 32 * i < a.hd)
-                dst[lane + 32 * i] = out_of<T>(acc[i] * inv);
+        store(row, col, v, l);
     }
-    if (a.cs > 1)
-        cluster_sync_all();  // peers read this CTA's part until here
+    cluster_sync_all();  // peers read this CTA's part until here
+}
+
+// Few keys (all in one step) and many rows: the bandwidth of Q and O. A CTA
+// reads the keys and values of one key head once and walks over tiles of 64
+// rows, each warp its 16 rows through three cp.async buffers of its own (no
+// block barrier in the loop); one pass of softmax without a running maximum;
+// results go back through the rows' buffer so that they are stored as 16-byte
+// vectors.
+template <typename T, int HDP, int KT>
+__global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constant__ XaArgs a)
+{
+    using TL = Tile<T, HDP>;
+    constexpr int NK = KT * 16, CPR = TL::CPR, EPC = 8, NT = KT * 2, DT = HDP / 8, QB = 16 * TL::PITCH, ST = 3;
+    constexpr bool KEEP = HDP == 32;  // key and value fragments stay in registers
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint8_t *ks = smem, *vs = ks + NK * TL::PITCH;
+    __shared__ uint8_t vis[NK];
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, g4 = lane >> 2, t4 = lane & 3;
+    uint8_t *qs = vs + NK * TL::PITCH + warp * ST * QB;
+    const int split = (int)(blockIdx.x % a.cs), bh = (int)(blockIdx.x / a.cs);  // cs: CTAs walking over a head's tiles
+    const int b = bh / a.kvheads, kh = bh - b * a.kvheads;
+
+    griddep_wait();
+    griddep_launch();
+
+    const T *qb = reinterpret_cast<const T *>(a.q) + b * a.qs0 + (long)kh * a.g * a.qs1;
+    T *ob = reinterpret_cast<T *>(a.o) + b * a.os0 + (long)kh * a.g * a.os1;
+    const int hdc = a.hd / EPC;
+    const int ntile = split < a.nqt ? (a.nqt - 1 - split) / a.cs + 1 : 0;
+    auto row_at = [&](uint32_t gr, long ld, long s1) {
+        const uint32_t qi = quot(gr, a.dg);
+        return qi * ld + (gr - qi * a.dg.d) * s1;
+    };
+    auto load_q = [&](int i) {
+        if (i < ntile) {
+            const uint32_t r0 = (uint32_t)(split + i * a.cs) * 64 + warp * 16;
+#pragma unroll
+            for (int x = lane; x < 16 * CPR; x += 32) {
+                const int r = x / CPR, c = x % CPR;
+                const bool live = r0 + r < a.rows && c < hdc;
+                const T *src = live ? qb + row_at(r0 + r, a.qld, a.qs1) + c * EPC : qb;
+                uint8_t *dst = qs + (i % ST) * QB + TL::at(r, c);
+                if (a.qvec)
+                    cp16(smem_addr(dst), live ? src : a.q, live);
+                else {
+                    T w[EPC];
+#pragma unroll
+                    for (int e = 0; e < EPC; e++)
+                        w[e] = live ? src[e] : out_of<T>(0.0f);
+                    *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(w);
+                }
+            }
+        }
+        cp_commit();
+    };
+    int len = a.Nk;
+    if (a.klen)
+        len = min(max(__ldg(a.klen + b), 0), a.Nk);
+    {
+        const uint8_t *mask = a.kmask ? a.kmask + (long)b * a.Nk : nullptr;
+        const T *kb = reinterpret_cast<const T *>(a.k) + b * a.ks0 + kh * a.ks1;
+        const T *vb = reinterpret_cast<const T *>(a.v) + b * a.vs0 + kh * a.vs1;
+        for (int x = t; x < NK * CPR; x += kThreads) {
+            const int r = x / CPR, c = x % CPR;
+            bool see = r < len;
+            if (see && mask)
+                see = __ldg(mask + r) == 0;
+            const bool live = see && c < hdc;
+            const T *k1 = kb + r * a.kld + c * EPC, *v1 = vb + r * a.vld + c * EPC;
+            uint8_t *kd = ks + TL::at(r, c), *vd = vs + TL::at(r, c);
+            if (a.kvec) {
+                cp16(smem_addr(kd), live ? k1 : kb, live);
+                cp16(smem_addr(vd), live ? v1 : vb, live);
+            }
+            else {
+                T w[EPC], y[EPC];
+#pragma unroll
+                for (int e = 0; e < EPC; e++) {
+                    w[e] = live ? k1[e] : out_of<T>(0.0f);
+                    y[e] = live ? v1[e] : out_of<T>(0.0f);
+                }
+                *reinterpret_cast<uint4 *>(kd) = *reinterpret_cast<const uint4 *>(w);
+                *reinterpret_cast<uint4 *>(vd) = *reinterpret_cast<const uint4 *>(y);
+            }
+            if (c == 0)
+                vis[r] = see;
+        }
+        cp_commit();
+    }
+    load_q(0);
+    load_q(1);
+    cp_wait<2>();
+    __syncthreads();
+    // hidden keys among this lane's columns: bit 2 n + e of tile n, column e
+    uint32_t hide = 0;
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+            hide |= (vis[n * 8 + t4 * 2 + e] ? 0u : 1u) << (2 * n + e);
+    const uint32_t ka = smem_addr(ks), va = smem_addr(vs);
+    auto key_frag = [&](int kk, int n, uint32_t (&f)[4]) {
+        ldsm4(ka + TL::at(n * 8 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)), f);
+    };
+    auto value_frag = [&](int n, int d, uint32_t (&f)[4]) {
+        ldsm4t(va + TL::at(n * 8 + (lane & 15), d + (lane >> 4)), f);
+    };
+    uint32_t kf[KEEP ? HDP / 16 : 1][KEEP ? KT : 1][4], vf[KEEP ? KT : 1][KEEP ? DT / 2 : 1][4];
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int n = 0; n < KT; n++) {
+#pragma unroll
+            for (int kk = 0; kk < HDP / 16; kk++)
+                key_frag(kk, 2 * n, kf[kk][n]);
+#pragma unroll
+            for (int d = 0; d < DT / 2; d++)
+                value_frag(2 * n, 2 * d, vf[n][d]);
+        }
+    }
+    for (int i = 0; i < ntile; i++) {
+        load_q(i + 2);
+        cp_wait<2>();
+        __syncwarp();
+        uint8_t *buf = qs + (i % ST) * QB;
+        float sc[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                sc[n][e] = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < HDP / 16; kk++) {
+            uint32_t qf[4];
+            ldsm4(smem_addr(buf) + TL::at(lane & 15, kk * 2 + (lane >> 4)), qf);
+#pragma unroll
+            for (int n = 0; n < KT; n++) {
+                uint32_t f[4];
+                if constexpr (!KEEP)
+                    key_frag(kk, 2 * n, f);
+                const uint32_t(&k4)[4] = KEEP ? kf[KEEP ? kk : 0][KEEP ? n : 0] : f;
+                mma16<T>(sc[2 * n], qf, k4[0], k4[1]);
+                mma16<T>(sc[2 * n + 1], qf, k4[2], k4[3]);
+            }
+        }
+        if (hide) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                if ((hide >> (2 * n)) & 1)
+                    sc[n][0] = sc[n][2] = -INFINITY;
+                if ((hide >> (2 * n + 1)) & 1)
+                    sc[n][1] = sc[n][3] = -INFINITY;
+            }
+        }
+        __syncwarp();
+        float inv[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float m = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+                m = max3f(m, sc[n][2 * h], sc[n][2 * h + 1]);
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const float base = m == -INFINITY ? 0.0f : -m * a.scale_log2;
+            float s = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                sc[n][2 * h] = ex2_approx(fmaf(sc[n][2 * h], a.scale_log2, base));
+                sc[n][2 * h + 1] = ex2_approx(fmaf(sc[n][2 * h + 1], a.scale_log2, base));
+                s += sc[n][2 * h] + sc[n][2 * h + 1];
+            }
+            s += __shfl_xor_sync(0xffffffffu, s, 1);
+            s += __shfl_xor_sync(0xffffffffu, s, 2);
+            inv[h] = s > 0.0f || s != s ? 1.0f / s : 0.0f;
+        }
+        float o[DT][4];
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                o[d][e] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < KT; n++) {
+            const uint32_t pf[4] = {pack2<T>(sc[2 * n][0], sc[2 * n][1]), pack2<T>(sc[2 * n][2], sc[2 * n][3]),
+                                    pack2<T>(sc[2 * n + 1][0], sc[2 * n + 1][1]),
+                                    pack2<T>(sc[2 * n + 1][2], sc[2 * n + 1][3])};
+#pragma unroll
+            for (int d = 0; d < DT / 2; d++) {
+                uint32_t f[4];
+                if constexpr (!KEEP)
+                    value_frag(2 * n, 2 * d, f);
+                const uint32_t(&v4)[4] = KEEP ? vf[KEEP ? n : 0][KEEP ? d : 0] : f;
+                mma16<T>(o[2 * d], pf, v4[0], v4[1]);
+                mma16<T>(o[2 * d + 1], pf, v4[2], v4[3]);
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                *reinterpret_cast<uint32_t *>(buf + TL::at(g4 + 8 * h, d) + t4 * 4) =
+                    pack2<T>(o[d][2 * h] * inv[h], o[d][2 * h + 1] * inv[h]);
+        __syncwarp();
+        const uint32_t r0 = (uint32_t)(split + i * a.cs) * 64 + warp * 16;
+#pragma unroll
+        for (int x = lane; x < 16 * CPR; x += 32) {
+            const int r = x / CPR, c = x % CPR;
+            if (r0 + r < a.rows && c < hdc) {
+                T *dst = ob + row_at(r0 + r, a.old, a.os1) + c * EPC;
+                const uint4 w = *reinterpret_cast<const uint4 *>(buf + TL::at(r, c));
+                if (a.ovec)
+                    *reinterpret_cast<uint4 *>(dst) = w;
+                else {
+                    const T *e8 = reinterpret_cast<const T *>(&w);
+#pragma unroll
+                    for (int e = 0; e < EPC; e++)
+                        dst[e] = e8[e];
+                }
+            }
+        }
+        __syncwarp();
+    }
+    cp_wait<0>();
+}
+
+template <typename T, int HDP, int KT>
+int launch_few(XaArgs &a, int nb, cudaStream_t s)
+{
+    using TL = Tile<T, HDP>;
+    constexpr int smem = 2 * KT * 16 * TL::PITCH + 4 * 3 * 16 * TL::PITCH;
+    const cudaError_t e = smem_limit_once<attn_few_kernel<T, HDP, KT>>(smem);
+    if (e != cudaSuccess)
+        return (int)e;
+    a.nqt = (int)((a.rows + 63) / 64);
+    // CTAs of a head: about kFewPerSm on every SM
+    constexpr int kFewPerSm = 8;
+    const long heads = (long)nb * a.kvheads, want = (long)kFewPerSm * device_sms() / heads;
+    a.cs = (int)(want < 1 ? 1 : (want < a.nqt ? want : a.nqt));
+    if (heads > 0x7fffffffL / a.cs)
+        return K_EARG;
+    return launch_pdl(attn_few_kernel<T, HDP, KT>, dim3((unsigned)(heads * a.cs)), dim3(kThreads), smem, s,
+                      (const XaArgs)a);
+}
+
+template <typename T, int HDP>
+int launch_few_k(XaArgs &a, int nb, cudaStream_t s)
+{
+    switch ((a.Nk + 15) / 16) {
+    case 1:
+        return launch_few<T, HDP, 1>(a, nb, s);
+    case 2:
+        return launch_few<T, HDP, 2>(a, nb, s);
+    case 3:
+        return launch_few<T, HDP, 3>(a, nb, s);
+    default:
+        return launch_few<T, HDP, 4>(a, nb, s);
+    }
 }
 
 template <auto Kern>
@@ -599,6 +870,11 @@ template <typename T>
 int launch_t(XaArgs &a, int nb, cudaStream_t s)
 {
     const bool few = a.rows <= 16;
+    if constexpr (sizeof(T) == 2) {
+        if (a.Nk <= 64 && !few && a.rows < 0x7fffff00L)
+            return a.hd <= 32 ? launch_few_k<T, 32>(a, nb, s)
+                              : (a.hd <= 64 ? launch_few_k<T, 64>(a, nb, s) : launch_few_k<T, 128>(a, nb, s));
+    }
     if (a.hd <= 32)
         return few ? launch<T, 32, 1>(a, nb, s) : launch<T, 32, 4>(a, nb, s);
     if (a.hd <= 64)
@@ -648,6 +924,9 @@ extern "C" int k_cross_attend(const struct k_rows *Q, const struct k_rows *K, co
     a.qvec = vec(Q);
     a.kvec = vec(K) && vec(V);
     a.ovec = pairs(O);
+    a.dg = make_div(a.g);
+    if (es == 2 && Nk <= 64 && a.rows > 16)
+        a.ovec = vec(O);  // the form for few keys stores 16 bytes
     a.scale_log2 = (float)(scale * 1.4426950408889634);
     a.err = err;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(s);

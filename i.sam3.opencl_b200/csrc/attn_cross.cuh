@@ -3,6 +3,7 @@
 // share: their arguments and the rounding of pairs.
 #pragma once
 
+#include "div.cuh"
 #include "kernels.h"
 #include "tc_ptx.cuh"
 
@@ -21,6 +22,7 @@ struct XaArgs {
     long rows;    // Nq * g rows of one key head
     int nqt, cs;  // tiles of rows, CTAs sharing a tile's keys
     int kvec, qvec, ovec;  // 16-byte accesses allowed
+    Div dg;                // g, for rows < 2^31
     float scale_log2;
     int *err;  // device error word (bounded waits of the tcgen05 form)
 };

@@ -284,7 +284,7 @@ struct k_rows {
 };
 
 /* cs[p * rot / 2 + j] = amp (cos, sin) of (first + p) * turns[j] turns. */
-int k_rope_table(long npos, int rot, long first, const double *turns, float amp,
+int k_rope_table(int npos, int rot, long first, const double *turns, float amp,
                  float *cs, k_stream s);
 /* Y = X with the first rot columns of every head rotated by table row pos[b *
  * N + n] (pos NULL: pos0 + n), rows outside the table copied; X may be Y. */

@@ -2,6 +2,7 @@
 // Rotary positions: tables of angles made on the device, and the rotation of
 // rows by them. The table has the layout of cb_rope_apply: [npos, rot / 2]
 // (cos, sin) pairs in fp32.
+#include "div.cuh"
 #include "kernels.h"
 #include "pdl.cuh"
 #include "tc_ptx.cuh"
@@ -15,17 +16,29 @@ namespace sam3 {
 namespace {
 
 // cos and sin of the angle of `turns` turns. The turns are reduced to a
-// quadrant and a remainder in [-1/8, 1/8] in 64 bits (exact, so far
-// positions lose nothing), the remainder goes through sincospif in 32.
+// quadrant q and a remainder in [-1/8, 1/8] in 64 bits (exact, so far
+// positions lose nothing); sine and cosine of the remainder's angle |x| <= pi / 4
+// are their Taylor polynomials in 32 bits, the first terms left out being
+// x^11 / 11! < 2e-9 and x^12 / 12! < 2e-10.
 __device__ __forceinline__ float2 cos_sin_turns(double turns)
 {
-    const long long q = __double2ll_rn(4.0 * turns);
-    const float r = (float)fma(-0.25, (double)q, turns);
-    float s, c;
-    sincospif(2.0f * r, &s, &c);
+    const double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
+    const double m = fma(4.0, turns, kMagic);
+    const int q = __double2loint(m);
+    const float x = (float)fma(-0.25, m - kMagic, turns) * 6.2831853071795865f;
+    const float z = x * x;
+    float s = fmaf(z, 2.7557319e-6f, -1.9841270e-4f);
+    s = fmaf(s, z, 8.3333333e-3f);
+    s = fmaf(s, z, -0.16666667f);
+    s = fmaf(s * z, x, x);
+    float c = fmaf(z, -2.7557319e-7f, 2.4801587e-5f);
+    c = fmaf(c, z, -1.3888889e-3f);
+    c = fmaf(c, z, 4.1666667e-2f);
+    c = fmaf(c, z, -0.5f);
+    c = fmaf(c, z, 1.0f);
     const float c1 = (q & 1) ? s : c, s1 = (q & 1) ? c : s;
-    const bool neg_c = ((q + 1) & 2) != 0, neg_s = (q & 2) != 0;
-    return make_float2(neg_c ? -c1 : c1, neg_s ? -s1 : s1);
+    return make_float2(__uint_as_float(__float_as_uint(c1) ^ ((uint32_t)(q + 1) << 30 & 0x80000000u)),
+                       __uint_as_float(__float_as_uint(s1) ^ ((uint32_t)q << 30 & 0x80000000u)));
 }
 
 // Frequencies in turns per position, by value (captured graphs keep them).
@@ -33,19 +46,40 @@ struct Freqs {
     double t[K_ROPE_MAX / 2];
 };
 
-// One thread per table entry, entries of a position adjacent: write bound.
+// A thread keeps one pair j (two adjacent ones when half is even) and steps over
+// positions; a block's threads are adjacent entries of the table. Write bound:
+// 131072 positions x 64 pairs in 13.2 us, 5.1 TB/s (63 us with a 64-bit division per entry
+// and sincospif).
+template <int PAIRS>
 __global__ void __launch_bounds__(256) rope_table_kernel(const __grid_constant__ Freqs f, int half,
-                                                         long first, long n, float amp,
+                                                         long first, int npos, float amp,
                                                          float2 *__restrict__ cs)
 {
+    const int width = half / PAIRS, rows = 256 / width;  // threads of a position, positions of a block
+    const int row = threadIdx.x / width, j = (threadIdx.x - row * width) * PAIRS;
     griddep_wait();
     griddep_launch();
-    for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n;
-         i += (long)gridDim.x * blockDim.x) {
-        const long p = i / half;
-        const int j = (int)(i - p * half);
-        const float2 v = cos_sin_turns((double)(first + p) * f.t[j]);
-        cs[i] = make_float2(v.x * amp, v.y * amp);
+    if (row >= rows)
+        return;
+    double w[PAIRS];
+#pragma unroll
+    for (int i = 0; i < PAIRS; i++)
+        w[i] = f.t[j + i];
+    const int step = gridDim.x * rows;
+    float2 *dst = cs + ((long)blockIdx.x * rows + row) * half + j;
+    for (long p = (long)blockIdx.x * rows + row; p < npos; p += step, dst += (long)step * half) {
+        const double pos = (double)(first + p);
+        float2 v[PAIRS];
+#pragma unroll
+        for (int i = 0; i < PAIRS; i++) {
+            v[i] = cos_sin_turns(pos * w[i]);
+            v[i].x *= amp;
+            v[i].y *= amp;
+        }
+        if constexpr (PAIRS == 2)
+            *reinterpret_cast<float4 *>(dst) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        else
+            *dst = v[0];
     }
 }
 
@@ -55,10 +89,11 @@ struct RotArgs {
     const float2 *cs;
     const int *pos;
     long ldx, sx0, sx1, ldy, sy0, sy1;  // elements: row, sequence and head strides
-    long rows;                          // nb * N
-    int N, heads, hd, half, pos0, npos;
-    int nrot, nch;  // chunks of a head: rotated, all (the rest is copied)
-    int nhg, hpt;   // head groups of a row; heads per thread
+    uint32_t row0;                      // first row (of nb * N) of this launch
+    uint32_t total;                     // threads with work, < 2^31
+    int heads, half, pos0, npos;
+    int nrot;             // rotated chunks of a head, the others are copied
+    Div nch, nhg, N;      // chunks of a head, head groups of a row, rows of a sequence
 };
 
 template <typename T>
@@ -104,14 +139,14 @@ __global__ void __launch_bounds__(256) rope_rotate_kernel(const __grid_constant_
     using VO = Vec<TO, W>;
     griddep_wait();
     griddep_launch();
-    const long total = a.rows * a.nhg * a.nch;
-    for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-         i += (long)gridDim.x * blockDim.x) {
-        const long rg = i / a.nch;
-        const int c = (int)(i - rg * a.nch);
-        const long row = rg / a.nhg;
-        const int hg = (int)(rg - row * a.nhg);
-        const long b = row / a.N, n = row - b * a.N;
+    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+    if (i < a.total) {
+        const uint32_t rg = quot(i, a.nch);
+        const int c = (int)(i - rg * a.nch.d);
+        const uint32_t rl = quot(rg, a.nhg);
+        const int hg = (int)(rg - rl * a.nhg.d);
+        const uint32_t row = a.row0 + rl;
+        const long b = quot(row, a.N), n = row - (uint32_t)b * a.N.d;
         const long p = a.pos ? (long)__ldg(a.pos + row) : a.pos0 + n;
         const bool turn = c < a.nrot && p >= 0 && p < a.npos;
         const TI *x = reinterpret_cast<const TI *>(a.x) + b * a.sx0 + n * a.ldx;
@@ -139,7 +174,7 @@ __global__ void __launch_bounds__(256) rope_rotate_kernel(const __grid_constant_
                                    : 2 * a.half + (c - a.nrot) * W;
         const int col2 = HALVES ? col + a.half : col + 1;
 #pragma unroll 4
-        for (int h = hg; h < a.heads; h += a.nhg) {
+        for (int h = hg; h < a.heads; h += a.nhg.d) {
             const TI *xh = x + h * a.sx1;
             TO *yh = y + h * a.sy1;
             const VI u = *reinterpret_cast<const VI *>(xh + col);
@@ -178,42 +213,55 @@ __global__ void __launch_bounds__(256) rope_rotate_kernel(const __grid_constant_
 }
 
 template <typename TI, typename TO, int W, bool HALVES>
-int launch(RotArgs &a, bool in_place, cudaStream_t s)
+int launch(RotArgs &a, long rows, int N, int hd, bool in_place, cudaStream_t s)
 {
     const int rot = 2 * a.half;
     a.nrot = HALVES ? a.half / W : (W > 1 ? rot / W : a.half);
-    a.nch = a.nrot + (in_place ? 0 : (a.hd - rot) / W);
+    const int nch = a.nrot + (in_place ? 0 : (hd - rot) / W);
     // Heads per thread: 4 when that leaves a few waves of threads.
-    const long one = a.rows * a.heads * a.nch;
-    const long fill = (long)device_sms() * 2048 * 2;
-    a.hpt = one >= 4 * fill ? 4 : (one >= 2 * fill ? 2 : 1);
-    a.nhg = (a.heads + a.hpt - 1) / a.hpt;
-    const long total = a.rows * a.nhg * a.nch, blocks = (total + 255) / 256;
-    return launch_pdl(rope_rotate_kernel<TI, TO, W, HALVES>,
-                      dim3((unsigned)(blocks < 0x7fffffffL ? blocks : 0x7fffffffL)), dim3(256), 0, s,
-                      (const RotArgs)a);
+    const double one = (double)rows * a.heads * nch;
+    const double fill = (double)device_sms() * 2048 * 2;
+    const int hpt = one >= 4 * fill ? 4 : (one >= 2 * fill ? 2 : 1);
+    const int nhg = (a.heads + hpt - 1) / hpt;
+    a.nch = make_div(nch);
+    a.nhg = make_div(nhg);
+    a.N = make_div(N);
+    // one launch up to 2^31 - 256 threads, which only larger tensors pass
+    const long most = 0x7fffff00L / ((long)nch * nhg);
+    if (most < 1 || rows > 0x7fffffffL)
+        return K_EARG;
+    for (long r = 0; r < rows; r += most) {
+        const long n = rows - r < most ? rows - r : most;
+        a.row0 = (uint32_t)r;
+        a.total = (uint32_t)(n * nch * nhg);
+        const int rc = launch_pdl(rope_rotate_kernel<TI, TO, W, HALVES>, dim3((a.total + 255) / 256), dim3(256),
+                                  0, s, (const RotArgs)a);
+        if (rc)
+            return rc;
+    }
+    return 0;
 }
 
 template <typename TI, typename TO>
-int launch_w(RotArgs &a, int layout, bool in_place, cudaStream_t s)
+int launch_w(RotArgs &a, long rows, int N, int hd, int layout, bool in_place, cudaStream_t s)
 {
     constexpr int W = 16 / sizeof(TI);
     const int rot = 2 * a.half;
     auto whole = [&](long v) { return v % W == 0; };
     const bool vec = whole(a.ldx) && whole(a.sx0) && whole(a.sx1) && whole(a.ldy) && whole(a.sy0) &&
                      whole(a.sy1) && whole(layout == K_ROPE_HALVES ? a.half : rot) &&
-                     (in_place || whole(a.hd)) && !(reinterpret_cast<uintptr_t>(a.x) & 15) &&
+                     (in_place || whole(hd)) && !(reinterpret_cast<uintptr_t>(a.x) & 15) &&
                      reinterpret_cast<uintptr_t>(a.y) % (W * sizeof(TO)) == 0 &&
                      !(reinterpret_cast<uintptr_t>(a.cs) & 15);
     if (layout == K_ROPE_HALVES)
-        return vec ? launch<TI, TO, W, true>(a, in_place, s) : launch<TI, TO, 1, true>(a, in_place, s);
-    return vec ? launch<TI, TO, W, false>(a, in_place, s) : launch<TI, TO, 1, false>(a, in_place, s);
+        return vec ? launch<TI, TO, W, true>(a, rows, N, hd, in_place, s) : launch<TI, TO, 1, true>(a, rows, N, hd, in_place, s);
+    return vec ? launch<TI, TO, W, false>(a, rows, N, hd, in_place, s) : launch<TI, TO, 1, false>(a, rows, N, hd, in_place, s);
 }
 
 }  // namespace
 }  // namespace sam3
 
-extern "C" int k_rope_table(long npos, int rot, long first, const double *turns, float amp, float *cs,
+extern "C" int k_rope_table(int npos, int rot, long first, const double *turns, float amp, float *cs,
                             k_stream s)
 {
     using namespace sam3;
@@ -224,10 +272,15 @@ extern "C" int k_rope_table(long npos, int rot, long first, const double *turns,
         f.t[j] = turns[j];
     for (int j = rot / 2; j < K_ROPE_MAX / 2; j++)
         f.t[j] = 0.0;
-    const long n = npos * (rot / 2), blocks = (n + 255) / 256, most = (long)device_sms() * 8;
-    return launch_pdl(rope_table_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0,
-                      reinterpret_cast<cudaStream_t>(s), f, rot / 2, first, n, amp,
-                      reinterpret_cast<float2 *>(cs));
+    const int half = rot / 2, pairs = half % 2 == 0 && !(reinterpret_cast<uintptr_t>(cs) & 15) ? 2 : 1;
+    const int rows = 256 / (half / pairs);
+    const long blocks = (npos + rows - 1) / rows, most = (long)device_sms() * 8;
+    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(s);
+    return pairs == 2 ? launch_pdl(rope_table_kernel<2>, grid, dim3(256), 0, st, f, half, first, npos, amp,
+                                   reinterpret_cast<float2 *>(cs))
+                      : launch_pdl(rope_table_kernel<1>, grid, dim3(256), 0, st, f, half, first, npos, amp,
+                                   reinterpret_cast<float2 *>(cs));
 }
 
 extern "C" int k_rope_rotate(const struct k_rows *X, const struct k_rows *Y, int nb, int N, int heads,
@@ -250,22 +303,19 @@ extern "C" int k_rope_rotate(const struct k_rows *X, const struct k_rows *Y, int
     a.pos = pos;
     a.pos0 = pos0;
     a.npos = npos;
-    a.N = N;
-    a.rows = (long)nb * N;
     a.heads = heads;
-    a.hd = hd;
     a.half = rot / 2;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(s);
     const bool in_place = X->p == Y->p;  // the caller has checked that the layouts agree
     if (X->dt == K_F32 && Y->dt == K_F32)
-        return launch_w<float, float>(a, layout, in_place, st);
+        return launch_w<float, float>(a, (long)nb * N, N, hd, layout, in_place, st);
     if (X->dt == K_F32 && Y->dt == K_BF16)
-        return launch_w<float, __nv_bfloat16>(a, layout, in_place, st);
+        return launch_w<float, __nv_bfloat16>(a, (long)nb * N, N, hd, layout, in_place, st);
     if (X->dt == K_F32 && Y->dt == K_F16)
-        return launch_w<float, __half>(a, layout, in_place, st);
+        return launch_w<float, __half>(a, (long)nb * N, N, hd, layout, in_place, st);
     if (X->dt == K_BF16 && Y->dt == K_BF16)
-        return launch_w<__nv_bfloat16, __nv_bfloat16>(a, layout, in_place, st);
+        return launch_w<__nv_bfloat16, __nv_bfloat16>(a, (long)nb * N, N, hd, layout, in_place, st);
     if (X->dt == K_F16 && Y->dt == K_F16)
-        return launch_w<__half, __half>(a, layout, in_place, st);
+        return launch_w<__half, __half>(a, (long)nb * N, N, hd, layout, in_place, st);
     return K_EARG;
 }

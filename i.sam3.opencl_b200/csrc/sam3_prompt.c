@@ -182,8 +182,8 @@ int cb_rope_rotate(cb_backend *b, int nb, int N, int heads, int hd, int rot, int
     struct rows x, y;
     int rc;
 
-    if (!b || nb <= 0 || N <= 0 || N > MAX_ROWS || heads <= 0 || hd <= 0 || rot <= 0 || rot % 2 ||
-        rot > hd || npos <= 0 || (layout != CB_ROPE_PAIRS && layout != CB_ROPE_HALVES) ||
+    if (!b || nb <= 0 || N <= 0 || N > MAX_ROWS || (int64_t)nb * N > INT32_MAX || heads <= 0 ||
+        hd <= 0 || hd > (1 << 16) || heads > (1 << 14) || rot <= 0 || rot % 2 || rot > hd || npos <= 0 || (layout != CB_ROPE_PAIRS && layout != CB_ROPE_HALVES) ||
         !vec_ok(cs, CB_F32, (int64_t)npos * rot) || (uintptr_t)cs->ptr % 8)
         return cbi_fail(b, CB_EARG, "rope_rotate");
     if (pos ? (pos0 != 0 || !vec_ok(pos, CB_I32, (int64_t)nb * N))
