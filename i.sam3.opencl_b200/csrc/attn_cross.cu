@@ -90,6 +90,22 @@ __device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// D = A B + C with C the same for both row halves.
+template <typename T>
+__device__ __forceinline__ void mma16_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
+                                           float c1)
+{
+    if constexpr (__is_same(T, __half))
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+                     "{%8,%9}, {%10,%11,%10,%11};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+                     "{%8,%9}, {%10,%11,%10,%11};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
 __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
@@ -97,13 +113,14 @@ __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo: hi rounded to tf32's 11 significand bits, lo the rest rounded
-// the same way.
+// x = hi + lo: hi rounded to tf32's 11 significand bits, lo what is left of the
+// 24, cut to 11 (off by 2^-22 of x at most).
 __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo)
 {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
+
 // Shared memory of a tile in 16-byte chunks. 16-bit types: rows of HDP * 2
 // bytes with the chunk index XORed by the row (no conflicts for ldmatrix);
 // fp32: rows padded by 16 bytes (fragment loads of 4 rows x 8 columns hit 32
@@ -489,6 +506,8 @@ __global__ void __launch_bounds__(kThreads) attn_cross_kernel(const __grid_const
 #pragma unroll
         for (int i = 0; i < NE; i++) {
             const int idx = t + i * kThreads, row = idx / HDP, col = idx % HDP;
+            if (row >= live)
+                continue;
             float2 q[WK];
             float m = -INFINITY;
 #pragma unroll
@@ -509,12 +528,14 @@ __global__ void __launch_bounds__(kThreads) attn_cross_kernel(const __grid_const
 #pragma unroll
         for (int i = 0; i < NE; i++) {
             const int idx = t + i * kThreads, row = idx / HDP, col = idx % HDP;
+            if (row >= live)
+                continue;
             if (a.cs > 1) {
                 part[row * PR + col] = v[i];
                 if (col == 0)
                     *reinterpret_cast<float2 *>(part + row * PR + HDP) = ml[i];
             }
-            else if (row < live)
+            else
                 store(row, col, v[i], ml[i].y);
         }
         if (a.cs == 1)
@@ -527,28 +548,35 @@ __global__ void __launch_bounds__(kThreads) attn_cross_kernel(const __grid_const
     for (int idx = rank * kThreads + t; idx < live * HDP; idx += a.cs * kThreads) {
         const int row = idx / HDP, col = idx % HDP;
         const uint32_t at = base + (uint32_t)(row * PR) * 4;
-        float pm[kMaxCluster], pl[kMaxCluster], po[kMaxCluster];
-        float m = -INFINITY;
+        constexpr int B = 8;  // parts at a time
+        float m = -INFINITY, v = 0.0f, l = 0.0f;
+#pragma unroll 1
+        for (int p0 = 0; p0 < a.cs; p0 += B) {
+            float pm[B], pl[B], po[B], mb = m;
 #pragma unroll
-        for (int p = 0; p < kMaxCluster; p++) {
-            pm[p] = -INFINITY;
-            pl[p] = po[p] = 0.0f;
-            if (p < a.cs) {
-                const uint32_t src = mapa_shared(at, p);
-                pm[p] = ld_dsmem(src + HDP * 4);
-                pl[p] = ld_dsmem(src + HDP * 4 + 4);
-                po[p] = ld_dsmem(src + col * 4);
+            for (int p = 0; p < B; p++) {
+                pm[p] = -INFINITY;
+                pl[p] = po[p] = 0.0f;
+                if (p0 + p < a.cs) {
+                    const uint32_t src = mapa_shared(at, p0 + p);
+                    pm[p] = ld_dsmem(src + HDP * 4);
+                    pl[p] = ld_dsmem(src + HDP * 4 + 4);
+                    po[p] = ld_dsmem(src + col * 4);
+                }
             }
-        }
 #pragma unroll
-        for (int p = 0; p < kMaxCluster; p++)
-            m = fmaxf(m, pm[p]);
-        float v = 0.0f, l = 0.0f;
+            for (int p = 0; p < B; p++)
+                mb = fmaxf(mb, pm[p]);
+            const float c = m == -INFINITY ? 1.0f : exp2f(m - mb);
+            v *= c;
+            l *= c;
+            m = mb;
 #pragma unroll
-        for (int p = 0; p < kMaxCluster; p++) {
-            const float w = pm[p] == -INFINITY ? 0.0f : exp2f(pm[p] - m);
-            v = fmaf(po[p], w, v);
-            l = fmaf(pl[p], w, l);
+            for (int p = 0; p < B; p++) {
+                const float w = pm[p] == -INFINITY ? 0.0f : exp2f(pm[p] - m);
+                v = fmaf(po[p], w, v);
+                l = fmaf(pl[p], w, l);
+            }
         }
         store(row, col, v, l);
     }
@@ -583,6 +611,8 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
     const int hdc = a.hd / EPC;
     const int ntile = split < a.nqt ? (a.nqt - 1 - split) / a.cs + 1 : 0;
     auto row_at = [&](uint32_t gr, long ld, long s1) {
+        if (a.g == 1)
+            return gr * ld;
         const uint32_t qi = quot(gr, a.dg);
         return qi * ld + (gr - qi * a.dg.d) * s1;
     };
@@ -646,13 +676,14 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
     load_q(1);
     cp_wait<2>();
     __syncthreads();
-    // hidden keys among this lane's columns: bit 2 n + e of tile n, column e
-    uint32_t hide = 0;
+    // What a lane's columns of the scores start from: -inf where the key is
+    // hidden (its row of K is zero)
+    float start[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int e = 0; e < 2; e++)
-            hide |= (vis[n * 8 + t4 * 2 + e] ? 0u : 1u) << (2 * n + e);
+            start[n][e] = vis[n * 8 + t4 * 2 + e] ? 0.0f : -INFINITY;
     const uint32_t ka = smem_addr(ks), va = smem_addr(vs);
     auto key_frag = [&](int kk, int n, uint32_t (&f)[4]) {
         ldsm4(ka + TL::at(n * 8 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)), f);
@@ -679,11 +710,6 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
         uint8_t *buf = qs + (i % ST) * QB;
         float sc[NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                sc[n][e] = 0.0f;
-#pragma unroll
         for (int kk = 0; kk < HDP / 16; kk++) {
             uint32_t qf[4];
             ldsm4(smem_addr(buf) + TL::at(lane & 15, kk * 2 + (lane >> 4)), qf);
@@ -693,17 +719,14 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
                 if constexpr (!KEEP)
                     key_frag(kk, 2 * n, f);
                 const uint32_t(&k4)[4] = KEEP ? kf[KEEP ? kk : 0][KEEP ? n : 0] : f;
-                mma16<T>(sc[2 * n], qf, k4[0], k4[1]);
-                mma16<T>(sc[2 * n + 1], qf, k4[2], k4[3]);
-            }
-        }
-        if (hide) {
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                if ((hide >> (2 * n)) & 1)
-                    sc[n][0] = sc[n][2] = -INFINITY;
-                if ((hide >> (2 * n + 1)) & 1)
-                    sc[n][1] = sc[n][3] = -INFINITY;
+                if (kk == 0) {
+                    mma16_from<T>(sc[2 * n], qf, k4[0], k4[1], start[2 * n][0], start[2 * n][1]);
+                    mma16_from<T>(sc[2 * n + 1], qf, k4[2], k4[3], start[2 * n + 1][0], start[2 * n + 1][1]);
+                }
+                else {
+                    mma16<T>(sc[2 * n], qf, k4[0], k4[1]);
+                    mma16<T>(sc[2 * n + 1], qf, k4[2], k4[3]);
+                }
             }
         }
         __syncwarp();
@@ -778,6 +801,25 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
     cp_wait<0>();
 }
 
+// CTAs of a kernel that run at the same time, asked once per device.
+template <auto Kern>
+long resident(int smem)
+{
+    static int known[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 && known[dev])
+        n = known[dev];
+    else {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kern, kThreads, smem) != cudaSuccess || n < 1) {
+            (void)cudaGetLastError();
+            n = 1;
+        }
+        if (dev >= 0 && dev < 64)
+            known[dev] = n;
+    }
+    return (long)n * device_sms();
+}
+
 template <typename T, int HDP, int KT>
 int launch_few(XaArgs &a, int nb, cudaStream_t s)
 {
@@ -787,9 +829,8 @@ int launch_few(XaArgs &a, int nb, cudaStream_t s)
     if (e != cudaSuccess)
         return (int)e;
     a.nqt = (int)((a.rows + 63) / 64);
-    // CTAs of a head: about kFewPerSm on every SM
-    constexpr int kFewPerSm = 8;
-    const long heads = (long)nb * a.kvheads, want = (long)kFewPerSm * device_sms() / heads;
+    // CTAs of a head: all that run at once
+    const long heads = (long)nb * a.kvheads, want = resident<attn_few_kernel<T, HDP, KT>>(smem) / heads;
     a.cs = (int)(want < 1 ? 1 : (want < a.nqt ? want : a.nqt));
     if (heads > 0x7fffffffL / a.cs)
         return K_EARG;
@@ -841,9 +882,9 @@ int launch(XaArgs &a, int nb, cudaStream_t s)
         return K_EARG;
     a.nqt = (int)nqt;
     const long items = (long)nb * a.kvheads * nqt;
-    // CTAs sharing a tile's keys: until two CTAs per SM are busy, each with
-    // at least two steps.
-    const long slots = 2L * device_sms(), steps = (a.Nk + Cfg<T, HDP>::BK - 1) / Cfg<T, HDP>::BK;
+    // CTAs sharing a tile's keys: while all run at once, each with at least
+    // two steps.
+    const long slots = resident<attn_cross_kernel<T, HDP, WM>>(smem), steps = (a.Nk + Cfg<T, HDP>::BK - 1) / Cfg<T, HDP>::BK;
     a.cs = 1;
     while (a.cs < kMaxCluster && items * a.cs * 2 <= slots && steps >= a.cs * 4)
         a.cs *= 2;
