@@ -159,7 +159,8 @@ constexpr int smem_bytes()
 }
 
 template <typename T, int HDP, int WM>
-__global__ void __launch_bounds__(kThreads) attn_cross_kernel(const __grid_constant__ XaArgs a)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 5 : 1)
+    attn_cross_kernel(const __grid_constant__ XaArgs a)
 {
     using TL = Tile<T, HDP>;
     using CF = Cfg<T, HDP>;
@@ -185,7 +186,6 @@ __global__ void __launch_bounds__(kThreads) attn_cross_kernel(const __grid_const
     const long r0 = (long)qt * BM;
 
     griddep_wait();
-    griddep_launch();
 
     int len = a.Nk;
     if (a.klen)
@@ -441,6 +441,10 @@ __global__ void __launch_bounds__(kThreads) attn_cross_kernel(const __grid_const
         }
     }
     cp_wait<0>();
+    // The next kernel's CTAs may come now: earlier they would take the free
+    // slots of some SMs and leave it badly spread (201 queries over 5184 keys in
+    // 32 bits: 83 us alone, 100 us in a row of such calls).
+    griddep_launch();
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
@@ -604,7 +608,6 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
     const int b = bh / a.kvheads, kh = bh - b * a.kvheads;
 
     griddep_wait();
-    griddep_launch();
 
     const T *qb = reinterpret_cast<const T *>(a.q) + b * a.qs0 + (long)kh * a.g * a.qs1;
     T *ob = reinterpret_cast<T *>(a.o) + b * a.os0 + (long)kh * a.g * a.os1;
@@ -685,6 +688,8 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
         for (int e = 0; e < 2; e++)
             start[n][e] = vis[n * 8 + t4 * 2 + e] ? 0.0f : -INFINITY;
     const uint32_t ka = smem_addr(ks), va = smem_addr(vs);
+    constexpr uint32_t kOnes = __is_same(T, __half) ? 0x3c003c00u : 0x3f803f80u;
+    const uint64_t sl2x2 = f2_make(a.scale_log2, a.scale_log2);
     auto key_frag = [&](int kk, int n, uint32_t (&f)[4]) {
         ldsm4(ka + TL::at(n * 8 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)), f);
     };
@@ -740,23 +745,16 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
             const float base = m == -INFINITY ? 0.0f : -m * a.scale_log2;
-            float s = 0.0f;
+            const uint64_t base2 = f2_make(base, base);
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                sc[n][2 * h] = ex2_approx(fmaf(sc[n][2 * h], a.scale_log2, base));
-                sc[n][2 * h + 1] = ex2_approx(fmaf(sc[n][2 * h + 1], a.scale_log2, base));
-                s += sc[n][2 * h] + sc[n][2 * h + 1];
+                float x, y;
+                f2_split(fma2(f2_make(sc[n][2 * h], sc[n][2 * h + 1]), sl2x2, base2), x, y);
+                sc[n][2 * h] = ex2_approx(x);
+                sc[n][2 * h + 1] = ex2_approx(y);
             }
-            s += __shfl_xor_sync(0xffffffffu, s, 1);
-            s += __shfl_xor_sync(0xffffffffu, s, 2);
-            inv[h] = s > 0.0f || s != s ? 1.0f / s : 0.0f;
         }
-        float o[DT][4];
-#pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                o[d][e] = 0.0f;
+        float o[DT][4], sums[4];  // sums: a row's P times ones
 #pragma unroll
         for (int n = 0; n < KT; n++) {
             const uint32_t pf[4] = {pack2<T>(sc[2 * n][0], sc[2 * n][1]), pack2<T>(sc[2 * n][2], sc[2 * n][3]),
@@ -768,10 +766,23 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
                 if constexpr (!KEEP)
                     value_frag(2 * n, 2 * d, f);
                 const uint32_t(&v4)[4] = KEEP ? vf[KEEP ? n : 0][KEEP ? d : 0] : f;
-                mma16<T>(o[2 * d], pf, v4[0], v4[1]);
-                mma16<T>(o[2 * d + 1], pf, v4[2], v4[3]);
+                if (n == 0) {
+                    mma16_from<T>(o[2 * d], pf, v4[0], v4[1], 0.0f, 0.0f);
+                    mma16_from<T>(o[2 * d + 1], pf, v4[2], v4[3], 0.0f, 0.0f);
+                }
+                else {
+                    mma16<T>(o[2 * d], pf, v4[0], v4[1]);
+                    mma16<T>(o[2 * d + 1], pf, v4[2], v4[3]);
+                }
             }
+            if (n == 0)
+                mma16_from<T>(sums, pf, kOnes, kOnes, 0.0f, 0.0f);
+            else
+                mma16<T>(sums, pf, kOnes, kOnes);
         }
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            inv[h] = sums[2 * h] > 0.0f || sums[2 * h] != sums[2 * h] ? 1.0f / sums[2 * h] : 0.0f;
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -799,6 +810,7 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
         __syncwarp();
     }
     cp_wait<0>();
+    griddep_launch();
 }
 
 // CTAs of a kernel that run at the same time, asked once per device.

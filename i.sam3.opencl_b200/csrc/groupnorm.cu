@@ -206,7 +206,6 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
     const long dx = a.rows * a.ldx, dy = a.rows * a.ldy;
 
     griddep_wait();
-    griddep_launch();
 
     // Batches of kUnroll steps, bpk per block of vectors, in order: this thread's
     // vectors of the next one into its slots of the ring. All ring indexes
@@ -431,6 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
     if (a.cs > 1)
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
+    griddep_launch();
     // Back from the last batch; those before the ring's are re-read as its slots
     // come free.
     const float lowest = a.act == K_ACT_RELU ? 0.0f : -INFINITY;
