@@ -24,6 +24,7 @@
 // sum M2_i + n_i (mean_i - mean)^2 in a fixed order, so a result does not depend
 // on timing. Per-channel pairs cost about as many instructions as one pair per
 // vector and let a vector span groups of any width.
+#include "div.cuh"
 #include "kernels.h"
 #include "pdl.cuh"
 #include "tc_ptx.cuh"
@@ -36,12 +37,12 @@
 namespace sam3 {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kUnroll = 4;
 constexpr int kSlabBytes = 64;
 constexpr int kMaxSlabGroups = 128;
 constexpr int kMaxCluster = 16;
-constexpr int kRing = 24;  // slots of 16-byte vectors, 6 batches
+constexpr int kRing = 48;  // slots of 16-byte vectors, 12 batches
 constexpr int kRingBytes = kThreads * kRing * 16;  // per CTA, one per SM
 
 struct GnArgs {
@@ -51,6 +52,7 @@ struct GnArgs {
     long ldx, sx, ldy, sy;  // elements: pixel and sample strides
     long per, extra;        // pixels of a CTA; the first `extra` ranks have one more
     int steps, srem;        // per / rows, per % rows
+    Div dcg;                // cg
     int cg, gps, S, nslab;  // group width, groups and channels per slab, slabs
     int lpp;                // vectors per pixel of a slab
     int rows, nk;           // pixels per step, blocks of vectors per pixel (lpp > kThreads)
@@ -180,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
     // ring of slots, then the threads' statistics: (mean, M2) per thread, or per channel of it
     extern __shared__ __align__(16) uint8_t dyn[];
     constexpr int VB = (int)sizeof(VI);
-    constexpr int kAhead = 2;  // batches in flight; the ring has at least one more
+    constexpr int kAhead = 4;  // batches in flight; the ring has at least one more
     uint8_t *ring = dyn + threadIdx.x * VB;
     float2 *red = reinterpret_cast<float2 *>(dyn + (size_t)a.nring * kUnroll * kThreads * VB);
     __shared__ float pub[kMaxSlabGroups][3];  // this CTA's (n, mean, M2), read by the cluster
@@ -242,6 +244,21 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
         fetch_commit();
     }
     int i = 0, islot = 0;  // batch at hand
+    // gamma, beta and group of this thread's channels in block k of vectors
+    // (the first block to be written is read while X arrives)
+    float cgam[2 * NP], cbet[2 * NP];
+    int cgrp[2 * NP];
+    auto channel_params = [&](int k) {
+        const int lane = lane0 + k * kThreads;
+#pragma unroll
+        for (int e = 0; e < 2 * NP; e++) {
+            const int ch = (lane < a.lpp ? lane : 0) * V + (e < V ? e : 0);
+            cgrp[e] = a.gps == 1 ? 0 : (int)quot(ch, a.dcg);
+            cgam[e] = __ldg(a.g + c0 + ch);
+            cbet[e] = __ldg(a.b + c0 + ch);
+        }
+    };
+    channel_params(a.nk - 1);
     float tn = 0.0f, tmean = 0.0f, tm2 = 0.0f;  // the thread's, over its vectors (not span)
     for (int k = 0; k < a.nk; k++) {
         const int lane = lane0 + k * kThreads;
@@ -443,13 +460,14 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
         uint64_t nm[NP], ga[NP], be[NP];  // -mean, gamma rstd, beta
         {
             float sm[2 * NP], sg[2 * NP], sb[2 * NP];
+            if (k < a.nk - 1)
+                channel_params(k);
 #pragma unroll
             for (int e = 0; e < 2 * NP; e++) {
-                const int ch = (lane < a.lpp ? lane : 0) * V + (e < V ? e : 0);
-                const float2 st = gstat[ch / a.cg];
+                const float2 st = gstat[cgrp[e]];
                 sm[e] = -st.x;
-                sg[e] = __ldg(a.g + c0 + ch) * st.y;
-                sb[e] = __ldg(a.b + c0 + ch);
+                sg[e] = cgam[e] * st.y;
+                sb[e] = cbet[e];
             }
 #pragma unroll
             for (int e = 0; e < NP; e++) {
@@ -574,8 +592,8 @@ int launch_a(GnArgs &a, int nb, long npix, int C, cudaStream_t s)
     // than a step
     const long steps = (npix + a.rows - 1) / a.rows;
     a.cs = 1;
-    for (int c = 2; c <= kMaxCluster; c *= 2)
-        if (units <= clusters_at_once<TI, TO, V, GELU>(c) && c <= steps)
+    for (int c = 2; c <= kMaxCluster && c <= steps; c++)
+        if (units <= clusters_at_once<TI, TO, V, GELU>(c))
             a.cs = c;
     a.per = npix / a.cs;
     a.extra = npix - a.per * a.cs;
@@ -670,6 +688,7 @@ extern "C" int k_groupnorm(const void *X, int xt, long ldx, long sx, void *Y, in
     a.ldy = ldy;
     a.sy = sy;
     a.cg = C / groups;
+    a.dcg = make_div(a.cg);
     a.eps = eps;
     a.act = act;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(s);
