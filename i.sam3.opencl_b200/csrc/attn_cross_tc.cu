@@ -100,7 +100,7 @@ struct TcArgs {
     int qb0, qb1, kb0, kb1, vb0, vb1;  // 1: the map has that dimension (stride not 0)
 };
 
-template <typename T, int HDP, bool SPLIT>
+template <typename T, int HDP, bool SPLIT, bool MASK>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     attn_cross_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                          const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TcArgs ta)
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             const Item it = item_at(u);
             const bool rows_live = it.qt * BQ + quarter * 32 < a.Nq;
             const int q = it.qt * BQ + r;
-            const uint8_t *mask = a.kmask ? a.kmask + (long)it.seq * a.Nk : nullptr;
+            const uint8_t *mask = MASK ? a.kmask + (long)it.seq * a.Nk : nullptr;
             float m_used = -INFINITY;
             uint64_t lsum0 = 0, lsum1 = 0;
             uint8_t ahead[NW];  // mask bytes of the next tile, a key per lane
@@ -337,28 +337,27 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
                 for (int w = 0; w < NW; w++) {
                     const int key = (it.j0 + j) * BKV + w * 32 + lane;
-                    ahead[w] = mask && j < it.n && key < it.len ? __ldg(mask + key) : 0;
+                    ahead[w] = MASK && j < it.n && key < it.len ? __ldg(mask + key) : 0;
                 }
             };
             look(0);
             for (int j = 0; j < it.n; j++, g++) {
                 const int b = g & 1;
-                // visible keys of the tile
+                // visible keys of the tile; without a mask only the last tile
+                // can hold hidden ones
                 uint32_t vis[NW];
-                bool whole = true;
-#pragma unroll
-                for (int w = 0; w < NW; w++)
-                    vis[w] = 0xffffffffu;
-                if (mask || j == it.n - 1) {
+                bool whole = MASK || j < it.n - 1 || (it.j0 + it.n) * BKV <= it.len;
+                if (MASK || !whole) {
 #pragma unroll
                     for (int w = 0; w < NW; w++) {
                         const int left = it.len - (it.j0 + j) * BKV - w * 32;
                         vis[w] = left >= 32 ? 0xffffffffu : (left > 0 ? (1u << left) - 1 : 0u);
-                        if (mask)
+                        if (MASK) {
                             vis[w] &= __ballot_sync(0xffffffffu, ahead[w] == 0);
-                        whole = whole && vis[w] == 0xffffffffu;
+                            whole = whole && vis[w] == 0xffffffffu;
+                        }
                     }
-                    if (mask)
+                    if (MASK)
                         look(j + 1);
                 }
                 if (!whole) {
@@ -446,10 +445,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                         auto chunk = [&](int c, uint32_t (&s)[32]) {
                             tmem_ld32(tS + 32 * c, s);
                             tmem_wait_ld();
-                            uint32_t seen = vis[0];
+                            uint32_t seen = 0xffffffffu;
+                            if (!whole) {
 #pragma unroll
-                            for (int w = 1; w < NW; w++)
-                                seen = c == w ? vis[w] : seen;
+                                for (int w = 0; w < NW; w++)
+                                    seen = c == w ? vis[w] : seen;
+                            }
 #pragma unroll
                             for (int e = 0; e < 32; e++)
                                 if (!((seen >> e) & 1))
@@ -658,10 +659,10 @@ bool make_map(CUtensorMap *map, bool bf16, const void *p, int hd, long rows, int
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int HDP, bool SPLIT>
+template <typename T, int HDP, bool SPLIT, bool MASK>
 int launch(TcArgs &ta, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, int grid, cudaStream_t s)
 {
-    const cudaError_t e = smem_limit_once<attn_cross_tc_kernel<T, HDP, SPLIT>>(Geo<HDP>::SMEM);
+    const cudaError_t e = smem_limit_once<attn_cross_tc_kernel<T, HDP, SPLIT, MASK>>(Geo<HDP>::SMEM);
     if (e != cudaSuccess)
         return (int)e;
     cudaLaunchAttribute attr[2];
@@ -678,7 +679,7 @@ int launch(TcArgs &ta, const CUtensorMap &tq, const CUtensorMap &tk, const CUten
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = SPLIT ? 2 : 1;
-    return (int)cudaLaunchKernelEx(&cfg, attn_cross_tc_kernel<T, HDP, SPLIT>, tq, tk, tv, (const TcArgs)ta);
+    return (int)cudaLaunchKernelEx(&cfg, attn_cross_tc_kernel<T, HDP, SPLIT, MASK>, tq, tk, tv, (const TcArgs)ta);
 }
 
 template <typename T, int HDP>
@@ -703,9 +704,12 @@ int run(XaArgs &x, int nb, bool bf16, cudaStream_t s)
         cs *= 2;
     x.cs = cs;
     ta.x = x;
+    const int grid = cs > 1 ? (int)items * cs : (items < slots ? (int)items : slots);
     if (cs > 1)
-        return launch<T, HDP, true>(ta, tq, tk, tv, (int)items * cs, s);
-    return launch<T, HDP, false>(ta, tq, tk, tv, items < slots ? (int)items : slots, s);
+        return x.kmask ? launch<T, HDP, true, true>(ta, tq, tk, tv, grid, s)
+                       : launch<T, HDP, true, false>(ta, tq, tk, tv, grid, s);
+    return x.kmask ? launch<T, HDP, false, true>(ta, tq, tk, tv, grid, s)
+                   : launch<T, HDP, false, false>(ta, tq, tk, tv, grid, s);
 }
 
 }  // namespace
