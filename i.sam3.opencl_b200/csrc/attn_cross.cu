@@ -280,6 +280,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 5 : 1)
 #pragma unroll
         for (int e = 0; e < 4; e++)
             o[d][e] = 0.0f;
+    const bool busy = r0 + wm * 16 < a.rows;
     float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
     uint32_t qf[F32 ? 1 : HDP / 16][4];
 
@@ -290,6 +291,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 5 : 1)
             load(s + STAGES - 1, see);
         cp_commit();
         look(s + STAGES, see);
+        if (!busy)
+            continue;  // only loads: none of the warp's rows exist
         const int st = s % STAGES;
         const uint8_t *ks = ring + st * CF::STAGE_BYTES, *vs = ks + CF::KV_BYTES;
         const uint32_t ka = smem_addr(ks), va = smem_addr(vs);

@@ -409,22 +409,30 @@ class Backend:
         return o
 
     def rope_table(self, npos, rot, first, scaling, cs):
-        self.check(lib().cb_rope_table(self.h, npos, rot, first,
-                                       C.byref(scaling) if scaling is not None else None, cs.h))
+        rc = lib().cb_rope_table(self.h, npos, rot, first,
+                                 C.byref(scaling) if scaling is not None else None, cs.h)
+        if rc:
+            self.check(rc)
 
     def rope_rotate(self, nb, N, heads, hd, rot, layout, X, Y, cs, npos, pos=None, pos0=0):
-        self.check(lib().cb_rope_rotate(self.h, nb, N, heads, hd, rot, layout, X, Y, cs.h, npos,
-                                        pos.h if pos else None, pos0))
+        rc = lib().cb_rope_rotate(self.h, nb, N, heads, hd, rot, layout, X, Y, cs.h, npos,
+                                  pos.h if pos else None, pos0)
+        if rc:
+            self.check(rc)
 
     def cross_attend(self, nb, Nq, Nk, heads, kvheads, hd, Q, K, V, O, klen=None, kmask=None,
                      scale=None):
         """scale: hd ** -0.5 when None."""
-        self.check(lib().cb_cross_attend(self.h, nb, Nq, Nk, heads, kvheads, hd, Q, K, V, O,
-                                         klen.h if klen else None, kmask.h if kmask else None,
-                                         hd ** -0.5 if scale is None else scale))
+        rc = lib().cb_cross_attend(self.h, nb, Nq, Nk, heads, kvheads, hd, Q, K, V, O,
+                                   klen.h if klen else None, kmask.h if kmask else None,
+                                   hd ** -0.5 if scale is None else scale)
+        if rc:
+            self.check(rc)
 
     def groupnorm(self, nb, npix, Cn, groups, X, Y, g, b, eps=1e-5, act=ACT_NONE):
-        self.check(lib().cb_groupnorm(self.h, nb, npix, Cn, groups, X, Y, g.h, b.h, eps, act))
+        rc = lib().cb_groupnorm(self.h, nb, npix, Cn, groups, X, Y, g.h, b.h, eps, act)
+        if rc:
+            self.check(rc)
 
     def mask_logits(self, U, hyper, out, P, npix):
         self.check(lib().cb_mask_logits(self.h, U.h, hyper.h, out.h, P, npix))
