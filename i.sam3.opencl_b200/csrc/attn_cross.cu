@@ -76,7 +76,7 @@ template <>
 __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4],
                                                      uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
                  "{%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -85,7 +85,7 @@ template <>
 __device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                               uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
                  "{%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -96,19 +96,19 @@ __device__ __forceinline__ void mma16_from(float (&d)[4], const uint32_t (&a)[4]
                                            float c1)
 {
     if constexpr (__is_same(T, __half))
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
                      "{%8,%9}, {%10,%11,%10,%11};"
                      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
                      "{%8,%9}, {%10,%11,%10,%11};"
                      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
                  "{%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -159,7 +159,7 @@ constexpr int smem_bytes()
 }
 
 template <typename T, int HDP, int WM>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 5 : 1)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
     attn_cross_kernel(const __grid_constant__ XaArgs a)
 {
     using TL = Tile<T, HDP>;
@@ -175,15 +175,22 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 5 : 1)
     constexpr int PART = WK * BM * (HDP + 4) * 4;
     uint8_t *vis = ring + (RING > PART ? RING : PART);
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-    const int wm = warp % WM, wk = warp / WM;
+    const int wk = warp / WM;
     const int g4 = lane >> 2, t4 = lane & 3;
 
     const int rank = (int)(blockIdx.x % a.cs);
     const long item = blockIdx.x / a.cs;
     const int qt = (int)(item % a.nqt);
+    // the warp's group of 16 rows: turned by the CTA, so that a tile's missing
+    // group falls on another quarter of the SM each time
+    const int wm = (int)((warp + item + rank) % WM);
     const long bh = item / a.nqt;
     const int b = (int)(bh / a.kvheads), kh = (int)(bh - (long)b * a.kvheads);
-    const long r0 = (long)qt * BM;
+    // groups of 16 rows dealt evenly to the tiles (201 rows: 3, 3, 3 and 4
+    // groups, not 4, 4, 4 and 1)
+    const long groups = (a.rows + 15) / 16;
+    const long r0 = groups * qt / a.nqt * 16;
+    const long r1 = min(a.rows, groups * (qt + 1) / a.nqt * 16);
 
     griddep_wait();
 
@@ -205,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 5 : 1)
             const int r = i / CPR, c = i % CPR;
             const long gr = r0 + r, qi = gr / a.g;
             const T *src = qb + qi * a.qld + (gr - qi * a.g) * a.qs1 + c * EPC;
-            const bool live = gr < a.rows && c < hdc;
+            const bool live = gr < r1 && c < hdc;
             const uint32_t dst = smem_addr(smem + TL::at(r, c));
             if (a.qvec)
                 cp16(dst, live ? src : a.q, live);
@@ -280,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 5 : 1)
 #pragma unroll
         for (int e = 0; e < 4; e++)
             o[d][e] = 0.0f;
-    const bool busy = r0 + wm * 16 < a.rows;
+    const bool busy = r0 + wm * 16 < r1;
     float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
     uint32_t qf[F32 ? 1 : HDP / 16][4];
 
@@ -333,14 +340,25 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 5 : 1)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     split_tf32(qs[(e & 1) * 8 * (TL::PITCH / 4) + kk * 8 + (e >> 1) * 4], ah[e], al[e]);
+                // four tiles side by side: a product waits for the one four before it
+                constexpr int NB = NT < 4 ? NT : 4;
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    uint32_t bh0, bl0, bh1, bl1;
-                    split_tf32(kf[n * 8 * (TL::PITCH / 4) + kk * 8], bh0, bl0);
-                    split_tf32(kf[n * 8 * (TL::PITCH / 4) + kk * 8 + 4], bh1, bl1);
-                    mma8(sc[n], al, bh0, bh1);
-                    mma8(sc[n], ah, bl0, bl1);
-                    mma8(sc[n], ah, bh0, bh1);
+                for (int n0 = 0; n0 < NT; n0 += NB) {
+                    uint32_t bh[NB][2], bl[NB][2];
+#pragma unroll
+                    for (int n = 0; n < NB; n++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            split_tf32(kf[(n0 + n) * 8 * (TL::PITCH / 4) + kk * 8 + 4 * e], bh[n][e], bl[n][e]);
+#pragma unroll
+                    for (int n = 0; n < NB; n++)
+                        mma8(sc[n0 + n], al, bh[n][0], bh[n][1]);
+#pragma unroll
+                    for (int n = 0; n < NB; n++)
+                        mma8(sc[n0 + n], ah, bl[n][0], bl[n][1]);
+#pragma unroll
+                    for (int n = 0; n < NB; n++)
+                        mma8(sc[n0 + n], ah, bh[n][0], bh[n][1]);
                 }
             }
         }
@@ -426,20 +444,36 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 5 : 1)
                 split_tf32(sc[n][3], ph[n][3], pl[n][3]);
             }
 #pragma unroll
-            for (int d = 0; d < DT; d++) {
-                float hi[4] = {0.0f, 0.0f, 0.0f, 0.0f}, lo[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int d0 = 0; d0 < DT; d0 += 4) {
+                float hi[4][4], lo[4][4];
+#pragma unroll
+                for (int d = 0; d < 4; d++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        hi[d][e] = lo[d][e] = 0.0f;
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    uint32_t bh0, bl0, bh1, bl1;
-                    split_tf32(vf[n * 8 * (TL::PITCH / 4) + d * 8], bh0, bl0);
-                    split_tf32(vf[(n * 8 + 1) * (TL::PITCH / 4) + d * 8], bh1, bl1);
-                    mma8(lo, pl[n], bh0, bh1);
-                    mma8(lo, ph[n], bl0, bl1);
-                    mma8(hi, ph[n], bh0, bh1);
+                    uint32_t bh[4][2], bl[4][2];
+#pragma unroll
+                    for (int d = 0; d < 4; d++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            split_tf32(vf[(n * 8 + e) * (TL::PITCH / 4) + (d0 + d) * 8], bh[d][e], bl[d][e]);
+#pragma unroll
+                    for (int d = 0; d < 4; d++)
+                        mma8(lo[d], pl[n], bh[d][0], bh[d][1]);
+#pragma unroll
+                    for (int d = 0; d < 4; d++)
+                        mma8(hi[d], ph[n], bh[d][0], bh[d][1]);
+#pragma unroll
+                    for (int d = 0; d < 4; d++)
+                        mma8(lo[d], ph[n], bl[d][0], bl[d][1]);
                 }
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    o[d][e] += hi[e] + lo[e];
+                for (int d = 0; d < 4; d++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        o[d0 + d][e] += hi[d][e] + lo[d][e];
             }
         }
     }
@@ -459,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 5 : 1)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const long gr = r0 + wm * 16 + g4 + 8 * h, qi = gr / a.g;
-            if (gr >= a.rows)
+            if (gr >= r1)
                 continue;
             T *dst = ob + qi * a.old + (gr - qi * a.g) * a.os1;
             const float inv = sum[h] > 0.0f || sum[h] != sum[h] ? 1.0f / sum[h] : 0.0f;
@@ -496,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 5 : 1)
         if (t4 == 0)
             *reinterpret_cast<float2 *>(pr + HDP) = make_float2(mx[h], sum[h]);
     }
-    const int live = (int)min((long)BM, a.rows - r0);
+    const int live = (int)(r1 - r0);
     auto store = [&](int row, int col, float v, float l) {
         const long gr = r0 + row, qi = gr / a.g;
         if (col < a.hd)
