@@ -166,10 +166,13 @@ __device__ __forceinline__ void fetch_wait()
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ float ld_cluster(uint32_t addr)
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr)
 {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
     return v;
 }
 
@@ -185,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
     constexpr int kAhead = 4;  // batches in flight; the ring has at least one more
     uint8_t *ring = dyn + threadIdx.x * VB;
     float2 *red = reinterpret_cast<float2 *>(dyn + (size_t)a.nring * kUnroll * kThreads * VB);
-    __shared__ float pub[kMaxSlabGroups][3];  // this CTA's (n, mean, M2), read by the cluster
+    __shared__ float4 pub[kMaxSlabGroups];    // this CTA's (n, mean, M2) per part, read by the cluster
     __shared__ float2 gstat[kMaxSlabGroups];  // mean, 1 / sqrt(var + eps)
     const int t = threadIdx.x;
     const int rank = (int)(blockIdx.x % a.cs), unit = (int)(blockIdx.x / a.cs);
@@ -350,37 +353,36 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
         red[t] = make_float2(tmean, tm2);
     __syncthreads();
     // The members of a group are the threads of its vectors, or its (row,
-    // channel) pairs; nparts warps share a group: means first, then sum
-    // n_i (mean_i - mean)^2.
+    // channel) pairs; nparts warps share a group and each publishes its own
+    // (n, mean, M2): the mean of its members first, then sum M2_i + n_i (mean_i -
+    // mean)^2. All parts of the cluster are then merged at once in the same way.
     constexpr int NW = kThreads / 32;
-    __shared__ float psum[kMaxSlabGroups], psq[kMaxSlabGroups];
     const int warp = t >> 5, lane32 = t & 31;
     const int nparts = a.gps >= NW ? 1 : NW / a.gps;
     const int width = a.span ? a.cg : (a.nk == 1 ? a.cg / V : kThreads);
     const int pitch = a.span ? a.S : a.lpp;
     const int members = a.rows * width;
-    const float sn = (float)np * (float)a.cg;
     const int dr = nparts * 32 / width, di = nparts * 32 - dr * width;  // to a lane's next member
     auto size = [&](int r, int i) {  // values behind member i of row r
         if (a.nk == 1)
             return (float)count(r) * (a.span ? 1 : V);
         return (float)np * V * (float)(i < a.lpp ? (a.lpp - 1 - i) / kThreads + 1 : 0);
     };
+    for (int w = warp; w < a.gps * nparts; w += NW) {
+        const int gi = w / nparts, part = w - gi * nparts;
+        const int m0 = part * 32 + lane32, r0 = m0 / width, i0 = m0 - r0 * width;
+        const float2 *mine_at = red + gi * width;
+        float n = 0.0f, mu = 0.0f, s = 0.0f;
 #pragma unroll
-    for (int pass = 0; pass < 2; pass++) {
-        for (int w = warp; w < a.gps * nparts; w += NW) {
-            const int gi = w / nparts, part = w - gi * nparts;
-            float mu = 0.0f, s = 0.0f;
-            if (pass == 1) {
-                for (int i = 0; i < nparts; i++)
-                    mu += psum[gi * nparts + i];
-                mu /= sn;
-            }
-            int r = (part * 32 + lane32) / width, i = part * 32 + lane32 - r * width;
-            for (int m = part * 32 + lane32; m < members; m += nparts * 32) {
+        for (int pass = 0; pass < 2; pass++) {
+            int r = r0, i = i0;
+            s = 0.0f;
+            for (int m = m0; m < members; m += nparts * 32) {
                 const float c = size(r, i);
                 if (c > 0.0f) {
-                    const float2 st = red[r * pitch + gi * width + i];
+                    const float2 st = mine_at[r * pitch + i];
+                    if (pass == 0)
+                        n += c;
                     s += pass == 0 ? c * st.x : fmaf((st.x - mu) * (st.x - mu), c, st.y);
                 }
                 i += di;
@@ -391,56 +393,55 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
                 }
             }
 #pragma unroll
-            for (int o = 16; o; o >>= 1)
+            for (int o = 16; o; o >>= 1) {
                 s += __shfl_xor_sync(0xffffffffu, s, o);
-            if (lane32 == 0) {
                 if (pass == 0)
-                    psum[w] = s;
-                else {
-                    psq[w] = s;
-                    if (part == 0) {
-                        pub[gi][0] = sn;
-                        pub[gi][1] = mu;
-                    }
-                }
+                    n += __shfl_xor_sync(0xffffffffu, n, o);
             }
+            if (pass == 0)
+                mu = n > 0.0f ? s / n : 0.0f;
         }
-        __syncthreads();
-    }
-    if (t < a.gps) {
-        float s = 0.0f;
-        for (int i = 0; i < nparts; i++)
-            s += psq[t * nparts + i];
-        pub[t][2] = s;
+        if (lane32 == 0)
+            pub[w] = make_float4(n, mu, s, 0.0f);
     }
     if (a.cs > 1)
         cluster_sync_all();
     else
         __syncthreads();
-    // a half warp per group, lane = CTA of the cluster
-    for (int g0 = 0; g0 < a.gps; g0 += kThreads / 16) {
-        const int gi = g0 + (t >> 4), r = t & 15;
-        float pn = 0.0f, pm = 0.0f, pq = 0.0f;
-        if (gi < a.gps && r < a.cs) {
-            const uint32_t own = smem_addr(&pub[gi][0]);
-            const uint32_t p = a.cs > 1 ? mapa_shared(own, r) : own;
-            pn = ld_cluster(p);
-            pm = ld_cluster(p + 4);
-            pq = ld_cluster(p + 8);
-        }
-        float sn = pn, ss = pn > 0.0f ? pn * pm : 0.0f;
+    // 16 or 32 lanes per group, a lane up to kParts of its parts
+    constexpr int kParts = kMaxCluster * NW / 32;
+    const int nall = a.cs * nparts, lw = nall > 16 ? 32 : 16;
+    for (int g0 = 0; g0 < a.gps; g0 += kThreads / lw) {
+        const int gi = g0 + t / lw, l = t & (lw - 1);
+        float4 q[kParts];
+        float n = 0.0f, s = 0.0f;
 #pragma unroll
-        for (int o = 8; o; o >>= 1) {
-            sn += __shfl_xor_sync(0xffffffffu, sn, o);
-            ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        for (int k = 0; k < kParts; k++) {
+            const int e = l + k * lw, r = e / nparts;
+            q[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (gi < a.gps && e < nall) {
+                const uint32_t own = smem_addr(&pub[gi * nparts + (e - r * nparts)]);
+                q[k] = ld_cluster4(a.cs > 1 ? mapa_shared(own, r) : own);
+            }
         }
-        const float mu = ss / sn;
-        float sq = pn > 0.0f ? fmaf((pm - mu) * (pm - mu), pn, pq) : 0.0f;
 #pragma unroll
-        for (int o = 8; o; o >>= 1)
-            sq += __shfl_xor_sync(0xffffffffu, sq, o);
-        if (r == 0 && gi < a.gps)
-            gstat[gi] = make_float2(mu, 1.0f / sqrtf(sq / sn + a.eps));
+        for (int k = 0; k < kParts; k++) {
+            n += q[k].x;
+            s += q[k].x > 0.0f ? q[k].x * q[k].y : 0.0f;
+        }
+        for (int o = lw / 2; o; o >>= 1) {
+            n += __shfl_xor_sync(0xffffffffu, n, o);
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+        }
+        const float mu = s / n;
+        s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kParts; k++)
+            s += q[k].x > 0.0f ? fmaf((q[k].y - mu) * (q[k].y - mu), q[k].x, q[k].z) : 0.0f;
+        for (int o = lw / 2; o; o >>= 1)
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (l == 0 && gi < a.gps)
+            gstat[gi] = make_float2(mu, 1.0f / sqrtf(s / n + a.eps));
     }
     __syncthreads();
     // no CTA may exit while another still reads its published statistics
