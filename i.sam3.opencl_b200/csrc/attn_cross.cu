@@ -154,7 +154,7 @@ constexpr int smem_bytes()
 {
     const int q = 16 * WM * Tile<T, HDP>::PITCH;
     const int ring = Cfg<T, HDP>::STAGES * Cfg<T, HDP>::STAGE_BYTES;
-    const int part = (4 / WM) * 16 * WM * (HDP + 4) * 4;
+    const int part = (4 / WM) * 16 * WM * Parts<HDP>::PR * 4;
     return q + (ring > part ? ring : part) + Cfg<T, HDP>::VIS_BYTES + 16;
 }
 
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t *ring = smem + BM * TL::PITCH;
     constexpr int RING = STAGES * CF::STAGE_BYTES;
-    constexpr int PART = WK * BM * (HDP + 4) * 4;
+    constexpr int PART = WK * BM * Parts<HDP>::PR * 4;
     uint8_t *vis = ring + (RING > PART ? RING : PART);
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
     const int wk = warp / WM;
@@ -517,111 +517,51 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
         }
         return;
     }
-    // ---- partial results: [wk][row][HDP + 4] fp32, (max, sum) at HDP
-    __syncthreads();
-    constexpr int PR = HDP + 4;
+    // ---- partial results of the warps' key parts and the cluster's CTAs
+    using PT = Parts<HDP>;
+    const int rl = BM / a.cs;  // rows of the tile a CTA merges: r % cs == rank
     float *part = reinterpret_cast<float *>(ring);
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        float *pr = part + (long)(wk * BM + wm * 16 + g4 + 8 * h) * PR;
-#pragma unroll
-        for (int d = 0; d < DT; d++)
-            *reinterpret_cast<float2 *>(pr + d * 8 + t4 * 2) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
-        if (t4 == 0)
-            *reinterpret_cast<float2 *>(pr + HDP) = make_float2(mx[h], sum[h]);
-    }
-    const int live = (int)(r1 - r0);
-    auto store = [&](int row, int col, float v, float l) {
-        const long gr = r0 + row, qi = gr / a.g;
-        if (col < a.hd)
-            ob[qi * a.old + (gr - qi * a.g) * a.os1 + col] =
-                out_of<T>(v * (l > 0.0f || l != l ? 1.0f / l : 0.0f));
-    };
-    __syncthreads();
-    // The warps' parts of an element: O = sum_p O_p 2^(max_p - max), the same
-    // for the sums; kept in the first part (or written, without a cluster).
-    if constexpr (WK > 1) {
-        constexpr int NE = BM * HDP / kThreads;  // elements of a thread
-        float v[NE];
-        float2 ml[NE];
-#pragma unroll
-        for (int i = 0; i < NE; i++) {
-            const int idx = t + i * kThreads, row = idx / HDP, col = idx % HDP;
-            if (row >= live)
-                continue;
-            float2 q[WK];
-            float m = -INFINITY;
-#pragma unroll
-            for (int p = 0; p < WK; p++) {
-                q[p] = *reinterpret_cast<const float2 *>(part + (p * BM + row) * PR + HDP);
-                m = fmaxf(m, q[p].x);
-            }
-            ml[i] = make_float2(m, 0.0f);
-            v[i] = 0.0f;
-#pragma unroll
-            for (int p = 0; p < WK; p++) {
-                const float w = q[p].x == -INFINITY ? 0.0f : exp2f(q[p].x - m);
-                v[i] = fmaf(part[(p * BM + row) * PR + col], w, v[i]);
-                ml[i].y = fmaf(q[p].y, w, ml[i].y);
-            }
-        }
+    if (a.cs > 1)
+        cluster_sync_all();  // no CTA reads its stages any more
+    else
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < NE; i++) {
-            const int idx = t + i * kThreads, row = idx / HDP, col = idx % HDP;
-            if (row >= live)
-                continue;
-            if (a.cs > 1) {
-                part[row * PR + col] = v[i];
-                if (col == 0)
-                    *reinterpret_cast<float2 *>(part + row * PR + HDP) = ml[i];
-            }
-            else
-                store(row, col, v[i], ml[i].y);
-        }
-        if (a.cs == 1)
-            return;
-    }
-    // The CTAs' parts: the tile's elements are dealt out to the cluster, every
-    // load of an element in flight at once.
-    cluster_sync_all();
-    const uint32_t base = smem_addr(part);
-    for (int idx = rank * kThreads + t; idx < live * HDP; idx += a.cs * kThreads) {
-        const int row = idx / HDP, col = idx % HDP;
-        const uint32_t at = base + (uint32_t)(row * PR) * 4;
-        constexpr int B = 8;  // parts at a time
-        float m = -INFINITY, v = 0.0f, l = 0.0f;
-#pragma unroll 1
-        for (int p0 = 0; p0 < a.cs; p0 += B) {
-            float pm[B], pl[B], po[B], mb = m;
+    for (int h = 0; h < 2; h++) {
+        const int r = wm * 16 + g4 + 8 * h, p = rank * WK + wk;
+        if (r0 + r >= r1)
+            continue;
+        const uint32_t own = smem_addr(part + (p * rl + r / a.cs) * PT::PR);
+        const uint32_t dst = a.cs > 1 ? mapa_shared(own, r % a.cs) : own;
 #pragma unroll
-            for (int p = 0; p < B; p++) {
-                pm[p] = -INFINITY;
-                pl[p] = po[p] = 0.0f;
-                if (p0 + p < a.cs) {
-                    const uint32_t src = mapa_shared(at, p0 + p);
-                    pm[p] = ld_dsmem(src + HDP * 4);
-                    pl[p] = ld_dsmem(src + HDP * 4 + 4);
-                    po[p] = ld_dsmem(src + col * 4);
+        for (int d = 0; d < DT; d++)
+            st_dsmem2(dst + (d * 8 + t4 * 2) * 4, o[d][2 * h], o[d][2 * h + 1]);
+        if (t4 == 0)
+            st_dsmem2(dst + HDP * 4, mx[h], sum[h]);
+    }
+    if (a.cs > 1)
+        cluster_sync_all();
+    else
+        __syncthreads();
+    const int rows = (int)(r1 - r0), live = rows > rank ? (rows - 1 - rank) / a.cs + 1 : 0;
+    PT::template merge<kThreads>(part, a.cs * WK, rl, live, [&](int i, int c, float x, float y, float z, float w) {
+        const long gr = r0 + i * a.cs + rank, qi = gr / a.g;
+        T *dst = ob + qi * a.old + (gr - qi * a.g) * a.os1 + c;
+        const float v[4] = {x, y, z, w};
+#pragma unroll
+        for (int e = 0; e < 4; e += 2)
+            if (c + e < a.hd) {
+                if (a.ovec) {
+                    if constexpr (F32)
+                        *reinterpret_cast<float2 *>(dst + e) = make_float2(v[e], v[e + 1]);
+                    else
+                        *reinterpret_cast<uint32_t *>(dst + e) = pack2<T>(v[e], v[e + 1]);
+                }
+                else {
+                    dst[e] = out_of<T>(v[e]);
+                    dst[e + 1] = out_of<T>(v[e + 1]);
                 }
             }
-#pragma unroll
-            for (int p = 0; p < B; p++)
-                mb = fmaxf(mb, pm[p]);
-            const float c = m == -INFINITY ? 1.0f : exp2f(m - mb);
-            v *= c;
-            l *= c;
-            m = mb;
-#pragma unroll
-            for (int p = 0; p < B; p++) {
-                const float w = pm[p] == -INFINITY ? 0.0f : exp2f(pm[p] - m);
-                v = fmaf(po[p], w, v);
-                l = fmaf(pl[p], w, l);
-            }
-        }
-        store(row, col, v, l);
-    }
-    cluster_sync_all();  // peers read this CTA's part until here
+    });
 }
 
 // Few keys (all in one step) and many rows: the bandwidth of Q and O. A CTA

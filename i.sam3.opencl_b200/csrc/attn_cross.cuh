@@ -65,6 +65,129 @@ __device__ __forceinline__ __half out_of<__half>(float v)
     return __float2half_rn(v);
 }
 
+__device__ __forceinline__ void st_dsmem4(uint32_t a, float x, float y, float z, float w)
+{
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(x), "f"(y), "f"(z), "f"(w)
+                 : "memory");
+}
+__device__ __forceinline__ void st_dsmem2(uint32_t a, float x, float y)
+{
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(x), "f"(y) : "memory");
+}
+
+// The parts of a tile's rows, merged over a cluster. Row r of the tile belongs
+// to CTA r % cs; every part of it is pushed into that CTA's shared memory (remote
+// stores, nothing waits for them; pulling cost a round trip per row or
+// element: 64 queries x 384 keys 15 us against 7), as part[(p * rl + r / cs) * PR]
+// with HDP columns of output, then its maximum and sum. After a cluster
+// barrier each CTA merges its own rows: O = sum_p O_p 2^(max_p - max) / sum_p
+// l_p 2^(max_p - max). A part without a visible key has maximum -inf and
+// counts nothing, unless its sum is NaN.
+template <int HDP>
+struct Parts {
+    static constexpr int PR = HDP + 4;
+    // rl: rows a CTA holds of each part; live: rows of its own that exist
+    template <int THREADS, typename Store>
+    static __device__ __forceinline__ void merge(float *part, int np, int rl, int live, const Store &store)
+    {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        // Weights of a row's parts and 1 / sum: a thread per row for few parts
+        // (many rows then), a warp per row for more.
+        constexpr int kFew = 8;
+        for (int i = threadIdx.x; np <= kFew && i < live; i += THREADS) {
+            float2 ml[kFew];
+            float m = -INFINITY, l = 0.0f;
+#pragma unroll
+            for (int p = 0; p < kFew; p++) {
+                ml[p] = p < np ? *reinterpret_cast<const float2 *>(part + (p * rl + i) * PR + HDP)
+                               : make_float2(-INFINITY, 0.0f);
+                m = fmaxf(m, ml[p].x);
+            }
+#pragma unroll
+            for (int p = 0; p < kFew; p++) {
+                const bool none = ml[p].x == -INFINITY;
+                const float w = none ? 0.0f : exp2f(ml[p].x - m);
+                l += none ? (ml[p].y == ml[p].y ? 0.0f : ml[p].y) : ml[p].y * w;
+                if (p < np)
+                    part[(p * rl + i) * PR + HDP] = w;
+            }
+            part[i * PR + HDP + 2] = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        }
+        for (int i = warp; np > kFew && i < live; i += THREADS / 32) {
+            float2 ml[2];  // up to 64 parts
+            float m = -INFINITY, l = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int p = lane + 32 * k;
+                ml[k] = p < np ? *reinterpret_cast<const float2 *>(part + (p * rl + i) * PR + HDP)
+                               : make_float2(-INFINITY, 0.0f);
+                m = fmaxf(m, ml[k].x);
+            }
+#pragma unroll
+            for (int x = 16; x; x >>= 1)
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int p = lane + 32 * k;
+                const float w = ml[k].x == -INFINITY ? 0.0f : exp2f(ml[k].x - m);
+                l += ml[k].x == -INFINITY ? (ml[k].y == ml[k].y ? 0.0f : ml[k].y) : ml[k].y * w;
+                if (p < np)
+                    part[(p * rl + i) * PR + HDP] = w;
+            }
+#pragma unroll
+            for (int x = 16; x; x >>= 1)
+                l += __shfl_xor_sync(0xffffffffu, l, x);
+            if (lane == 0)
+                part[i * PR + HDP + 2] = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        }
+        __syncthreads();
+        const int ne = live * (HDP / 4);  // elements, four columns each
+        if (np > kFew) {  // eight lanes to an element
+            const int g = lane & 7;
+            for (int e0 = warp * 4; e0 < ne; e0 += THREADS / 8) {
+                const int e = min(e0 + (lane >> 3), ne - 1), i = e / (HDP / 4), c = (e % (HDP / 4)) * 4;
+                float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                for (int p = g; p < np; p += 8) {
+                    const float *src = part + (p * rl + i) * PR;
+                    const float w = src[HDP];
+                    const float4 v = *reinterpret_cast<const float4 *>(src + c);
+                    acc.x = fmaf(v.x, w, acc.x);
+                    acc.y = fmaf(v.y, w, acc.y);
+                    acc.z = fmaf(v.z, w, acc.z);
+                    acc.w = fmaf(v.w, w, acc.w);
+                }
+#pragma unroll
+                for (int x = 4; x; x >>= 1) {
+                    acc.x += __shfl_xor_sync(0xffffffffu, acc.x, x);
+                    acc.y += __shfl_xor_sync(0xffffffffu, acc.y, x);
+                    acc.z += __shfl_xor_sync(0xffffffffu, acc.z, x);
+                    acc.w += __shfl_xor_sync(0xffffffffu, acc.w, x);
+                }
+                const float inv = part[i * PR + HDP + 2];
+                if (g == 0 && e0 + (lane >> 3) < ne)
+                    store(i, c, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            }
+            return;
+        }
+        for (int e = threadIdx.x; e < ne; e += THREADS) {
+            const int i = e / (HDP / 4), c = (e % (HDP / 4)) * 4;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int p = 0; p < np; p++) {
+                const float *src = part + (p * rl + i) * PR;
+                const float w = src[HDP];
+                const float4 v = *reinterpret_cast<const float4 *>(src + c);
+                acc.x = fmaf(v.x, w, acc.x);
+                acc.y = fmaf(v.y, w, acc.y);
+                acc.z = fmaf(v.z, w, acc.z);
+                acc.w = fmaf(v.w, w, acc.w);
+            }
+            const float inv = part[i * PR + HDP + 2];
+            store(i, c, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        }
+    }
+};
+
 // The tcgen05 form (attn_cross_tc.cu): whether it takes a call's operands (16-bit,
 // 16-byte aligned starts and strides), and the call.
 bool attn_cross_tc_takes(const XaArgs &a, int nb, int dt);

@@ -55,10 +55,9 @@ struct Geo {
     static constexpr int NBAR = 2 * NQ + 4 * KST + 2 + 2 + 2 + 1;
     static constexpr int SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
     static constexpr uint32_t TM_O = 2 * BKV, TM_COLS = 256;
-    static constexpr int PART_ROW = HDP + 4;  // output, max, sum of a row
     static_assert(kCtasPerSm * SMEM <= 232448 - 2048, "two CTAs per SM");
     static_assert(TM_O + HDP <= TM_COLS, "tensor memory");
-    static_assert(BQ * PART_ROW * 4 <= OFF_BAR, "partial rows");
+    static_assert(BQ * Parts<HDP>::PR * 4 <= OFF_BAR, "partial rows");
 };
 
 template <typename T>
@@ -174,6 +173,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         it.n = (SPLIT ? (int)((long)nt * (rank + 1) / a.cs) : nt) - it.j0;
         return it;
     };
+
+    // what a split item's rows leave for the merge
+    float part_max = -INFINITY, part_sum = 0.0f;
+    int part_tiles = 0;
 
     if (warp == kProducerWarp) {
         if (lane < 2) {
@@ -533,13 +536,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                     break;
                 tc_fence_after();
             }
-            if (rows_live) {
+            if (SPLIT) {  // pushed behind the cluster barrier below
+                float la, lb, lc, ld;
+                f2_split(lsum0, la, lb);
+                f2_split(lsum1, lc, ld);
+                part_max = m_used;
+                part_sum = (la + lb) + (lc + ld);
+                part_tiles = it.n;
+            }
+            else if (rows_live) {
                 float la, lb, lc, ld;
                 f2_split(lsum0, la, lb);
                 f2_split(lsum1, lc, ld);
                 const float lsum = (la + lb) + (lc + ld);
                 const float inv = m_used == -INFINITY && lsum == lsum ? 0.0f : 1.0f / lsum;
-                float *part = reinterpret_cast<float *>(smem) + r * G::PART_ROW;
                 T *dst = reinterpret_cast<T *>(a.o) + it.seq * a.os0 + (long)q * a.old + it.head * a.os1;
 #pragma unroll
                 for (int c = 0; c < HDP; c += 32) {
@@ -553,12 +563,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                         for (int e = 0; e < 32; e++)
                             ov[e] = 0;
                     }
-                    if (SPLIT) {  // every copy has landed and every product is done: the stages are free
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<uint4 *>(part + c + e) = make_uint4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
-                    }
-                    else if (q < a.Nq) {
+                    if (q < a.Nq) {
 #pragma unroll
                         for (int e = 0; e < 32; e += 8) {
                             if (c + e >= a.hd)
@@ -578,57 +583,59 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                         }
                     }
                 }
-                if (SPLIT) {
-                    part[HDP] = m_used;
-                    part[HDP + 1] = lsum;
-                }
                 tc_fence_before();
             }
         }
     }
     if constexpr (SPLIT) {
+        using PT = Parts<HDP>;
+        const Item it = item_at(first);
+        const int live = min(BQ, a.Nq - it.qt * BQ), rl = BQ / a.cs;
+        float *part = reinterpret_cast<float *>(smem);
+        __syncwarp();
+        cluster_sync_all();  // every copy has landed and every product is done in all CTAs: the stages are free
+        if (warp < kProducerWarp && warp * 32 < live) {
+            const int r = warp * 32 + lane;
+            const uint32_t tO = tmem_base + ((uint32_t)(warp * 32) << 16) + G::TM_O;
+            const uint32_t dst =
+                mapa_shared(smem_addr(part + (rank * rl + r / a.cs) * PT::PR), r % a.cs);
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HDP; c += 32) {
+                uint32_t ov[32];
+                if (part_tiles > 0) {
+                    tmem_ld32(tO + c, ov);
+                    tmem_wait_ld();
+                }
+                else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++)
+                        ov[e] = 0;
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    st_dsmem4(dst + (c + e) * 4, __uint_as_float(ov[e]), __uint_as_float(ov[e + 1]),
+                              __uint_as_float(ov[e + 2]), __uint_as_float(ov[e + 3]));
+            }
+            st_dsmem2(dst + HDP * 4, part_max, part_sum);
+        }
         __syncwarp();
         cluster_sync_all();
-        // row i of the tile belongs to CTA i % cs, a warp per row
-        const Item it = item_at(first);
-        const int live = min(BQ, a.Nq - it.qt * BQ);
-        const uint32_t base = smem_addr(smem);
-        for (int i = rank + a.cs * warp; i < live; i += a.cs * (kThreads / 32)) {
-            const uint32_t row = base + (uint32_t)(i * G::PART_ROW) * 4;
-            const uint32_t peer = mapa_shared(row, lane < a.cs ? lane : 0);
-            const float mp = lane < a.cs ? ld_dsmem(peer + HDP * 4) : -INFINITY;
-            float m = mp;
-#pragma unroll
-            for (int x = 4; x; x >>= 1)
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-            m = __shfl_sync(0xffffffffu, m, 0);
-            const float w = mp == -INFINITY ? 0.0f : exp2f(mp - m);
-            float l = lane < a.cs ? ld_dsmem(peer + (HDP + 1) * 4) : 0.0f;
-            // a part without a visible key adds nothing, one with a NaN sum all of it
-            l = mp == -INFINITY && l == l ? 0.0f : l * (mp == -INFINITY ? 1.0f : w);
-#pragma unroll
-            for (int x = 4; x; x >>= 1)
-                l += __shfl_xor_sync(0xffffffffu, l, x);
-            l = __shfl_sync(0xffffffffu, l, 0);
-            float acc[HDP / 32];
-#pragma unroll
-            for (int c = 0; c < HDP / 32; c++)
-                acc[c] = 0.0f;
-            for (int p = 0; p < a.cs; p++) {
-                const float wp = __shfl_sync(0xffffffffu, w, p);
-                const uint32_t src = mapa_shared(row, p) + lane * 4;
-#pragma unroll
-                for (int c = 0; c < HDP / 32; c++)
-                    acc[c] = fmaf(ld_dsmem(src + c * 128), wp, acc[c]);
+        const int mine = live > rank ? (live - 1 - rank) / a.cs + 1 : 0;
+        T *ob = reinterpret_cast<T *>(a.o) + it.seq * a.os0 + it.head * a.os1;
+        PT::template merge<kThreads>(part, a.cs, rl, mine, [&](int i, int c, float x, float y, float z, float w) {
+            if (c >= a.hd)
+                return;
+            T *dst = ob + (long)(it.qt * BQ + i * a.cs + rank) * a.old + c;
+            if (a.ovec)
+                *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<T>(x, y), pack2<T>(z, w));
+            else {
+                dst[0] = out_of<T>(x);
+                dst[1] = out_of<T>(y);
+                dst[2] = out_of<T>(z);
+                dst[3] = out_of<T>(w);
             }
-            const float inv = m == -INFINITY && l == l ? 0.0f : 1.0f / l;
-            T *dst = reinterpret_cast<T *>(a.o) + it.seq * a.os0 + (long)(it.qt * BQ + i) * a.old + it.head * a.os1;
-#pragma unroll
-            for (int c = 0; c < HDP / 32; c++)
-                if (c * 32 + lane < a.hd)
-                    dst[c * 32 + lane] = out_of<T>(acc[c] * inv);
-        }
-        cluster_sync_all();  // peers read this CTA's rows until here
+        });
     }
     tc_fence_before();
     __syncthreads();
