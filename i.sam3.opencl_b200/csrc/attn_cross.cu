@@ -40,6 +40,7 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kMaxCluster = 16;
+constexpr int kSplitSteps = 4;  // steps of a CTA from which two share them
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live)
 {
@@ -138,24 +139,27 @@ struct Tile {
     }
 };
 
-template <typename T, int HDP>
+template <typename T, int HDP, int WM>
 struct Cfg {
-    static constexpr int BK = sizeof(T) == 4 && HDP == 128 ? 32 : 64;  // keys per step
-    static constexpr int STAGES = sizeof(T) == 4 ? 2 : (HDP == 128 ? 3 : 4);
+    // keys per step: with all warps on 16 rows, enough for 32 keys a warp
+    static constexpr int BK = sizeof(T) == 4 ? (HDP == 128 ? 32 : 64) : (WM == 1 && HDP <= 64 ? 128 : 64);
+    static constexpr int STAGES = sizeof(T) == 4 ? 2 : (HDP == 128 || BK == 128 ? 3 : 4);
     static constexpr int KV_BYTES = BK * Tile<T, HDP>::PITCH;
     static constexpr int STAGE_BYTES = 2 * KV_BYTES;
-    static constexpr int VIS_BYTES = STAGES * BK;
+    static constexpr int BM = 16 * WM, WK = 4 / WM;
+    // shared memory: query rows, stages, visible keys of the stages, and, when
+    // parts are merged, the parts of this CTA's rows
+    static constexpr int OFF_RING = BM * Tile<T, HDP>::PITCH;
+    static constexpr int OFF_VIS = OFF_RING + STAGES * STAGE_BYTES;
+    static constexpr int OFF_PART = OFF_VIS + (STAGES * BK + 15) / 16 * 16;
+    static constexpr int SMEM_WHOLE = OFF_PART;
+    static constexpr int SMEM_PARTS = OFF_PART + WK * BM * Parts<HDP>::PR * 4;
 };
 
-// Rows of a tile (16 WM), partial outputs (fp32) of its WK = 4 / WM key parts:
-// (max, sum) then HDP columns per row, over the stages' memory.
-template <typename T, int HDP, int WM>
-constexpr int smem_bytes()
+// Query row of row gr of a key head's (query, head) rows.
+__device__ __forceinline__ long query_of(const XaArgs &a, long gr)
 {
-    const int q = 16 * WM * Tile<T, HDP>::PITCH;
-    const int ring = Cfg<T, HDP>::STAGES * Cfg<T, HDP>::STAGE_BYTES;
-    const int part = (4 / WM) * 16 * WM * Parts<HDP>::PR * 4;
-    return q + (ring > part ? ring : part) + Cfg<T, HDP>::VIS_BYTES + 16;
+    return gr < 0x7fffffffL ? (long)quot((uint32_t)gr, a.dg) : gr / a.g;
 }
 
 template <typename T, int HDP, int WM>
@@ -163,17 +167,14 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
     attn_cross_kernel(const __grid_constant__ XaArgs a)
 {
     using TL = Tile<T, HDP>;
-    using CF = Cfg<T, HDP>;
+    using CF = Cfg<T, HDP, WM>;
     constexpr int WK = 4 / WM, BM = 16 * WM, BK = CF::BK, KW = BK / WK;
     constexpr int CPR = TL::CPR, EPC = 16 / (int)sizeof(T);  // elements per chunk
     constexpr int STAGES = CF::STAGES;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int NT = KW / 8, DT = HDP / 8;  // score and output tiles of a warp
     extern __shared__ __align__(16) uint8_t smem[];
-    uint8_t *ring = smem + BM * TL::PITCH;
-    constexpr int RING = STAGES * CF::STAGE_BYTES;
-    constexpr int PART = WK * BM * Parts<HDP>::PR * 4;
-    uint8_t *vis = ring + (RING > PART ? RING : PART);
+    uint8_t *ring = smem + CF::OFF_RING, *vis = smem + CF::OFF_VIS;
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
     const int wk = warp / WM;
     const int g4 = lane >> 2, t4 = lane & 3;
@@ -186,6 +187,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
     const int wm = (int)((warp + item + rank) % WM);
     const long bh = item / a.nqt;
     const int b = (int)(bh / a.kvheads), kh = (int)(bh - (long)b * a.kvheads);
+    // (every CTA of the cluster runs once the wait before the merge is over)
+    if (a.cs > 1)
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     // groups of 16 rows dealt evenly to the tiles (201 rows: 3, 3, 3 and 4
     // groups, not 4, 4, 4 and 1)
     const long groups = (a.rows + 15) / 16;
@@ -210,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
         const T *qb = reinterpret_cast<const T *>(a.q) + b * a.qs0 + (long)kh * a.g * a.qs1;
         for (int i = t; i < BM * CPR; i += kThreads) {
             const int r = i / CPR, c = i % CPR;
-            const long gr = r0 + r, qi = gr / a.g;
+            const long gr = r0 + r, qi = query_of(a, gr);
             const T *src = qb + qi * a.qld + (gr - qi * a.g) * a.qs1 + c * EPC;
             const bool live = gr < r1 && c < hdc;
             const uint32_t dst = smem_addr(smem + TL::at(r, c));
@@ -492,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
     if (WK == 1 && a.cs == 1) {  // the tile is whole: straight from registers
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const long gr = r0 + wm * 16 + g4 + 8 * h, qi = gr / a.g;
+            const long gr = r0 + wm * 16 + g4 + 8 * h, qi = query_of(a, gr);
             if (gr >= r1)
                 continue;
             T *dst = ob + qi * a.old + (gr - qi * a.g) * a.os1;
@@ -520,11 +524,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
     // ---- partial results of the warps' key parts and the cluster's CTAs
     using PT = Parts<HDP>;
     const int rl = BM / a.cs;  // rows of the tile a CTA merges: r % cs == rank
-    float *part = reinterpret_cast<float *>(ring);
+    float *part = reinterpret_cast<float *>(smem + CF::OFF_PART);
     if (a.cs > 1)
-        cluster_sync_all();  // no CTA reads its stages any more
-    else
-        __syncthreads();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const int r = wm * 16 + g4 + 8 * h, p = rank * WK + wk;
@@ -544,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
         __syncthreads();
     const int rows = (int)(r1 - r0), live = rows > rank ? (rows - 1 - rank) / a.cs + 1 : 0;
     PT::template merge<kThreads>(part, a.cs * WK, rl, live, [&](int i, int c, float x, float y, float z, float w) {
-        const long gr = r0 + i * a.cs + rank, qi = gr / a.g;
+        const long gr = r0 + i * a.cs + rank, qi = query_of(a, gr);
         T *dst = ob + qi * a.old + (gr - qi * a.g) * a.os1 + c;
         const float v[4] = {x, y, z, w};
 #pragma unroll
@@ -861,8 +863,8 @@ cudaError_t prepare_once(int smem)
 template <typename T, int HDP, int WM>
 int launch(XaArgs &a, int nb, cudaStream_t s)
 {
-    constexpr int smem = smem_bytes<T, HDP, WM>();
-    const cudaError_t pe = prepare_once<attn_cross_kernel<T, HDP, WM>>(smem);
+    using CF = Cfg<T, HDP, WM>;
+    const cudaError_t pe = prepare_once<attn_cross_kernel<T, HDP, WM>>(CF::SMEM_PARTS);
     if (pe != cudaSuccess)
         return (int)pe;
     constexpr int BM = 16 * WM;
@@ -873,12 +875,13 @@ int launch(XaArgs &a, int nb, cudaStream_t s)
     const long items = (long)nb * a.kvheads * nqt;
     // CTAs sharing a tile's keys: while all run at once, each with at least
     // two steps.
-    const long slots = resident<attn_cross_kernel<T, HDP, WM>>(smem), steps = (a.Nk + Cfg<T, HDP>::BK - 1) / Cfg<T, HDP>::BK;
+    const long slots = resident<attn_cross_kernel<T, HDP, WM>>(CF::SMEM_PARTS), steps = (a.Nk + CF::BK - 1) / CF::BK;
     a.cs = 1;
-    while (a.cs < kMaxCluster && items * a.cs * 2 <= slots && steps >= a.cs * 4)
+    while (a.cs < kMaxCluster && items * a.cs * 2 <= slots && steps >= a.cs * kSplitSteps)
         a.cs *= 2;
     if (items > 0x7fffffffL / a.cs)
         return K_EARG;
+    const int smem = CF::WK > 1 || a.cs > 1 ? CF::SMEM_PARTS : CF::SMEM_WHOLE;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -960,8 +963,20 @@ extern "C" int k_cross_attend(const struct k_rows *Q, const struct k_rows *K, co
     a.scale_log2 = (float)(scale * 1.4426950408889634);
     a.err = err;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(s);
-    // many rows over many keys: tcgen05
-    if (Nq >= 96 && Nk >= 192 && attn_cross_tc_takes(a, nb, Q->dt)) {
+    // Many rows over many keys: tcgen05. Both forms were measured over 1 to 1024
+    // queries and 96 to 4096 keys (us, tcgen05 / this file): 128 columns a head
+    // 128 x 16 heads, 1 query x 1024 keys 16.0 / 21.6, 128 x 4096 53 / 145;
+    // 64 columns, 32 heads, 48 x 384 7.0 / 8.4, 48 x 1024 11.6 / 12.1 (1.6 M
+    // scores), 128 x 1024 14.4 / 12.1 (4.2 M), 256 x 1024 15.1 / 17.0 (8.4 M);
+    // 32 columns, 64 heads, 64 x 192 5.6 / 4.8, 64 x 384 7.2 / 7.2, 96 x 1024
+    // 14.2 / 13.7 (6.3 M), 96 x 2048 17.1 / 22.7. Heads sharing keys are rows of
+    // one tile here, so few queries of theirs stay.
+    const double scores = (double)nb * heads * Nq * Nk;
+    const bool mid = Nk < 640, big = scores >= 6e6;
+    const bool many = hd > 64   ? Nk >= 96 && (a.g == 1 || Nq >= 16)
+                      : hd > 32 ? Nq >= 24 && (mid ? Nk >= 96 : big)
+                                : (Nq >= 64 && mid && Nk >= 256) || (Nq >= 24 && Nk >= 96 && big);
+    if (many && attn_cross_tc_takes(a, nb, Q->dt)) {
         a.ovec = vec(O);
         const int rc = attn_cross_tc(a, nb, Q->dt, st);
         if (rc != K_ETMAP)

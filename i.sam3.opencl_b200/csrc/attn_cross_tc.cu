@@ -363,6 +363,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                     if (MASK)
                         look(j + 1);
                 }
+                ok = __all_sync(0xffffffffu, mbar_wait(&s_full[b], (g >> 1) & 1, a.err, abort_flag));
+                if (!ok)
+                    break;
+                tc_fence_after();
+                // The hidden keys' rows of V, a thread per key. Only after the
+                // scores: S(g) follows P.V(g - 2), so the load of this stage
+                // before this one is complete and the wait below cannot take it
+                // for this one's (two stages a ring; a parity names every other
+                // load of a stage).
                 if (!whole) {
                     const int st = g % KST;
                     ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (g / KST) & 1, a.err, abort_flag));
@@ -384,10 +393,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                     }
                     fence_proxy_async_smem();
                 }
-                ok = __all_sync(0xffffffffu, mbar_wait(&s_full[b], (g >> 1) & 1, a.err, abort_flag));
-                if (!ok)
-                    break;
-                tc_fence_after();
                 const uint32_t tS = tL + b * BKV;
                 bool resc = false;
                 float factor = 1.0f;
@@ -705,9 +710,12 @@ int run(XaArgs &x, int nb, bool bf16, cudaStream_t s)
     if (items > 0x3fffffffL)
         return K_EARG;
     ta.nitems = (int)items;
-    // CTAs sharing an item's keys: while all parts run at once, 4 tiles each
+    // CTAs sharing an item's keys: as many as run at once (cluster scheduling
+    // leaves a few slots), from ten tiles on: a tile takes about 0.75 us alone, the
+    // merge 3.5 us (64 (sequence, head) pairs x 128 queries, cs 1 and 4: 8
+    // tiles 11.8 and 12.6 us, 11 tiles 14.6 and 13.7 us).
     int cs = 1;
-    while (cs < kMaxSplit && items * cs * 2 <= slots && nkv >= cs * 8)
+    while (nkv >= 10 && cs < kMaxSplit && items * cs * 2 <= slots - slots / 16)
         cs *= 2;
     x.cs = cs;
     ta.x = x;

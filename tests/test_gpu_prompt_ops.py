@@ -304,6 +304,39 @@ def test_cross_attend_lengths_and_masks(be, Nq, Nk, h, kv, hd, dt, with_len, wit
     assert torch.equal(o, o2)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("masked", [False, True])
+def test_cross_attend_hidden_keys_many_times(be, hd, masked):
+    """Short sequences of other lengths after one another in each CTA's rings: what lies behind their ends (the
+    type's largest values) must never be taken for values, however loads and products interleave."""
+    nb, Nq, Nk, h = 40, 300, 500, 4
+    g = gen(77)
+    dt = torch.float16
+    q, k, v = (randn(g, nb, n, h, hd).to(dt) for n in (Nq, Nk, Nk))
+    klen = torch.randint(1, Nk + 1, (nb,), device="cuda", generator=g, dtype=torch.int32)
+    see = torch.arange(Nk, device="cuda") < klen[:, None]
+    kmask = None
+    if masked:
+        kmask = (torch.rand(nb, Nk, device="cuda", generator=g) < 0.3).to(torch.uint8)
+        see &= kmask == 0
+    v[~see] = math.inf
+    k[~see] = math.nan
+    first = None
+    def d(t):
+        return op(be, t, 0, t.stride(1), t.stride(0), t.stride(2))
+    for _ in range(25):
+        o = torch.full_like(q, 3.0)
+        be.cross_attend(nb, Nq, Nk, h, h, hd, d(q), d(k), d(v), d(o), be.wrap(klen),
+                        be.wrap(kmask) if masked else None)
+        be.sync()
+        first = o if first is None else first
+        assert torch.equal(o, first)
+    assert first.isfinite().all()
+    want, A, big = attend_ref(q.double(), torch.where(see[:, :, None, None], k, 0).double(),
+                              torch.where(see[:, :, None, None], v, 0).double(), see, hd ** -0.5)
+    assert ((first.double() - want).abs() <= attend_tol(dt, want, A, big, hd, Nk)).all()
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("Nq,Nk,hd,shift", [(4, 200, 64, 0), (150, 300, 32, 1), (150, 300, 32, 2), (200, 700, 64, 4),
                                             (200, 700, 128, 8)])
