@@ -141,19 +141,19 @@ struct Tile {
 
 template <typename T, int HDP, int WM>
 struct Cfg {
-    // keys per step: with all warps on 16 rows, enough for 32 keys a warp
-    static constexpr int BK = sizeof(T) == 4 ? (HDP == 128 ? 32 : 64) : (WM == 1 && HDP <= 64 ? 128 : 64);
-    static constexpr int STAGES = sizeof(T) == 4 ? 2 : (HDP == 128 || BK == 128 ? 3 : 4);
+    static constexpr int BK = sizeof(T) == 4 && HDP == 128 ? 32 : 64;  // keys per step
+    static constexpr int STAGES = sizeof(T) == 4 ? 2 : (HDP == 128 ? 3 : 4);
     static constexpr int KV_BYTES = BK * Tile<T, HDP>::PITCH;
     static constexpr int STAGE_BYTES = 2 * KV_BYTES;
     static constexpr int BM = 16 * WM, WK = 4 / WM;
-    // shared memory: query rows, stages, visible keys of the stages, and, when
-    // parts are merged, the parts of this CTA's rows
+    // shared memory: query rows, stages, visible keys of the stages, and in a
+    // cluster the parts of the rows that this CTA merges
     static constexpr int OFF_RING = BM * Tile<T, HDP>::PITCH;
     static constexpr int OFF_VIS = OFF_RING + STAGES * STAGE_BYTES;
     static constexpr int OFF_PART = OFF_VIS + (STAGES * BK + 15) / 16 * 16;
     static constexpr int SMEM_WHOLE = OFF_PART;
-    static constexpr int SMEM_PARTS = OFF_PART + WK * BM * Parts<HDP>::PR * 4;
+    static constexpr int SMEM_PARTS = OFF_PART + BM * Parts<HDP>::PR * 4;
+    static_assert(WK * BM * Parts<HDP>::PR * 4 <= STAGES * STAGE_BYTES, "the warps' parts lie over the stages");
 };
 
 // Query row of row gr of a key head's (query, head) rows.
@@ -521,34 +521,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
         }
         return;
     }
-    // ---- partial results of the warps' key parts and the cluster's CTAs
+    // ---- results of the warps' key parts and of the cluster's CTAs
     using PT = Parts<HDP>;
-    const int rl = BM / a.cs;  // rows of the tile a CTA merges: r % cs == rank
-    float *part = reinterpret_cast<float *>(smem + CF::OFF_PART);
-    if (a.cs > 1)
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int r = wm * 16 + g4 + 8 * h, p = rank * WK + wk;
-        if (r0 + r >= r1)
-            continue;
-        const uint32_t own = smem_addr(part + (p * rl + r / a.cs) * PT::PR);
-        const uint32_t dst = a.cs > 1 ? mapa_shared(own, r % a.cs) : own;
-#pragma unroll
-        for (int d = 0; d < DT; d++)
-            st_dsmem2(dst + (d * 8 + t4 * 2) * 4, o[d][2 * h], o[d][2 * h + 1]);
-        if (t4 == 0)
-            st_dsmem2(dst + HDP * 4, mx[h], sum[h]);
-    }
-    if (a.cs > 1)
-        cluster_sync_all();
-    else
-        __syncthreads();
-    const int rows = (int)(r1 - r0), live = rows > rank ? (rows - 1 - rank) / a.cs + 1 : 0;
-    PT::template merge<kThreads>(part, a.cs * WK, rl, live, [&](int i, int c, float x, float y, float z, float w) {
-        const long gr = r0 + i * a.cs + rank, qi = query_of(a, gr);
+    const int rows = (int)(r1 - r0);
+    auto store = [&](int r, int c, const float (&v)[4]) {  // columns c .. c + 3 of the tile's row r
+        const long gr = r0 + r, qi = query_of(a, gr);
         T *dst = ob + qi * a.old + (gr - qi * a.g) * a.os1 + c;
-        const float v[4] = {x, y, z, w};
 #pragma unroll
         for (int e = 0; e < 4; e += 2)
             if (c + e < a.hd) {
@@ -563,6 +541,85 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
                     dst[e + 1] = out_of<T>(v[e + 1]);
                 }
             }
+    };
+    const int rl = BM / a.cs;  // rows of the tile a CTA merges: r % cs == rank
+    float *part = reinterpret_cast<float *>(smem + CF::OFF_PART);
+    auto owner = [&](int r) {  // where this CTA's part of row r goes
+        return mapa_shared(smem_addr(part + (rank * rl + r / a.cs) * PT::PR), r % a.cs);
+    };
+    if constexpr (WK > 1) {
+        // the warps' parts first, over the stages
+        float *mine = reinterpret_cast<float *>(ring);
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int r = g4 + 8 * h;
+            float *pr = mine + (wk * BM + r) * PT::PR;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+                *reinterpret_cast<float2 *>(pr + d * 8 + t4 * 2) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
+            if (t4 == 0)
+                *reinterpret_cast<float2 *>(pr + HDP) = make_float2(mx[h], sum[h]);
+        }
+        if (a.cs > 1)
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        __syncthreads();
+        for (int e = t; e < rows * (HDP / 4); e += kThreads) {
+            const int r = e / (HDP / 4), c = (e % (HDP / 4)) * 4;
+            float2 ml[WK];
+            float m = -INFINITY, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int p = 0; p < WK; p++) {
+                ml[p] = *reinterpret_cast<const float2 *>(mine + (p * BM + r) * PT::PR + HDP);
+                m = fmaxf(m, ml[p].x);
+            }
+#pragma unroll
+            for (int p = 0; p < WK; p++) {
+                const bool none = ml[p].x == -INFINITY;
+                const float w = none ? 0.0f : exp2f(ml[p].x - m);
+                const float4 x = *reinterpret_cast<const float4 *>(mine + (p * BM + r) * PT::PR + c);
+                l += none ? (ml[p].y == ml[p].y ? 0.0f : ml[p].y) : ml[p].y * w;
+                v[0] = fmaf(x.x, w, v[0]);
+                v[1] = fmaf(x.y, w, v[1]);
+                v[2] = fmaf(x.z, w, v[2]);
+                v[3] = fmaf(x.w, w, v[3]);
+            }
+            if (a.cs == 1) {
+                const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    v[i] *= inv;
+                store(r, c, v);
+            }
+            else {
+                st_dsmem4(owner(r) + c * 4, v[0], v[1], v[2], v[3]);
+                if (c == 0)
+                    st_dsmem2(owner(r) + HDP * 4, m, l);
+            }
+        }
+        if (a.cs == 1)
+            return;
+    }
+    else {
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int r = wm * 16 + g4 + 8 * h;
+            if (r >= rows)
+                continue;
+            const uint32_t dst = owner(r);
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+                st_dsmem2(dst + (d * 8 + t4 * 2) * 4, o[d][2 * h], o[d][2 * h + 1]);
+            if (t4 == 0)
+                st_dsmem2(dst + HDP * 4, mx[h], sum[h]);
+        }
+    }
+    cluster_sync_all();
+    const int live = rows > rank ? (rows - 1 - rank) / a.cs + 1 : 0;
+    PT::template merge<kThreads>(part, a.cs, rl, live, [&](int i, int c, float x, float y, float z, float w) {
+        const float v[4] = {x, y, z, w};
+        store(i * a.cs + rank, c, v);
     });
 }
 
@@ -881,7 +938,7 @@ int launch(XaArgs &a, int nb, cudaStream_t s)
         a.cs *= 2;
     if (items > 0x7fffffffL / a.cs)
         return K_EARG;
-    const int smem = CF::WK > 1 || a.cs > 1 ? CF::SMEM_PARTS : CF::SMEM_WHOLE;
+    const int smem = a.cs > 1 ? CF::SMEM_PARTS : CF::SMEM_WHOLE;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -965,7 +1022,8 @@ extern "C" int k_cross_attend(const struct k_rows *Q, const struct k_rows *K, co
     cudaStream_t st = reinterpret_cast<cudaStream_t>(s);
     // Many rows over many keys: tcgen05. Both forms were measured over 1 to 1024
     // queries and 96 to 4096 keys (us, tcgen05 / this file): 128 columns a head
-    // 128 x 16 heads, 1 query x 1024 keys 16.0 / 21.6, 128 x 4096 53 / 145;
+    // 128 heads, 1 query x 4096 keys 46 / 71 (8 heads, 8192 keys 22.0 / 18.8), 128 x
+    // 4096 53 / 145;
     // 64 columns, 32 heads, 48 x 384 7.0 / 8.4, 48 x 1024 11.6 / 12.1 (1.6 M
     // scores), 128 x 1024 14.4 / 12.1 (4.2 M), 256 x 1024 15.1 / 17.0 (8.4 M);
     // 32 columns, 64 heads, 64 x 192 5.6 / 4.8, 64 x 384 7.2 / 7.2, 96 x 1024
@@ -973,7 +1031,7 @@ extern "C" int k_cross_attend(const struct k_rows *Q, const struct k_rows *K, co
     // one tile here, so few queries of theirs stay.
     const double scores = (double)nb * heads * Nq * Nk;
     const bool mid = Nk < 640, big = scores >= 6e6;
-    const bool many = hd > 64   ? Nk >= 96 && (a.g == 1 || Nq >= 16)
+    const bool many = hd > 64   ? Nk >= 96 && (Nq >= 16 || (a.g == 1 && (long)nb * heads >= 64))
                       : hd > 32 ? Nq >= 24 && (mid ? Nk >= 96 : big)
                                 : (Nq >= 64 && mid && Nk >= 256) || (Nq >= 24 && Nk >= 96 && big);
     if (many && attn_cross_tc_takes(a, nb, Q->dt)) {

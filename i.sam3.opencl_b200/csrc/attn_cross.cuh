@@ -90,89 +90,33 @@ struct Parts {
     template <int THREADS, typename Store>
     static __device__ __forceinline__ void merge(float *part, int np, int rl, int live, const Store &store)
     {
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        // Weights of a row's parts and 1 / sum: a thread per row for few parts
-        // (many rows then), a warp per row for more.
-        constexpr int kFew = 8;
-        for (int i = threadIdx.x; np <= kFew && i < live; i += THREADS) {
-            float2 ml[kFew];
+        // weights of a row's parts and 1 / sum, a thread per row
+        constexpr int kMost = 16;  // CTAs of a cluster
+        for (int i = threadIdx.x; i < live; i += THREADS) {
             float m = -INFINITY, l = 0.0f;
+            float2 ml[kMost];
 #pragma unroll
-            for (int p = 0; p < kFew; p++) {
+            for (int p = 0; p < kMost; p++) {
                 ml[p] = p < np ? *reinterpret_cast<const float2 *>(part + (p * rl + i) * PR + HDP)
                                : make_float2(-INFINITY, 0.0f);
                 m = fmaxf(m, ml[p].x);
             }
 #pragma unroll
-            for (int p = 0; p < kFew; p++) {
-                const bool none = ml[p].x == -INFINITY;
-                const float w = none ? 0.0f : exp2f(ml[p].x - m);
-                l += none ? (ml[p].y == ml[p].y ? 0.0f : ml[p].y) : ml[p].y * w;
-                if (p < np)
+            for (int p = 0; p < kMost; p++)
+                if (p < np) {
+                    const bool none = ml[p].x == -INFINITY;
+                    const float w = none ? 0.0f : exp2f(ml[p].x - m);
+                    l += none ? (ml[p].y == ml[p].y ? 0.0f : ml[p].y) : ml[p].y * w;
                     part[(p * rl + i) * PR + HDP] = w;
-            }
+                }
             part[i * PR + HDP + 2] = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        }
-        for (int i = warp; np > kFew && i < live; i += THREADS / 32) {
-            float2 ml[2];  // up to 64 parts
-            float m = -INFINITY, l = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const int p = lane + 32 * k;
-                ml[k] = p < np ? *reinterpret_cast<const float2 *>(part + (p * rl + i) * PR + HDP)
-                               : make_float2(-INFINITY, 0.0f);
-                m = fmaxf(m, ml[k].x);
-            }
-#pragma unroll
-            for (int x = 16; x; x >>= 1)
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const int p = lane + 32 * k;
-                const float w = ml[k].x == -INFINITY ? 0.0f : exp2f(ml[k].x - m);
-                l += ml[k].x == -INFINITY ? (ml[k].y == ml[k].y ? 0.0f : ml[k].y) : ml[k].y * w;
-                if (p < np)
-                    part[(p * rl + i) * PR + HDP] = w;
-            }
-#pragma unroll
-            for (int x = 16; x; x >>= 1)
-                l += __shfl_xor_sync(0xffffffffu, l, x);
-            if (lane == 0)
-                part[i * PR + HDP + 2] = l > 0.0f || l != l ? 1.0f / l : 0.0f;
         }
         __syncthreads();
         const int ne = live * (HDP / 4);  // elements, four columns each
-        if (np > kFew) {  // eight lanes to an element
-            const int g = lane & 7;
-            for (int e0 = warp * 4; e0 < ne; e0 += THREADS / 8) {
-                const int e = min(e0 + (lane >> 3), ne - 1), i = e / (HDP / 4), c = (e % (HDP / 4)) * 4;
-                float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                for (int p = g; p < np; p += 8) {
-                    const float *src = part + (p * rl + i) * PR;
-                    const float w = src[HDP];
-                    const float4 v = *reinterpret_cast<const float4 *>(src + c);
-                    acc.x = fmaf(v.x, w, acc.x);
-                    acc.y = fmaf(v.y, w, acc.y);
-                    acc.z = fmaf(v.z, w, acc.z);
-                    acc.w = fmaf(v.w, w, acc.w);
-                }
-#pragma unroll
-                for (int x = 4; x; x >>= 1) {
-                    acc.x += __shfl_xor_sync(0xffffffffu, acc.x, x);
-                    acc.y += __shfl_xor_sync(0xffffffffu, acc.y, x);
-                    acc.z += __shfl_xor_sync(0xffffffffu, acc.z, x);
-                    acc.w += __shfl_xor_sync(0xffffffffu, acc.w, x);
-                }
-                const float inv = part[i * PR + HDP + 2];
-                if (g == 0 && e0 + (lane >> 3) < ne)
-                    store(i, c, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-            }
-            return;
-        }
         for (int e = threadIdx.x; e < ne; e += THREADS) {
             const int i = e / (HDP / 4), c = (e % (HDP / 4)) * 4;
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
             for (int p = 0; p < np; p++) {
                 const float *src = part + (p * rl + i) * PR;
                 const float w = src[HDP];

@@ -427,11 +427,12 @@ int cb_attend(cb_backend *b, int Nq, int Nk, int heads, int hd, cb_mem Q,
  * n, h, d) of a [nb, rows, heads, hd] operand lies at off + b * s0 + n * ld + h
  * * s1 + d; strides are not negative (0 repeats an input), and no two elements
  * of an output share an address. Any alignment of the element type is taken;
- * 16-byte aligned starts and strides run fastest. Each call enqueues one
- * kernel on the backend's stream, allocates nothing and uses no scratch
- * buffer, so it may be captured into a graph and several captured calls may
- * replay at once on their own buffers. An output may not overlap an input,
- * except where in-place use is named. */
+ * 16-byte aligned starts and strides run fastest. Each call enqueues its
+ * kernel (one, or several for rotations of more than 2^31 chunks) on the
+ * backend's stream, allocates nothing and uses no scratch buffer, so it may be
+ * captured into a graph, as its first call too, and several captured calls
+ * may replay at once on their own buffers. An output may not overlap an
+ * input, except where in-place use is named. */
 
 /* Frequencies of a table: pair j of rot columns turns by w_j per position,
  *   NONE:   w_j = theta^(-2j / rot);
@@ -468,7 +469,8 @@ int cb_rope_table(cb_backend *b, int npos, int rot, int64_t first,
  * 0), or pos0 + n when pos is NULL (pos0 + N <= npos). A position outside [0,
  * npos) leaves its row as it is. X and Y of one type, or X F32 and Y BF16 /
  * F16; rotated in 32 bits and rounded once. Y may be X (same layout). Queries
- * and keys of one fused row are rotated by one call over their heads. */
+ * and keys of one fused row are rotated by one call over their heads. At most
+ * 2^31 - 1 rows in all, 2^30 a sequence, 2^14 heads of 2^16 columns. */
 #define CB_ROPE_PAIRS 0
 #define CB_ROPE_HALVES 1
 int cb_rope_rotate(cb_backend *b, int nb, int N, int heads, int hd, int rot,

@@ -377,6 +377,88 @@ def test_cross_attend_one_encoder_for_all_and_large_scores(be, dt):
     check_attend(be, q1, k.expand(nb, Nk, h, hd), v.expand(nb, Nk, h, hd), scale=1.0)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("Nq,Nk,hd", [(2, 150, 64), (50, 40, 32), (300, 450, 64), (200, 300, 128)])
+def test_cross_attend_nan_and_infinities_of_visible_keys(be, Nq, Nk, hd, dt):
+    """A key that is seen and not a number makes every row NaN wherever it lies, one whose scores are -inf for all
+    queries counts nothing, an infinite value shows in its column."""
+    h = 2
+    g = gen(9)
+    q = randn(g, 1, Nq, h, hd).abs().to(DT[dt]) + 0.25
+    k, v = (randn(g, 1, Nk, h, hd).to(DT[dt]) for _ in range(2))
+    def d(t):
+        return op(be, t, 0, t.stride(1), t.stride(0), t.stride(2))
+    def run(k, v):
+        o = torch.empty_like(q)
+        be.cross_attend(1, Nq, Nk, h, h, hd, d(q), d(k), d(v), d(o))
+        be.sync()
+        return o
+    for j in (0, 13, 14, 31, Nk - 1):
+        kn = k.clone()
+        kn[0, j, :, 3] = math.nan
+        assert run(kn, v).isnan().all()
+        if dt != "f32":  # 32-bit operands are split into parts: finite values only
+            kn = k.clone()
+            kn[0, j, :, 3] = math.inf
+            assert run(kn, v).isnan().all()
+            kn[0, j, :, 3] = -math.inf  # q is positive
+            keep = torch.arange(Nk, device="cuda") != j
+            klen = torch.tensor([Nk], device="cuda", dtype=torch.int32)
+            mask = (~keep).to(torch.uint8)
+            o = torch.empty_like(q)
+            be.cross_attend(1, Nq, Nk, h, h, hd, d(q), d(k), d(v), d(o), be.wrap(klen), be.wrap(mask))
+            be.sync()
+            assert ((run(kn, v) - o).abs() <= 4 * u(DT[dt]) * v.abs().max()).all()
+            vn = v.clone()
+            vn[0, j, :, 5] = math.inf
+            o = run(k, vn)
+            assert (o[..., 5] == math.inf).all() and o[..., :5].isfinite().all()
+
+
+def test_operands_far_into_a_buffer(be, sb):
+    """Offsets past 2^31 elements."""
+    far = 2 ** 31 + 64
+    buf = torch.empty(far + (1 << 20), device="cuda", dtype=torch.bfloat16)
+    g = gen(2)
+    n = 60 * 128
+    tail = buf[far:]
+    tail[:4 * n] = randn(g, 4 * n).bfloat16()
+    near = tail[:4 * n].clone()
+    m, mn = be.wrap(buf), be.wrap(near)
+    out = torch.empty(2, n, device="cuda", dtype=torch.bfloat16)
+    mo = be.wrap(out)
+    cs = torch.empty(60, 32, 2, device="cuda")
+    be.rope_table(60, 64, 0, None, be.wrap(cs))
+    for i, (b, o) in enumerate(((m, far), (mn, 0))):
+        be.rope_rotate(1, 60, 2, 64, 64, 0, be.bmat(b, o, 128, 0, 64), be.bmat(mo, i * n, 128, 0, 64), be.wrap(cs), 60)
+    be.sync()
+    assert torch.equal(out[0], out[1])
+    for i, (b, o) in enumerate(((m, far), (mn, 0))):
+        be.cross_attend(1, 60, 60, 2, 2, 64, *(be.bmat(b, o + j * n, 128, 0, 64) for j in range(3)),
+                        be.bmat(mo, i * n, 128, 0, 64))
+    be.sync()
+    assert torch.equal(out[0], out[1])
+    gamma, beta = torch.ones(128, device="cuda"), torch.zeros(128, device="cuda")
+    for i, (b, o) in enumerate(((m, far), (mn, 0))):
+        be.groupnorm(1, 60, 128, 8, be.bmat(b, o, 128), be.bmat(mo, i * n, 128), be.wrap(gamma), be.wrap(beta))
+    be.sync()
+    assert torch.equal(out[0], out[1])
+    # results written there, rows 2^29 elements apart
+    ld = 2 ** 29
+    x = randn(g, 4, 64).bfloat16()
+    be.groupnorm(1, 4, 64, 8, op(be, x, 0, 64), be.bmat(m, 0, ld), be.wrap(gamma), be.wrap(beta))
+    be.groupnorm(1, 4, 64, 8, op(be, x, 0, 64), be.bmat(mo, 0, 64), be.wrap(gamma), be.wrap(beta))
+    be.sync()
+    assert all(torch.equal(buf[i * ld:i * ld + 64], out.view(-1)[i * 64:i * 64 + 64]) for i in range(4))
+    q = randn(g, 1, 100, 1, 64).bfloat16()
+    for i in range(4):
+        buf[i * ld:i * ld + 128] = randn(g, 128).bfloat16()
+    k = torch.stack([buf[i * ld:i * ld + 64] for i in range(4)]).view(1, 4, 1, 64)
+    v = torch.stack([buf[i * ld + 64:i * ld + 128] for i in range(4)]).view(1, 4, 1, 64)
+    o = torch.empty_like(q)
+    check_attend(be, q, k, v, o=o, args=[op(be, q, 0, 64), be.bmat(m, 0, ld), be.bmat(m, 64, ld), op(be, o, 0, 64)])
+
+
 # ------------------------------------------------------------------ group norm
 def norm_ref(x, G, gamma, beta, eps, act):
     nb, n, Cn = x.shape
@@ -580,6 +662,48 @@ def test_together_captured_and_replayed(sb):
     for b in bes + [b3]:
         b.sync()
         b.close()
+
+
+def test_first_call_of_a_process_may_be_captured():
+    """Nothing that a call sets up once is refused during a capture."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = """
+import sys, torch
+sys.path.insert(0, %r)
+import conftest
+sb = conftest.load_product()
+import test_gpu_prompt_ops as T
+x = T.chain_inputs(5, torch.bfloat16, N=300, Nk=700)
+b = sb.Backend(0)
+s = torch.cuda.Stream()
+b.set_stream(s.cuda_stream)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    T.chain(b, sb, x)
+g.replay()
+torch.cuda.synchronize()
+y = x["y"].clone()
+b.set_stream(1)
+T.chain(b, sb, x)
+b.sync()
+assert torch.equal(x["y"], y) and y.float().abs().sum() > 0
+""" % here
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_profile_names(be, sb):
+    be.profile(True)
+    chain(be, sb, chain_inputs(3, torch.bfloat16))
+    table = be.profile_table()
+    be.profile(False)
+    assert {n: table[n]["calls"] for n in ("rope_table", "rope_rotate", "cross_attend", "groupnorm")} == \
+        {"rope_table": 1, "rope_rotate": 2, "cross_attend": 1, "groupnorm": 1}
+    assert all(table[n]["ms"] > 0 and table[n]["bytes"] > 0 for n in table)
 
 
 def test_same_result_each_time(be, sb):
