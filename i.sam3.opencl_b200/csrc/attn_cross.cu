@@ -623,18 +623,22 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
     });
 }
 
-// Few keys (all in one step) and many rows: the bandwidth of Q and O. A CTA
-// reads the keys and values of one key head once and walks over tiles of 64
-// rows, each warp its 16 rows through three cp.async buffers of its own (no
-// block barrier in the loop); one pass of softmax without a running maximum;
-// results go back through the rows' buffer so that they are stored as 16-byte
-// vectors.
+// Few keys (all in one step) and many rows. A CTA reads the keys and values of
+// one key head once and walks over tiles of 64 rows, each warp its 16 rows
+// through three cp.async buffers of its own (no block barrier in the loop);
+// one pass of softmax without a running maximum, row sums as a product with
+// ones, -inf of hidden keys as the scores' first accumulator; results go back
+// through the rows' buffer so that they are stored as 16-byte vectors. 8 x 5184
+// rows x 8 heads of 32 columns over 39 keys: 13.5 us, 3.1 TB/s; the same loop
+// without its arithmetic copies at 5.9 TB/s, so the instructions per row bound
+// it (issue slots half full at 16 warps per SM; key and value fragments kept in
+// registers 14.0 us, 5 or 6 CTAs per SM 15.2 and 16.4, two row groups per
+// warp 15.9).
 template <typename T, int HDP, int KT>
-__global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constant__ XaArgs a)
+__global__ void __launch_bounds__(kThreads, HDP <= 64 ? 4 : 3) attn_few_kernel(const __grid_constant__ XaArgs a)
 {
     using TL = Tile<T, HDP>;
     constexpr int NK = KT * 16, CPR = TL::CPR, EPC = 8, NT = KT * 2, DT = HDP / 8, QB = 16 * TL::PITCH, ST = 3;
-    constexpr bool KEEP = HDP == 32;  // key and value fragments stay in registers
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t *ks = smem, *vs = ks + NK * TL::PITCH;
     __shared__ uint8_t vis[NK];
@@ -650,30 +654,43 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
     const int hdc = a.hd / EPC;
     const int ntile = split < a.nqt ? (a.nqt - 1 - split) / a.cs + 1 : 0;
     auto row_at = [&](uint32_t gr, long ld, long s1) {
-        if (a.g == 1)
-            return gr * ld;
         const uint32_t qi = quot(gr, a.dg);
         return qi * ld + (gr - qi * a.dg.d) * s1;
     };
+    // A lane's chunks of a tile are RS rows apart. Without shared heads their
+    // addresses step by a constant from tile to tile.
+    constexpr int NC = 16 * CPR / 32, RS = 32 / CPR;
+    const int lr = lane / CPR, lc = lane % CPR;
+    const bool plain = a.g == 1, col = lc < hdc;
+    const uint32_t w0 = (uint32_t)split * 64 + warp * 16;  // first row of the warp's first tile
+    const T *qp = qb + (w0 + lr) * a.qld + lc * EPC;
+    T *op = ob + (w0 + lr) * a.old + lc * EPC;
+    const long qstep = (long)a.cs * 64 * a.qld, ostep = (long)a.cs * 64 * a.old;
+    long qleft = a.rows - w0 - lr;  // rows from the lane's first one to the last
+    const uint32_t slot0 = smem_addr(qs);
+    int qslot = 0;
     auto load_q = [&](int i) {
         if (i < ntile) {
-            const uint32_t r0 = (uint32_t)(split + i * a.cs) * 64 + warp * 16;
+            uint8_t *buf = qs + qslot * QB;
 #pragma unroll
-            for (int x = lane; x < 16 * CPR; x += 32) {
-                const int r = x / CPR, c = x % CPR;
-                const bool live = r0 + r < a.rows && c < hdc;
-                const T *src = live ? qb + row_at(r0 + r, a.qld, a.qs1) + c * EPC : qb;
-                uint8_t *dst = qs + (i % ST) * QB + TL::at(r, c);
+            for (int k = 0; k < NC; k++) {
+                const int r = lr + k * RS;
+                const bool live = col && qleft > k * RS;
+                const T *src = plain ? qp + k * RS * a.qld
+                                     : qb + (live ? row_at(w0 + (uint32_t)i * a.cs * 64 + r, a.qld, a.qs1) : 0) + lc * EPC;
                 if (a.qvec)
-                    cp16(smem_addr(dst), live ? src : a.q, live);
+                    cp16(slot0 + qslot * QB + TL::at(r, lc), live ? src : a.q, live);
                 else {
                     T w[EPC];
 #pragma unroll
                     for (int e = 0; e < EPC; e++)
                         w[e] = live ? src[e] : out_of<T>(0.0f);
-                    *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(w);
+                    *reinterpret_cast<uint4 *>(buf + TL::at(r, lc)) = *reinterpret_cast<const uint4 *>(w);
                 }
             }
+            qp += qstep;
+            qleft -= a.cs * 64;
+            qslot = qslot + 1 == ST ? 0 : qslot + 1;
         }
         cp_commit();
     };
@@ -732,23 +749,14 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
     auto value_frag = [&](int n, int d, uint32_t (&f)[4]) {
         ldsm4t(va + TL::at(n * 8 + (lane & 15), d + (lane >> 4)), f);
     };
-    uint32_t kf[KEEP ? HDP / 16 : 1][KEEP ? KT : 1][4], vf[KEEP ? KT : 1][KEEP ? DT / 2 : 1][4];
-    if constexpr (KEEP) {
-#pragma unroll
-        for (int n = 0; n < KT; n++) {
-#pragma unroll
-            for (int kk = 0; kk < HDP / 16; kk++)
-                key_frag(kk, 2 * n, kf[kk][n]);
-#pragma unroll
-            for (int d = 0; d < DT / 2; d++)
-                value_frag(2 * n, 2 * d, vf[n][d]);
-        }
-    }
+    long left = a.rows - w0 - lr;
+    int slot = 0;
     for (int i = 0; i < ntile; i++) {
         load_q(i + 2);
         cp_wait<2>();
         __syncwarp();
-        uint8_t *buf = qs + (i % ST) * QB;
+        uint8_t *buf = qs + slot * QB;
+        slot = slot + 1 == ST ? 0 : slot + 1;
         float sc[NT][4];
 #pragma unroll
         for (int kk = 0; kk < HDP / 16; kk++) {
@@ -756,10 +764,8 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
             ldsm4(smem_addr(buf) + TL::at(lane & 15, kk * 2 + (lane >> 4)), qf);
 #pragma unroll
             for (int n = 0; n < KT; n++) {
-                uint32_t f[4];
-                if constexpr (!KEEP)
-                    key_frag(kk, 2 * n, f);
-                const uint32_t(&k4)[4] = KEEP ? kf[KEEP ? kk : 0][KEEP ? n : 0] : f;
+                uint32_t k4[4];
+                key_frag(kk, 2 * n, k4);
                 if (kk == 0) {
                     mma16_from<T>(sc[2 * n], qf, k4[0], k4[1], start[2 * n][0], start[2 * n][1]);
                     mma16_from<T>(sc[2 * n + 1], qf, k4[2], k4[3], start[2 * n + 1][0], start[2 * n + 1][1]);
@@ -798,10 +804,8 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
                                     pack2<T>(sc[2 * n + 1][2], sc[2 * n + 1][3])};
 #pragma unroll
             for (int d = 0; d < DT / 2; d++) {
-                uint32_t f[4];
-                if constexpr (!KEEP)
-                    value_frag(2 * n, 2 * d, f);
-                const uint32_t(&v4)[4] = KEEP ? vf[KEEP ? n : 0][KEEP ? d : 0] : f;
+                uint32_t v4[4];
+                value_frag(2 * n, 2 * d, v4);
                 if (n == 0) {
                     mma16_from<T>(o[2 * d], pf, v4[0], v4[1], 0.0f, 0.0f);
                     mma16_from<T>(o[2 * d + 1], pf, v4[2], v4[3], 0.0f, 0.0f);
@@ -818,7 +822,7 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
         }
 #pragma unroll
         for (int h = 0; h < 2; h++)
-            inv[h] = sums[2 * h] > 0.0f || sums[2 * h] != sums[2 * h] ? 1.0f / sums[2 * h] : 0.0f;
+            inv[h] = sums[2 * h] > 0.0f || sums[2 * h] != sums[2 * h] ? rcp_approx(sums[2 * h]) : 0.0f;
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -826,13 +830,13 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
                 *reinterpret_cast<uint32_t *>(buf + TL::at(g4 + 8 * h, d) + t4 * 4) =
                     pack2<T>(o[d][2 * h] * inv[h], o[d][2 * h + 1] * inv[h]);
         __syncwarp();
-        const uint32_t r0 = (uint32_t)(split + i * a.cs) * 64 + warp * 16;
 #pragma unroll
-        for (int x = lane; x < 16 * CPR; x += 32) {
-            const int r = x / CPR, c = x % CPR;
-            if (r0 + r < a.rows && c < hdc) {
-                T *dst = ob + row_at(r0 + r, a.old, a.os1) + c * EPC;
-                const uint4 w = *reinterpret_cast<const uint4 *>(buf + TL::at(r, c));
+        for (int k = 0; k < NC; k++) {
+            const int r = lr + k * RS;
+            if (col && left > k * RS) {
+                T *dst = plain ? op + k * RS * a.old
+                               : ob + row_at(w0 + (uint32_t)i * a.cs * 64 + r, a.old, a.os1) + lc * EPC;
+                const uint4 w = *reinterpret_cast<const uint4 *>(buf + TL::at(r, lc));
                 if (a.ovec)
                     *reinterpret_cast<uint4 *>(dst) = w;
                 else {
@@ -843,6 +847,8 @@ __global__ void __launch_bounds__(kThreads) attn_few_kernel(const __grid_constan
                 }
             }
         }
+        op += ostep;
+        left -= a.cs * 64;
         __syncwarp();
     }
     cp_wait<0>();
