@@ -958,7 +958,7 @@ int launch(XaArgs &a, int nb, cudaStream_t s)
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = a.cs > 1 ? 2 : 1;
     return (int)cudaLaunchKernelEx(&cfg, attn_cross_kernel<T, HDP, WM>, (const XaArgs)a);
 }
 

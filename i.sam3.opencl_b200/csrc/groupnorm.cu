@@ -622,7 +622,7 @@ int launch_a(GnArgs &a, int nb, long npix, int C, cudaStream_t s)
     cfg.dynamicSmemBytes = (size_t)a.nring * batch + red;
     cfg.stream = s;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = a.cs > 1 ? 2 : 1;
     return (int)cudaLaunchKernelEx(&cfg, groupnorm_kernel<TI, TO, V, GELU>, (const GnArgs)a);
 }
 
