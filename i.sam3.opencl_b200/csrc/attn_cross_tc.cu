@@ -21,7 +21,10 @@
 // with a visible key, exponentials of later tiles are taken against it, and a
 // tile whose sum reaches 2^13 (or is not a number) is taken again with a raised
 // offset, then without the polynomial exponential, so that infinities and NaN
-// of visible keys come out as such.
+// of visible keys come out as such. Measured: 8 x 5184 queries x 5184 keys x 16
+// heads of 64 columns 1012 us, 870 TFLOP/s (the softmax warps bound it as in
+// attn_tc.cu: 884); 4 x 4096 x 4096 x 16 heads of 128 columns 467 us, 1177
+// TFLOP/s; with a key mask 1164 us, every tile in the rolled path.
 #include "attn_cross.cuh"
 #include "kernels.h"
 #include "pdl.cuh"

@@ -129,7 +129,8 @@ struct alignas(sizeof(T) * V) Vec {
 // (cos, sin) pairs are read once for all of them. W columns are 16 bytes of
 // input, or 1 (a pair of columns 2 j, 2 j + 1 without HALVES) for rows that
 // are not 16-byte aligned. Memory bound: X read and Y written once, the
-// table rows from L2.
+// table rows from L2; 41472 rows of 24 heads of 64 bf16 columns 48 us, 5.3 TB/s
+// (81 % of a copy). Indexes without divisions (56 us with 64-bit ones).
 template <typename TI, typename TO, int W, bool HALVES>
 __global__ void __launch_bounds__(256) rope_rotate_kernel(const __grid_constant__ RotArgs a)
 {
