@@ -119,11 +119,23 @@ __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo: hi rounded to tf32's 11 significand bits, lo what is left of the
-// 24, cut to 11 (off by 2^-22 of x at most).
-__device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo)
+// x = hi + lo, hi with tf32's 11 significand bits, off by 2^-22 of x at most.
+// Only one factor of a product has hi cut, the other has it rounded: lo * lo is
+// dropped, and with both cut it would always have the product's sign. Cutting
+// (K, V): the largest numbers do not round up to infinity.
+__device__ __forceinline__ void split_cut(float x, uint32_t &hi, uint32_t &lo)
 {
-    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    hi = __float_as_uint(x) & 0xffffe000u;
+    lo = (__float_as_uint(x - __uint_as_float(hi)) + 0x1000u) & 0xffffe000u;
+}
+// Rounding (weights, at most 1; queries with MOST, which keeps them finite)
+template <bool MOST>
+__device__ __forceinline__ void split_near(float x, uint32_t &hi, uint32_t &lo)
+{
+    const uint32_t u = __float_as_uint(x);
+    hi = (u + 0x1000u) & 0xffffe000u;
+    if (MOST && (hi & 0x7fffffffu) == 0x7f800000u)
+        hi = u & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 
@@ -343,31 +355,53 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
         else {
             const float *qs = reinterpret_cast<const float *>(smem) + (wm * 16 + g4) * (TL::PITCH / 4) + t4;
             const float *kf = reinterpret_cast<const float *>(ks) + (jw + g4) * (TL::PITCH / 4) + t4;
-#pragma unroll 2
-            for (int kk = 0; kk < HDP / 8; kk++) {
-                uint32_t ah[4], al[4];
+            // As P V below: 16 columns sum from zero and are added outside the
+            // matrix unit. Output of 300 queries x 2000 keys, 128 columns: 3.6e-7
+            // off, all columns in one chain 1.2e-6 (201 x 5184 x 32 columns 70 us,
+            // then 67; 8 columns at a time 71).
+#pragma unroll 1
+            for (int kk = 0; kk < HDP / 8; kk += 2) {
+                uint32_t ah[2][4], al[2][4];
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    split_tf32(qs[(e & 1) * 8 * (TL::PITCH / 4) + kk * 8 + (e >> 1) * 4], ah[e], al[e]);
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        split_near<true>(qs[(e & 1) * 8 * (TL::PITCH / 4) + (kk + u) * 8 + (e >> 1) * 4], ah[u][e],
+                                         al[u][e]);
                 // four tiles side by side: a product waits for the one four before it
                 constexpr int NB = NT < 4 ? NT : 4;
 #pragma unroll
                 for (int n0 = 0; n0 < NT; n0 += NB) {
-                    uint32_t bh[NB][2], bl[NB][2];
+                    float part[NB][4];
 #pragma unroll
                     for (int n = 0; n < NB; n++)
 #pragma unroll
-                        for (int e = 0; e < 2; e++)
-                            split_tf32(kf[(n0 + n) * 8 * (TL::PITCH / 4) + kk * 8 + 4 * e], bh[n][e], bl[n][e]);
+                        for (int e = 0; e < 4; e++)
+                            part[n][e] = 0.0f;
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        uint32_t bh[NB][2], bl[NB][2];
+#pragma unroll
+                        for (int n = 0; n < NB; n++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++)
+                                split_cut(kf[(n0 + n) * 8 * (TL::PITCH / 4) + (kk + u) * 8 + 4 * e], bh[n][e],
+                                          bl[n][e]);
+#pragma unroll
+                        for (int n = 0; n < NB; n++)
+                            mma8(part[n], al[u], bh[n][0], bh[n][1]);
+#pragma unroll
+                        for (int n = 0; n < NB; n++)
+                            mma8(part[n], ah[u], bl[n][0], bl[n][1]);
+#pragma unroll
+                        for (int n = 0; n < NB; n++)
+                            mma8(part[n], ah[u], bh[n][0], bh[n][1]);
+                    }
 #pragma unroll
                     for (int n = 0; n < NB; n++)
-                        mma8(sc[n0 + n], al, bh[n][0], bh[n][1]);
 #pragma unroll
-                    for (int n = 0; n < NB; n++)
-                        mma8(sc[n0 + n], ah, bl[n][0], bl[n][1]);
-#pragma unroll
-                    for (int n = 0; n < NB; n++)
-                        mma8(sc[n0 + n], ah, bh[n][0], bh[n][1]);
+                        for (int e = 0; e < 4; e++)
+                            sc[n0 + n][e] += part[n][e];
                 }
             }
         }
@@ -400,17 +434,22 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
                 m = max3f(m, sc[n][2 * h], sc[n][2 * h + 1]);
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            const float mn = fmaxf(mx[h], m * a.scale_log2);
+            // 32 bits: a whole number, so that neither the shift below nor the
+            // corrections round
+            const float mn = fmaxf(mx[h], F32 ? ceilf(m * a.scale_log2) : m * a.scale_log2);
             const float base = mn == -INFINITY ? 0.0f : mn;
             const float corr = exp2f(mx[h] - base);
+            // 32 bits: weights below 2^-shift < 1 / (2 Nk), so that their sum with
+            // values of any size stays finite (the factor is in O and in the sum)
+            const float off = F32 ? -(base + a.shift) : -base;
             mx[h] = mn;
             float add = 0.0f;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                sc[n][2 * h] = F32 ? exp2f(fmaf(sc[n][2 * h], a.scale_log2, -base))
-                                   : ex2_approx(fmaf(sc[n][2 * h], a.scale_log2, -base));
-                sc[n][2 * h + 1] = F32 ? exp2f(fmaf(sc[n][2 * h + 1], a.scale_log2, -base))
-                                       : ex2_approx(fmaf(sc[n][2 * h + 1], a.scale_log2, -base));
+                sc[n][2 * h] = F32 ? exp2f(fmaf(sc[n][2 * h], a.scale_log2, off))
+                                   : ex2_approx(fmaf(sc[n][2 * h], a.scale_log2, off));
+                sc[n][2 * h + 1] = F32 ? exp2f(fmaf(sc[n][2 * h + 1], a.scale_log2, off))
+                                       : ex2_approx(fmaf(sc[n][2 * h + 1], a.scale_log2, off));
                 add += sc[n][2 * h] + sc[n][2 * h + 1];
             }
             sum[h] = fmaf(sum[h], corr, add);
@@ -447,10 +486,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
             uint32_t ph[NT][4], pl[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                split_tf32(sc[n][0], ph[n][0], pl[n][0]);
-                split_tf32(sc[n][2], ph[n][1], pl[n][1]);
-                split_tf32(sc[n][1], ph[n][2], pl[n][2]);
-                split_tf32(sc[n][3], ph[n][3], pl[n][3]);
+                split_near<false>(sc[n][0], ph[n][0], pl[n][0]);
+                split_near<false>(sc[n][2], ph[n][1], pl[n][1]);
+                split_near<false>(sc[n][1], ph[n][2], pl[n][2]);
+                split_near<false>(sc[n][3], ph[n][3], pl[n][3]);
             }
 #pragma unroll
             for (int d0 = 0; d0 < DT; d0 += 4) {
@@ -467,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
                     for (int d = 0; d < 4; d++)
 #pragma unroll
                         for (int e = 0; e < 2; e++)
-                            split_tf32(vf[(n * 8 + e) * (TL::PITCH / 4) + (d0 + d) * 8], bh[d][e], bl[d][e]);
+                            split_cut(vf[(n * 8 + e) * (TL::PITCH / 4) + (d0 + d) * 8], bh[d][e], bl[d][e]);
 #pragma unroll
                     for (int d = 0; d < 4; d++)
                         mma8(lo[d], pl[n], bh[d][0], bh[d][1]);
@@ -1029,6 +1068,9 @@ extern "C" int k_cross_attend(const struct k_rows *Q, const struct k_rows *K, co
     if (es == 2 && Nk <= 64 && a.rows > 16)
         a.ovec = vec(O);  // the form for few keys stores 16 bytes
     a.scale_log2 = (float)(scale * 1.4426950408889634);
+    for (int n = Nk; n > 0; n >>= 1)
+        a.shift += 1.0f;
+    a.shift += 1.0f;
     a.err = err;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(s);
     // Many rows over many keys: tcgen05. Both forms were measured over 1 to 1024

@@ -24,6 +24,7 @@ struct XaArgs {
     int kvec, qvec, ovec;  // 16-byte accesses allowed
     Div dg;                // g, for rows < 2^31
     float scale_log2;
+    float shift;  // of the weights' exponents in 32 bits, 2^shift > 2 Nk
     int *err;  // device error word (bounded waits of the tcgen05 form)
 };
 

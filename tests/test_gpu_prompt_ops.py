@@ -415,6 +415,21 @@ def test_cross_attend_nan_and_infinities_of_visible_keys(be, Nq, Nk, hd, dt):
             assert (o[..., 5] == math.inf).all() and o[..., :5].isfinite().all()
 
 
+def test_cross_attend_largest_numbers(be):
+    """Values next to the largest of 32 bits come through (an operand is split into parts that must not overflow)."""
+    g = gen(15)
+    q, k = randn(g, 1, 40, 1, 32), randn(g, 1, 90, 1, 32)
+    big = torch.finfo(torch.float32).max
+    v = torch.where(randn(g, 1, 90, 1, 32) > 0, big, -big)
+    v[..., :8] = big
+    o = torch.empty_like(q)
+    be.cross_attend(1, 40, 90, 1, 1, 32, op(be, q, 0, 32), op(be, k, 0, 32), op(be, v, 0, 32), op(be, o, 0, 32))
+    be.sync()
+    assert not o.isnan().any() and (o[..., 8:].abs() < math.inf).all()
+    # an average of equal numbers is that number up to the errors of the weights' sum, infinite where these exceed it
+    assert ((o[..., :8] == math.inf) | ((o[..., :8] / big - 1).abs() <= (32 + 16 + 90 + 16) * 2.0 ** -23)).all()
+
+
 def test_operands_far_into_a_buffer(be, sb):
     """Offsets past 2^31 elements."""
     far = 2 ** 31 + 64
