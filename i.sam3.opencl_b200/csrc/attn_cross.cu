@@ -673,7 +673,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
 // one pass of softmax without a running maximum, row sums as a product with
 // ones, -inf of hidden keys as the scores' first accumulator; results go back
 // through the rows' buffer so that they are stored as 16-byte vectors. 8 x 5184
-// rows x 8 heads of 32 columns over 39 keys: 13.5 us, 3.1 TB/s; the same loop
+// rows x 8 heads of 32 columns over 39 keys: 13.9 us, 3.0 TB/s (13.5 us before
+// hidden keys were hidden twice; the variants below against that); the same loop
 // without its arithmetic copies at 5.9 TB/s, so the instructions per row bound
 // it (issue slots half full at 16 warps per SM; key and value fragments kept in
 // registers 14.0 us, 5 or 6 CTAs per SM 15.2 and 16.4, two row groups per
@@ -821,16 +822,29 @@ __global__ void __launch_bounds__(kThreads, HDP <= 64 ? 4 : 3) attn_few_kernel(c
             }
         }
         __syncwarp();
-        float inv[2];
+        float inv[2], m[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            float m = -INFINITY;
+            m[h] = -INFINITY;
 #pragma unroll
             for (int n = 0; n < NT; n++)
-                m = max3f(m, sc[n][2 * h], sc[n][2 * h + 1]);
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            const float base = m == -INFINITY ? 0.0f : -m * a.scale_log2;
+                m[h] = max3f(m[h], sc[n][2 * h], sc[n][2 * h + 1]);
+            m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 1));
+            m[h] = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 2));
+        }
+        // Infinities of a query times a hidden key's zeros are NaN: where no score
+        // is left such keys are hidden again (a score of +inf gives NaN anyway).
+        if (__any_sync(0xffffffffu, fminf(m[0], m[1]) == -INFINITY)) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (start[n][e & 1] < 0.0f)
+                        sc[n][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const float base = m[h] == -INFINITY ? 0.0f : -m[h] * a.scale_log2;
             const uint64_t base2 = f2_make(base, base);
 #pragma unroll
             for (int n = 0; n < NT; n++) {

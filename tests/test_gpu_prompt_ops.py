@@ -430,6 +430,39 @@ def test_cross_attend_largest_numbers(be):
     assert ((o[..., :8] == math.inf) | ((o[..., :8] / big - 1).abs() <= (32 + 16 + 90 + 16) * 2.0 ** -23)).all()
 
 
+@pytest.mark.parametrize("Nk", [16, 39, 64, 200, 300])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_cross_attend_infinite_query(be, Nk, dt):
+    """A query of infinities: zeros where every visible score is -inf, NaN where one is +inf, other rows as always."""
+    g = gen(16)
+    hd = 32
+    q, k, v = (randn(g, 1, n, 1, hd).to(dt) for n in (70, Nk, Nk))
+    k[:, :, :, 0] = k[:, :, :, 0].abs() + 0.5
+    out = []
+    for low, high in ((0.0, 0.0), (-math.inf, math.inf)):
+        qi = q.clone()
+        qi[0, 3, 0, 0], qi[0, 20, 0, 0], qi[0, 69, 0, 0] = low, high, low
+        kmask = torch.zeros(1, Nk, dtype=torch.uint8, device="cuda")
+        kmask[0, 5] = 1
+        o = torch.empty_like(q)
+        be.cross_attend(1, 70, Nk, 1, 1, hd, op(be, qi, 0, hd), op(be, k, 0, hd), op(be, v, 0, hd),
+                        op(be, o, 0, hd), None, be.wrap(kmask))
+        be.sync()
+        out.append(o[0, :, 0])
+    assert (out[1][[3, 69]] == 0).all() and out[1][20].isnan().all()
+    rest = [r for r in range(70) if r not in (3, 20, 69)]
+    if Nk <= 200:
+        assert torch.equal(out[0][rest], out[1][rest])
+    else:
+        # The tcgen05 form takes a tile again for 32 rows at once, so a neighbour's weights are evaluated twice, each
+        # time rounded to the type (u = eps / 2) and off by the exponential's 2^-12 at most: weights w, w' of sum 1
+        # with |w - w'| <= (2 u + 2 * 2^-12) w in numerator and, unrounded, 2 * 2^-12 w in the sum, then both
+        # results rounded: |o - o'| <= (2 u + 4 * 2^-12 + 2 u) max |v|.
+        u = torch.finfo(dt).eps / 2
+        lim = (4 * u + 2.0 ** -10) * v.float().abs().max()
+        assert ((out[0][rest].float() - out[1][rest].float()).abs() <= lim).all()
+
+
 def test_operands_far_into_a_buffer(be, sb):
     """Offsets past 2^31 elements."""
     far = 2 ** 31 + 64
