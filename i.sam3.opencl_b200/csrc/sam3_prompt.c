@@ -127,7 +127,7 @@ int cb_rope_table(cb_backend *b, int npos, int rot, int64_t first,
     if (!b || npos <= 0 || rot <= 0 || rot % 2 || rot > K_ROPE_MAX ||
         first < -((int64_t)1 << 31) || first > ((int64_t)1 << 31) - npos ||
         !vec_ok(cs, CB_F32, (int64_t)npos * rot) || (uintptr_t)cs->ptr % 8 ||
-        !(theta > 1.0) || !isfinite(theta) || !(sc->amplitude > 0.0) || !isfinite(sc->amplitude))
+        !(theta > 1.0) || !isfinite(theta) || !(sc->amplitude > 0.0) || !isfinite((float)sc->amplitude))
         return cbi_fail(b, CB_EARG, "rope_table");
     if (sc->kind != CB_ROPE_SCALE_NONE && (!(sc->factor >= 1.0) || !isfinite(sc->factor)))
         return cbi_fail(b, CB_EARG, "rope_table: factor");
@@ -183,7 +183,8 @@ int cb_rope_rotate(cb_backend *b, int nb, int N, int heads, int hd, int rot, int
     int rc;
 
     if (!b || nb <= 0 || N <= 0 || N > MAX_ROWS || (int64_t)nb * N > INT32_MAX || heads <= 0 ||
-        hd <= 0 || hd > (1 << 16) || heads > (1 << 14) || rot <= 0 || rot % 2 || rot > hd || npos <= 0 || (layout != CB_ROPE_PAIRS && layout != CB_ROPE_HALVES) ||
+        hd <= 0 || hd > (1 << 16) || heads > (1 << 14) || rot <= 0 || rot % 2 || rot > hd ||
+        npos <= 0 || (layout != CB_ROPE_PAIRS && layout != CB_ROPE_HALVES) ||
         !vec_ok(cs, CB_F32, (int64_t)npos * rot) || (uintptr_t)cs->ptr % 8)
         return cbi_fail(b, CB_EARG, "rope_rotate");
     if (pos ? (pos0 != 0 || !vec_ok(pos, CB_I32, (int64_t)nb * N))
@@ -219,7 +220,7 @@ int cb_cross_attend(cb_backend *b, int nb, int Nq, int Nk, int heads, int kvhead
 
     if (!b || nb <= 0 || Nq <= 0 || Nq > MAX_ROWS || Nk <= 0 || Nk > MAX_ROWS || heads <= 0 ||
         kvheads <= 0 || heads % kvheads || hd <= 0 || hd > 128 || hd % 8 || !(scale > 0.0f) ||
-        !isfinite(scale))
+        scale > 1e38f) /* its product with log2(e) is formed in 32 bits */
         return cbi_fail(b, CB_EARG, "cross_attend");
     if ((klen && !vec_ok(klen, CB_I32, nb)) || (kmask && !vec_ok(kmask, CB_U8, (int64_t)nb * Nk)))
         return cbi_fail(b, CB_EARG, "cross_attend: key lengths or mask");

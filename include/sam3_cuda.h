@@ -480,7 +480,7 @@ int cb_rope_rotate(cb_backend *b, int nb, int N, int heads, int hd, int rot,
 /* O[b, i, h] = softmax over visible j of (scale Q[b, i, h] . K[b, j, h']) V[b,
  * j, h'], h' = h / (heads / kvheads): Q, O [nb, Nq, heads, hd], K, V [nb, Nk,
  * kvheads, hd], one type (F32, BF16, F16), hd a multiple of 8 up to 128, scale
- * > 0. Key j of sequence b is visible when j < klen[b] (CB_I32 [nb], clamped
+ * in (0, 1e38]. Key j of sequence b is visible when j < klen[b] (CB_I32 [nb], clamped
  * to [0, Nk]; NULL: all) and kmask[b * Nk + j] is 0 (CB_U8 [nb, Nk], nonzero
  * marks padding; NULL: none). What masked and absent rows of K and V hold does
  * not enter the result; a row without a visible key, or whose visible scores

@@ -100,6 +100,7 @@ def test_cross_attend_refusals(sb, fake):
     assert call(ks=(32, 0, 16), vs=(32, 0, 16)) == CB_ECUDA  # one encoder for every sequence
     for bad in (dict(nb=0), dict(Nq=0), dict(Nk=0), dict(heads=0), dict(kv=0), dict(kv=3), dict(hd=0), dict(hd=12),
                 dict(hd=136), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
+                dict(scale=3e38),
                 dict(klen=F, nl=1), dict(klen=F, ldt=sb.F32), dict(klen=F + 2), dict(kmask=G, nm=13),
                 dict(kmask=G, mdt=sb.I32), dict(nq=383), dict(nk=447), dict(nv=447), dict(no=383),
                 dict(os_=(64, 0, 16)), dict(os_=(64, 192, 8)), dict(os_=(48, 192, 16)), dict(ks=(-32, 224, 16)),
