@@ -276,7 +276,7 @@ extern "C" int k_rope_table(int npos, int rot, long first, const double *turns, 
         f.t[j] = 0.0;
     const int half = rot / 2, pairs = half % 2 == 0 && !(reinterpret_cast<uintptr_t>(cs) & 15) ? 2 : 1;
     const int rows = 256 / (half / pairs);
-    const long blocks = (npos + rows - 1) / rows, most = (long)device_sms() * 8;
+    const long blocks = ((long)npos + rows - 1) / rows, most = (long)device_sms() * 8;
     const dim3 grid((unsigned)(blocks < most ? blocks : most));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(s);
     return pairs == 2 ? launch_pdl(rope_table_kernel<2>, grid, dim3(256), 0, st, f, half, first, npos, amp,

@@ -463,6 +463,23 @@ def test_cross_attend_infinite_query(be, Nk, dt):
         assert ((out[0][rest].float() - out[1][rest].float()).abs() <= lim).all()
 
 
+def test_rope_table_of_every_position(be):
+    """As many positions as the call takes."""
+    npos = 2 ** 31 - 8
+    buf = torch.empty(npos, 2, device="cuda")
+    be.rope_table(npos, 2, 8, None, be.wrap(buf))
+    be.sync()
+    for at in (0, npos // 2, npos - 300):
+        p = torch.arange(at + 8, at + 308, dtype=torch.float64, device="cuda")
+        want = torch.stack([p.cos(), p.sin()], -1)
+        # the angle in turns off by half a step of 64 bits for the frequency and as much for the product, each
+        # 2^-53 of up to 2^31 / (2 pi) turns, so 2^-52 2^31 in the angle; the rest rounds in 32 bits: the
+        # remainder's angle (pi / 4, three roundings), the polynomial's five steps
+        assert (buf[at:at + 300].double() - want).abs().max() <= 2.0 ** -21 + 8 * 2.0 ** -24
+    del buf
+    torch.cuda.empty_cache()
+
+
 def test_operands_far_into_a_buffer(be, sb):
     """Offsets past 2^31 elements."""
     far = 2 ** 31 + 64
