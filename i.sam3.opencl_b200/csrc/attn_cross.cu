@@ -28,7 +28,7 @@
 // the operands' own precision). fp32: each operand is split into two tf32 parts
 // and x y taken as hi hi + hi lo + lo hi on mma.m16n8k8, off by about 2^-21 of a
 // product; the dropped lo lo is of that size. 201 queries x 5184 keys x 8 heads
-// of 32 columns x 2: 66 us, bound by the splits' dependent arithmetic (issue
+// of 32 columns x 2: 69 us, bound by the splits' dependent arithmetic (issue
 // slots 40 % busy at 16 warps per SM; the products alone need 25 us).
 #include "attn_cross.cuh"
 #include "kernels.h"
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
             const float *kf = reinterpret_cast<const float *>(ks) + (jw + g4) * (TL::PITCH / 4) + t4;
             // As P V below: 16 columns sum from zero and are added outside the
             // matrix unit. Output of 300 queries x 2000 keys, 128 columns: 3.6e-7
-            // off, all columns in one chain 1.2e-6 (201 x 5184 x 32 columns 70 us,
+            // off, all columns in one chain 1.2e-6 (201 x 5184 x 32 columns 69 us,
             // then 67; 8 columns at a time 71).
 #pragma unroll 1
             for (int kk = 0; kk < HDP / 8; kk += 2) {
