@@ -25,7 +25,8 @@
 //
 // bf16 / f16: products on mma.m16n8k16 with fp32 accumulation, P rounded to
 // the operands' type (half a unit in the last place, 2^-8 / 2^-11 of a weight,
-// the operands' own precision). fp32: each operand is split into two tf32 parts
+// the operands' own precision; f16 by 2^-40 of the row's largest at least,
+// kWeightShift). fp32: each operand is split into two tf32 parts
 // and x y taken as hi hi + hi lo + lo hi on mma.m16n8k8, off by about 2^-21 of a
 // product; the dropped lo lo is of that size. 201 queries x 5184 keys x 8 heads
 // of 32 columns x 2: 68.6 us, bound by the splits' dependent arithmetic (issue
@@ -443,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
             // values of any size stays finite (the factor is in O and in the sum).
             // Weights below 2^-126 become 0: 2^-93 of the row's largest at most,
             // which is 2^-33 or more (exp2f, which keeps them, took 1.1 us of 69.7).
-            const float off = F32 ? -(base + a.shift) : -base;
+            const float off = F32 ? -(base + a.shift) : kWeightShift<T> - base;
             mx[h] = mn;
             float add = 0.0f;
 #pragma unroll
@@ -844,7 +845,7 @@ __global__ void __launch_bounds__(kThreads, HDP <= 64 ? 4 : 3) attn_few_kernel(c
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const float base = m[h] == -INFINITY ? 0.0f : -m[h] * a.scale_log2;
+            const float base = m[h] == -INFINITY ? 0.0f : kWeightShift<T> - m[h] * a.scale_log2;
             const uint64_t base2 = f2_make(base, base);
 #pragma unroll
             for (int n = 0; n < NT; n++) {

@@ -42,6 +42,15 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// Weights are formed times 2^kWeightShift, in the products with V and in the
+// sums alike. f16 holds the weights of a row down to 2^-14 of the largest with
+// all its bits and loses those below 2^-25, while the sum of the 32-bit
+// weights keeps them (one key 18 nats above 5184 others: all of these were
+// lost); times 2^15, the most that stays below 65504, they are whole down to
+// 2^-29 and rounded by 2^-40 below. bf16 and 32 bits have the exponents.
+template <typename T>
+constexpr float kWeightShift = __is_same(T, __half) ? 15.0f : 0.0f;
+
 __device__ __forceinline__ float ld_dsmem(uint32_t a)
 {
     float v;

@@ -19,7 +19,7 @@
 //     shared memory: no workspace, one launch.
 // Softmax as in attn_tc.cu: the row's offset is the maximum of its first tile
 // with a visible key, exponentials of later tiles are taken against it, and a
-// tile whose sum reaches 2^13 (or is not a number) is taken again with a raised
+// tile whose sum reaches kOverflowSum (or is not a number) is taken again with a raised
 // offset, then without the polynomial exponential, so that infinities and NaN
 // of visible keys come out as such. Measured: 8 x 5184 queries x 5184 keys x 16
 // heads of 64 columns 1012 us, 870 TFLOP/s (the softmax warps bound it as in
@@ -41,7 +41,13 @@ constexpr int kThreads = 32 * 6;
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxSplit = 8;
 constexpr int kPolyPairsPer8 = 2;  // of 8 pairs, on the FMA pipe (attn_tc.cu)
-constexpr float kOverflowSum = 8192.0f;
+// Weights times 2^kShift (as kWeightShift, attn_cross.cuh). f16: 96 weights of the
+// first tile, 2^9 at most, stay below the limit and each weight below it fits the
+// type: whole down to 2^-23 of the offset's weight and rounded by 2^-34 below.
+template <typename T>
+constexpr float kShift = __is_same(T, __half) ? 9.0f : 0.0f;
+template <typename T>
+constexpr float kOverflowSum = __is_same(T, __half) ? 61440.0f : 8192.0f;
 
 template <int HDP>
 struct Geo {
@@ -417,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                             }
                             m_used = fmaxf(mx0, mx1) * a.scale_log2;
                         }
-                        const float base = m_used == -INFINITY ? 0.0f : -m_used;
+                        const float base = m_used == -INFINITY ? 0.0f : kShift<T> - m_used;
                         const uint64_t negm = f2_make(base, base);
 #pragma unroll
                         for (int e = 0; e < BKV; e += 2) {
@@ -440,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                         float u0, u1, u2, u3;
                         f2_split(t0, u0, u1);
                         f2_split(t1, u2, u3);
-                        over = __any_sync(0xffffffffu, !(((u0 + u1) + (u2 + u3)) < kOverflowSum));
+                        over = __any_sync(0xffffffffu, !(((u0 + u1) + (u2 + u3)) < kOverflowSum<T>));
                         if (!over) {
                             tmem_st32(tS, *reinterpret_cast<const uint32_t(*)[32]>(s));
                             if constexpr (BKV == 96)
@@ -486,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                             lsum0 = mul2(lsum0, f2_make(factor, factor));
                             lsum1 = mul2(lsum1, f2_make(factor, factor));
                         }
-                        const float base = m_used == -INFINITY ? 0.0f : -m_used;
+                        const float base = m_used == -INFINITY ? 0.0f : kShift<T> - m_used;
                         t0 = t1 = 0;
 #pragma unroll 1
                         for (int c = 0; c < NW; c++) {
