@@ -19,12 +19,13 @@
 //     shared memory: no workspace, one launch.
 // Softmax as in attn_tc.cu: the row's offset is the maximum of its first tile
 // with a visible key, exponentials of later tiles are taken against it, and a
-// tile whose sum reaches kOverflowSum (or is not a number) is taken again with a raised
-// offset, then without the polynomial exponential, so that infinities and NaN
-// of visible keys come out as such. Measured: 8 x 5184 queries x 5184 keys x 16
-// heads of 64 columns 1012 us, 870 TFLOP/s (the softmax warps bound it as in
-// attn_tc.cu: 884); 4 x 4096 x 4096 x 16 heads of 128 columns 467 us, 1177
-// TFLOP/s; with a key mask 1164 us, every tile in the rolled path.
+// tile whose sum reaches kOverflowSum (or is not a number) or whose exponents
+// pass the polynomial's range is taken again with a raised offset, without the
+// polynomial, so that infinities and NaN of visible keys come out as such.
+// Measured: 8 x 5184 queries x 5184 keys x 16 heads of 64 columns 1012 us, 870
+// TFLOP/s (the softmax warps bound it as in attn_tc.cu: 884); 4 x 4096 x 4096 x
+// 16 heads of 128 columns 467 us, 1177 TFLOP/s; with a key mask 1164 us, every
+// tile in the rolled path.
 #include "attn_cross.cuh"
 #include "kernels.h"
 #include "pdl.cuh"
@@ -48,6 +49,10 @@ template <typename T>
 constexpr float kShift = __is_same(T, __half) ? 9.0f : 0.0f;
 template <typename T>
 constexpr float kOverflowSum = __is_same(T, __half) ? 61440.0f : 8192.0f;
+// From 2^128 on the polynomial's exponent field wraps and the sum does not show
+// it, so its exponents are looked at themselves: one at or above this sends
+// the tile through again.
+constexpr float kPolyMost = 64.0f;
 
 template <int HDP>
 struct Geo {
@@ -78,7 +83,7 @@ __host__ __device__ constexpr uint32_t idesc(int M, int N, int b_mn_major)
            ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// 2^x of two values as exp2_poly2 (tc_ptx.cuh), but a NaN becomes NaN or huge
+// 2^x of two values below 128 as exp2_poly2 (tc_ptx.cuh), but a NaN becomes NaN or huge
 // instead of 2^-125, so that the tile's sum shows it: the clamp at -125 is a
 // minimum of the bit patterns, which grow with the magnitude of a negative
 // number and are smaller for positive ones and for the NaN of an fma.
@@ -425,14 +430,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                         }
                         const float base = m_used == -INFINITY ? 0.0f : kShift<T> - m_used;
                         const uint64_t negm = f2_make(base, base);
+                        float xm = -INFINITY;  // largest exponent of the polynomial
 #pragma unroll
                         for (int e = 0; e < BKV; e += 2) {
                             const uint64_t x2 = fma2(f2_make(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
                                                      sl2x2, negm);
                             float x0, x1, p0, p1;
                             f2_split(x2, x0, x1);
-                            if (((e >> 1) & 7) >= 8 - kPolyPairsPer8)
+                            if (((e >> 1) & 7) >= 8 - kPolyPairsPer8) {
+                                xm = max3f(xm, x0, x1);
                                 exp2_poly2_nan(x0, x1, p0, p1);
+                            }
                             else {
                                 p0 = ex2_approx(x0);
                                 p1 = ex2_approx(x1);
@@ -446,7 +454,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                         float u0, u1, u2, u3;
                         f2_split(t0, u0, u1);
                         f2_split(t1, u2, u3);
-                        over = __any_sync(0xffffffffu, !(((u0 + u1) + (u2 + u3)) < kOverflowSum<T>));
+                        over = __any_sync(0xffffffffu,
+                                          !(((u0 + u1) + (u2 + u3)) < kOverflowSum<T> && xm < kPolyMost));
                         if (!over) {
                             tmem_st32(tS, *reinterpret_cast<const uint32_t(*)[32]>(s));
                             if constexpr (BKV == 96)

@@ -36,3 +36,38 @@ def test_cross_attend_f16_sink(be, Nq, Nk, h, hd, nats):
     tol = attend_tol(torch.float16, want, A, big, hd, Nk) + 2.0 ** -34 * v.double().abs().sum(1, keepdim=True)
     err = (o.double() - want).abs()
     assert (err <= tol).all(), (float((err / tol).max()), float((err / want.abs()).max()))
+
+
+# ------------------------------------------------------------------ scores far above those of the first keys
+def late_key(g, dt, nb, Nq, Nk, h, hd, at, gap, scale):
+    """Scores of about 0 with a deviation of half a nat, key `at` at `gap` powers of two above for every row."""
+    q, k = randn(g, nb, Nq, h, hd), 0.5 * randn(g, nb, Nk, h, hd)
+    q[..., 0], k[..., 0] = 16.0, 0.0
+    k[:, at] = 0.0
+    k[:, at, :, 0] = gap * math.log(2.0) / (16.0 * scale)
+    return q.to(dt), k.to(dt), (randn(g, nb, Nk, h, hd) + 0.5).to(dt)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("nb,Nq,Nk,h,hd,tile,first", [
+    (2, 300, 480, 2, 64, 96, 3),     # whole tiles of 96 keys
+    (2, 200, 448, 2, 128, 64, 4),    # of 64 keys
+    (1, 1, 448, 64, 128, 64, 4),     # one live row of a tile
+    (1, 1, 320, 64, 80, 64, 2),
+    (1, 300, 1152, 20, 64, 96, 4),   # keys shared by a cluster, the late key in a CTA's second tile
+    (2, 40, 60, 2, 32, 60, 0),       # few keys
+    (1, 70, 200, 3, 32, 64, 2),      # 64-row tiles, few rows
+    (1, 1, 300, 4, 64, 64, 1),
+])
+@pytest.mark.parametrize("masked", [False, True])
+def test_cross_attend_late_score(be, nb, Nq, Nk, h, hd, tile, first, masked, dt):
+    """One key's score 20 to 500 powers of two above all before it, at each kind of column of a tile."""
+    g = gen(hd + Nk)
+    kmask = None
+    if masked:  # a hidden key in the first tile, so that later tiles are whole
+        kmask = torch.zeros(nb, Nk, dtype=torch.uint8, device="cuda")
+        kmask[:, 5] = 1
+    for gap in (20, 100, 130, 150, 200, 260, 300, 400, 500):
+        for col in (16, 28, 29, 31):
+            q, k, v = late_key(g, DT[dt], nb, Nq, Nk, h, hd, first * tile + col, gap, hd ** -0.5)
+            check_attend(be, q, k, v, None, kmask)
