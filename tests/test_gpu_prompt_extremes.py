@@ -71,3 +71,20 @@ def test_cross_attend_late_score(be, nb, Nq, Nk, h, hd, tile, first, masked, dt)
         for col in (16, 28, 29, 31):
             q, k, v = late_key(g, DT[dt], nb, Nq, Nk, h, hd, first * tile + col, gap, hd ** -0.5)
             check_attend(be, q, k, v, None, kmask)
+
+
+@pytest.mark.parametrize("gap", [20, 100, 130, 150, 200, 260, 300, 400, 500])
+@pytest.mark.parametrize("col", [0, 12, 13, 15])
+def test_attention_late_score(be, sb, gap, col):
+    """cb_attention on 16-bit rows, as above. Its output is 32-bit: u(bf16) only of the weights."""
+    nb, N, h, hd = 2, 576, 16, 64
+    E = h * hd
+    q, k, v = late_key(gen(gap + col), torch.bfloat16, nb, N, N, h, hd, 3 * 96 + 16 + col, gap, 0.125)
+    qkv = torch.cat([t.reshape(nb * N, E) for t in (q, k, v)], 1).contiguous()
+    o = torch.empty(nb * N, E, device="cuda")
+    be.attention(be.wrap(qkv), nb, N, E, h, hd, None, 0, 0.125, sb.ATTN_TC, be.wrap(o))
+    be.sync()
+    want, A, big = attend_ref(q.double(), k.double(), v.double(), torch.ones(nb, N, dtype=torch.bool, device="cuda"), 0.125)
+    # its exponentials are within 7.5e-5 (2^-13.7) of the weight, not 2^-20
+    tol = attend_tol(torch.bfloat16, want, A, big, hd, N) + 2.0 ** -13 * A
+    assert ((o.view(nb, N, h, hd).double() - want).abs() <= tol).all()
