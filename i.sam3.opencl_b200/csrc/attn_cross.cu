@@ -435,22 +435,26 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
                 m = max3f(m, sc[n][2 * h], sc[n][2 * h + 1]);
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            // 32 bits: a whole number, so that neither the shift below nor the
-            // corrections round
-            const float mn = fmaxf(mx[h], F32 ? ceilf(m * a.scale_log2) : m * a.scale_log2);
-            const float base = mn == -INFINITY ? 0.0f : mn;
-            const float corr = exp2f(mx[h] - base);
+            // Differences of scores are taken before they are scaled: a product
+            // m scale rounded on its own would leave 2^(its rounding) in every
+            // weight, past 2^30 more than 32 bits hold.
+            const float mn = fmaxf(mx[h], m), base = mn == -INFINITY ? 0.0f : mn;
+            const float corr = exp2f((mx[h] - base) * a.scale_log2);
             // 32 bits: weights below 2^-shift < 1 / (2 Nk), so that their sum with
             // values of any size stays finite (the factor is in O and in the sum).
             // Weights below 2^-126 become 0: 2^-93 of the row's largest at most,
-            // which is 2^-33 or more (exp2f, which keeps them, took 1.1 us of 69.7).
-            const float off = F32 ? -(base + a.shift) : kWeightShift<T> - base;
+            // which is 2^-32 (exp2f, which keeps them, took 1.1 us of 69.7).
+            const float shift = F32 ? -a.shift : kWeightShift<T>;
             mx[h] = mn;
+            const uint64_t neg2 = f2_make(-base, -base), sl2 = f2_make(a.scale_log2, a.scale_log2),
+                           shift2 = f2_make(shift, shift);
             float add = 0.0f;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                sc[n][2 * h] = ex2_approx(fmaf(sc[n][2 * h], a.scale_log2, off));
-                sc[n][2 * h + 1] = ex2_approx(fmaf(sc[n][2 * h + 1], a.scale_log2, off));
+                float x, y;
+                f2_split(fma2(add2(f2_make(sc[n][2 * h], sc[n][2 * h + 1]), neg2), sl2, shift2), x, y);
+                sc[n][2 * h] = ex2_approx(x);
+                sc[n][2 * h + 1] = ex2_approx(y);
                 add += sc[n][2 * h] + sc[n][2 * h + 1];
             }
             sum[h] = fmaf(sum[h], corr, add);
@@ -621,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
 #pragma unroll
             for (int p = 0; p < WK; p++) {
                 const bool none = ml[p].x == -INFINITY;
-                const float w = none ? 0.0f : exp2f(ml[p].x - m);
+                const float w = none ? 0.0f : exp2f((ml[p].x - m) * a.scale_log2);
                 const float4 x = *reinterpret_cast<const float4 *>(mine + (p * BM + r) * PT::PR + c);
                 l += none ? (ml[p].y == ml[p].y ? 0.0f : ml[p].y) : ml[p].y * w;
                 v[0] = fmaf(x.x, w, v[0]);
@@ -662,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
     }
     cluster_sync_all();
     const int live = rows > rank ? (rows - 1 - rank) / a.cs + 1 : 0;
-    PT::template merge<kThreads>(part, a.cs, rl, live, [&](int i, int c, float x, float y, float z, float w) {
+    PT::template merge<kThreads>(part, a.cs, rl, live, a.scale_log2, [&](int i, int c, float x, float y, float z, float w) {
         const float v[4] = {x, y, z, w};
         store(i * a.cs + rank, c, v);
     });
@@ -788,7 +792,7 @@ __global__ void __launch_bounds__(kThreads, HDP <= 64 ? 4 : 3) attn_few_kernel(c
             start[n][e] = vis[n * 8 + t4 * 2 + e] ? 0.0f : -INFINITY;
     const uint32_t ka = smem_addr(ks), va = smem_addr(vs);
     constexpr uint32_t kOnes = __is_same(T, __half) ? 0x3c003c00u : 0x3f803f80u;
-    const uint64_t sl2x2 = f2_make(a.scale_log2, a.scale_log2);
+    const uint64_t sl2x2 = f2_make(a.scale_log2, a.scale_log2), shift2 = f2_make(kWeightShift<T>, kWeightShift<T>);
     auto key_frag = [&](int kk, int n, uint32_t (&f)[4]) {
         ldsm4(ka + TL::at(n * 8 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)), f);
     };
@@ -845,12 +849,12 @@ __global__ void __launch_bounds__(kThreads, HDP <= 64 ? 4 : 3) attn_few_kernel(c
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const float base = m[h] == -INFINITY ? 0.0f : kWeightShift<T> - m[h] * a.scale_log2;
+            const float base = m[h] == -INFINITY ? 0.0f : -m[h];
             const uint64_t base2 = f2_make(base, base);
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 float x, y;
-                f2_split(fma2(f2_make(sc[n][2 * h], sc[n][2 * h + 1]), sl2x2, base2), x, y);
+                f2_split(fma2(add2(f2_make(sc[n][2 * h], sc[n][2 * h + 1]), base2), sl2x2, shift2), x, y);
                 sc[n][2 * h] = ex2_approx(x);
                 sc[n][2 * h + 1] = ex2_approx(y);
             }

@@ -89,16 +89,17 @@ __device__ __forceinline__ void st_dsmem2(uint32_t a, float x, float y)
 // to CTA r % cs; every part of it is pushed into that CTA's shared memory (remote
 // stores, nothing waits for them; pulling cost a round trip per row or
 // element: 64 queries x 384 keys 15 us against 7), as part[(p * rl + r / cs) * PR]
-// with HDP columns of output, then its maximum and sum. After a cluster
-// barrier each CTA merges its own rows: O = sum_p O_p 2^(max_p - max) / sum_p
-// l_p 2^(max_p - max). A part without a visible key has maximum -inf and
+// with HDP columns of output, then its largest score (not scaled) and sum. After
+// a cluster barrier each CTA merges its own rows: O = sum_p O_p w_p / sum_p l_p
+// w_p, w_p = 2^((max_p - max) scale_log2). A part without a visible key has maximum -inf and
 // counts nothing, unless its sum is NaN.
 template <int HDP>
 struct Parts {
     static constexpr int PR = HDP + 4;
     // rl: rows a CTA holds of each part; live: rows of its own that exist
     template <int THREADS, typename Store>
-    static __device__ __forceinline__ void merge(float *part, int np, int rl, int live, const Store &store)
+    static __device__ __forceinline__ void merge(float *part, int np, int rl, int live, float scale_log2,
+                                                 const Store &store)
     {
         // weights of a row's parts and 1 / sum, a thread per row
         constexpr int kMost = 16;  // CTAs of a cluster
@@ -115,7 +116,7 @@ struct Parts {
             for (int p = 0; p < kMost; p++)
                 if (p < np) {
                     const bool none = ml[p].x == -INFINITY;
-                    const float w = none ? 0.0f : exp2f(ml[p].x - m);
+                    const float w = none ? 0.0f : exp2f((ml[p].x - m) * scale_log2);
                     l += none ? (ml[p].y == ml[p].y ? 0.0f : ml[p].y) : ml[p].y * w;
                     part[(p * rl + i) * PR + HDP] = w;
                 }

@@ -53,6 +53,11 @@ constexpr float kOverflowSum = __is_same(T, __half) ? 61440.0f : 8192.0f;
 // it, so its exponents are looked at themselves: one at or above this sends
 // the tile through again.
 constexpr float kPolyMost = 64.0f;
+// An offset is a score; its product with the scale is rounded, which leaves a
+// power of two of that rounding in every weight of the row. Products below this
+// leave 2^-12 at most, less than the weights' own rounding; beyond it a tile
+// goes through again, where differences are taken before they are scaled.
+constexpr float kFarOffset = 4096.0f;
 
 template <int HDP>
 struct Geo {
@@ -347,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             const bool rows_live = it.qt * BQ + quarter * 32 < a.Nq;
             const int q = it.qt * BQ + r;
             const uint8_t *mask = MASK ? a.kmask + (long)it.seq * a.Nk : nullptr;
-            float m_used = -INFINITY;
+            float m_used = -INFINITY;  // offset, a score before scaling
             uint64_t lsum0 = 0, lsum1 = 0;
             uint8_t ahead[NW];  // mask bytes of the next tile, a key per lane
             auto look = [&](int j) {
@@ -426,10 +431,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                                 mx0 = max3f(mx0, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
                                 mx1 = max3f(mx1, __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
                             }
-                            m_used = fmaxf(mx0, mx1) * a.scale_log2;
+                            m_used = fmaxf(mx0, mx1);
                         }
-                        const float base = m_used == -INFINITY ? 0.0f : kShift<T> - m_used;
-                        const uint64_t negm = f2_make(base, base);
+                        const float top = m_used == -INFINITY ? 0.0f : m_used * a.scale_log2;
+                        const uint64_t negm = f2_make(kShift<T> - top, kShift<T> - top);
                         float xm = -INFINITY;  // largest exponent of the polynomial
 #pragma unroll
                         for (int e = 0; e < BKV; e += 2) {
@@ -455,7 +460,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                         f2_split(t0, u0, u1);
                         f2_split(t1, u2, u3);
                         over = __any_sync(0xffffffffu,
-                                          !(((u0 + u1) + (u2 + u3)) < kOverflowSum<T> && xm < kPolyMost));
+                                          !(((u0 + u1) + (u2 + u3)) < kOverflowSum<T> && xm < kPolyMost &&
+                                            fabsf(top) < kFarOffset));
                         if (!over) {
                             tmem_st32(tS, *reinterpret_cast<const uint32_t(*)[32]>(s));
                             if constexpr (BKV == 96)
@@ -491,17 +497,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                             for (int e = 0; e < 32; e += 2)
                                 mx = max3f(mx, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
                         }
-                        const float m_tile = mx * a.scale_log2;
                         if (m_used == -INFINITY)
-                            m_used = m_tile;
-                        else if (m_tile > m_used) {
+                            m_used = mx;
+                        else if (mx > m_used) {
                             resc = true;
-                            factor = ex2_approx(m_used - m_tile);
-                            m_used = m_tile;
+                            factor = ex2_approx((m_used - mx) * a.scale_log2);
+                            m_used = mx;
                             lsum0 = mul2(lsum0, f2_make(factor, factor));
                             lsum1 = mul2(lsum1, f2_make(factor, factor));
                         }
-                        const float base = m_used == -INFINITY ? 0.0f : kShift<T> - m_used;
+                        const float base = m_used == -INFINITY ? 0.0f : -m_used;
+                        const uint64_t base2 = f2_make(base, base), shift2 = f2_make(kShift<T>, kShift<T>);
                         t0 = t1 = 0;
 #pragma unroll 1
                         for (int c = 0; c < NW; c++) {
@@ -509,8 +515,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                             chunk(c, s);
 #pragma unroll
                             for (int e = 0; e < 32; e += 2) {
-                                const float p0 = ex2_approx(fmaf(__uint_as_float(s[e]), a.scale_log2, base));
-                                const float p1 = ex2_approx(fmaf(__uint_as_float(s[e + 1]), a.scale_log2, base));
+                                float x0, x1;
+                                f2_split(fma2(add2(f2_make(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), base2),
+                                              sl2x2, shift2),
+                                         x0, x1);
+                                const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
                                 t0 = add2(t0, f2_make(p0, p1));
                                 p[e >> 1] = pack2<T>(p0, p1);
                             }
@@ -646,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         cluster_sync_all();
         const int mine = live > rank ? (live - 1 - rank) / a.cs + 1 : 0;
         T *ob = reinterpret_cast<T *>(a.o) + it.seq * a.os0 + it.head * a.os1;
-        PT::template merge<kThreads>(part, a.cs, rl, mine, [&](int i, int c, float x, float y, float z, float w) {
+        PT::template merge<kThreads>(part, a.cs, rl, mine, a.scale_log2, [&](int i, int c, float x, float y, float z, float w) {
             if (c >= a.hd)
                 return;
             T *dst = ob + (long)(it.qt * BQ + i * a.cs + rank) * a.old + c;

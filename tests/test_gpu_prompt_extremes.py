@@ -88,3 +88,72 @@ def test_attention_late_score(be, sb, gap, col):
     # its exponentials are within 7.5e-5 (2^-13.7) of the weight, not 2^-20
     tol = attend_tol(torch.bfloat16, want, A, big, hd, N) + 2.0 ** -13 * A
     assert ((o.view(nb, N, h, hd).double() - want).abs() <= tol).all()
+
+
+# ------------------------------------------------------------------ scores of any size
+FORMS = [(2, 40, 60, 2, 32),      # few keys
+         (1, 1, 300, 4, 64),      # one row, the keys dealt to four warps
+         (1, 1, 5000, 2, 128),    # and to a cluster
+         (1, 70, 200, 3, 32),     # 64-row tiles
+         (1, 40, 3000, 1, 32),    # shared by a cluster
+         (2, 300, 480, 2, 64),    # tcgen05
+         (2, 200, 448, 2, 128),
+         (1, 300, 1152, 20, 64)]  # tcgen05, keys shared by a cluster
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("nb,Nq,Nk,h,hd", FORMS)
+def test_cross_attend_huge_scores(be, nb, Nq, Nk, h, hd, dt):
+    """Whole-number scores times scales up to 1e38: the largest score has all the weight, so a row is that key's value up
+    to the value's own rounding (16 bits: none but the type's; 32 bits: its two parts, 2^-21, and the sum's 2^-22)."""
+    g = gen(Nk + hd)
+    t = DT[dt]
+    q = torch.zeros(nb, Nq, h, hd, device="cuda")
+    q[..., 0] = 2.0 ** torch.randint(0, 3, (nb, Nq, h), device="cuda", generator=g) * \
+        (1 - 2 * torch.randint(0, 2, (nb, Nq, h), device="cuda", generator=g))
+    k = randn(g, nb, Nk, h, hd)
+    k[..., 0] = torch.randint(-50, 51, (nb, Nk, h), device="cuda", generator=g).float()
+    v = (randn(g, nb, Nk, h, hd) + 0.5).to(t)
+    for most, least in ((Nk - 1, 3), (3, Nk // 2), (Nk // 2 + 5, Nk - 3)):
+        ki = k.clone()
+        ki[:, most, :, 0], ki[:, least, :, 0] = 113.0, -107.0
+        want = torch.where((q[..., :1] > 0), v[:, most][:, None].float(), v[:, least][:, None].float())
+        for scale in (100.0, 1e6, 1e8, 1e10, 1e20, 1e30, 1e38):
+            o = torch.full_like(v[:, :1].expand(nb, Nq, h, hd), 5.0).contiguous()
+            qd, kd = q.to(t), ki.to(t)
+            be.cross_attend(nb, Nq, Nk, h, h, hd, *(op(be, x, 0, h * hd, x.shape[1] * h * hd, hd) for x in (qd, kd, v, o)),
+                            None, None, scale)
+            be.sync()
+            tol = (2.0 ** -20 if dt == "f32" else u(t)) * want.abs()
+            assert ((o.float() - want).abs() <= tol).all(), (scale, most)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("nb,Nq,Nk,h,hd", FORMS)
+@pytest.mark.parametrize("common", [2.0 ** 11, 2.0 ** 14, 2.0 ** 15])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_cross_attend_large_common_score(be, nb, Nq, Nk, h, hd, common, sign, dt):
+    """All scores near one large number, which must drop out. They are sums of whole numbers, exact in 32 bits; the
+    offset may be rounded twice at 2^-24 of up to 2^12 powers of two (2^-12 in a weight's exponent, ln 2 of it in the
+    weight), larger ones are not formed before the difference is taken."""
+    g = gen(Nk + hd + int(common))
+    t = DT[dt]
+    q, k = torch.zeros(nb, Nq, h, hd, device="cuda"), torch.zeros(nb, Nk, h, hd, device="cuda")
+    q[..., 0], q[..., 1] = 64.0, 1.0
+    k[..., 0] = sign * common / 64.0
+    k[..., 1] = torch.randint(0, 21, (nb, Nk, h), device="cuda", generator=g).float()
+    v = randn(g, nb, Nk, h, hd)
+    for scale in (0.25, 1.0, 64.0):
+        qd, kd, vd = q.to(t), k.to(t), v.to(t)
+        o = torch.full_like(qd, 5.0)
+        be.cross_attend(nb, Nq, Nk, h, h, hd, *(op(be, x, 0, h * hd, x.shape[1] * h * hd, hd) for x in (qd, kd, vd, o)),
+                        None, None, scale)
+        be.sync()
+        see = torch.ones(nb, Nk, dtype=torch.bool, device="cuda")
+        want, A, _ = attend_ref(qd.double(), kd.double(), vd.double(), see, scale)
+        # the differences alone: at most 20 scale each, rounded
+        tol = attend_tol(t, want, A, 20.0 * scale, hd, Nk)
+        top = min(2.0 ** 12, (common + 20.0) * scale * 1.4427)
+        tol = tol + 4 * 2.0 ** -24 * top * A + (2.0 ** -34 * vd.double().abs().sum(1, keepdim=True) if dt == "f16" else 0.0)
+        err = (o.double() - want).abs()
+        assert (err <= tol).all(), (scale, float((err / tol).max()))
