@@ -28,7 +28,10 @@
 // the operands' own precision; f16 by 2^-40 of the row's largest at least,
 // kWeightShift). fp32: each operand is split into two tf32 parts
 // and x y taken as hi hi + hi lo + lo hi on mma.m16n8k8, off by about 2^-21 of a
-// product; the dropped lo lo is of that size. 201 queries x 5184 keys x 8 heads
+// product; the dropped lo lo is of that size. Sums that may have overflowed, and
+// values so small that their second parts fall below the smallest numbers, are
+// seen at the end of a CTA's keys and taken again with V times a power of two
+// (Retake). 201 queries x 5184 keys x 8 heads
 // of 32 columns x 2: 68.6 us, bound by the splits' dependent arithmetic (issue
 // slots 40 % busy at 16 warps per SM; the products alone need 25 us).
 #include "attn_cross.cuh"
@@ -180,6 +183,18 @@ __device__ __forceinline__ long query_of(const XaArgs &a, long gr)
     return gr < 0x7fffffffL ? (long)quot((uint32_t)gr, a.dg) : gr / a.g;
 }
 
+// 32 bits: unnormalised outputs from kMostOut on, or none of kLeastOut, make a
+// CTA take its keys again with the values times 2^k that puts the largest of them
+// near 2^kTargetExp: every sum of up to 2^30 of them stays finite, parts
+// of numbers down to the smallest are normal ones. 2^k is 2^64 at most, so that
+// weights times 2^-k are normal too. (A factor of 1 / (2 Nk) in all weights,
+// which needs no second pass, took those bits from values below 2^-100.)
+struct Retake {
+    static constexpr float kMostOut = 2.6584560e36f;    // 2^121: parts of 4 warps and 16 CTAs add up
+    static constexpr float kLeastOut = 8.2718061e-25f;  // 2^-80
+    static constexpr int kTargetExp = 64, kSmallExp = -70;
+};
+
 template <typename T, int HDP, int WM>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
     attn_cross_kernel(const __grid_constant__ XaArgs a)
@@ -293,244 +308,306 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
                 see[p] = __ldg(mask + j) == 0;
         }
     };
-    bool see[PER];
-#pragma unroll 1
-    for (int s = 0; s < STAGES - 1; s++) {
-        look(s, see);
-        if (s < nsteps)
-            load(s, see);
-        cp_commit();
-    }
-    look(STAGES - 1, see);
-
-    float o[DT][4];
-#pragma unroll
-    for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            o[d][e] = 0.0f;
-    const bool busy = r0 + wm * 16 < r1;
-    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-    uint32_t qf[F32 ? 1 : HDP / 16][4];
-
-    for (int s = 0; s < nsteps; s++) {
-        cp_wait<STAGES - 2>();
+    // 32 bits, rare (Retake): exponent of the largest finite value of this CTA's
+    // visible keys, below -149 for none
+    [[maybe_unused]] auto largest_value = [&]() {
+        uint32_t big = 0;
+        const long j0 = (long)s0 * BK, n = (min((long)(s0 + nsteps) * BK, (long)len) - j0) * a.hd;
+        for (long i = t; i < n; i += kThreads) {
+            const long j = j0 + i / a.hd;
+            if (mask && __ldg(mask + j))
+                continue;
+            const uint32_t u = __float_as_uint((float)vb[j * a.vld + i % a.hd]) & 0x7fffffffu;
+            if (u < 0x7f800000u)
+                big = max(big, u);
+        }
+        __shared__ uint32_t warps[kThreads / 32];
+        big = __reduce_max_sync(0xffffffffu, big);
+        if (lane == 0)
+            warps[warp] = big;
         __syncthreads();
-        if (s + STAGES - 1 < nsteps)
-            load(s + STAGES - 1, see);
-        cp_commit();
-        look(s + STAGES, see);
-        if (!busy)
-            continue;  // only loads: none of the warp's rows exist
-        const int st = s % STAGES;
-        const uint8_t *ks = ring + st * CF::STAGE_BYTES, *vs = ks + CF::KV_BYTES;
-        const uint32_t ka = smem_addr(ks), va = smem_addr(vs);
-        const int jw = wk * KW;  // this warp's first key of the step
-
-        float sc[NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int w = 0; w < kThreads / 32; w++)
+            big = max(big, warps[w]);
+        return big ? ilogbf(__uint_as_float(big)) : -1000;
+    };
+    // a thread's own chunks of the values of stage st, before others read them
+    [[maybe_unused]] auto scale_values = [&](int st, int ex) {
+        const float f = __int_as_float((127 + ex) << 23);
+#pragma unroll 1
+        for (int i = t; i < BK * CPR; i += kThreads) {
+            float4 *x = reinterpret_cast<float4 *>(ring + st * CF::STAGE_BYTES + CF::KV_BYTES + TL::at(i / CPR, i % CPR));
+            const float4 v = *x;
+            *x = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+        }
+    };
+    const bool busy = r0 + wm * 16 < r1;
+    float o[DT][4], mx[2], sum[2];
+    uint32_t qf[F32 ? 1 : HDP / 16][4];
+    [[maybe_unused]] int vexp = 0;  // V is taken times 2^vexp (32 bits)
+
+    for (;;) {
+        bool see[PER];
+#pragma unroll 1
+        for (int s = 0; s < STAGES - 1; s++) {
+            look(s, see);
+            if (s < nsteps)
+                load(s, see);
+            cp_commit();
+        }
+        look(STAGES - 1, see);
+#pragma unroll
+        for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                sc[n][e] = 0.0f;
-        if constexpr (!F32) {
-            if (s == 0) {
-#pragma unroll
-                for (int kk = 0; kk < HDP / 16; kk++)
-                    ldsm4(smem_addr(smem) + TL::at(wm * 16 + (lane & 15), kk * 2 + (lane >> 4)), qf[kk]);
+                o[d][e] = 0.0f;
+        mx[0] = mx[1] = -INFINITY;
+        sum[0] = sum[1] = 0.0f;
+
+        for (int s = 0; s < nsteps; s++) {
+            cp_wait<STAGES - 2>();
+            if constexpr (F32) {
+                if (vexp != 0)
+                    scale_values(s % STAGES, vexp);
             }
-#pragma unroll
-            for (int kk = 0; kk < HDP / 16; kk++) {
-#pragma unroll
-                for (int n = 0; n < NT; n += 2) {
-                    // keys n*8 .. n*8+15, columns kk*16 .. kk*16+15
-                    uint32_t kf[4];
-                    ldsm4(ka + TL::at(jw + n * 8 + (lane & 7) + ((lane >> 4) << 3),
-                                      kk * 2 + ((lane >> 3) & 1)),
-                          kf);
-                    mma16<T>(sc[n], qf[kk], kf[0], kf[1]);
-                    mma16<T>(sc[n + 1], qf[kk], kf[2], kf[3]);
-                }
-            }
-        }
-        else {
-            const float *qs = reinterpret_cast<const float *>(smem) + (wm * 16 + g4) * (TL::PITCH / 4) + t4;
-            const float *kf = reinterpret_cast<const float *>(ks) + (jw + g4) * (TL::PITCH / 4) + t4;
-            // As P V below: 16 columns sum from zero and are added outside the
-            // matrix unit. Output of 300 queries x 2000 keys, 128 columns: 3.6e-7
-            // off, all columns in one chain 1.2e-6 (201 x 5184 x 32 columns 69 us,
-            // then 67; 8 columns at a time 71).
-#pragma unroll 1
-            for (int kk = 0; kk < HDP / 8; kk += 2) {
-                uint32_t ah[2][4], al[2][4];
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        split_near<true>(qs[(e & 1) * 8 * (TL::PITCH / 4) + (kk + u) * 8 + (e >> 1) * 4], ah[u][e],
-                                         al[u][e]);
-                // four tiles side by side: a product waits for the one four before it
-                constexpr int NB = NT < 4 ? NT : 4;
-#pragma unroll
-                for (int n0 = 0; n0 < NT; n0 += NB) {
-                    float part[NB][4];
-#pragma unroll
-                    for (int n = 0; n < NB; n++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            part[n][e] = 0.0f;
-#pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        uint32_t bh[NB][2], bl[NB][2];
-#pragma unroll
-                        for (int n = 0; n < NB; n++)
-#pragma unroll
-                            for (int e = 0; e < 2; e++)
-                                split_cut(kf[(n0 + n) * 8 * (TL::PITCH / 4) + (kk + u) * 8 + 4 * e], bh[n][e],
-                                          bl[n][e]);
-#pragma unroll
-                        for (int n = 0; n < NB; n++)
-                            mma8(part[n], al[u], bh[n][0], bh[n][1]);
-#pragma unroll
-                        for (int n = 0; n < NB; n++)
-                            mma8(part[n], ah[u], bl[n][0], bl[n][1]);
-#pragma unroll
-                        for (int n = 0; n < NB; n++)
-                            mma8(part[n], ah[u], bh[n][0], bh[n][1]);
-                    }
-#pragma unroll
-                    for (int n = 0; n < NB; n++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            sc[n0 + n][e] += part[n][e];
-                }
-            }
-        }
-        // ---- online softmax of rows g4 and g4 + 8
-        const int j0 = (s0 + s) * BK + jw;
-        if (mask) {
-            const uint8_t *vw = vis + st * BK + jw;
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const uint16_t two = *reinterpret_cast<const uint16_t *>(vw + n * 8 + t4 * 2);
-                if (!(two & 0xff))
-                    sc[n][0] = sc[n][2] = -INFINITY;
-                if (!(two >> 8))
-                    sc[n][1] = sc[n][3] = -INFINITY;
-            }
-        }
-        else if (j0 + KW > len) {
+            __syncthreads();
+            if (s + STAGES - 1 < nsteps)
+                load(s + STAGES - 1, see);
+            cp_commit();
+            look(s + STAGES, see);
+            if (!busy)
+                continue;  // only loads: none of the warp's rows exist
+            const int st = s % STAGES;
+            const uint8_t *ks = ring + st * CF::STAGE_BYTES, *vs = ks + CF::KV_BYTES;
+            const uint32_t ka = smem_addr(ks), va = smem_addr(vs);
+            const int jw = wk * KW;  // this warp's first key of the step
+
+            float sc[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    if (j0 + n * 8 + t4 * 2 + (e & 1) >= len)
-                        sc[n][e] = -INFINITY;
-        }
+                    sc[n][e] = 0.0f;
+            if constexpr (!F32) {
+                if (s == 0) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float m = -INFINITY;
+                    for (int kk = 0; kk < HDP / 16; kk++)
+                        ldsm4(smem_addr(smem) + TL::at(wm * 16 + (lane & 15), kk * 2 + (lane >> 4)), qf[kk]);
+                }
 #pragma unroll
-            for (int n = 0; n < NT; n++)
-                m = max3f(m, sc[n][2 * h], sc[n][2 * h + 1]);
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            // Differences of scores are taken before they are scaled: a product
-            // m scale rounded on its own would leave 2^(its rounding) in every
-            // weight, past 2^30 more than 32 bits hold.
-            const float mn = fmaxf(mx[h], m), base = mn == -INFINITY ? 0.0f : mn;
-            const float corr = exp2f((mx[h] - base) * a.scale_log2);
-            // 32 bits: weights below 2^-shift < 1 / (2 Nk), so that their sum with
-            // values of any size stays finite (the factor is in O and in the sum).
-            // Weights below 2^-126 become 0: 2^-93 of the row's largest at most,
-            // which is 2^-32 (exp2f, which keeps them, took 1.1 us of 69.7).
-            const float shift = F32 ? -a.shift : kWeightShift<T>;
-            mx[h] = mn;
-            const uint64_t neg2 = f2_make(-base, -base), sl2 = f2_make(a.scale_log2, a.scale_log2),
-                           shift2 = f2_make(shift, shift);
-            float add = 0.0f;
+                for (int kk = 0; kk < HDP / 16; kk++) {
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                float x, y;
-                f2_split(fma2(add2(f2_make(sc[n][2 * h], sc[n][2 * h + 1]), neg2), sl2, shift2), x, y);
-                sc[n][2 * h] = ex2_approx(x);
-                sc[n][2 * h + 1] = ex2_approx(y);
-                add += sc[n][2 * h] + sc[n][2 * h + 1];
-            }
-            sum[h] = fmaf(sum[h], corr, add);
-#pragma unroll
-            for (int d = 0; d < DT; d++) {
-                o[d][2 * h] *= corr;
-                o[d][2 * h + 1] *= corr;
-            }
-        }
-        // ---- O += P V
-        if constexpr (!F32) {
-#pragma unroll
-            for (int n = 0; n < NT; n += 2) {
-                const uint32_t pf[4] = {pack2<T>(sc[n][0], sc[n][1]), pack2<T>(sc[n][2], sc[n][3]),
-                                        pack2<T>(sc[n + 1][0], sc[n + 1][1]),
-                                        pack2<T>(sc[n + 1][2], sc[n + 1][3])};
-#pragma unroll
-                for (int d = 0; d < DT; d += 2) {
-                    uint32_t vf[4];
-                    ldsm4t(va + TL::at(jw + n * 8 + (lane & 15), d + (lane >> 4)), vf);
-                    mma16<T>(o[d], pf, vf[0], vf[1]);
-                    mma16<T>(o[d + 1], pf, vf[2], vf[3]);
+                    for (int n = 0; n < NT; n += 2) {
+                        // keys n*8 .. n*8+15, columns kk*16 .. kk*16+15
+                        uint32_t kf[4];
+                        ldsm4(ka + TL::at(jw + n * 8 + (lane & 7) + ((lane >> 4) << 3),
+                                          kk * 2 + ((lane >> 3) & 1)),
+                              kf);
+                        mma16<T>(sc[n], qf[kk], kf[0], kf[1]);
+                        mma16<T>(sc[n + 1], qf[kk], kf[2], kf[3]);
+                    }
                 }
             }
-        }
-        else {
-            // The product's k index runs over keys in any order as long as both
-            // operands agree: index t4 is key 2 t4, t4 + 4 is key 2 t4 + 1, as
-            // the scores already lie.
-            // Each step's sum starts from zero and is added to O outside the
-            // matrix unit, whose own additions truncate (5184 keys in one chain
-            // were 8e-6 off).
-            const float *vf = reinterpret_cast<const float *>(vs) + (jw + 2 * t4) * (TL::PITCH / 4) + g4;
-            uint32_t ph[NT][4], pl[NT][4];
+            else {
+                const float *qs = reinterpret_cast<const float *>(smem) + (wm * 16 + g4) * (TL::PITCH / 4) + t4;
+                const float *kf = reinterpret_cast<const float *>(ks) + (jw + g4) * (TL::PITCH / 4) + t4;
+                // As P V below: 16 columns sum from zero and are added outside the
+                // matrix unit. Output of 300 queries x 2000 keys, 128 columns: 2.8e-7
+                // off, all columns in one chain 1.2e-6 (201 x 5184 x 32 columns 69 us,
+                // then 67; 8 columns at a time 71).
+#pragma unroll 1
+                for (int kk = 0; kk < HDP / 8; kk += 2) {
+                    uint32_t ah[2][4], al[2][4];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                split_near<false>(sc[n][0], ph[n][0], pl[n][0]);
-                split_near<false>(sc[n][2], ph[n][1], pl[n][1]);
-                split_near<false>(sc[n][1], ph[n][2], pl[n][2]);
-                split_near<false>(sc[n][3], ph[n][3], pl[n][3]);
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            split_near<true>(qs[(e & 1) * 8 * (TL::PITCH / 4) + (kk + u) * 8 + (e >> 1) * 4], ah[u][e],
+                                             al[u][e]);
+                    // four tiles side by side: a product waits for the one four before it
+                    constexpr int NB = NT < 4 ? NT : 4;
+#pragma unroll
+                    for (int n0 = 0; n0 < NT; n0 += NB) {
+                        float part[NB][4];
+#pragma unroll
+                        for (int n = 0; n < NB; n++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                part[n][e] = 0.0f;
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            uint32_t bh[NB][2], bl[NB][2];
+#pragma unroll
+                            for (int n = 0; n < NB; n++)
+#pragma unroll
+                                for (int e = 0; e < 2; e++)
+                                    split_cut(kf[(n0 + n) * 8 * (TL::PITCH / 4) + (kk + u) * 8 + 4 * e], bh[n][e],
+                                              bl[n][e]);
+#pragma unroll
+                            for (int n = 0; n < NB; n++)
+                                mma8(part[n], al[u], bh[n][0], bh[n][1]);
+#pragma unroll
+                            for (int n = 0; n < NB; n++)
+                                mma8(part[n], ah[u], bl[n][0], bl[n][1]);
+#pragma unroll
+                            for (int n = 0; n < NB; n++)
+                                mma8(part[n], ah[u], bh[n][0], bh[n][1]);
+                        }
+#pragma unroll
+                        for (int n = 0; n < NB; n++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                sc[n0 + n][e] += part[n][e];
+                    }
+                }
             }
-#pragma unroll
-            for (int d0 = 0; d0 < DT; d0 += 4) {
-                float hi[4][4], lo[4][4];
-#pragma unroll
-                for (int d = 0; d < 4; d++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        hi[d][e] = lo[d][e] = 0.0f;
+            // ---- online softmax of rows g4 and g4 + 8
+            const int j0 = (s0 + s) * BK + jw;
+            if (mask) {
+                const uint8_t *vw = vis + st * BK + jw;
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    uint32_t bh[4][2], bl[4][2];
-#pragma unroll
-                    for (int d = 0; d < 4; d++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++)
-                            split_cut(vf[(n * 8 + e) * (TL::PITCH / 4) + (d0 + d) * 8], bh[d][e], bl[d][e]);
-#pragma unroll
-                    for (int d = 0; d < 4; d++)
-                        mma8(lo[d], pl[n], bh[d][0], bh[d][1]);
-#pragma unroll
-                    for (int d = 0; d < 4; d++)
-                        mma8(hi[d], ph[n], bh[d][0], bh[d][1]);
-#pragma unroll
-                    for (int d = 0; d < 4; d++)
-                        mma8(lo[d], ph[n], bl[d][0], bl[d][1]);
+                    const uint16_t two = *reinterpret_cast<const uint16_t *>(vw + n * 8 + t4 * 2);
+                    if (!(two & 0xff))
+                        sc[n][0] = sc[n][2] = -INFINITY;
+                    if (!(two >> 8))
+                        sc[n][1] = sc[n][3] = -INFINITY;
                 }
+            }
+            else if (j0 + KW > len) {
 #pragma unroll
-                for (int d = 0; d < 4; d++)
+                for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        o[d0 + d][e] += hi[d][e] + lo[d][e];
+                        if (j0 + n * 8 + t4 * 2 + (e & 1) >= len)
+                            sc[n][e] = -INFINITY;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float m = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+                    m = max3f(m, sc[n][2 * h], sc[n][2 * h + 1]);
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                // Differences of scores are taken before they are scaled: a product
+                // m scale rounded on its own would leave 2^(its rounding) in every
+                // weight, past 2^30 more than 32 bits hold.
+                const float mn = fmaxf(mx[h], m), base = mn == -INFINITY ? 0.0f : mn;
+                const float corr = exp2f((mx[h] - base) * a.scale_log2);
+                mx[h] = mn;
+                const uint64_t neg2 = f2_make(-base, -base), sl2 = f2_make(a.scale_log2, a.scale_log2),
+                               shift2 = f2_make(kWeightShift<T>, kWeightShift<T>);
+                float add = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    float x, y;
+                    f2_split(fma2(add2(f2_make(sc[n][2 * h], sc[n][2 * h + 1]), neg2), sl2, shift2), x, y);
+                    sc[n][2 * h] = ex2_approx(x);
+                    sc[n][2 * h + 1] = ex2_approx(y);
+                    add += sc[n][2 * h] + sc[n][2 * h + 1];
+                }
+                sum[h] = fmaf(sum[h], corr, add);
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    o[d][2 * h] *= corr;
+                    o[d][2 * h + 1] *= corr;
+                }
+            }
+            // ---- O += P V
+            if constexpr (!F32) {
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+                    const uint32_t pf[4] = {pack2<T>(sc[n][0], sc[n][1]), pack2<T>(sc[n][2], sc[n][3]),
+                                            pack2<T>(sc[n + 1][0], sc[n + 1][1]),
+                                            pack2<T>(sc[n + 1][2], sc[n + 1][3])};
+#pragma unroll
+                    for (int d = 0; d < DT; d += 2) {
+                        uint32_t vf[4];
+                        ldsm4t(va + TL::at(jw + n * 8 + (lane & 15), d + (lane >> 4)), vf);
+                        mma16<T>(o[d], pf, vf[0], vf[1]);
+                        mma16<T>(o[d + 1], pf, vf[2], vf[3]);
+                    }
+                }
+            }
+            else {
+                // The product's k index runs over keys in any order as long as both
+                // operands agree: index t4 is key 2 t4, t4 + 4 is key 2 t4 + 1, as
+                // the scores already lie.
+                // Each step's sum starts from zero and is added to O outside the
+                // matrix unit, whose own additions truncate (5184 keys in one chain
+                // were 8e-6 off).
+                const float *vf = reinterpret_cast<const float *>(vs) + (jw + 2 * t4) * (TL::PITCH / 4) + g4;
+                uint32_t ph[NT][4], pl[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    split_near<false>(sc[n][0], ph[n][0], pl[n][0]);
+                    split_near<false>(sc[n][2], ph[n][1], pl[n][1]);
+                    split_near<false>(sc[n][1], ph[n][2], pl[n][2]);
+                    split_near<false>(sc[n][3], ph[n][3], pl[n][3]);
+                }
+#pragma unroll
+                for (int d0 = 0; d0 < DT; d0 += 4) {
+                    float hi[4][4], lo[4][4];
+#pragma unroll
+                    for (int d = 0; d < 4; d++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            hi[d][e] = lo[d][e] = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        uint32_t bh[4][2], bl[4][2];
+#pragma unroll
+                        for (int d = 0; d < 4; d++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++)
+                                split_cut(vf[(n * 8 + e) * (TL::PITCH / 4) + (d0 + d) * 8], bh[d][e], bl[d][e]);
+#pragma unroll
+                        for (int d = 0; d < 4; d++)
+                            mma8(lo[d], pl[n], bh[d][0], bh[d][1]);
+#pragma unroll
+                        for (int d = 0; d < 4; d++)
+                            mma8(hi[d], ph[n], bh[d][0], bh[d][1]);
+#pragma unroll
+                        for (int d = 0; d < 4; d++)
+                            mma8(lo[d], ph[n], bl[d][0], bl[d][1]);
+                    }
+#pragma unroll
+                    for (int d = 0; d < 4; d++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            o[d0 + d][e] += hi[d][e] + lo[d][e];
+                }
             }
         }
+        cp_wait<0>();
+        if constexpr (!F32)
+            break;
+        else {
+            if (vexp != 0 || nsteps == 0)
+                break;
+            bool most = false, least = false;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    most |= !(fabsf(o[d][e]) < Retake::kMostOut);
+                    least |= fabsf(o[d][e]) >= Retake::kLeastOut;
+                }
+            if (!__syncthreads_or(busy && (most || !least)))
+                break;
+            most = __syncthreads_or(most);
+            least = __syncthreads_or(least);
+            if (!most && least)
+                break;
+            const int top = largest_value();
+            if (top < -149 || (!most && top >= Retake::kSmallExp))
+                break;  // nothing but zeros; or small sums of larger values
+            vexp = min(Retake::kTargetExp - top, 64);
+            if (vexp == 0)
+                break;
+        }
     }
-    cp_wait<0>();
     // The next kernel's CTAs may come now: earlier they would take the free
     // slots of some SMs and leave it badly spread (201 queries over 5184 keys in
     // 32 bits: 83 us alone, 100 us in a row of such calls).
@@ -541,6 +618,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
         sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
     }
     T *ob = reinterpret_cast<T *>(a.o) + b * a.os0 + (long)kh * a.g * a.os1;
+    const float unscale = F32 ? __int_as_float((127 - vexp) << 23) : 1.0f;
 
     if (WK == 1 && a.cs == 1) {  // the tile is whole: straight from registers
 #pragma unroll
@@ -555,7 +633,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
                 const int c = d * 8 + t4 * 2;
                 if (c >= a.hd)
                     continue;
-                const float x = o[d][2 * h] * inv, y = o[d][2 * h + 1] * inv;
+                float x = o[d][2 * h] * inv, y = o[d][2 * h + 1] * inv;
+                if constexpr (F32) {
+                    x *= unscale;
+                    y *= unscale;
+                }
                 if (a.ovec) {
                     if constexpr (F32)
                         *reinterpret_cast<float2 *>(dst + c) = make_float2(x, y);
@@ -637,13 +719,13 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
                 const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    v[i] *= inv;
+                    v[i] = v[i] * inv * unscale;
                 store(r, c, v);
             }
             else {
                 st_dsmem4(owner(r) + c * 4, v[0], v[1], v[2], v[3]);
                 if (c == 0)
-                    st_dsmem2(owner(r) + HDP * 4, m, l);
+                    st_dsmem4(owner(r) + HDP * 4, m, l, unscale, 0.0f);
             }
         }
         if (a.cs == 1)
@@ -661,12 +743,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
             for (int d = 0; d < DT; d++)
                 st_dsmem2(dst + (d * 8 + t4 * 2) * 4, o[d][2 * h], o[d][2 * h + 1]);
             if (t4 == 0)
-                st_dsmem2(dst + HDP * 4, mx[h], sum[h]);
+                st_dsmem4(dst + HDP * 4, mx[h], sum[h], unscale, 0.0f);
         }
     }
     cluster_sync_all();
     const int live = rows > rank ? (rows - 1 - rank) / a.cs + 1 : 0;
-    PT::template merge<kThreads>(part, a.cs, rl, live, a.scale_log2, [&](int i, int c, float x, float y, float z, float w) {
+    PT::template merge<kThreads, F32>(part, a.cs, rl, live, a.scale_log2, [&](int i, int c, float x, float y, float z, float w) {
         const float v[4] = {x, y, z, w};
         store(i * a.cs + rank, c, v);
     });
@@ -1087,9 +1169,6 @@ extern "C" int k_cross_attend(const struct k_rows *Q, const struct k_rows *K, co
     if (es == 2 && Nk <= 64 && a.rows > 16)
         a.ovec = vec(O);  // the form for few keys stores 16 bytes
     a.scale_log2 = (float)(scale * 1.4426950408889634);
-    for (int n = Nk; n > 0; n >>= 1)
-        a.shift += 1.0f;
-    a.shift += 1.0f;
     a.err = err;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(s);
     // Many rows over many keys: tcgen05. Both forms were measured over 1 to 1024

@@ -24,7 +24,6 @@ struct XaArgs {
     int kvec, qvec, ovec;  // 16-byte accesses allowed
     Div dg;                // g, for rows < 2^31
     float scale_log2;
-    float shift;  // of the weights' exponents in 32 bits, 2^shift > 2 Nk
     int *err;  // device error word (bounded waits of the tcgen05 form)
 };
 
@@ -91,17 +90,20 @@ __device__ __forceinline__ void st_dsmem2(uint32_t a, float x, float y)
 // element: 64 queries x 384 keys 15 us against 7), as part[(p * rl + r / cs) * PR]
 // with HDP columns of output, then its largest score (not scaled) and sum. After
 // a cluster barrier each CTA merges its own rows: O = sum_p O_p w_p / sum_p l_p
-// w_p, w_p = 2^((max_p - max) scale_log2). A part without a visible key has maximum -inf and
-// counts nothing, unless its sum is NaN.
+// w_p, w_p = 2^((max_p - max) scale_log2). SCALED: a part's output is times a
+// power of two whose inverse follows the sum; where these differ, the weights
+// are divided by the sum and brought to the largest inverse first, so that
+// nothing overflows and the smallest numbers are rounded once.
+// A part without a visible key has maximum -inf and counts nothing, unless its sum is NaN.
 template <int HDP>
 struct Parts {
     static constexpr int PR = HDP + 4;
     // rl: rows a CTA holds of each part; live: rows of its own that exist
-    template <int THREADS, typename Store>
+    template <int THREADS, bool SCALED, typename Store>
     static __device__ __forceinline__ void merge(float *part, int np, int rl, int live, float scale_log2,
                                                  const Store &store)
     {
-        // weights of a row's parts and 1 / sum, a thread per row
+        // weights of a row's parts and the last factor, a thread per row
         constexpr int kMost = 16;  // CTAs of a cluster
         for (int i = threadIdx.x; i < live; i += THREADS) {
             float m = -INFINITY, l = 0.0f;
@@ -120,7 +122,33 @@ struct Parts {
                     l += none ? (ml[p].y == ml[p].y ? 0.0f : ml[p].y) : ml[p].y * w;
                     part[(p * rl + i) * PR + HDP] = w;
                 }
-            part[i * PR + HDP + 2] = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            float last = inv;  // what the sum is multiplied by
+            if constexpr (SCALED) {
+                float lo = INFINITY, hi = 0.0f;
+#pragma unroll
+                for (int p = 0; p < kMost; p++)
+                    if (p < np && ml[p].x != -INFINITY) {
+                        const float f = part[(p * rl + i) * PR + HDP + 2];
+                        lo = fminf(lo, f);
+                        hi = fmaxf(hi, f);
+                    }
+                if (lo >= hi)  // of one scale
+                    last = inv * hi;
+                else {
+                    hi = 0.0f;
+                    for (int p = 0; p < np; p++) {
+                        const float *at = part + (p * rl + i) * PR + HDP;
+                        hi = at[0] != 0.0f ? fmaxf(hi, at[2]) : hi;
+                    }
+                    for (int p = 0; p < np; p++) {
+                        float *at = part + (p * rl + i) * PR + HDP;
+                        at[0] = at[0] != 0.0f ? at[0] * inv * (at[2] / hi) : 0.0f;
+                    }
+                    last = inv == inv ? hi : inv;
+                }
+            }
+            part[i * PR + HDP + 2] = last;
         }
         __syncthreads();
         const int ne = live * (HDP / 4);  // elements, four columns each
@@ -137,8 +165,8 @@ struct Parts {
                 acc.z = fmaf(v.z, w, acc.z);
                 acc.w = fmaf(v.w, w, acc.w);
             }
-            const float inv = part[i * PR + HDP + 2];
-            store(i, c, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            const float last = part[i * PR + HDP + 2];
+            store(i, c, acc.x * last, acc.y * last, acc.z * last, acc.w * last);
         }
     }
 };

@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         cluster_sync_all();
         const int mine = live > rank ? (live - 1 - rank) / a.cs + 1 : 0;
         T *ob = reinterpret_cast<T *>(a.o) + it.seq * a.os0 + it.head * a.os1;
-        PT::template merge<kThreads>(part, a.cs, rl, mine, a.scale_log2, [&](int i, int c, float x, float y, float z, float w) {
+        PT::template merge<kThreads, false>(part, a.cs, rl, mine, a.scale_log2, [&](int i, int c, float x, float y, float z, float w) {
             if (c >= a.hd)
                 return;
             T *dst = ob + (long)(it.qt * BQ + i * a.cs + rank) * a.old + c;

@@ -157,3 +157,97 @@ def test_cross_attend_large_common_score(be, nb, Nq, Nk, h, hd, common, sign, dt
         tol = tol + 4 * 2.0 ** -24 * top * A + (2.0 ** -34 * vd.double().abs().sum(1, keepdim=True) if dt == "f16" else 0.0)
         err = (o.double() - want).abs()
         assert (err <= tol).all(), (scale, float((err / tol).max()))
+
+
+# ------------------------------------------------------------------ 32-bit values of any size
+F32_FORMS = [(2, 1, 40, 3, 32), (1, 3, 300, 4, 64), (1, 1, 5000, 2, 128), (2, 90, 60, 2, 32), (1, 600, 700, 4, 40),
+             (1, 70, 3000, 2, 128), (1, 40, 3000, 1, 24)]
+
+
+def check_f32_values(be, q, k, v, klen=None, kmask=None):
+    """As check_attend, without its allowance for small numbers: what is allowed is half a step of the smallest ones for
+    the result and as much for each of the two products that bring it to its size."""
+    nb, Nq, h, hd = q.shape
+    Nk, kv = k.shape[1], k.shape[2]
+    o = torch.full_like(q, 5.0)
+    be.cross_attend(nb, Nq, Nk, h, kv, hd, *(op(be, x, 0, x.stride(1), x.stride(0), x.stride(2)) for x in (q, k, v, o)),
+                    be.wrap(klen) if klen is not None else None, be.wrap(kmask) if kmask is not None else None)
+    be.sync()
+    see = torch.ones(nb, Nk, dtype=torch.bool, device="cuda")
+    if klen is not None:
+        see &= torch.arange(Nk, device="cuda") < klen[:, None]
+    if kmask is not None:
+        see &= kmask == 0
+    want, A, big = attend_ref(q.double(), k.double(), v.double(), see, hd ** -0.5)
+    w = 2 * (hd + 16) * 2.0 ** -23 * big + 2.0 ** -20 + (Nk + 16) * 2.0 ** -23
+    tol = (u(torch.float32) * want.abs() + w * (1 + u(torch.float32)) * A) * 1.01 + 1.5 * 2.0 ** -149
+    err = (o.double() - want).abs()
+    assert (err <= tol).all(), (float((err / tol).max()), float(err.max()))
+
+
+@pytest.mark.parametrize("nb,Nq,Nk,h,hd", F32_FORMS)
+@pytest.mark.parametrize("ex", [-147, -140, -130, -122, -115, -105, -90, -75, -20, 90, 115, 123])
+def test_cross_attend_f32_value_sizes(be, nb, Nq, Nk, h, hd, ex):
+    """Values of any size keep their bits, with weights spread over many keys and with nearly all of it on one."""
+    g = gen(Nk + hd)
+    q, k = randn(g, nb, Nq, h, hd), randn(g, nb, Nk, h, hd)
+    v = (randn(g, nb, Nk, h, hd).double() * 2.0 ** ex).float()
+    assert v.isfinite().all() and v.abs().max() > 0
+    check_f32_values(be, q, k, v)
+    k[:, Nk // 2] += 4.0 * q[:, 0].mean(1, keepdim=True)
+    check_f32_values(be, q, k, v)
+
+
+@pytest.mark.parametrize("nb,Nq,Nk,h,hd", F32_FORMS)
+@pytest.mark.parametrize("low,high", [(-140, -120), (-120, 0), (-120, 124), (0, 126), (-30, 60)])
+def test_cross_attend_f32_values_of_two_sizes(be, nb, Nq, Nk, h, hd, low, high):
+    """One half of the keys with small values, the other with large ones, either half hidden in some sequences (lengths
+    and masks): what is hidden decides nothing, and small values beside larger ones keep what the larger ones leave."""
+    nb = 4
+    g = gen(Nk + hd + high)
+    q, k = randn(g, nb, Nq, h, hd), randn(g, nb, Nk, h, hd)
+    ex = torch.where(torch.arange(Nk, device="cuda") < Nk // 2, float(low), float(high)).double()
+    sign = torch.where(randn(g, nb, Nk, h, hd) > 0, 1.0, -1.0)
+    v = (sign * (1.0 + torch.rand(nb, Nk, h, hd, device="cuda", generator=g).double()) * 2.0 ** ex[:, None, None]).float()
+    klen = torch.tensor([Nk, Nk // 2, Nk, 0], device="cuda", dtype=torch.int32)
+    kmask = torch.zeros(nb, Nk, dtype=torch.uint8, device="cuda")
+    kmask[2, Nk // 2:] = 1
+    check_f32_values(be, q, k, v, klen, kmask)
+
+
+def test_cross_attend_f32_values_that_cancel(be):
+    """Sums of nothing, or next to it, of values of ordinary size."""
+    g = gen(3)
+    q, k, v = randn(g, 1, 40, 2, 32), randn(g, 1, 80, 2, 32), randn(g, 1, 80, 2, 32)
+    k[:, 1::2], v[:, 1::2] = k[:, 0::2], -v[:, 0::2]
+    check_f32_values(be, q, k, v)
+    check_f32_values(be, q, k, v * 2.0 ** 100)
+    check_f32_values(be, q, k, torch.zeros_like(v))
+
+
+@pytest.mark.parametrize("nb,Nq,Nk,h,hd", F32_FORMS)
+def test_cross_attend_f32_not_a_number(be, nb, Nq, Nk, h, hd):
+    """A visible key that is not a number makes every row NaN, an infinite value its column, whatever the other values'
+    sizes; other columns stay what they were."""
+    g = gen(5)
+    q, k = randn(g, nb, Nq, h, hd).abs() + 0.25, randn(g, nb, Nk, h, hd)
+    for ex in (0, -120, 122):
+        v = (randn(g, nb, Nk, h, hd).double() * 2.0 ** ex).float()
+
+        def run(k, v):
+            o = torch.full_like(q, 5.0)
+            be.cross_attend(nb, Nq, Nk, h, h, hd, *(op(be, x, 0, h * hd, x.shape[1] * h * hd, hd) for x in (q, k, v, o)))
+            be.sync()
+            return o
+        for j in (0, Nk // 2, Nk - 1):
+            kn = k.clone()
+            kn[:, j, :, 3] = math.nan
+            assert run(kn, v).isnan().all()
+            vn = v.clone()
+            vn[:, j, :, 5] = math.inf
+            o, want = run(k, vn), run(k, v)
+            rest = torch.arange(hd, device="cuda") != 5
+            assert (~o[..., 5].isfinite()).all()
+            # the same sums, perhaps of values times another power of two
+            lim = 2.0 ** -18 * v[..., rest].abs().amax((1, 3))[:, None, :, None]
+            assert ((o - want)[..., rest].abs() <= lim).all()
