@@ -42,13 +42,16 @@ constexpr int kThreads = 32 * 6;
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxSplit = 8;
 constexpr int kPolyPairsPer8 = 2;  // of 8 pairs, on the FMA pipe (attn_tc.cu)
-// Weights times 2^kShift (as kWeightShift, attn_cross.cuh). f16: 96 weights of the
-// first tile, 2^9 at most, stay below the limit and each weight below it fits the
-// type: whole down to 2^-23 of the offset's weight and rounded by 2^-34 below.
+// Weights times 2^kShift (as kWeightShift, attn_cross.cuh), and the sum of a tile's
+// from which it is taken again. f16: 96 weights of the first tile, 2^9 at most,
+// stay below the limit and each weight below it fits the type: whole down to
+// 2^-23 of the offset's weight and rounded by 2^-34 below. bf16: weights stay
+// below 1, so that their sums with values are finite as far as the plain ones
+// are, and 2^-13 of the smallest normal value still has the type's bits.
 template <typename T>
-constexpr float kShift = __is_same(T, __half) ? 9.0f : 0.0f;
+constexpr float kShift = __is_same(T, __half) ? 9.0f : -13.0f;
 template <typename T>
-constexpr float kOverflowSum = __is_same(T, __half) ? 61440.0f : 8192.0f;
+constexpr float kOverflowSum = __is_same(T, __half) ? 61440.0f : 1.0f;
 // From 2^128 on the polynomial's exponent field wraps and the sum does not show
 // it, so its exponents are looked at themselves: one at or above this sends
 // the tile through again.

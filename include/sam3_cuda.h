@@ -489,8 +489,7 @@ int cb_rope_rotate(cb_backend *b, int nb, int N, int heads, int hd, int rot,
  * 2^-100 beside far larger ones of the same head keep fewer), BF16 / F16
  * weights are rounded to the operands' type before the product with V (F16: by
  * half a step of the type or 2^-34 of the row's largest weight, whichever is
- * more). The weights of BF16 are divided by their sum last: values of V below
- * 2^120 / Nk. */
+ * more) and divided by their sum last: BF16 values of V below 2^127 / Nk. */
 int cb_cross_attend(cb_backend *b, int nb, int Nq, int Nk, int heads,
                     int kvheads, int hd, struct cb_opnd Q, struct cb_opnd K,
                     struct cb_opnd V, struct cb_opnd O, cb_mem klen,

@@ -251,3 +251,27 @@ def test_cross_attend_f32_not_a_number(be, nb, Nq, Nk, h, hd):
             # the same sums, perhaps of values times another power of two
             lim = 2.0 ** -18 * v[..., rest].abs().amax((1, 3))[:, None, :, None]
             assert ((o - want)[..., rest].abs() <= lim).all()
+
+
+@pytest.mark.parametrize("nb,Nq,Nk,h,hd", FORMS)
+@pytest.mark.parametrize("size", ["large", "small"])
+def test_cross_attend_bf16_value_sizes(be, nb, Nq, Nk, h, hd, size):
+    """bf16 values up to 2^127 / Nk and down to the smallest normal ones, with scores that rise by up to 12 powers of two
+    after the first keys. Allowed besides: half a step of the type's smallest numbers (2^-134), and half a step
+    of 32 bits' (2^-150) for each of Nk products with weights of 2^-13 of the plain ones, so 2^-137 each."""
+    g = gen(Nk + hd)
+    q, k, v = late_key(g, torch.bfloat16, nb, Nq, Nk, h, hd, Nk * 2 // 3, 12.0, hd ** -0.5)
+    top = 2.0 ** (126 - math.ceil(math.log2(Nk)))
+    ex = top if size == "large" else 2.0 ** -126
+    v = ((1.0 + torch.rand(nb, Nk, h, hd, device="cuda", generator=g).double()) * ex *
+         torch.where(randn(g, nb, Nk, h, hd) > 0, 1.0, -1.0)).bfloat16()
+    o = torch.full_like(q, 5.0)
+    be.cross_attend(nb, Nq, Nk, h, h, hd, *(op(be, x, 0, h * hd, x.shape[1] * h * hd, hd) for x in (q, k, v, o)))
+    be.sync()
+    want, A, big = attend_ref(q.double(), k.double(), v.double(), torch.ones(nb, Nk, dtype=torch.bool, device="cuda"),
+                              hd ** -0.5)
+    e = (hd + 16) * 2.0 ** -23 * big
+    w = u(torch.bfloat16) + 2 * e + 2.0 ** -13 + (Nk + 16) * 2.0 ** -23
+    tol = (u(torch.bfloat16) * want.abs() + w * (1 + u(torch.bfloat16)) * A) * 1.01 + 2.0 ** -134 + Nk * 2.0 ** -137
+    err = (o.double() - want).abs()
+    assert (err <= tol).all(), (float((err / tol).max()), float(err.max()))
