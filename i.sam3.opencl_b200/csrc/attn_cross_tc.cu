@@ -19,9 +19,9 @@
 //     shared memory: no workspace, one launch.
 // Softmax as in attn_tc.cu: the row's offset is the maximum of its first tile
 // with a visible key, exponentials of later tiles are taken against it, and a
-// tile whose sum reaches kOverflowSum (or is not a number) or whose exponents
-// pass the polynomial's range is taken again with a raised offset, without the
-// polynomial, so that infinities and NaN of visible keys come out as such.
+// tile whose sum reaches kOverflowSum (or is not a number; the polynomial
+// exponential makes 2^125 of one) is taken again with a raised offset, without
+// the polynomial, so that infinities and NaN of visible keys come out as such.
 // Measured: 8 x 5184 queries x 5184 keys x 16 heads of 64 columns 1012 us, 870
 // TFLOP/s (the softmax warps bound it as in attn_tc.cu: 884); 4 x 4096 x 4096 x
 // 16 heads of 128 columns 467 us, 1177 TFLOP/s; with a key mask 1164 us, every
@@ -52,10 +52,6 @@ template <typename T>
 constexpr float kShift = __is_same(T, __half) ? 9.0f : -13.0f;
 template <typename T>
 constexpr float kOverflowSum = __is_same(T, __half) ? 61440.0f : 1.0f;
-// From 2^128 on the polynomial's exponent field wraps and the sum does not show
-// it, so its exponents are looked at themselves: one at or above this sends
-// the tile through again.
-constexpr float kPolyMost = 64.0f;
 // An offset is a score; its product with the scale is rounded, which leaves a
 // power of two of that rounding in every weight of the row. Products below this
 // leave 2^-12 at most, less than the weights' own rounding; beyond it a tile
@@ -89,30 +85,6 @@ __host__ __device__ constexpr uint32_t idesc(int M, int N, int b_mn_major)
     const uint32_t f = sizeof(T) == 2 && !__is_same(T, __half) ? 1u : 0u;
     return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)b_mn_major << 16) |
            ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-
-// 2^x of two values below 128 as exp2_poly2 (tc_ptx.cuh), but a NaN becomes NaN or huge
-// instead of 2^-125, so that the tile's sum shows it: the clamp at -125 is a
-// minimum of the bit patterns, which grow with the magnitude of a negative
-// number and are smaller for positive ones and for the NaN of an fma.
-__device__ __forceinline__ void exp2_poly2_nan(float x0, float x1, float &y0, float &y1)
-{
-    x0 = __uint_as_float(min(__float_as_uint(x0), 0xc2fa0000u));
-    x1 = __uint_as_float(min(__float_as_uint(x1), 0xc2fa0000u));
-    const float kMagic = 12582912.0f;
-    const uint64_t x = f2_make(x0, x1);
-    const uint64_t j = add2(x, f2_make(kMagic, kMagic));
-    const uint64_t n = add2(j, f2_make(-kMagic, -kMagic));
-    const uint64_t f = fma2(n, f2_make(-1.0f, -1.0f), x);
-    uint64_t p = fma2(f2_make(0.05517221987247467f, 0.05517221987247467f), f,
-                      f2_make(0.24261115491390228f, 0.24261115491390228f));
-    p = fma2(p, f, f2_make(0.6932608485221863f, 0.6932608485221863f));
-    p = fma2(p, f, f2_make(0.9999280571937561f, 0.9999280571937561f));
-    float p0, p1, j0, j1;
-    f2_split(p, p0, p1);
-    f2_split(j, j0, j1);
-    y0 = __uint_as_float(__float_as_uint(j0) * 8388608u + __float_as_uint(p0));
-    y1 = __uint_as_float(__float_as_uint(j1) * 8388608u + __float_as_uint(p1));
 }
 
 struct TcArgs {
@@ -438,17 +410,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                         }
                         const float top = m_used == -INFINITY ? 0.0f : m_used * a.scale_log2;
                         const uint64_t negm = f2_make(kShift<T> - top, kShift<T> - top);
-                        float xm = -INFINITY;  // largest exponent of the polynomial
 #pragma unroll
                         for (int e = 0; e < BKV; e += 2) {
                             const uint64_t x2 = fma2(f2_make(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
                                                      sl2x2, negm);
                             float x0, x1, p0, p1;
                             f2_split(x2, x0, x1);
-                            if (((e >> 1) & 7) >= 8 - kPolyPairsPer8) {
-                                xm = max3f(xm, x0, x1);
-                                exp2_poly2_nan(x0, x1, p0, p1);
-                            }
+                            if (((e >> 1) & 7) >= 8 - kPolyPairsPer8)
+                                exp2_poly2(x0, x1, p0, p1);
                             else {
                                 p0 = ex2_approx(x0);
                                 p1 = ex2_approx(x1);
@@ -463,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                         f2_split(t0, u0, u1);
                         f2_split(t1, u2, u3);
                         over = __any_sync(0xffffffffu,
-                                          !(((u0 + u1) + (u2 + u3)) < kOverflowSum<T> && xm < kPolyMost &&
+                                          !(((u0 + u1) + (u2 + u3)) < kOverflowSum<T> &&
                                             fabsf(top) < kFarOffset));
                         if (!over) {
                             tmem_st32(tS, *reinterpret_cast<const uint32_t(*)[32]>(s));

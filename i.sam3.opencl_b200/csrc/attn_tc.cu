@@ -77,14 +77,10 @@ constexpr int kCtasPerSm = 2;
 // (exp2_poly2) instead of two MUFU instructions: the MUFU unit runs 16
 // exponentials per clock per SM against 256 MMA flops per score.
 constexpr int kPolyPairsPer8 = 2;
-// A row's tile sum at or above this (some P >= 2^13, or inf / NaN) sends
-// the tile through the maximum pass again with a raised offset.
+// A row's tile sum at or above this (some P >= 2^13, 2^125 at most from the
+// polynomial, or inf / NaN) sends the tile through the maximum pass again with
+// a raised offset.
 constexpr float kOverflowSum = 8192.0f;
-// So does an exponent of the polynomial at or above this: from 2^128 on its
-// exponent field wraps and the sum would not show it. (Their maximum is one
-// instruction a pair, a clamp of each from above would be two; 0.7 % of the
-// backbone's step.)
-constexpr float kPolyMost = 64.0f;
 constexpr int Q_BYTES = BQ * HD * 2;
 constexpr int KV_BYTES = BKV * HD * 2;
 constexpr int OFF_Q = 0;                       // [buffer], one query tile each
@@ -469,7 +465,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                         const uint64_t negm = f2_make(-m_used, -m_used);
                         t0 = 0;
                         t1 = 0;
-                        float xm = -INFINITY;  // largest exponent of the polynomial
 #pragma unroll
                         for (int e = 0; e < BKV; e += 2) {
                             const uint64_t x2 = fma2(f2_make(__uint_as_float(s[e]),
@@ -477,10 +472,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                                                      sl2x2, negm);
                             float x0, x1, p0, p1;
                             f2_split(x2, x0, x1);
-                            if (((e >> 1) & 7) >= 8 - kPolyPairsPer8) {
-                                xm = max3f(xm, x0, x1);
+                            if (((e >> 1) & 7) >= 8 - kPolyPairsPer8)
                                 exp2_poly2(x0, x1, p0, p1);
-                            }
                             else {
                                 p0 = ex2_approx(x0);
                                 p1 = ex2_approx(x1);
@@ -494,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                         float u0, u1, u2, u3;
                         f2_split(t0, u0, u1);
                         f2_split(t1, u2, u3);
-                        const bool over = !(((u0 + u1) + (u2 + u3)) < kOverflowSum && xm < kPolyMost);
+                        const bool over = !(((u0 + u1) + (u2 + u3)) < kOverflowSum);
                         if (pass == 1 || !__any_sync(0xffffffffu, over))
                             break;
 #pragma unroll

@@ -595,19 +595,28 @@ __device__ __forceinline__ float max3f(float a, float b, float c)
     return d;
 }
 
-// 2^x for two values x <= 0 on the FMA pipe, leaving the MUFU unit to the
+// x clamped to [-most, most] in one instruction (the smaller magnitude with
+// x's sign; most > 0). A NaN, which an fma makes with a clear sign bit, becomes most.
+__device__ __forceinline__ float clamp_abs(float x, float most)
+{
+    float y;
+    asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(most));
+    return y;
+}
+
+// 2^x for two values on the FMA pipe, leaving the MUFU unit to the
 // other exponentials of the softmax. Method: Cody-Waite style range
 // reduction x = n + f with n = round(x) (add and subtract 1.5 * 2^23, exact
 // for |x| < 2^22) and f in [-0.5, 0.5]; 2^f from a degree-3 polynomial whose
 // coefficients minimise the maximum relative error on [-0.5, 0.5] (fitted
 // for this kernel by linear programming: 7.5e-5 max relative error in fp32
 // Horner form); 2^n applied by adding n to the exponent field. x is clamped
-// to -125 so the result stays a normal number (2^-125 ~ 2.4e-38, i.e. 0 for
-// a softmax weight). Accuracy is far below the bf16 rounding of P (2^-9).
+// to [-125, 125] so the result stays a normal number (2^-125 ~ 2.4e-38, i.e. 0 for
+// a softmax weight; 2^125, as for a NaN, is far above what a softmax accepts). Accuracy is far below the bf16 rounding of P (2^-9).
 __device__ __forceinline__ void exp2_poly2(float x0, float x1, float &y0, float &y1)
 {
     const float kMagic = 12582912.0f;  // 1.5 * 2^23
-    const uint64_t x = f2_make(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f));
+    const uint64_t x = f2_make(clamp_abs(x0, 125.0f), clamp_abs(x1, 125.0f));
     const uint64_t j = add2(x, f2_make(kMagic, kMagic));
     const uint64_t n = add2(j, f2_make(-kMagic, -kMagic));
     const uint64_t f = fma2(n, f2_make(-1.0f, -1.0f), x);
