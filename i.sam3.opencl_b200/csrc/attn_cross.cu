@@ -35,6 +35,7 @@
 // of 32 columns x 2: 68.6 us, bound by the splits' dependent arithmetic (issue
 // slots 40 % busy at 16 warps per SM; the products alone need 25 us).
 #include "attn_cross.cuh"
+#include "cluster.cuh"
 #include "kernels.h"
 #include "pdl.cuh"
 #include "tc_ptx.cuh"
@@ -48,7 +49,7 @@ namespace sam3 {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kMaxCluster = 16;
+constexpr int kMaxCluster = kMaxClusterCtas;
 constexpr int kSplitSteps = 4;  // steps of a CTA from which two share them
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live)
@@ -1052,27 +1053,11 @@ int launch_few_k(XaArgs &a, int nb, cudaStream_t s)
     }
 }
 
-template <auto Kern>
-cudaError_t prepare_once(int smem)
-{
-    static int done[64];
-    int dev = 0;
-    const bool known = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
-    if (known && done[dev])
-        return cudaSuccess;
-    cudaError_t e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(Kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess && known)
-        done[dev] = 1;
-    return e;
-}
-
 template <typename T, int HDP, int WM>
 int launch(XaArgs &a, int nb, cudaStream_t s)
 {
     using CF = Cfg<T, HDP, WM>;
-    const cudaError_t pe = prepare_once<attn_cross_kernel<T, HDP, WM>>(CF::SMEM_PARTS);
+    const cudaError_t pe = cluster_prepare_once<attn_cross_kernel<T, HDP, WM>>(CF::SMEM_PARTS);
     if (pe != cudaSuccess)
         return (int)pe;
     constexpr int BM = 16 * WM;
@@ -1082,10 +1067,11 @@ int launch(XaArgs &a, int nb, cudaStream_t s)
     a.nqt = (int)nqt;
     const long items = (long)nb * a.kvheads * nqt;
     // CTAs sharing a tile's keys: while all run at once, each with at least
-    // two steps.
+    // two steps, and a cluster of them fits the device.
     const long slots = resident<attn_cross_kernel<T, HDP, WM>>(CF::SMEM_PARTS), steps = (a.Nk + CF::BK - 1) / CF::BK;
     a.cs = 1;
-    while (a.cs < kMaxCluster && items * a.cs * 2 <= slots && steps >= a.cs * kSplitSteps)
+    while (a.cs < kMaxCluster && items * a.cs * 2 <= slots && steps >= a.cs * kSplitSteps &&
+           clusters_at_once<attn_cross_kernel<T, HDP, WM>>(a.cs * 2, kThreads, CF::SMEM_PARTS) > 0)
         a.cs *= 2;
     if (items > 0x7fffffffL / a.cs)
         return K_EARG;

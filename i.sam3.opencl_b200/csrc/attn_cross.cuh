@@ -3,6 +3,7 @@
 // share: their arguments and the rounding of pairs.
 #pragma once
 
+#include "cluster.cuh"
 #include "div.cuh"
 #include "kernels.h"
 #include "tc_ptx.cuh"
@@ -104,7 +105,7 @@ struct Parts {
                                                  const Store &store)
     {
         // weights of a row's parts and the last factor, a thread per row
-        constexpr int kMost = 16;  // CTAs of a cluster
+        constexpr int kMost = kMaxClusterCtas;
         for (int i = threadIdx.x; i < live; i += THREADS) {
             float m = -INFINITY, l = 0.0f;
             float2 ml[kMost];

@@ -27,6 +27,7 @@
 // 16 heads of 128 columns 467 us, 1177 TFLOP/s; with a key mask 1164 us, every
 // tile in the rolled path.
 #include "attn_cross.cuh"
+#include "cluster.cuh"
 #include "kernels.h"
 #include "pdl.cuh"
 #include "tc_ptx.cuh"
@@ -673,7 +674,7 @@ bool make_map(CUtensorMap *map, bool bf16, const void *p, int hd, long rows, int
 template <typename T, int HDP, bool SPLIT, bool MASK>
 int launch(TcArgs &ta, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, int grid, cudaStream_t s)
 {
-    const cudaError_t e = smem_limit_once<attn_cross_tc_kernel<T, HDP, SPLIT, MASK>>(Geo<HDP>::SMEM);
+    const cudaError_t e = cluster_prepare_once<attn_cross_tc_kernel<T, HDP, SPLIT, MASK>>(Geo<HDP>::SMEM);
     if (e != cudaSuccess)
         return (int)e;
     cudaLaunchAttribute attr[2];
@@ -691,6 +692,14 @@ int launch(TcArgs &ta, const CUtensorMap &tq, const CUtensorMap &tk, const CUten
     cfg.attrs = attr;
     cfg.numAttrs = SPLIT ? 2 : 1;
     return (int)cudaLaunchKernelEx(&cfg, attn_cross_tc_kernel<T, HDP, SPLIT, MASK>, tq, tk, tv, (const TcArgs)ta);
+}
+
+// Whether a cluster of c CTAs fits the device.
+template <typename T, int HDP, bool MASK>
+bool cluster_fits(int c)
+{
+    return cluster_prepare_once<attn_cross_tc_kernel<T, HDP, true, MASK>>(Geo<HDP>::SMEM) == cudaSuccess &&
+           clusters_at_once<attn_cross_tc_kernel<T, HDP, true, MASK>>(c, kThreads, Geo<HDP>::SMEM) > 0;
 }
 
 template <typename T, int HDP>
@@ -714,7 +723,8 @@ int run(XaArgs &x, int nb, bool bf16, cudaStream_t s)
     // merge 3.5 us (64 (sequence, head) pairs x 128 queries, cs 1 and 4: 8
     // tiles 11.8 and 12.6 us, 11 tiles 14.6 and 13.7 us).
     int cs = 1;
-    while (nkv >= 10 && cs < kMaxSplit && items * cs * 2 <= slots - slots / 16)
+    while (nkv >= 10 && cs < kMaxSplit && items * cs * 2 <= slots - slots / 16 &&
+           (x.kmask ? cluster_fits<T, HDP, true>(cs * 2) : cluster_fits<T, HDP, false>(cs * 2)))
         cs *= 2;
     x.cs = cs;
     ta.x = x;

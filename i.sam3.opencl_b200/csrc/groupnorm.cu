@@ -27,6 +27,7 @@
 // CTAs); 72 x 72 x 256 6.8 us, of which the exchange takes 2.5.
 // Per-channel pairs cost about as many instructions as one pair per
 // vector and let a vector span groups of any width.
+#include "cluster.cuh"
 #include "div.cuh"
 #include "kernels.h"
 #include "pdl.cuh"
@@ -44,7 +45,7 @@ constexpr int kThreads = 256;
 constexpr int kUnroll = 4;
 constexpr int kSlabBytes = 64;
 constexpr int kMaxSlabGroups = 128;
-constexpr int kMaxCluster = 16;
+constexpr int kMaxCluster = kMaxClusterCtas;
 constexpr int kRing = 48;  // slots of 16-byte vectors, 12 batches
 constexpr int kRingBytes = kThreads * kRing * 16;  // per CTA, one per SM
 
@@ -529,59 +530,11 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Shared-memory limit and clusters above 8 CTAs, once per kernel and device.
-template <auto Kern, int V>
-cudaError_t prepare_once()
-{
-    static int done[64];
-    int dev = 0;
-    const bool known = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
-    if (known && done[dev])
-        return cudaSuccess;
-    cudaError_t e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kRingBytes + kThreads * (int)sizeof(float2));
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(Kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess && known)
-        done[dev] = 1;
-    return e;
-}
-
-// Clusters of c CTAs (with the whole ring) that run at the same time, asked
-// once per device.
-template <typename TI, typename TO, int V, bool GELU>
-long clusters_at_once(int c)
-{
-    static int known[64][kMaxCluster + 1];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
-        return 0;
-    if (!known[dev][c]) {
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = c;
-        attr[0].val.clusterDim.y = 1;
-        attr[0].val.clusterDim.z = 1;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(c);
-        cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = kRingBytes;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, groupnorm_kernel<TI, TO, V, GELU>, &cfg) != cudaSuccess) {
-            (void)cudaGetLastError();
-            return 0;
-        }
-        known[dev][c] = n + 1;
-    }
-    return known[dev][c] - 1;
-}
-
 template <typename TI, typename TO, int V, bool GELU>
 int launch_a(GnArgs &a, int nb, long npix, int C, cudaStream_t s)
 {
-    const cudaError_t pe = prepare_once<groupnorm_kernel<TI, TO, V, GELU>, V>();
+    const cudaError_t pe =
+        cluster_prepare_once<groupnorm_kernel<TI, TO, V, GELU>>(kRingBytes + kThreads * (int)sizeof(float2));
     if (pe != cudaSuccess)
         return (int)pe;
     a.nslab = C / a.S;
@@ -597,7 +550,7 @@ int launch_a(GnArgs &a, int nb, long npix, int C, cudaStream_t s)
     const long steps = (npix + a.rows - 1) / a.rows;
     a.cs = 1;
     for (int c = 2; c <= kMaxCluster && c <= steps; c++)
-        if (units <= clusters_at_once<TI, TO, V, GELU>(c))
+        if (units <= clusters_at_once<groupnorm_kernel<TI, TO, V, GELU>>(c, kThreads, kRingBytes))
             a.cs = c;
     a.per = npix / a.cs;
     a.extra = npix - a.per * a.cs;

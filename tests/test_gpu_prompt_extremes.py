@@ -275,3 +275,15 @@ def test_cross_attend_bf16_value_sizes(be, nb, Nq, Nk, h, hd, size):
     tol = (u(torch.bfloat16) * want.abs() + w * (1 + u(torch.bfloat16)) * A) * 1.01 + 2.0 ** -134 + Nk * 2.0 ** -137
     err = (o.double() - want).abs()
     assert (err <= tol).all(), (float((err / tol).max()), float(err.max()))
+
+
+# ------------------------------------------------------------------ the largest clusters
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("Nq,Nk,h,kv,hd", [(10, 5000, 8, 1, 64), (20, 6000, 5, 1, 32), (15, 4500, 8, 1, 128),
+                                           (100, 9000, 1, 1, 128), (1, 9000, 1, 1, 32), (300, 9000, 1, 1, 64)])
+def test_cross_attend_sixteen_ctas(be, Nq, Nk, h, kv, hd, dt):
+    """Tiles of 64 rows (and others) whose keys 16 CTAs (tcgen05: 8) share, with lengths that leave some of them none."""
+    g = gen(Nk)
+    q, k, v = (randn(g, 1, n, hh, hd).to(DT[dt]) for n, hh in ((Nq, h), (Nk, kv), (Nk, kv)))
+    for n in (Nk, 3 * Nk // 4 + 1, 70, 1, 0):
+        check_attend(be, q, k, v, torch.tensor([n], device="cuda", dtype=torch.int32))
