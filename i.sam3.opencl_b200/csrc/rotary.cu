@@ -119,6 +119,17 @@ __device__ __forceinline__ __half wr<__half>(float v)
     return __float2half_rn(v);
 }
 
+// A value that is not turned: its bits where the types agree (a NaN keeps its
+// payload), else rounded.
+template <typename TO, typename TI>
+__device__ __forceinline__ TO copied(TI v)
+{
+    if constexpr (__is_same(TI, TO))
+        return v;
+    else
+        return wr<TO>(rd(v));
+}
+
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
     T v[V];
@@ -185,8 +196,8 @@ __global__ void __launch_bounds__(256) rope_rotate_kernel(const __grid_constant_
             VO ou, ow;
 #pragma unroll
             for (int e = 0; e < W; e++) {
-                ou.v[e] = wr<TO>(rd(u.v[e]));
-                ow.v[e] = wr<TO>(rd(w.v[e]));
+                ou.v[e] = copied<TO>(u.v[e]);
+                ow.v[e] = copied<TO>(w.v[e]);
             }
             if (turn) {
                 if (HALVES || W == 1) {

@@ -287,3 +287,32 @@ def test_cross_attend_sixteen_ctas(be, Nq, Nk, h, kv, hd, dt):
     q, k, v = (randn(g, 1, n, hh, hd).to(DT[dt]) for n, hh in ((Nq, h), (Nk, kv), (Nk, kv)))
     for n in (Nk, 3 * Nk // 4 + 1, 70, 1, 0):
         check_attend(be, q, k, v, torch.tensor([n], device="cuda", dtype=torch.int32))
+
+
+# ------------------------------------------------------------------ rotation: what is copied
+@pytest.mark.parametrize("halves", [False, True])
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("off,hd,rot", [(0, 64, 32), (1, 48, 10), (0, 80, 64)])
+def test_rope_rotate_copies_bits(be, sb, dt, halves, off, hd, rot):
+    """Columns behind the rotated ones and rows without a position keep every bit: NaN payloads, signalling NaN, -0,
+    subnormals, in place and not."""
+    nb, N, h = 2, 33, 3
+    g = gen(hd)
+    it = torch.int32 if dt == "f32" else torch.int16
+    info = torch.iinfo(it)
+    bits = torch.randint(info.min, info.max, (nb * N * h * hd + off,), device="cuda", generator=g, dtype=torch.int64).to(it)
+    nan = {"bf16": 0x7f81, "f16": 0x7c05, "f32": 0x7f800123}[dt]
+    bits[::5] = nan
+    bits[1::7] = nan - 2 ** 16 + 2 ** 15 if dt != "f32" else nan - 2 ** 31
+    x = bits.view(DT[dt])
+    pos = torch.where(torch.arange(nb * N, device="cuda") % 3 == 0, -1, 2).int()
+    cs = randn(g, 4, rot // 2, 2)
+    for place in (False, True):
+        y = x.clone() if place else torch.zeros_like(x)
+        src = y if place else x
+        be.rope_rotate(nb, N, h, hd, rot, int(halves), op(be, src, off, h * hd, N * h * hd, hd),
+                       op(be, y, off, h * hd, N * h * hd, hd), be.wrap(cs), 4, be.wrap(pos))
+        be.sync()
+        got, want = (t[off:].view(it).view(nb * N, h, hd) for t in (y, x))
+        assert torch.equal(got[pos < 0], want[pos < 0])
+        assert torch.equal(got[..., rot:], want[..., rot:])
