@@ -316,3 +316,31 @@ def test_rope_rotate_copies_bits(be, sb, dt, halves, off, hd, rot):
         got, want = (t[off:].view(it).view(nb * N, h, hd) for t in (y, x))
         assert torch.equal(got[pos < 0], want[pos < 0])
         assert torch.equal(got[..., rot:], want[..., rot:])
+
+
+# ------------------------------------------------------------------ group norm: the tail of GELU
+@pytest.mark.parametrize("tx,ty", [("f32", "f32"), ("f32", "bf16"), ("f32", "f16"), ("bf16", "bf16"), ("f16", "f16")])
+def test_groupnorm_gelu_tail(be, tx, ty):
+    """GELU over -13 to 7 (gamma 0, so that z = beta exactly) is off by the output's rounding and
+    16 bits: |z| h, h = erfc(|z| / sqrt 2) / 2, off by the fit's 3.7e-6 of h, about 20 roundings of 2^-23 for t, the
+      polynomial and the products, and three of the exponent z^2 log2(e) / 2: (3.7e-6 + (z^2 + 20) 2^-23) |z| h, and the last
+      sum's 2^-24;
+    32 bits: 0.5 z (1 + erf): erf off by 2 units and the sum rounded, 2.5 * 2^-24 |z| / 2, and three more roundings."""
+    Cn = 4096
+    z = torch.linspace(-13.0, 7.0, Cn, device="cuda")
+    x = randn(gen(1), 1, 40, Cn).to(DT[tx])
+    y = torch.empty(1, 40, Cn, device="cuda", dtype=DT[ty])
+    gamma = torch.zeros(Cn, device="cuda")
+    be.groupnorm(1, 40, Cn, 32, op(be, x, 0, Cn), op(be, y, 0, Cn), be.wrap(gamma), be.wrap(z), 1e-5, 1)
+    be.sync()
+    d = z.double()
+    want = 0.5 * d * torch.special.erfc(d * -math.sqrt(0.5))
+    h = 0.5 * torch.special.erfc(d.abs() * math.sqrt(0.5))
+    if ty == "f32":
+        own = 1.25 * 2.0 ** -24 * d.abs() + 3 * 2.0 ** -24 * want.abs()
+    else:
+        own = (3.7e-6 + (d * d + 20.0) * 2.0 ** -23) * d.abs() * h + 2.0 ** -24 * want.abs()
+    least = {"f32": 2.0 ** -149, "f16": 2.0 ** -25, "bf16": 2.0 ** -134}[ty]
+    tol = u(DT[ty]) * want.abs() + own * (1 + u(DT[ty])) + least
+    err = (y[0].double() - want).abs()
+    assert (err <= tol).all(), (float((err / tol).max()), float(z[(err / tol).amax(0).argmax()]))
