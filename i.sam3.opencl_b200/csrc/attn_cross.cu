@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
                 T w[EPC];
 #pragma unroll
                 for (int e = 0; e < EPC; e++)
-                    w[e] = live && c * EPC + e < a.hd ? src[e] : out_of<T>(0.0f);
+                    w[e] = live && c * EPC + e < a.hd ? src[e] : from_f<T>(0.0f);
                 *reinterpret_cast<uint4 *>(smem + TL::at(r, c)) = *reinterpret_cast<const uint4 *>(w);
             }
         }
@@ -288,8 +288,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
 #pragma unroll
                 for (int e = 0; e < EPC; e++) {
                     const bool in = live && c * EPC + e < a.hd;
-                    w[e] = in ? ks[e] : out_of<T>(0.0f);
-                    x[e] = in ? vs[e] : out_of<T>(0.0f);
+                    w[e] = in ? ks[e] : from_f<T>(0.0f);
+                    x[e] = in ? vs[e] : from_f<T>(0.0f);
                 }
                 *reinterpret_cast<uint4 *>(kd + off) = *reinterpret_cast<const uint4 *>(w);
                 *reinterpret_cast<uint4 *>(vd + off) = *reinterpret_cast<const uint4 *>(x);
@@ -646,8 +646,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
                         *reinterpret_cast<uint32_t *>(dst + c) = pack2<T>(x, y);
                 }
                 else {
-                    dst[c] = out_of<T>(x);
-                    dst[c + 1] = out_of<T>(y);
+                    dst[c] = from_f<T>(x);
+                    dst[c + 1] = from_f<T>(y);
                 }
             }
         }
@@ -669,8 +669,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
                         *reinterpret_cast<uint32_t *>(dst + e) = pack2<T>(v[e], v[e + 1]);
                 }
                 else {
-                    dst[e] = out_of<T>(v[e]);
-                    dst[e + 1] = out_of<T>(v[e + 1]);
+                    dst[e] = from_f<T>(v[e]);
+                    dst[e + 1] = from_f<T>(v[e + 1]);
                 }
             }
     };
@@ -817,7 +817,7 @@ __global__ void __launch_bounds__(kThreads, HDP <= 64 ? 4 : 3) attn_few_kernel(c
                     T w[EPC];
 #pragma unroll
                     for (int e = 0; e < EPC; e++)
-                        w[e] = live ? src[e] : out_of<T>(0.0f);
+                        w[e] = live ? src[e] : from_f<T>(0.0f);
                     *reinterpret_cast<uint4 *>(buf + TL::at(r, lc)) = *reinterpret_cast<const uint4 *>(w);
                 }
             }
@@ -850,8 +850,8 @@ __global__ void __launch_bounds__(kThreads, HDP <= 64 ? 4 : 3) attn_few_kernel(c
                 T w[EPC], y[EPC];
 #pragma unroll
                 for (int e = 0; e < EPC; e++) {
-                    w[e] = live ? k1[e] : out_of<T>(0.0f);
-                    y[e] = live ? v1[e] : out_of<T>(0.0f);
+                    w[e] = live ? k1[e] : from_f<T>(0.0f);
+                    y[e] = live ? v1[e] : from_f<T>(0.0f);
                 }
                 *reinterpret_cast<uint4 *>(kd) = *reinterpret_cast<const uint4 *>(w);
                 *reinterpret_cast<uint4 *>(vd) = *reinterpret_cast<const uint4 *>(y);

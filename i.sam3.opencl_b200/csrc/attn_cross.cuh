@@ -7,9 +7,7 @@
 #include "div.cuh"
 #include "kernels.h"
 #include "tc_ptx.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include "vec.cuh"
 
 namespace sam3 {
 
@@ -50,30 +48,6 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
 // 2^-29 and rounded by 2^-40 below. bf16 and 32 bits have the exponents.
 template <typename T>
 constexpr float kWeightShift = __is_same(T, __half) ? 15.0f : 0.0f;
-
-__device__ __forceinline__ float ld_dsmem(uint32_t a)
-{
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-    return v;
-}
-template <typename T>
-__device__ __forceinline__ T out_of(float v);
-template <>
-__device__ __forceinline__ float out_of<float>(float v)
-{
-    return v;
-}
-template <>
-__device__ __forceinline__ __nv_bfloat16 out_of<__nv_bfloat16>(float v)
-{
-    return __float2bfloat16_rn(v);
-}
-template <>
-__device__ __forceinline__ __half out_of<__half>(float v)
-{
-    return __float2half_rn(v);
-}
 
 __device__ __forceinline__ void st_dsmem4(uint32_t a, float x, float y, float z, float w)
 {

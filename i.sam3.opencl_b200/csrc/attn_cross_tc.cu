@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                             else {
 #pragma unroll
                                 for (int i = 0; i < 8; i++)
-                                    dst[c + e + i] = out_of<T>(__uint_as_float(ov[e + i]) * inv);
+                                    dst[c + e + i] = from_f<T>(__uint_as_float(ov[e + i]) * inv);
                             }
                         }
                     }
@@ -635,10 +635,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             if (a.ovec)
                 *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<T>(x, y), pack2<T>(z, w));
             else {
-                dst[0] = out_of<T>(x);
-                dst[1] = out_of<T>(y);
-                dst[2] = out_of<T>(z);
-                dst[3] = out_of<T>(w);
+                dst[0] = from_f<T>(x);
+                dst[1] = from_f<T>(y);
+                dst[2] = from_f<T>(z);
+                dst[3] = from_f<T>(w);
             }
         });
     }

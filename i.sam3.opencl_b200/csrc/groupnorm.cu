@@ -33,9 +33,8 @@
 #include "pdl.cuh"
 #include "tc_ptx.cuh"
 #include "tmap.cuh"
+#include "vec.cuh"
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 namespace sam3 {
@@ -65,46 +64,6 @@ struct GnArgs {
     int span;               // a vector may hold channels of several groups
     float eps;
     int act;
-};
-
-template <typename T>
-__device__ __forceinline__ float to_f(T v);
-template <>
-__device__ __forceinline__ float to_f<float>(float v)
-{
-    return v;
-}
-template <>
-__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v)
-{
-    return __bfloat162float(v);
-}
-template <>
-__device__ __forceinline__ float to_f<__half>(__half v)
-{
-    return __half2float(v);
-}
-template <typename T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ float from_f<float>(float v)
-{
-    return v;
-}
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v)
-{
-    return __float2bfloat16_rn(v);
-}
-template <>
-__device__ __forceinline__ __half from_f<__half>(float v)
-{
-    return __float2half_rn(v);
-}
-
-template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-    T v[V];
 };
 
 // Values 2 e and 2 e + 1 of a vector (one value and 0 when V is 1).

@@ -7,17 +7,17 @@
 #include "pdl.cuh"
 #include "tc_ptx.cuh"
 #include "tmap.cuh"
+#include "vec.cuh"
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 namespace sam3 {
 namespace {
 
 // cos and sin of the angle of `turns` turns. The turns are reduced to a
-// quadrant q and a remainder in [-1/8, 1/8] in 64 bits (exact, so far
-// positions lose nothing); sine and cosine of the remainder's angle |x| <= pi / 4
+// quadrant q and a remainder in [-1/8, 1/8] in 64 bits, exactly; what far
+// positions lose is the rounding of the turns, position times frequency in
+// 64 bits (2^-21 of an angle at position 2^31); sine and cosine of the remainder's angle |x| <= pi / 4
 // are their Taylor polynomials in 32 bits, the first terms left out being
 // x^11 / 11! < 2e-9 and x^12 / 12! < 2e-10.
 __device__ __forceinline__ float2 cos_sin_turns(double turns)
@@ -96,29 +96,6 @@ struct RotArgs {
     Div nch, nhg, N;      // chunks of a head, head groups of a row, rows of a sequence
 };
 
-template <typename T>
-__device__ __forceinline__ float rd(T v)
-{
-    return (float)v;
-}
-template <typename T>
-__device__ __forceinline__ T wr(float v);
-template <>
-__device__ __forceinline__ float wr<float>(float v)
-{
-    return v;
-}
-template <>
-__device__ __forceinline__ __nv_bfloat16 wr<__nv_bfloat16>(float v)
-{
-    return __float2bfloat16_rn(v);
-}
-template <>
-__device__ __forceinline__ __half wr<__half>(float v)
-{
-    return __float2half_rn(v);
-}
-
 // A value that is not turned: its bits where the types agree (a NaN keeps its
 // payload), else rounded.
 template <typename TO, typename TI>
@@ -127,13 +104,8 @@ __device__ __forceinline__ TO copied(TI v)
     if constexpr (__is_same(TI, TO))
         return v;
     else
-        return wr<TO>(rd(v));
+        return from_f<TO>(to_f(v));
 }
-
-template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-    T v[V];
-};
 
 // A thread takes one chunk of W adjacent columns (HALVES: the W columns at j
 // and the W at half + j) of up to hpt heads of one row, so that the chunk's
@@ -203,17 +175,17 @@ __global__ void __launch_bounds__(256) rope_rotate_kernel(const __grid_constant_
                 if (HALVES || W == 1) {
 #pragma unroll
                     for (int e = 0; e < W; e++) {
-                        const float p0 = rd(u.v[e]), p1 = rd(w.v[e]);
-                        ou.v[e] = wr<TO>(p0 * cs[e].x - p1 * cs[e].y);
-                        ow.v[e] = wr<TO>(p0 * cs[e].y + p1 * cs[e].x);
+                        const float p0 = to_f(u.v[e]), p1 = to_f(w.v[e]);
+                        ou.v[e] = from_f<TO>(p0 * cs[e].x - p1 * cs[e].y);
+                        ow.v[e] = from_f<TO>(p0 * cs[e].y + p1 * cs[e].x);
                     }
                 }
                 else {
 #pragma unroll
                     for (int e = 0; e + 1 < W; e += 2) {
-                        const float p0 = rd(u.v[e]), p1 = rd(u.v[e + 1]);
-                        ou.v[e] = wr<TO>(p0 * cs[e / 2].x - p1 * cs[e / 2].y);
-                        ou.v[e + 1] = wr<TO>(p0 * cs[e / 2].y + p1 * cs[e / 2].x);
+                        const float p0 = to_f(u.v[e]), p1 = to_f(u.v[e + 1]);
+                        ou.v[e] = from_f<TO>(p0 * cs[e / 2].x - p1 * cs[e / 2].y);
+                        ou.v[e + 1] = from_f<TO>(p0 * cs[e / 2].y + p1 * cs[e / 2].x);
                     }
                 }
             }
