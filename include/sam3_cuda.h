@@ -432,7 +432,8 @@ int cb_attend(cb_backend *b, int Nq, int Nk, int heads, int hd, cb_mem Q,
  * backend's stream, allocates nothing and uses no scratch buffer, so it may be
  * captured into a graph, as its first call too, and several captured calls
  * may replay at once on their own buffers. An output may not overlap an
- * input, except where in-place use is named. */
+ * input, except where in-place use is named: the spans from the first to the
+ * last element of both, so interleaved operands of one buffer are refused. */
 
 /* Frequencies of a table: pair j of rot columns turns by w_j per position,
  *   NONE:   w_j = theta^(-2j / rot);
@@ -486,10 +487,12 @@ int cb_rope_rotate(cb_backend *b, int nb, int N, int heads, int hd, int rot,
  * not enter the result; a row without a visible key, or whose visible scores
  * are all -inf, gets zeros. Softmax and sums in 32 bits; F32 operands keep
  * about 21 bits of each product (finite values, any size of V; numbers below
- * 2^-100 beside far larger ones of the same head keep fewer), BF16 / F16
- * weights are rounded to the operands' type before the product with V (F16: by
- * half a step of the type or 2^-34 of the row's largest weight, whichever is
- * more) and divided by their sum last: BF16 values of V below 2^127 / Nk. */
+ * 2^-100 beside far larger ones of the same head keep fewer). Of BF16 / F16
+ * over many keys a quarter of the exponentials are off by 7.5e-5 of
+ * themselves; their weights are rounded to the operands' type before the
+ * product with V (F16: by half a step of the type or 2^-34 of the row's largest
+ * weight, whichever is more) and divided by their sum last: BF16 values of V
+ * below 2^127 / Nk. */
 int cb_cross_attend(cb_backend *b, int nb, int Nq, int Nk, int heads,
                     int kvheads, int hd, struct cb_opnd Q, struct cb_opnd K,
                     struct cb_opnd V, struct cb_opnd O, cb_mem klen,
@@ -500,7 +503,8 @@ int cb_cross_attend(cb_backend *b, int nb, int Nq, int Nk, int heads,
  * + bias[c]), mean and variance over the npix pixels and C / groups adjacent
  * channels of (b, group), in 32 bits. X, Y: [nb, npix, C] with pixel stride ld
  * and sample stride s0 (s1 0); one type, or X F32 and Y BF16 / F16; g, bias
- * F32 [C]. Y may be X (same layout). */
+ * F32 [C]. GELU is 0.5 z (1 + erf(z / sqrt 2)) as written for F32 results; for
+ * BF16 / F16 ones its negative tail keeps its bits. Y may be X (same layout). */
 int cb_groupnorm(cb_backend *b, int nb, int64_t npix, int C, int groups,
                  struct cb_opnd X, struct cb_opnd Y, cb_mem g, cb_mem bias,
                  float eps, int act);
