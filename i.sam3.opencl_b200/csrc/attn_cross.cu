@@ -20,8 +20,7 @@
 // and merges (max, sum, output) through distributed shared memory (Parts in
 // attn_cross.cuh). Measured: 8 sequences x 1 query of 16 heads over 1500 keys
 // of 4 heads of 64 columns 8.5 us (1 CTA a tile 19; three steps 3.3 us, the
-// exchange 1.3), 32 x 1 query over 2048 keys of 8 heads of 128 columns 48 us, 5.6
-// TB/s.
+// exchange 1.3).
 //
 // bf16 / f16: products on mma.m16n8k16 with fp32 accumulation, P rounded to
 // the operands' type (half a unit in the last place, 2^-8 / 2^-11 of a weight,
@@ -761,12 +760,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
 // one pass of softmax without a running maximum, row sums as a product with
 // ones, -inf of hidden keys as the scores' first accumulator; results go back
 // through the rows' buffer so that they are stored as 16-byte vectors. 8 x 5184
-// rows x 8 heads of 32 columns over 39 keys: 13.9 us, 3.0 TB/s (13.5 us before
-// hidden keys were hidden twice; the variants below against that); the same loop
-// without its arithmetic copies at 5.9 TB/s, so the instructions per row bound
-// it (issue slots half full at 16 warps per SM; key and value fragments kept in
-// registers 14.0 us, 5 or 6 CTAs per SM 15.2 and 16.4, two row groups per
-// warp 15.9).
+// rows x 8 heads of 32 columns over 39 keys: 14.5 us, 2.9 TB/s. No unit is full
+// (issue slots 53 %, matrix unit 31 %, half the copy rate): what a warp waits for
+// is its own chain of fragment loads, products, maxima, exponentials, products
+// and the way out, at 14 warps per SM; the same loop without its arithmetic
+// copies at 5.9 TB/s. Key and value fragments kept in registers, 5 or 6 CTAs per SM
+// and two row groups per warp were slower (by 3 %, 11 to 20 %, 16 %).
 template <typename T, int HDP, int KT>
 __global__ void __launch_bounds__(kThreads, HDP <= 64 ? 4 : 3) attn_few_kernel(const __grid_constant__ XaArgs a)
 {

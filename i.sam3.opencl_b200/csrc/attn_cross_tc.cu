@@ -22,10 +22,11 @@
 // tile whose sum reaches kOverflowSum (or is not a number; the polynomial
 // exponential makes 2^125 of one) is taken again with a raised offset, without
 // the polynomial, so that infinities and NaN of visible keys come out as such.
-// Measured: 8 x 5184 queries x 5184 keys x 16 heads of 64 columns 1012 us, 870
-// TFLOP/s (the softmax warps bound it as in attn_tc.cu: 884); 4 x 4096 x 4096 x
-// 16 heads of 128 columns 467 us, 1177 TFLOP/s; with a key mask 1164 us, every
-// tile in the rolled path.
+// Measured: 8 x 5184 queries x 5184 keys x 16 heads of 64 columns 1028 us, 857
+// TFLOP/s (the softmax warps bound it as in attn_tc.cu: 879), with a key mask, every
+// tile in the rolled path, 1173 us; 4 x 4096 x 4096 x 16 heads of 128 columns 483
+// us, 1138 TFLOP/s (tensor pipe 60 %); 32 x 1 query over 2048 keys of 8 heads of 128
+// columns 45 us, 5.9 TB/s.
 #include "attn_cross.cuh"
 #include "cluster.cuh"
 #include "kernels.h"
