@@ -18,9 +18,9 @@
 // A thread owns a vector of channels and steps over pixels. Statistics in
 // fp32 without the cancellation of E[x^2] - E[x]^2: per channel, kUnroll
 // pixels at a time are reduced to their own mean and M2 = sum (x - mean)^2 and
-// merged into the running pair (mean += d f, M2 += M2' + d^2 n f, d = mean' -
-// mean, f = n' / (n + n'); Chan, Golub and LeVeque 1979), two channels to an
-// instruction; channels, threads and CTAs are merged by sum n_i mean_i / n and
+// merged into the running pair (mean += d f, M2 += M2' + (n f d) d, d = mean' -
+// mean, f = n' / (n + n'); Chan, Golub and LeVeque 1979; with the first n = 0 no
+// square of a mean is formed, which may pass 32 bits), two channels to an instruction; channels, threads and CTAs are merged by sum n_i mean_i / n and
 // sum M2_i + n_i (mean_i - mean)^2 in a fixed order, so a result does not depend
 // on timing. 4 x 288 x 288 x 256 bf16, 8 groups: 88 us, 5.3 TB/s over the 459 MB
 // that cross HBM (X 1.7 times, Y once); one sample 31 us (clusters of 10, 80
@@ -62,6 +62,7 @@ struct GnArgs {
     int cs;                 // cluster size
     int bpk, nring;         // batches of kUnroll steps per block of vectors, of the ring
     int span;               // a vector may hold channels of several groups
+    float share;            // 1 / values of a group
     float eps;
     int act;
 };
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
                     }
                     const uint64_t d = fma2(mean[e], neg, mu);
                     mean[e] = fma2(d, f2, mean[e]);
-                    m2[e] = add2(m2[e], fma2(mul2(d, d), w2, q));
+                    m2[e] = add2(m2[e], fma2(mul2(d, w2), d, q));
                 }
             }
             else {
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
                     for (int e = 0; e < NP; e++) {
                         const uint64_t d = fma2(mean[e], f2_make(-1.0f, -1.0f), pair<TI, V>(v, e));
                         mean[e] = fma2(d, f2, mean[e]);
-                        m2[e] = fma2(mul2(d, d), w2, m2[e]);
+                        m2[e] = fma2(mul2(d, w2), d, m2[e]);
                     }
                 }
             }
@@ -332,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
                 q += fmaf((me[e] - mu) * (me[e] - mu), c, qe[e]);
             const float nn = c * V, n1 = tn + nn, f = nn / n1, d = mu - tmean;
             tmean = fmaf(d, f, tmean);
-            tm2 += fmaf(d * d, tn * f, q);
+            tm2 += fmaf(d * (tn * f), d, q);
             tn = n1;
         }
     }
@@ -342,7 +343,9 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
     // The members of a group are the threads of its vectors, or its (row,
     // channel) pairs; nparts warps share a group and each publishes its own
     // (n, mean, M2): the mean of its members first, then sum M2_i + n_i (mean_i -
-    // mean)^2. All parts of the cluster are then merged at once in the same way.
+    // mean)^2; n and M2 as shares of the group's values from here on, so that the
+    // sums are of the size of the mean and the variance. All parts of the
+    // cluster are then merged at once in the same way.
     constexpr int NW = kThreads / 32;
     const int warp = t >> 5, lane32 = t & 31;
     const int nparts = a.gps >= NW ? 1 : NW / a.gps;
@@ -350,10 +353,10 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
     const int pitch = a.span ? a.S : a.lpp;
     const int members = a.rows * width;
     const int dr = nparts * 32 / width, di = nparts * 32 - dr * width;  // to a lane's next member
-    auto size = [&](int r, int i) {  // values behind member i of row r
+    auto size = [&](int r, int i) {  // values behind member i of row r, as a share
         if (a.nk == 1)
-            return (float)count(r) * (a.span ? 1 : V);
-        return (float)np * V * (float)(i < a.lpp ? (a.lpp - 1 - i) / kThreads + 1 : 0);
+            return (float)count(r) * (a.span ? 1 : V) * a.share;
+        return (float)np * V * (float)(i < a.lpp ? (a.lpp - 1 - i) / kThreads + 1 : 0) * a.share;
     };
     for (int w = warp; w < a.gps * nparts; w += NW) {
         const int gi = w / nparts, part = w - gi * nparts;
@@ -370,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1) groupnorm_kernel(const __grid_con
                     const float2 st = mine_at[r * pitch + i];
                     if (pass == 0)
                         n += c;
-                    s += pass == 0 ? c * st.x : fmaf((st.x - mu) * (st.x - mu), c, st.y);
+                    s += pass == 0 ? c * st.x : fmaf((st.x - mu) * (st.x - mu), c, st.y * a.share);
                 }
                 i += di;
                 r += dr;
@@ -629,6 +632,7 @@ extern "C" int k_groupnorm(const void *X, int xt, long ldx, long sx, void *Y, in
     a.sy = sy;
     a.cg = C / groups;
     a.dcg = make_div(a.cg);
+    a.share = (float)(1.0 / ((double)npix * a.cg));
     a.eps = eps;
     a.act = act;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(s);

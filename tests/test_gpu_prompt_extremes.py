@@ -8,7 +8,7 @@ import math
 import pytest
 
 torch = pytest.importorskip("torch")
-from test_gpu_prompt_ops import (DT, attend_ref, attend_tol, be, check_attend, gen, op, randn, u)  # noqa: E402,F401
+from test_gpu_prompt_ops import (DT, attend_ref, attend_tol, be, check_attend, check_norm, gen, op, randn, u)  # noqa: E402,F401
 
 pytestmark = pytest.mark.gpu
 
@@ -344,3 +344,16 @@ def test_groupnorm_gelu_tail(be, tx, ty):
     tol = u(DT[ty]) * want.abs() + own * (1 + u(DT[ty])) + least
     err = (y[0].double() - want).abs()
     assert (err <= tol).all(), (float((err / tol).max()), float(z[(err / tol).amax(0).argmax()]))
+
+
+# ------------------------------------------------------------------ group norm: means whose squares pass 32 bits
+@pytest.mark.parametrize("nb,n,Cn,G,dt,ex", [(2, 3000, 32, 4, "f32", 57), (1, 3, 32, 4, "f32", 57), (1, 900, 60, 6, "f32", 55),
+                                             (1, 20000, 64, 8, "f32", 52), (1, 40, 2051, 1, "f32", 57),
+                                             (2, 500, 64, 8, "bf16", 60), (1, 2, 48, 4, "bf16", 62)])
+def test_groupnorm_means_of_any_size(be, nb, n, Cn, G, dt, ex):
+    """A mean near 2^67 (its square is 2^134) with deviations whose squares and their sums are finite."""
+    if dt == "f32":
+        x = (randn(gen(n), nb, n, Cn) + 1000.0) * 2.0 ** ex
+    else:
+        x = ((randn(gen(n), nb, n, Cn) + 16.0) * 2.0 ** ex).bfloat16()
+    check_norm(be, x, torch.empty_like(x), G, 0, steps=n // 16)
