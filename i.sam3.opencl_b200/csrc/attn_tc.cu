@@ -81,6 +81,9 @@ constexpr int kPolyPairsPer8 = 2;
 // polynomial, or inf / NaN) sends the tile through the maximum pass again with
 // a raised offset.
 constexpr float kOverflowSum = 8192.0f;
+// A row's sum at or above this (2^60) holds a score that is not a number: the
+// sums of finite ones stay below 2^13 a tile.
+constexpr float kNotANumber = 1.152921504606847e18f;
 constexpr int Q_BYTES = BQ * HD * 2;
 constexpr int KV_BYTES = BKV * HD * 2;
 constexpr int OFF_Q = 0;                       // [buffer], one query tile each
@@ -551,7 +554,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 float la, lb, lc, ld;
                 f2_split(lsum0, la, lb);
                 f2_split(lsum1, lc, ld);
-                const float lsum = (la + lb) + (lc + ld);
+                const float all = (la + lb) + (lc + ld);
+                const float lsum = all < kNotANumber ? all : NAN;
                 if (is_part && q < a.Nq) {
                     const long v = (long)blockIdx.x + (long)k * gridDim.x - a.nfull;
                     float *pr = a.part + (v * BQ + r) * kPartRow;

@@ -357,3 +357,20 @@ def test_groupnorm_means_of_any_size(be, nb, n, Cn, G, dt, ex):
     else:
         x = ((randn(gen(n), nb, n, Cn) + 16.0) * 2.0 ** ex).bfloat16()
     check_norm(be, x, torch.empty_like(x), G, 0, steps=n // 16)
+
+
+@pytest.mark.parametrize("N", [576, 130])
+def test_attention_not_a_number(be, sb, N):
+    """cb_attention: a key that is not a number makes every row of its head NaN at each kind of column of a tile, and no
+    row of another head or sequence."""
+    nb, h, hd = 2, 16, 64
+    E = h * hd
+    x = randn(gen(N), nb, N, 3, h, hd).bfloat16()
+    for j in (0, 12, 13, 14, 15, 100, N - 1):
+        y = x.clone()
+        y[1, j, 1, 3, 7] = math.nan
+        o = torch.zeros(nb * N, E, device="cuda")
+        be.attention(be.wrap(y.view(nb * N, 3 * E)), nb, N, E, h, hd, None, 0, 0.125, sb.ATTN_TC, be.wrap(o))
+        be.sync()
+        bad = o.view(nb, N, h, hd).isnan()
+        assert bad[1, :, 3].all() and int(bad.sum()) == N * hd
