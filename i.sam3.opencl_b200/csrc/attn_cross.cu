@@ -748,10 +748,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && HDP == 32 ? 4 : 1)
     }
     cluster_sync_all();
     const int live = rows > rank ? (rows - 1 - rank) / a.cs + 1 : 0;
-    PT::template merge<kThreads, F32>(part, a.cs, rl, live, a.scale_log2, [&](int i, int c, float x, float y, float z, float w) {
-        const float v[4] = {x, y, z, w};
-        store(i * a.cs + rank, c, v);
-    });
+    PT::template merge<kThreads, F32>(part, a.cs, rl, live, a.scale_log2,
+                                      [&](int i, int c, float x, float y, float z, float w) {
+                                          const float v[4] = {x, y, z, w};
+                                          store(i * a.cs + rank, c, v);
+                                      });
 }
 
 // Few keys (all in one step) and many rows. A CTA reads the keys and values of

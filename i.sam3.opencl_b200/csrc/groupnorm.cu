@@ -20,9 +20,10 @@
 // pixels at a time are reduced to their own mean and M2 = sum (x - mean)^2 and
 // merged into the running pair (mean += d f, M2 += M2' + (n f d) d, d = mean' -
 // mean, f = n' / (n + n'); Chan, Golub and LeVeque 1979; with the first n = 0 no
-// square of a mean is formed, which may pass 32 bits), two channels to an instruction; channels, threads and CTAs are merged by sum n_i mean_i / n and
-// sum M2_i + n_i (mean_i - mean)^2 in a fixed order, so a result does not depend
-// on timing. 4 x 288 x 288 x 256 bf16, 8 groups: 88 us, 5.3 TB/s over the 459 MB
+// square of a mean is formed, which may pass 32 bits), two channels to an
+// instruction; channels, threads and CTAs are merged by sum n_i mean_i / n and sum
+// M2_i + n_i (mean_i - mean)^2 in a fixed order, so a result does not depend on
+// timing. 4 x 288 x 288 x 256 bf16, 8 groups: 89 us, 5.2 TB/s over the 459 MB
 // that cross HBM (X 1.7 times, Y once); one sample 31 us (clusters of 10, 80
 // CTAs); 72 x 72 x 256 6.8 us, of which the exchange takes 2.5.
 // Per-channel pairs cost about as many instructions as one pair per
