@@ -384,9 +384,9 @@ def _handles(s):
 
 def _own(s):
     c = s["case"]
-    if "h" not in s:
-        s["h"] = _handles(s)
-    h, cb = s["h"], _lib["cb"]
+    if "handles" not in s:
+        s["handles"] = _handles(s)
+    h, cb = s["handles"], _lib["cb"]
     if c["op"] == "gemm":
         cb.gemm_e4m3(c["M"], c["N"], c["K"], h["a"], h["sa"], h["b"], h["sb"], h["c"], h["sc"], h["bias"], h["act"])
         return s["c"] if s["sc"] is None else (s["c"], s["sc"])
