@@ -22,10 +22,12 @@ NVCC = os.path.join(CUDA, "bin", "nvcc")
 
 CU = ["gemm_tc.cu", "attn_tc.cu", "attn_simt.cu", "attn_decoder.cu", "elementwise.cu", "attn_noalloc.cu",
       "decoder.cu", "neck.cu", "input.cu",
-      "detector.cu", "rotary.cu", "attn_cross.cu", "attn_cross_tc.cu", "groupnorm.cu"]
+      "detector.cu", "rotary.cu", "attn_cross.cu", "attn_cross_tc.cu", "groupnorm.cu",
+      "quantize.cu", "norm_residual.cu", "gemm_e4m3.cu"]
 C = ["cuda_backend.c", "sam3_ops.c", "sam3_encoder.c", "sam3_decoder.c", "sam3_neck.c", "sam3_input.c",
-     "sam3_prompt.c", "synth.c"]
-HEADERS = ["tc_ptx.cuh", "tmap.cuh", "pdl.cuh", "attn_cross.cuh", "cluster.cuh", "div.cuh", "vec.cuh", "kernels.h", "backend_internal.h"]
+     "sam3_prompt.c", "sam3_block.c", "synth.c"]
+HEADERS = ["tc_ptx.cuh", "tmap.cuh", "pdl.cuh", "attn_cross.cuh", "cluster.cuh", "div.cuh", "vec.cuh", "vec8.cuh", "act.cuh", "e4m3.cuh", "kernels.h",
+           "backend_internal.h", "operand.h"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC",

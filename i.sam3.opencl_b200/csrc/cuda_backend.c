@@ -19,6 +19,8 @@ size_t cbi_dtype_size(int dtype)
     case CB_F16:
         return 2;
     case CB_U8:
+    case CB_E4M3:
+    case CB_E8M0:
         return 1;
     default:
         return 0;

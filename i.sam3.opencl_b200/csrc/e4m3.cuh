@@ -1,0 +1,77 @@
+// SPDX-License-Identifier: Unlicense
+// Blocks of E4M3 values with a power-of-two scale.
+#pragma once
+
+#include "kernels.h"
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace sam3 {
+
+constexpr int kScaleBlock = 128;
+
+// Bits of |x| of a finite x, 0 of an infinity or NaN: largest by integer max.
+__device__ __forceinline__ uint32_t finite_bits(float x)
+{
+    const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
+    return u < 0x7f800000u ? u : 0u;
+}
+
+// The scale of a block whose largest finite magnitude has the bits u, as the
+// E8M0 byte e + 127: the smallest e >= -126 with the magnitude at most 448 2^e =
+// 1.75 * 2^(8 + e). Adding 2^21 - 1 carries into the exponent exactly when the
+// fraction is above 0.75.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t u)
+{
+    const uint32_t x = (u + 0x1fffffu) >> 23;
+    return x > 9 ? x - 8 : 1u;
+}
+__device__ __forceinline__ float scale_value(uint32_t byte)
+{
+    return __uint_as_float(byte << 23);
+}
+// 1 / scale (bytes 1 .. 247: a normal number).
+__device__ __forceinline__ float scale_inverse(uint32_t byte)
+{
+    return __uint_as_float((254u - byte) << 23);
+}
+
+// Four values times the inverse scale, to nearest; the product is exact or far
+// below E4M3's smallest number. x 0 added turns an infinity, which the
+// conversion would saturate, into NaN.
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d, float inv)
+{
+    uint16_t lo, hi;
+    a = fmaf(a, 0.0f, a * inv);
+    b = fmaf(b, 0.0f, b * inv);
+    c = fmaf(c, 0.0f, c * inv);
+    d = fmaf(d, 0.0f, d * inv);
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+
+// A scale as it is stored (E8M0 byte or fp32 bits) and its value.
+__device__ __forceinline__ uint32_t scale_raw(const void *p, int dt, long i)
+{
+    return dt == K_E8M0 ? (uint32_t)__ldg(reinterpret_cast<const uint8_t *>(p) + i)
+                        : __ldg(reinterpret_cast<const uint32_t *>(p) + i);
+}
+__device__ __forceinline__ float scale_of(uint32_t raw, int dt)
+{
+    if (dt != K_E8M0)
+        return __uint_as_float(raw);
+    // 2^-127 is below the normal numbers, 255 stands for NaN
+    return raw == 0 ? __uint_as_float(0x00400000u)
+                    : __uint_as_float(raw == 255 ? 0x7fffffffu : raw << 23);
+}
+__device__ __forceinline__ void put_scale(void *p, int dt, long i, uint32_t byte)
+{
+    if (dt == K_E8M0)
+        reinterpret_cast<uint8_t *>(p)[i] = (uint8_t)byte;
+    else
+        reinterpret_cast<float *>(p)[i] = scale_value(byte);
+}
+
+}  // namespace sam3

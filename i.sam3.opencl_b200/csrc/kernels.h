@@ -273,24 +273,36 @@ int k_attend_simt(int Nq, int Nk, int heads, int hd, const float *Q, int ldq,
 #define K_F32 0
 #define K_BF16 1
 #define K_F16 2
+#define K_E4M3 5 /* 8-bit floating point */
+#define K_E8M0 6 /* powers of two, scales of E4M3 blocks */
 #define K_ROPE_HALVES 1 /* pair j = columns (j, rot / 2 + j); 0: (2j, 2j + 1) */
 #define K_ROPE_MAX 256  /* rotated columns of a table */
 
 /* Rows of an operand: element (b, n, h, d) at p[b * s0 + n * ld + h * s1 + d]. */
 struct k_rows {
     void *p;
-    int dt; /* K_F32, K_BF16, K_F16 */
+    int dt; /* K_F32, K_BF16, K_F16, K_E4M3, K_E8M0 */
     long ld, s0, s1;
 };
 
 /* cs[p * rot / 2 + j] = amp (cos, sin) of (first + p) * turns[j] turns. */
 int k_rope_table(int npos, int rot, long first, const double *turns, float amp,
                  float *cs, k_stream s);
+/* Several axes: pair j turns by the position on axis[j], pos [nb, N, axes] or
+ * row n's coordinates in a grid (last axis fastest); sections: the pairs of an
+ * axis are adjacent. */
+#define K_ROPE_AXES 4
+struct k_rope_axes {
+    int axes, sections;
+    int grid[K_ROPE_AXES];
+    uint8_t axis[K_ROPE_MAX / 2];
+};
 /* Y = X with the first rot columns of every head rotated by table row pos[b *
- * N + n] (pos NULL: pos0 + n), rows outside the table copied; X may be Y. */
+ * N + n] (pos NULL: pos0 + n), rows outside the table copied; X may be Y. axes
+ * NULL: one. */
 int k_rope_rotate(const struct k_rows *X, const struct k_rows *Y, int nb, int N,
                   int heads, int hd, int rot, int layout, const int *pos, int pos0,
-                  int npos, const float *cs, k_stream s);
+                  int npos, const float *cs, const struct k_rope_axes *axes, k_stream s);
 /* Attention of Nq query rows over the visible ones of Nk key rows, heads /
  * kvheads query heads per key head; all operands of one type. */
 int k_cross_attend(const struct k_rows *Q, const struct k_rows *K,
@@ -302,6 +314,36 @@ int k_cross_attend(const struct k_rows *Q, const struct k_rows *K,
 int k_groupnorm(const void *X, int xt, long ldx, long sx, void *Y, int yt, long ldy,
                 long sy, const float *g, const float *b, int nb, long npix, int C,
                 int groups, float eps, int act, k_stream s);
+
+/* ---- 8-bit products and what stands around them in a block (sam3_block.c
+ * checks the arguments; blocks and scales: sam3_cuda.h) */
+/* Q E4M3 [nb, N, K] and S [nb, ceil(N / brows), ceil(K / 128)] of X; brows 1 or
+ * 128. */
+int k_quantize_e4m3(const struct k_rows *X, const struct k_rows *Q, const struct k_rows *S, int nb,
+                    int N, int K, int brows, k_stream s);
+/* C [M, N] = act(A B^T + bias) of E4M3 A [M, K], B [N, K] with scales SA [M, kb],
+ * SB [ceil(N / 128), kb]; C E4M3 with scales SC [M, ceil(N / 128)], or SC NULL. */
+int k_gemm_e4m3(int M, int N, int K, const struct k_rows *A, const struct k_rows *SA,
+                const struct k_rows *B, const struct k_rows *SB, const struct k_rows *C,
+                const struct k_rows *SC, const float *bias, int act, int *err, k_stream s);
+#define K_NORM_NONE 0
+#define K_NORM_LAYER 1
+#define K_NORM_RMS 2
+struct k_norm {
+    int kind;
+    float eps;
+    const float *g, *b; /* NULL: 1 and 0 */
+};
+/* h = post(H), r = X + alpha ls gate h (H.p NULL: r = X), R = r, Y = pre(r) (1 +
+ * scale) + shift; p NULL where an operand is absent (S: the scales of an E4M3 Y). */
+struct k_norm_args {
+    int nb, N, C;
+    struct k_rows X, H, gate, R, scale, shift, Y, S;
+    struct k_norm post, pre;
+    float alpha;
+    const float *ls;
+};
+int k_norm_residual(const struct k_norm_args *a, k_stream s);
 
 /* uint8 HWC tiles -> bf16 patch rows in window-major token order:
  * out[ntile * grid^2, kpad], column c*ps*ps + ky*ps + kx (the Conv2d weight

@@ -96,6 +96,16 @@ struct RotArgs {
     Div nch, nhg, N;      // chunks of a head, head groups of a row, rows of a sequence
 };
 
+// Several axes: the axis of each pair, and the extents a row's coordinates are
+// taken by when there are no positions.
+struct RotAxes {
+    int axes, sections;
+    Div grid[K_ROPE_AXES];
+    uint8_t axis[K_ROPE_MAX / 2];
+};
+struct OneAxis {
+};
+
 // A value that is not turned: its bits where the types agree (a NaN keeps its
 // payload), else rounded.
 template <typename TO, typename TI>
@@ -114,9 +124,13 @@ __device__ __forceinline__ TO copied(TI v)
 // are not 16-byte aligned. Memory bound: X read and Y written once, the
 // table rows from L2; 41472 rows of 24 heads of 64 bf16 columns 48 us, 5.3 TB/s
 // (81 % of a copy). Indexes without divisions (56 us with 64-bit ones).
-template <typename TI, typename TO, int W, bool HALVES>
-__global__ void __launch_bounds__(256) rope_rotate_kernel(const __grid_constant__ RotArgs a)
+// AX = RotAxes: each pair takes the table row of its own axis; pairs of one axis
+// as a vector where a chunk has no others.
+template <typename TI, typename TO, int W, bool HALVES, typename AX>
+__global__ void __launch_bounds__(256) rope_rotate_kernel(const __grid_constant__ RotArgs a,
+                                                          const __grid_constant__ AX ax)
 {
+    constexpr bool MANY = !__is_same(AX, OneAxis);
     constexpr int CW = HALVES || W > 1 ? W : 2;     // columns of a vector
     constexpr int NP = HALVES ? W : CW / 2;         // pairs of a chunk
     using VI = Vec<TI, W>;
@@ -131,25 +145,70 @@ __global__ void __launch_bounds__(256) rope_rotate_kernel(const __grid_constant_
         const int hg = (int)(rg - rl * a.nhg.d);
         const uint32_t row = a.row0 + rl;
         const long b = quot(row, a.N), n = row - (uint32_t)b * a.N.d;
-        const long p = a.pos ? (long)__ldg(a.pos + row) : a.pos0 + n;
-        const bool turn = c < a.nrot && p >= 0 && p < a.npos;
+        uint32_t turns = 0;  // bit e: pair e of the chunk is turned
         const TI *x = reinterpret_cast<const TI *>(a.x) + b * a.sx0 + n * a.ldx;
         TO *y = reinterpret_cast<TO *>(a.y) + b * a.sy0 + n * a.ldy;
         float2 cs[NP];
-        if (turn) {
-            const float2 *src = a.cs + p * a.half + c * NP;
-            if (NP % 2 == 0) {
+        if constexpr (MANY) {
+            int p[K_ROPE_AXES];
+            uint32_t left = (uint32_t)n;
 #pragma unroll
-                for (int e = 0; e < NP; e += 2) {
-                    const float4 v = __ldg(reinterpret_cast<const float4 *>(src + e));
-                    cs[e] = make_float2(v.x, v.y);
-                    cs[e + 1 < NP ? e + 1 : e] = make_float2(v.z, v.w);
+            for (int k = K_ROPE_AXES - 1; k >= 0; k--) {
+                p[k] = -1;
+                if (k < ax.axes && a.pos)
+                    p[k] = __ldg(a.pos + (long)row * ax.axes + k);
+                else if (k < ax.axes) {
+                    const uint32_t q = quot(left, ax.grid[k]);
+                    p[k] = (int)(left - q * ax.grid[k].d);
+                    left = q;
                 }
             }
-            else {
+            auto position = [&](int k) { return k == 0 ? p[0] : (k == 1 ? p[1] : (k == 2 ? p[2] : p[3])); };
+            if (c < a.nrot) {
+                const float2 *src = a.cs + c * NP;
+                const int k0 = ax.axis[c * NP];
+                if (NP % 2 == 0 && ax.sections && k0 == ax.axis[c * NP + NP - 1]) {
+                    const int pk = position(k0);
+                    if (pk >= 0 && pk < a.npos) {
+                        turns = (1u << NP) - 1;
 #pragma unroll
-                for (int e = 0; e < NP; e++)
-                    cs[e] = __ldg(src + e);
+                        for (int e = 0; e < NP; e += 2) {
+                            const float4 v = __ldg(reinterpret_cast<const float4 *>(src + (long)pk * a.half + e));
+                            cs[e] = make_float2(v.x, v.y);
+                            cs[e + 1 < NP ? e + 1 : e] = make_float2(v.z, v.w);
+                        }
+                    }
+                }
+                else {
+#pragma unroll
+                    for (int e = 0; e < NP; e++) {
+                        const int pk = position(ax.axis[c * NP + e]);
+                        if (pk >= 0 && pk < a.npos) {
+                            turns |= 1u << e;
+                            cs[e] = __ldg(src + (long)pk * a.half + e);
+                        }
+                    }
+                }
+            }
+        }
+        else {
+            const long p = a.pos ? (long)__ldg(a.pos + row) : a.pos0 + n;
+            if (c < a.nrot && p >= 0 && p < a.npos) {
+                turns = (1u << NP) - 1;
+                const float2 *src = a.cs + p * a.half + c * NP;
+                if (NP % 2 == 0) {
+#pragma unroll
+                    for (int e = 0; e < NP; e += 2) {
+                        const float4 v = __ldg(reinterpret_cast<const float4 *>(src + e));
+                        cs[e] = make_float2(v.x, v.y);
+                        cs[e + 1 < NP ? e + 1 : e] = make_float2(v.z, v.w);
+                    }
+                }
+                else {
+#pragma unroll
+                    for (int e = 0; e < NP; e++)
+                        cs[e] = __ldg(src + e);
+                }
             }
         }
         // copied chunks follow the rotated ones: single vectors from column 2 half on
@@ -171,10 +230,12 @@ __global__ void __launch_bounds__(256) rope_rotate_kernel(const __grid_constant_
                 ou.v[e] = copied<TO>(u.v[e]);
                 ow.v[e] = copied<TO>(w.v[e]);
             }
-            if (turn) {
+            if (turns) {
                 if (HALVES || W == 1) {
 #pragma unroll
                     for (int e = 0; e < W; e++) {
+                        if (MANY && !(turns >> e & 1))
+                            continue;
                         const float p0 = to_f(u.v[e]), p1 = to_f(w.v[e]);
                         ou.v[e] = from_f<TO>(p0 * cs[e].x - p1 * cs[e].y);
                         ow.v[e] = from_f<TO>(p0 * cs[e].y + p1 * cs[e].x);
@@ -183,6 +244,8 @@ __global__ void __launch_bounds__(256) rope_rotate_kernel(const __grid_constant_
                 else {
 #pragma unroll
                     for (int e = 0; e + 1 < W; e += 2) {
+                        if (MANY && !(turns >> (e / 2) & 1))
+                            continue;
                         const float p0 = to_f(u.v[e]), p1 = to_f(u.v[e + 1]);
                         ou.v[e] = from_f<TO>(p0 * cs[e / 2].x - p1 * cs[e / 2].y);
                         ou.v[e + 1] = from_f<TO>(p0 * cs[e / 2].y + p1 * cs[e / 2].x);
@@ -196,8 +259,8 @@ __global__ void __launch_bounds__(256) rope_rotate_kernel(const __grid_constant_
     }
 }
 
-template <typename TI, typename TO, int W, bool HALVES>
-int launch(RotArgs &a, long rows, int N, int hd, bool in_place, cudaStream_t s)
+template <typename TI, typename TO, int W, bool HALVES, typename AX>
+int launch(RotArgs &a, const AX &ax, long rows, int N, int hd, bool in_place, cudaStream_t s)
 {
     const int rot = 2 * a.half;
     a.nrot = HALVES ? a.half / W : (W > 1 ? rot / W : a.half);
@@ -219,16 +282,16 @@ int launch(RotArgs &a, long rows, int N, int hd, bool in_place, cudaStream_t s)
         const long n = rows - r < most ? rows - r : most;
         a.row0 = (uint32_t)r;
         a.total = (uint32_t)(n * nch * nhg);
-        const int rc = launch_pdl(rope_rotate_kernel<TI, TO, W, HALVES>, dim3((a.total + 255) / 256), dim3(256),
-                                  0, s, (const RotArgs)a);
+        const int rc = launch_pdl(rope_rotate_kernel<TI, TO, W, HALVES, AX>, dim3((a.total + 255) / 256), dim3(256),
+                                  0, s, (const RotArgs)a, ax);
         if (rc)
             return rc;
     }
     return 0;
 }
 
-template <typename TI, typename TO>
-int launch_w(RotArgs &a, long rows, int N, int hd, int layout, bool in_place, cudaStream_t s)
+template <typename TI, typename TO, typename AX>
+int launch_w(RotArgs &a, const AX &ax, long rows, int N, int hd, int layout, bool in_place, cudaStream_t s)
 {
     constexpr int W = 16 / sizeof(TI);
     const int rot = 2 * a.half;
@@ -239,8 +302,24 @@ int launch_w(RotArgs &a, long rows, int N, int hd, int layout, bool in_place, cu
                      reinterpret_cast<uintptr_t>(a.y) % (W * sizeof(TO)) == 0 &&
                      !(reinterpret_cast<uintptr_t>(a.cs) & 15);
     if (layout == K_ROPE_HALVES)
-        return vec ? launch<TI, TO, W, true>(a, rows, N, hd, in_place, s) : launch<TI, TO, 1, true>(a, rows, N, hd, in_place, s);
-    return vec ? launch<TI, TO, W, false>(a, rows, N, hd, in_place, s) : launch<TI, TO, 1, false>(a, rows, N, hd, in_place, s);
+        return vec ? launch<TI, TO, W, true>(a, ax, rows, N, hd, in_place, s) : launch<TI, TO, 1, true>(a, ax, rows, N, hd, in_place, s);
+    return vec ? launch<TI, TO, W, false>(a, ax, rows, N, hd, in_place, s) : launch<TI, TO, 1, false>(a, ax, rows, N, hd, in_place, s);
+}
+
+template <typename AX>
+int launch_t(RotArgs &a, const AX &ax, int xt, int yt, long rows, int N, int hd, int layout, bool in_place, cudaStream_t st)
+{
+    if (xt == K_F32 && yt == K_F32)
+        return launch_w<float, float>(a, ax, rows, N, hd, layout, in_place, st);
+    if (xt == K_F32 && yt == K_BF16)
+        return launch_w<float, __nv_bfloat16>(a, ax, rows, N, hd, layout, in_place, st);
+    if (xt == K_F32 && yt == K_F16)
+        return launch_w<float, __half>(a, ax, rows, N, hd, layout, in_place, st);
+    if (xt == K_BF16 && yt == K_BF16)
+        return launch_w<__nv_bfloat16, __nv_bfloat16>(a, ax, rows, N, hd, layout, in_place, st);
+    if (xt == K_F16 && yt == K_F16)
+        return launch_w<__half, __half>(a, ax, rows, N, hd, layout, in_place, st);
+    return K_EARG;
 }
 
 }  // namespace
@@ -270,7 +349,7 @@ extern "C" int k_rope_table(int npos, int rot, long first, const double *turns, 
 
 extern "C" int k_rope_rotate(const struct k_rows *X, const struct k_rows *Y, int nb, int N, int heads,
                              int hd, int rot, int layout, const int *pos, int pos0, int npos,
-                             const float *cs, k_stream s)
+                             const float *cs, const struct k_rope_axes *axes, k_stream s)
 {
     using namespace sam3;
     if (nb <= 0 || N <= 0 || heads <= 0 || rot <= 0 || (rot & 1) || rot > hd)
@@ -292,15 +371,17 @@ extern "C" int k_rope_rotate(const struct k_rows *X, const struct k_rows *Y, int
     a.half = rot / 2;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(s);
     const bool in_place = X->p == Y->p;  // the caller has checked that the layouts agree
-    if (X->dt == K_F32 && Y->dt == K_F32)
-        return launch_w<float, float>(a, (long)nb * N, N, hd, layout, in_place, st);
-    if (X->dt == K_F32 && Y->dt == K_BF16)
-        return launch_w<float, __nv_bfloat16>(a, (long)nb * N, N, hd, layout, in_place, st);
-    if (X->dt == K_F32 && Y->dt == K_F16)
-        return launch_w<float, __half>(a, (long)nb * N, N, hd, layout, in_place, st);
-    if (X->dt == K_BF16 && Y->dt == K_BF16)
-        return launch_w<__nv_bfloat16, __nv_bfloat16>(a, (long)nb * N, N, hd, layout, in_place, st);
-    if (X->dt == K_F16 && Y->dt == K_F16)
-        return launch_w<__half, __half>(a, (long)nb * N, N, hd, layout, in_place, st);
-    return K_EARG;
+    if (axes) {
+        RotAxes ax = {};
+        if (axes->axes < 1 || axes->axes > K_ROPE_AXES || rot > K_ROPE_MAX)
+            return K_EARG;
+        ax.axes = axes->axes;
+        ax.sections = axes->sections;
+        for (int k = 0; k < K_ROPE_AXES; k++)
+            ax.grid[k] = make_div(axes->grid[k] > 0 ? axes->grid[k] : 1);
+        for (int j = 0; j < rot / 2; j++)
+            ax.axis[j] = axes->axis[j];
+        return launch_t(a, ax, X->dt, Y->dt, (long)nb * N, N, hd, layout, in_place, st);
+    }
+    return launch_t(a, OneAxis{}, X->dt, Y->dt, (long)nb * N, N, hd, layout, in_place, st);
 }

@@ -5,129 +5,17 @@
  * enqueues one kernel on the backend stream; none uses the scratch buffer, so
  * captured graphs and other calls share no memory with them. */
 #include <math.h>
-#include <string.h>
 
-#include "backend_internal.h"
+#include "operand.h"
 
-#define MAX_ROWS (1 << 30) /* rows of one sequence */
-
-/* Elements an operand of counts n (strides st) and hd adjacent columns spans;
- * -1 when a stride is negative or the span passes 2^62. */
-static int64_t span(const int64_t *n, const int64_t *st, int k, int64_t hd)
+/* Turns per position of the pairs of a ladder of rot columns; CB_EARG. */
+static int rope_turns(cb_backend *b, int rot, const struct cb_rope_scaling *sc, double *turns)
 {
-    __int128 s = hd;
-    int i;
-
-    for (i = 0; i < k; i++) {
-        if (st[i] < 0)
-            return -1;
-        s += (__int128)(n[i] - 1) * st[i];
-        if (s > ((__int128)1 << 62))
-            return -1;
-    }
-    return (int64_t)s;
-}
-
-/* Whether no two of the operand's elements share an address. */
-static int distinct(const int64_t *n, const int64_t *st, int k, int64_t hd)
-{
-    int64_t extent = hd;
-    int done[3] = {0, 0, 0}, i, step;
-
-    for (step = 0; step < k; step++) {
-        int best = -1;
-
-        for (i = 0; i < k; i++)
-            if (!done[i] && (best < 0 || (n[i] > 1 ? st[i] : 0) < (n[best] > 1 ? st[best] : 0)))
-                best = i;
-        done[best] = 1;
-        if (n[best] == 1)
-            continue;
-        if (st[best] < extent)
-            return 0;
-        extent += (n[best] - 1) * st[best];
-    }
-    return 1;
-}
-
-struct rows {
-    struct k_rows k;
-    const char *lo, *hi; /* bytes it spans */
-};
-
-static int float_dt(int dt)
-{
-    return dt == CB_F32 || dt == CB_BF16 || dt == CB_F16;
-}
-
-/* Checks [nb, rows, heads, hd] at o and fills r; CB_EARG / CB_EDTYPE. */
-static int take(const struct cb_opnd *o, int64_t nb, int64_t rows, int64_t heads, int64_t hd,
-                int output, struct rows *r)
-{
-    const int64_t n[3] = {nb, rows, heads}, st[3] = {o->s0, o->ld, o->s1};
-    int64_t sp, es;
-
-    if (!o->buf || !o->buf->ptr)
-        return CB_EARG;
-    if (!float_dt(o->buf->dtype))
-        return CB_EDTYPE;
-    es = (int64_t)cbi_dtype_size(o->buf->dtype);
-    sp = span(n, st, 3, hd);
-    if (sp < 0 || o->off < 0 || o->off > (INT64_C(1) << 62) ||
-        (uint64_t)(o->off + sp) > (uint64_t)o->buf->bytes / (uint64_t)es ||
-        ((uintptr_t)o->buf->ptr % (uintptr_t)es) || (output && !distinct(n, st, 3, hd)))
-        return CB_EARG;
-    r->k.p = (char *)o->buf->ptr + o->off * es;
-    r->k.dt = o->buf->dtype;
-    r->k.ld = o->ld;
-    r->k.s0 = o->s0;
-    r->k.s1 = o->s1;
-    r->lo = (const char *)r->k.p;
-    r->hi = r->lo + sp * es;
-    return CB_OK;
-}
-
-static int overlap(const struct rows *a, const char *lo, const char *hi)
-{
-    return a->lo < hi && lo < a->hi;
-}
-
-/* Same type, address and layout (of the dimensions that have a second step). */
-static int same_place(const struct rows *a, const struct rows *b, int64_t nb, int64_t n,
-                      int64_t heads)
-{
-    return a->k.p == b->k.p && a->k.dt == b->k.dt && (nb == 1 || a->k.s0 == b->k.s0) &&
-           (n == 1 || a->k.ld == b->k.ld) && (heads == 1 || a->k.s1 == b->k.s1);
-}
-
-/* A vector of n elements of type dt (4-byte types on a 4-byte boundary). */
-static int vec_ok(cb_mem m, int dt, int64_t n)
-{
-    const uint64_t es = cbi_dtype_size(dt);
-
-    return m && m->ptr && m->dtype == dt && n >= 0 && (uint64_t)n <= (uint64_t)m->bytes / es &&
-           (uintptr_t)m->ptr % es == 0;
-}
-
-static int vec_overlap(const struct rows *a, cb_mem m, int64_t n)
-{
-    return m && overlap(a, (const char *)m->ptr,
-                        (const char *)m->ptr + n * (int64_t)cbi_dtype_size(m->dtype));
-}
-
-int cb_rope_table(cb_backend *b, int npos, int rot, int64_t first,
-                  const struct cb_rope_scaling *scaling, cb_mem cs)
-{
-    static const struct cb_rope_scaling plain = {10000.0, CB_ROPE_SCALE_NONE, 1.0, 0.0, 0.0, 0.0, 1.0};
-    const struct cb_rope_scaling *sc = scaling ? scaling : &plain;
     const double two_pi = 6.283185307179586476925286766559;
-    double turns[K_ROPE_MAX / 2], theta = sc->theta, lo = 0.0, hi = 0.0;
+    double theta = sc->theta, lo = 0.0, hi = 0.0;
     int j;
 
-    if (!b || npos <= 0 || rot <= 0 || rot % 2 || rot > K_ROPE_MAX ||
-        first < -((int64_t)1 << 31) || first > ((int64_t)1 << 31) - npos ||
-        !vec_ok(cs, CB_F32, (int64_t)npos * rot) || (uintptr_t)cs->ptr % 8 ||
-        !(theta > 1.0) || !isfinite(theta) || !(sc->amplitude > 0.0) || !isfinite((float)sc->amplitude))
+    if (!(theta > 1.0) || !isfinite(theta) || !(sc->amplitude > 0.0) || !isfinite((float)sc->amplitude))
         return cbi_fail(b, CB_EARG, "rope_table");
     if (sc->kind != CB_ROPE_SCALE_NONE && (!(sc->factor >= 1.0) || !isfinite(sc->factor)))
         return cbi_fail(b, CB_EARG, "rope_table: factor");
@@ -166,49 +54,172 @@ int cb_rope_table(cb_backend *b, int npos, int rot, int64_t first,
         }
         turns[j] = w / two_pi;
     }
-    CB_TRY(cbi_enter(b));
-    cbi_prof_begin(b, "rope_table", (double)npos * rot, 4.0 * npos * rot);
-    j = cbi_kstatus(b,
-                    k_rope_table(npos, rot, (long)first, turns, (float)sc->amplitude,
-                                 (float *)cs->ptr, (k_stream)b->stream),
-                    "rope_table");
-    cbi_prof_end(b);
-    return j;
+    return CB_OK;
 }
 
-int cb_rope_rotate(cb_backend *b, int nb, int N, int heads, int hd, int rot, int layout,
-                   struct cb_opnd X, struct cb_opnd Y, cb_mem cs, int npos, cb_mem pos, int pos0)
+static const struct cb_rope_scaling plain_rope = {10000.0, CB_ROPE_SCALE_NONE, 1.0, 0.0, 0.0, 0.0, 1.0};
+
+static int table_ok(int npos, int rot, int64_t first, cb_mem cs)
 {
-    struct rows x, y;
+    return npos > 0 && rot > 0 && rot % 2 == 0 && rot <= K_ROPE_MAX && first >= -((int64_t)1 << 31) &&
+           first <= ((int64_t)1 << 31) - npos && vec_ok(cs, CB_F32, (int64_t)npos * rot) &&
+           (uintptr_t)cs->ptr % 8 == 0;
+}
+
+static int enqueue_table(cb_backend *b, int npos, int rot, int64_t first, const double *turns,
+                         double amplitude, cb_mem cs)
+{
     int rc;
 
-    if (!b || nb <= 0 || N <= 0 || N > MAX_ROWS || (int64_t)nb * N > INT32_MAX || heads <= 0 ||
-        hd <= 0 || hd > (1 << 16) || heads > (1 << 14) || rot <= 0 || rot % 2 || rot > hd ||
-        npos <= 0 || (layout != CB_ROPE_PAIRS && layout != CB_ROPE_HALVES) ||
-        !vec_ok(cs, CB_F32, (int64_t)npos * rot) || (uintptr_t)cs->ptr % 8)
-        return cbi_fail(b, CB_EARG, "rope_rotate");
-    if (pos ? (pos0 != 0 || !vec_ok(pos, CB_I32, (int64_t)nb * N))
-            : (pos0 < 0 || (int64_t)pos0 + N > npos))
-        return cbi_fail(b, CB_EARG, "rope_rotate: positions");
-    if ((rc = take(&X, nb, N, heads, hd, 0, &x)) != CB_OK ||
-        (rc = take(&Y, nb, N, heads, hd, 1, &y)) != CB_OK)
+    CB_TRY(cbi_enter(b));
+    cbi_prof_begin(b, "rope_table", (double)npos * rot, 4.0 * npos * rot);
+    rc = cbi_kstatus(b,
+                     k_rope_table(npos, rot, (long)first, turns, (float)amplitude, (float *)cs->ptr,
+                                  (k_stream)b->stream),
+                     "rope_table");
+    cbi_prof_end(b);
+    return rc;
+}
+
+int cb_rope_table(cb_backend *b, int npos, int rot, int64_t first,
+                  const struct cb_rope_scaling *scaling, cb_mem cs)
+{
+    const struct cb_rope_scaling *sc = scaling ? scaling : &plain_rope;
+    double turns[K_ROPE_MAX / 2];
+
+    if (!b || !table_ok(npos, rot, first, cs))
+        return cbi_fail(b, CB_EARG, "rope_table");
+    CB_TRY(rope_turns(b, rot, sc, turns));
+    return enqueue_table(b, npos, rot, first, turns, sc->amplitude, cs);
+}
+
+/* The axis of each pair of the head; the pairs of all axes, 0 when the
+ * description is not valid (widths even and positive, with turns no axis
+ * behind the first wider than its places). */
+static int axes_pairs(const struct cb_rope_axes *ax, uint8_t *axis)
+{
+    int pairs = 0, count[K_ROPE_AXES] = {0, 0, 0, 0}, a, i, j;
+
+    if (!ax || ax->axes < 1 || ax->axes > K_ROPE_AXES ||
+        (ax->order != CB_ROPE_AXES_SECTIONS && ax->order != CB_ROPE_AXES_TURNS))
+        return 0;
+    for (a = 0; a < ax->axes; a++) {
+        if (ax->width[a] <= 0 || ax->width[a] % 2 || ax->width[a] > K_ROPE_MAX)
+            return 0;
+        pairs += ax->width[a] / 2;
+    }
+    if (pairs > K_ROPE_MAX / 2)
+        return 0;
+    if (ax->order == CB_ROPE_AXES_SECTIONS) {
+        for (a = 0, j = 0; a < ax->axes; a++)
+            for (i = 0; i < ax->width[a] / 2; i++)
+                axis[j++] = (uint8_t)a;
+        return pairs;
+    }
+    for (j = 0; j < pairs; j++) {
+        a = j % ax->axes;
+        axis[j] = (uint8_t)(j / ax->axes < ax->width[a] / 2 ? a : 0);
+        count[axis[j]]++;
+    }
+    for (a = 0; a < ax->axes; a++)
+        if (count[a] != ax->width[a] / 2)
+            return 0;
+    return pairs;
+}
+
+int cb_rope_axes_table(cb_backend *b, int npos, const struct cb_rope_axes *axes, int64_t first,
+                       const struct cb_rope_scaling *scaling, cb_mem cs)
+{
+    const struct cb_rope_scaling *sc = scaling ? scaling : &plain_rope;
+    double turns[K_ROPE_MAX / 2], own[K_ROPE_AXES][K_ROPE_MAX / 2];
+    uint8_t axis[K_ROPE_MAX / 2];
+    int at[K_ROPE_AXES] = {0, 0, 0, 0}, pairs, a, j;
+
+    if (!b || (pairs = axes_pairs(axes, axis)) == 0 || !table_ok(npos, 2 * pairs, first, cs))
+        return cbi_fail(b, CB_EARG, "rope_axes_table");
+    for (a = 0; a < axes->axes; a++)
+        CB_TRY(rope_turns(b, axes->width[a], sc, own[a]));
+    for (j = 0; j < pairs; j++)
+        turns[j] = own[axis[j]][at[axis[j]]++];
+    return enqueue_table(b, npos, 2 * pairs, first, turns, sc->amplitude, cs);
+}
+
+/* The part of the rotations that does not depend on where positions come
+ * from: operands, then the kernel. ax NULL: one axis. */
+static int rotate(cb_backend *b, int nb, int N, int heads, int hd, int rot, int layout,
+                  const struct cb_opnd *X, const struct cb_opnd *Y, cb_mem cs, int npos, cb_mem pos,
+                  int pos0, const struct k_rope_axes *ax, const char *what)
+{
+    struct rows x, y;
+    const int64_t npid = (int64_t)nb * N * (ax ? ax->axes : 1);
+    int rc;
+
+    if ((rc = take(X, nb, N, heads, hd, T_FLOAT, 0, &x)) != CB_OK ||
+        (rc = take(Y, nb, N, heads, hd, T_FLOAT, 1, &y)) != CB_OK)
         return cbi_fail(b, rc, "rope_rotate: operand");
     if (y.k.dt != x.k.dt && x.k.dt != CB_F32)
         return cbi_fail(b, CB_EDTYPE, "rope_rotate: output type");
     if ((overlap(&y, x.lo, x.hi) && !same_place(&x, &y, nb, N, heads)) ||
-        vec_overlap(&y, cs, (int64_t)npos * rot) || vec_overlap(&y, pos, (int64_t)nb * N))
+        vec_overlap(&y, cs, (int64_t)npos * rot) || vec_overlap(&y, pos, npid))
         return cbi_fail(b, CB_EARG, "rope_rotate: output overlaps an input");
     CB_TRY(cbi_enter(b));
-    cbi_prof_begin(b, "rope_rotate", 3.0 * nb * N * heads * rot,
+    cbi_prof_begin(b, what, 3.0 * nb * N * heads * rot,
                    (double)nb * N * heads * hd *
                        (cbi_dtype_size(x.k.dt) + cbi_dtype_size(y.k.dt)));
     rc = cbi_kstatus(b,
                      k_rope_rotate(&x.k, &y.k, nb, N, heads, hd, rot, layout,
                                    pos ? (const int *)pos->ptr : NULL, pos0, npos,
-                                   (const float *)cs->ptr, (k_stream)b->stream),
-                     "rope_rotate");
+                                   (const float *)cs->ptr, ax, (k_stream)b->stream),
+                     what);
     cbi_prof_end(b);
     return rc;
+}
+
+static int rotate_shape_ok(int nb, int N, int heads, int hd, int rot, int layout, cb_mem cs, int npos)
+{
+    return nb > 0 && N > 0 && N <= MAX_ROWS && (int64_t)nb * N <= INT32_MAX && heads > 0 && hd > 0 &&
+           hd <= (1 << 16) && heads <= (1 << 14) && rot > 0 && rot % 2 == 0 && rot <= hd && npos > 0 &&
+           (layout == CB_ROPE_PAIRS || layout == CB_ROPE_HALVES) &&
+           vec_ok(cs, CB_F32, (int64_t)npos * rot) && (uintptr_t)cs->ptr % 8 == 0;
+}
+
+int cb_rope_rotate(cb_backend *b, int nb, int N, int heads, int hd, int rot, int layout,
+                   struct cb_opnd X, struct cb_opnd Y, cb_mem cs, int npos, cb_mem pos, int pos0)
+{
+    if (!b || !rotate_shape_ok(nb, N, heads, hd, rot, layout, cs, npos))
+        return cbi_fail(b, CB_EARG, "rope_rotate");
+    if (pos ? (pos0 != 0 || !vec_ok(pos, CB_I32, (int64_t)nb * N))
+            : (pos0 < 0 || (int64_t)pos0 + N > npos))
+        return cbi_fail(b, CB_EARG, "rope_rotate: positions");
+    return rotate(b, nb, N, heads, hd, rot, layout, &X, &Y, cs, npos, pos, pos0, NULL, "rope_rotate");
+}
+
+int cb_rope_rotate_axes(cb_backend *b, int nb, int N, int heads, int hd, int rot, int layout,
+                        const struct cb_rope_axes *axes, struct cb_opnd X, struct cb_opnd Y,
+                        cb_mem cs, int npos, cb_mem pos, const int *grid)
+{
+    struct k_rope_axes ax = {0};
+    int a;
+
+    if (!b || !rotate_shape_ok(nb, N, heads, hd, rot, layout, cs, npos) || rot > K_ROPE_MAX ||
+        axes_pairs(axes, ax.axis) * 2 != rot)
+        return cbi_fail(b, CB_EARG, "rope_rotate_axes");
+    ax.axes = axes->axes;
+    ax.sections = axes->order == CB_ROPE_AXES_SECTIONS;
+    if (pos ? (grid || !vec_ok(pos, CB_I32, (int64_t)nb * N * ax.axes)) : !grid)
+        return cbi_fail(b, CB_EARG, "rope_rotate_axes: positions");
+    if (grid) {
+        int64_t cells = 1;
+
+        for (a = 0; a < ax.axes; a++) {
+            if (grid[a] <= 0 || (cells *= grid[a]) > INT32_MAX)
+                return cbi_fail(b, CB_EARG, "rope_rotate_axes: grid");
+            ax.grid[a] = grid[a];
+        }
+        if (N > cells)
+            return cbi_fail(b, CB_EARG, "rope_rotate_axes: grid");
+    }
+    return rotate(b, nb, N, heads, hd, rot, layout, &X, &Y, cs, npos, pos, 0, &ax, "rope_rotate_axes");
 }
 
 int cb_cross_attend(cb_backend *b, int nb, int Nq, int Nk, int heads, int kvheads, int hd,
@@ -224,10 +235,10 @@ int cb_cross_attend(cb_backend *b, int nb, int Nq, int Nk, int heads, int kvhead
         return cbi_fail(b, CB_EARG, "cross_attend");
     if ((klen && !vec_ok(klen, CB_I32, nb)) || (kmask && !vec_ok(kmask, CB_U8, (int64_t)nb * Nk)))
         return cbi_fail(b, CB_EARG, "cross_attend: key lengths or mask");
-    if ((rc = take(&Q, nb, Nq, heads, hd, 0, &q)) != CB_OK ||
-        (rc = take(&K, nb, Nk, kvheads, hd, 0, &k)) != CB_OK ||
-        (rc = take(&V, nb, Nk, kvheads, hd, 0, &v)) != CB_OK ||
-        (rc = take(&O, nb, Nq, heads, hd, 1, &o)) != CB_OK)
+    if ((rc = take(&Q, nb, Nq, heads, hd, T_FLOAT, 0, &q)) != CB_OK ||
+        (rc = take(&K, nb, Nk, kvheads, hd, T_FLOAT, 0, &k)) != CB_OK ||
+        (rc = take(&V, nb, Nk, kvheads, hd, T_FLOAT, 0, &v)) != CB_OK ||
+        (rc = take(&O, nb, Nq, heads, hd, T_FLOAT, 1, &o)) != CB_OK)
         return cbi_fail(b, rc, "cross_attend: operand");
     if (k.k.dt != q.k.dt || v.k.dt != q.k.dt || o.k.dt != q.k.dt)
         return cbi_fail(b, CB_EDTYPE, "cross_attend: operands of different types");
@@ -260,8 +271,8 @@ int cb_groupnorm(cb_backend *b, int nb, int64_t npix, int C, int groups, struct 
         return cbi_fail(b, CB_EARG, "groupnorm");
     if (X.s1 != 0 || Y.s1 != 0) /* channels are adjacent */
         return cbi_fail(b, CB_EARG, "groupnorm: channel stride");
-    if ((rc = take(&X, nb, npix, 1, C, 0, &x)) != CB_OK ||
-        (rc = take(&Y, nb, npix, 1, C, 1, &y)) != CB_OK)
+    if ((rc = take(&X, nb, npix, 1, C, T_FLOAT, 0, &x)) != CB_OK ||
+        (rc = take(&Y, nb, npix, 1, C, T_FLOAT, 1, &y)) != CB_OK)
         return cbi_fail(b, rc, "groupnorm: operand");
     if (y.k.dt != x.k.dt && x.k.dt != CB_F32)
         return cbi_fail(b, CB_EDTYPE, "groupnorm: output type");

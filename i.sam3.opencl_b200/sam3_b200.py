@@ -14,10 +14,12 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libsam3cuda.so")
 
-F32, BF16, F16, U8, I32 = 0, 1, 2, 3, 4
+F32, BF16, F16, U8, I32, E4M3, E8M0 = 0, 1, 2, 3, 4, 5, 6
 ACT_NONE, ACT_GELU, ACT_RELU = 0, 1, 2
 ATTN_TC, ATTN_F32 = 0, 1
 ROPE_PAIRS, ROPE_HALVES = 0, 1
+ROPE_AXES_SECTIONS, ROPE_AXES_TURNS = 0, 1
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
 ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_BASE, ROPE_SCALE_RAMP = 0, 1, 2, 3
 
 STATUS = {0: "CB_OK", 1: "CB_ENODEV", 2: "CB_EALLOC", 3: "CB_EARG",
@@ -42,6 +44,7 @@ EXPORTS = [
     "cb_decode", "cb_neck_create", "cb_neck_free", "cb_neck_init_random",
     "cb_neck_set_weight", "cb_neck_run", "cb_image_encoder_input",
     "cb_attend", "cb_rope_table", "cb_rope_rotate", "cb_cross_attend", "cb_groupnorm",
+    "cb_rope_axes_table", "cb_rope_rotate_axes", "cb_quantize_e4m3", "cb_gemm_e4m3", "cb_norm_residual",
     "sam3_synth_normal", "sam3_synth_u8", "sam3_synth_rope_axial",
 ]
 
@@ -99,6 +102,23 @@ class RopeScaling(C.Structure):
     def __init__(self, theta=10000.0, kind=0, factor=1.0, orig_len=0.0, turns_fast=32.0,
                  turns_slow=1.0, amplitude=1.0):
         super().__init__(theta, kind, factor, orig_len, turns_fast, turns_slow, amplitude)
+
+
+class RopeAxes(C.Structure):
+    """struct cb_rope_axes: the rotated columns of each axis and their order."""
+    _fields_ = [("axes", C.c_int), ("width", C.c_int * 4), ("order", C.c_int)]
+
+    def __init__(self, widths, order=ROPE_AXES_SECTIONS):
+        super().__init__(len(widths), (C.c_int * 4)(*widths[:4]), order)
+
+
+class Norm(C.Structure):
+    """struct cb_norm: kind (NORM_*), eps, weight and bias (Mem, F32, or None)."""
+    _fields_ = [("kind", C.c_int), ("eps", C.c_float), ("g", C.c_void_p), ("bias", C.c_void_p)]
+
+    def __init__(self, kind, eps=1e-5, g=None, bias=None):
+        super().__init__(kind, eps, g.h.value if g else None, bias.h.value if bias else None)
+        self.mems = (g, bias)  # kept alive
 
 
 class CBError(RuntimeError):
@@ -193,6 +213,14 @@ def lib():
         "cb_cross_attend": (i32, [vp, i32, i32, i32, i32, i32, i32, Opnd, Opnd, Opnd, Opnd, vp,
                                   vp, f32]),
         "cb_groupnorm": (i32, [vp, i32, i64, i32, i32, Opnd, Opnd, vp, vp, f32, i32]),
+        "cb_rope_axes_table": (i32, [vp, i32, C.POINTER(RopeAxes), i64, C.POINTER(RopeScaling), vp]),
+        "cb_rope_rotate_axes": (i32, [vp, i32, i32, i32, i32, i32, i32, C.POINTER(RopeAxes), Opnd, Opnd, vp,
+                                      i32, vp, C.POINTER(i32)]),
+        "cb_quantize_e4m3": (i32, [vp, i32, i32, i32, i32, Opnd, Opnd, Opnd]),
+        "cb_gemm_e4m3": (i32, [vp, i32, i32, i32, Opnd, Opnd, Opnd, Opnd, Opnd, C.POINTER(Opnd), vp, i32]),
+        "cb_norm_residual": (i32, [vp, i32, i32, i32, Opnd, C.POINTER(Opnd), C.POINTER(Norm), f32, vp,
+                                   C.POINTER(Opnd), C.POINTER(Opnd), C.POINTER(Norm), C.POINTER(Opnd),
+                                   C.POINTER(Opnd), C.POINTER(Opnd), C.POINTER(Opnd)]),
         "sam3_synth_normal": (None, [C.c_uint64, C.c_uint64, sz, f32, f32, vp]),
         "sam3_synth_u8": (None, [C.c_uint64, C.c_uint64, sz, vp]),
         "sam3_synth_rope_axial": (None, [i32, i32, C.c_double, vp]),
@@ -304,7 +332,8 @@ class Backend:
         import torch
         dt = dtype if dtype is not None else {
             torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16,
-            torch.uint8: U8, torch.int32: I32}[tensor.dtype]
+            torch.uint8: U8, torch.int32: I32, torch.float8_e4m3fn: E4M3,
+            torch.float8_e8m0fnu: E8M0}[tensor.dtype]
         m = C.c_void_p()
         self.check(lib().cb_wrap(self.h, C.c_void_p(tensor.data_ptr()),
                                  tensor.numel() * tensor.element_size(), dt,
@@ -431,6 +460,40 @@ class Backend:
 
     def groupnorm(self, nb, npix, Cn, groups, X, Y, g, b, eps=1e-5, act=ACT_NONE):
         rc = lib().cb_groupnorm(self.h, nb, npix, Cn, groups, X, Y, g.h, b.h, eps, act)
+        if rc:
+            self.check(rc)
+
+    def rope_axes_table(self, npos, axes, first, scaling, cs):
+        rc = lib().cb_rope_axes_table(self.h, npos, C.byref(axes), first,
+                                      C.byref(scaling) if scaling is not None else None, cs.h)
+        if rc:
+            self.check(rc)
+
+    def rope_rotate_axes(self, nb, N, heads, hd, rot, layout, axes, X, Y, cs, npos, pos=None, grid=None):
+        """pos: I32 Mem [nb, N, axes], or grid: the extents whose coordinates the rows have."""
+        rc = lib().cb_rope_rotate_axes(self.h, nb, N, heads, hd, rot, layout, C.byref(axes), X, Y, cs.h,
+                                       npos, pos.h if pos else None,
+                                       (C.c_int * 4)(*grid) if grid is not None else None)
+        if rc:
+            self.check(rc)
+
+    # ---- 8-bit products and the norms around them: operands are bmat() descriptors
+    def quantize_e4m3(self, nb, N, K, brows, X, Q, S):
+        rc = lib().cb_quantize_e4m3(self.h, nb, N, K, brows, X, Q, S)
+        if rc:
+            self.check(rc)
+
+    def gemm_e4m3(self, M, N, K, A, SA, B, SB, Cm, SC=None, bias=None, act=ACT_NONE):
+        """SC: the scales of an E4M3 Cm."""
+        rc = lib().cb_gemm_e4m3(self.h, M, N, K, A, SA, B, SB, Cm, SC, bias.h if bias else None, act)
+        if rc:
+            self.check(rc)
+
+    def norm_residual(self, nb, N, Cn, X, H=None, post=None, alpha=1.0, ls=None, gate=None, R=None, pre=None,
+                      scale=None, shift=None, Y=None, S=None):
+        """post, pre: Norm or None."""
+        rc = lib().cb_norm_residual(self.h, nb, N, Cn, X, H, post, alpha, ls.h if ls else None, gate, R, pre,
+                                    scale, shift, Y, S)
         if rc:
             self.check(rc)
 

@@ -35,6 +35,8 @@ extern "C" {
 #define CB_F16 2
 #define CB_U8 3
 #define CB_I32 4 /* positions and lengths */
+#define CB_E4M3 5 /* 8-bit floating point: 4 exponent and 3 mantissa bits, to 448, no infinity */
+#define CB_E8M0 6 /* 2^(byte - 127), 255 NaN: scales of blocks of E4M3 */
 
 /* Activations, as sam3_ops.h:11-13. */
 #define CB_ACT_NONE 0
@@ -478,6 +480,41 @@ int cb_rope_rotate(cb_backend *b, int nb, int N, int heads, int hd, int rot,
                    int layout, struct cb_opnd X, struct cb_opnd Y, cb_mem cs,
                    int npos, cb_mem pos, int pos0);
 
+/* Rotary positions with several axes (time, height, width of video and image
+ * tokens): pair j of a head turns by its row's position on the pair's axis.
+ * width[a]: rotated columns (even) of axis a, their sum is rot, at most 256.
+ *   SECTIONS: the first width[0] / 2 pairs are axis 0's, the next width[1] / 2
+ *             axis 1's, ...
+ *   TURNS:    pair j is axis j % axes' while that axis has pairs left (j / axes <
+ *             width / 2), else axis 0's; refused when an axis does not get its
+ *             width this way. */
+#define CB_ROPE_AXES_SECTIONS 0
+#define CB_ROPE_AXES_TURNS 1
+struct cb_rope_axes {
+    int axes; /* 1 to 4 */
+    int width[4];
+    int order;
+};
+
+/* The table of cb_rope_rotate_axes with a ladder of frequencies for each axis:
+ * the i-th pair of axis a turns as pair i of cb_rope_table(rot = width[a]) does.
+ * cs F32 [npos, rot / 2] (cos, sin), column j that of pair j; rows are positions
+ * first .. first + npos - 1 of every axis. (One ladder over all pairs is
+ * cb_rope_table's.) */
+int cb_rope_axes_table(cb_backend *b, int npos, const struct cb_rope_axes *axes,
+                       int64_t first, const struct cb_rope_scaling *scaling,
+                       cb_mem cs);
+
+/* cb_rope_rotate with several axes: row (b, n)'s position on axis a is pos[(b * N
+ * + n) * axes + a] (CB_I32; grid NULL) or, with pos NULL, its coordinate in a
+ * grid of grid[0] x ... x grid[axes - 1] rows, the last axis fastest (N at most
+ * their product). A position outside [0, npos) leaves the pairs of its axis as
+ * they are. */
+int cb_rope_rotate_axes(cb_backend *b, int nb, int N, int heads, int hd, int rot,
+                        int layout, const struct cb_rope_axes *axes,
+                        struct cb_opnd X, struct cb_opnd Y, cb_mem cs, int npos,
+                        cb_mem pos, const int *grid);
+
 /* O[b, i, h] = softmax over visible j of (scale Q[b, i, h] . K[b, j, h']) V[b,
  * j, h'], h' = h / (heads / kvheads): Q, O [nb, Nq, heads, hd], K, V [nb, Nk,
  * kvheads, hd], one type (F32, BF16, F16), hd a multiple of 8 up to 128, scale
@@ -508,6 +545,66 @@ int cb_cross_attend(cb_backend *b, int nb, int Nq, int Nk, int heads,
 int cb_groupnorm(cb_backend *b, int nb, int64_t npix, int C, int groups,
                  struct cb_opnd X, struct cb_opnd Y, cb_mem g, cb_mem bias,
                  float eps, int act);
+
+/* ------------------------------------------------------------ 8-bit products
+ * The products of a transformer block on 8-bit operands and the norms around
+ * them. Operands, streams, graphs and overlaps as on the prompt path; rows are
+ * cb_bmat() descriptors with s1 0.
+ *
+ * An E4M3 matrix has a scale for each block of 128 columns of a row (or of 128 x
+ * 128 values), the last block of a row or column shorter: it stands for q s. */
+
+/* Q (E4M3) and its scales S of X [nb, N, K] (F32, BF16, F16): s = 2^e with the
+ * smallest whole e >= -126 for which the block's largest finite |x| is at most
+ * 448 s; q = x / s to nearest (the division is exact). Infinities and NaN become
+ * NaN. brows 1: S [nb, N, ceil(K / 128)] (activations); 128: S [nb, ceil(N /
+ * 128), ceil(K / 128)] (weights). S E8M0 or F32. Elements of Q's rows behind
+ * column K are left as they were. */
+int cb_quantize_e4m3(cb_backend *b, int nb, int N, int K, int brows,
+                     struct cb_opnd X, struct cb_opnd Q, struct cb_opnd S);
+
+/* C[m, n] = act(sum over blocks kb of SA[m, kb] SB[n / 128, kb] (sum over k in kb
+ * of A[m, k] B[n, k]) + bias[n]), B in the Linear weight layout: A [M, K], B [N, K]
+ * E4M3; SA [M, ceil(K / 128)], SB [ceil(N / 128), ceil(K / 128)] E8M0 or F32 (any
+ * values, each its own type; a product of two scales stays within 32 bits);
+ * bias F32 [N] or NULL; C F32, BF16 or F16, rounded once, or E4M3, then SC [M,
+ * ceil(N / 128)] (E8M0 or F32) receives the scales cb_quantize_e4m3 (brows 1)
+ * would give act(...) in 32 bits. Sums in 32 bits. Rows of A and B start at
+ * multiples of 16 bytes (off and ld; what lies behind column K of a row is not
+ * used); C takes any ld. s0 is of no account. GELU as cb_groupnorm's. */
+int cb_gemm_e4m3(cb_backend *b, int M, int N, int K, struct cb_opnd A,
+                 struct cb_opnd SA, struct cb_opnd B, struct cb_opnd SB,
+                 struct cb_opnd C, const struct cb_opnd *SC, cb_mem bias, int act);
+
+/* Norm of a row v of C channels: LAYER (v - mean) / sqrt(var + eps) g + bias, RMS
+ * v / sqrt(mean of v^2 + eps) g + bias; g, bias F32 [C] or NULL (1, 0). */
+#define CB_NORM_NONE 0
+#define CB_NORM_LAYER 1
+#define CB_NORM_RMS 2
+struct cb_norm {
+    int kind;
+    float eps;
+    cb_mem g, bias;
+};
+
+/* What stands between two blocks of a transformer, in one pass over [nb, N, C]:
+ *   h = post(H)                                norm behind a block (post NULL: h = H)
+ *   r = X + alpha ls[c] gate[b, n, c] h        residual scale and gate (H NULL: r = X)
+ *   R = r                                      the residual stream (R NULL: not kept)
+ *   Y = pre(r) (1 + scale[b, n, c]) + shift[b, n, c]   norm before the next block
+ * in 32 bits, r not rounded before pre. ls F32 [C] or NULL (1); gate, scale, shift
+ * F32, BF16 or F16 operands, NULL for 1, 0, 0 (ld 0: one row for a sample, s0 0: for
+ * all). X F32, BF16 or F16; H and R of X's type, H also BF16 or F16 beside an F32
+ * X; Y of X's type, BF16 or F16 of an F32 X, or E4M3 with the scales S
+ * [nb, N, ceil(C / 128)] of cb_quantize_e4m3 (brows 1). R and Y may be X or H (same
+ * type and layout), not one another. R or Y is given; without Y: pre, scale, shift
+ * and S NULL; pre NULL: Y of r itself. */
+int cb_norm_residual(cb_backend *b, int nb, int N, int C, struct cb_opnd X,
+                     const struct cb_opnd *H, const struct cb_norm *post,
+                     float alpha, cb_mem ls, const struct cb_opnd *gate,
+                     const struct cb_opnd *R, const struct cb_norm *pre,
+                     const struct cb_opnd *scale, const struct cb_opnd *shift,
+                     const struct cb_opnd *Y, const struct cb_opnd *S);
 
 /* ------------------------------------------------------------ input path
  * image_encoder_input (image.c:346-371) on the device: the crop (x0, y0, w,
