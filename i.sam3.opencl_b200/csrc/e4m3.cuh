@@ -11,20 +11,28 @@ namespace sam3 {
 
 constexpr int kScaleBlock = 128;
 
-// Bits of |x| of a finite x, 0 of an infinity or NaN: largest by integer max.
-__device__ __forceinline__ uint32_t finite_bits(float x)
+// The larger of m and |x|; a NaN counts for nothing. A block's largest magnitude
+// that comes out infinite is taken again over its finite values (larger_finite).
+__device__ __forceinline__ float larger(float m, float x)
 {
-    const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
-    return u < 0x7f800000u ? u : 0u;
+    return fmaxf(m, fabsf(x));
+}
+__device__ __forceinline__ float larger_finite(float m, float x)
+{
+    const float a = fabsf(x);
+    return a < __int_as_float(0x7f800000) ? fmaxf(m, a) : m;
+}
+__device__ __forceinline__ bool infinite(float m)
+{
+    return m == __int_as_float(0x7f800000);
 }
 
-// The scale of a block whose largest finite magnitude has the bits u, as the
-// E8M0 byte e + 127: the smallest e >= -126 with the magnitude at most 448 2^e =
+// The scale of a block whose largest finite magnitude is m, as the E8M0 byte e + 127: the smallest e >= -126 with the magnitude at most 448 2^e =
 // 1.75 * 2^(8 + e). Adding 2^21 - 1 carries into the exponent exactly when the
 // fraction is above 0.75.
-__device__ __forceinline__ uint32_t scale_byte(uint32_t u)
+__device__ __forceinline__ uint32_t scale_byte(float m)
 {
-    const uint32_t x = (u + 0x1fffffu) >> 23;
+    const uint32_t x = (__float_as_uint(m) + 0x1fffffu) >> 23;
     return x > 9 ? x - 8 : 1u;
 }
 __device__ __forceinline__ float scale_value(uint32_t byte)
@@ -38,18 +46,27 @@ __device__ __forceinline__ float scale_inverse(uint32_t byte)
 }
 
 // Four values times the inverse scale, to nearest; the product is exact or far
-// below E4M3's smallest number. x 0 added turns an infinity, which the
-// conversion would saturate, into NaN.
+// below E4M3's smallest number. INF: some may be infinite, which the conversion
+// would saturate; 0 x added makes them NaN.
+template <bool INF>
 __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d, float inv)
 {
     uint16_t lo, hi;
-    a = fmaf(a, 0.0f, a * inv);
-    b = fmaf(b, 0.0f, b * inv);
-    c = fmaf(c, 0.0f, c * inv);
-    d = fmaf(d, 0.0f, d * inv);
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    if (INF) {
+        a = fmaf(a, 0.0f, a);
+        b = fmaf(b, 0.0f, b);
+        c = fmaf(c, 0.0f, c);
+        d = fmaf(d, 0.0f, d);
+    }
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b * inv), "f"(a * inv));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d * inv), "f"(c * inv));
     return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+__device__ __forceinline__ uint2 pack8_e4m3(const float (&v)[8], float inv, bool inf)
+{
+    if (inf)
+        return make_uint2(pack_e4m3<true>(v[0], v[1], v[2], v[3], inv), pack_e4m3<true>(v[4], v[5], v[6], v[7], inv));
+    return make_uint2(pack_e4m3<false>(v[0], v[1], v[2], v[3], inv), pack_e4m3<false>(v[4], v[5], v[6], v[7], inv));
 }
 
 // A scale as it is stored (E8M0 byte or fp32 bits) and its value.

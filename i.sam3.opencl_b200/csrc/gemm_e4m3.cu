@@ -31,12 +31,15 @@ namespace {
 constexpr int BM = 128, BK = 128;
 constexpr int kThreads = 384;
 constexpr int kStageTile = 32 * 128;  // a warp's 32 rows x 128 bytes of C
+constexpr int kChunk = 4;             // k-blocks whose scales are handed over at once
+constexpr int kScaleRing = 2 * kChunk * BM * 4;  // two chunks of a group's scales
 
 struct E4Args {
     int M, N, K;
     const void *sa, *sb;
     long ldsa, ldsb;
     int sadt, sbdt;
+    int savec, sbvec;  // rows of scales start at multiples of four
     const float *bias;
     void *c;
     long ldc;
@@ -54,47 +57,128 @@ struct E4Smem {
     static constexpr int A_BYTES = BM * BK;
     static constexpr int B_ROWS = PAIR ? BN / 2 : BN;
     static constexpr int STAGE_BYTES = A_BYTES + B_ROWS * BK;
-    static constexpr int STAGES = STAGE_BYTES > 32768 ? 4 : (STAGE_BYTES > 24576 ? 6 : 7);
+    static constexpr int STAGES = STAGE_BYTES > 32768 ? 3 : (STAGE_BYTES > 24576 ? 5 : 7);
     static constexpr int EPI_OFF = STAGES * STAGE_BYTES;
-    static constexpr int BAR_OFF = EPI_OFF + 8 * kStageTile;
-    // full[S], empty[S], tfull[4], tempty[4], drain, then tmem base + abort
-    static constexpr int BYTES = BAR_OFF + (2 * STAGES + 9) * 8 + 16 + 1024;
+    static constexpr int SCALE_OFF = EPI_OFF + 8 * kStageTile;
+    static constexpr int BAR_OFF = SCALE_OFF + 2 * kScaleRing;
+    // full[S], empty[S], tfull[4], tempty[4], sfull[2][2], sempty[2][2], drain, then
+    // tmem base + abort
+    static constexpr int BYTES = BAR_OFF + (2 * STAGES + 17) * 8 + 16 + 1024;
     static_assert(BYTES <= 232448, "shared memory");
 };
 
-// The scales of a thread's row and columns, four k-blocks ahead of their use, over
-// all tiles of the thread.
-struct Scales {
-    static constexpr int D = 4;
-    uint32_t a[D], b[D];
-    long ia, ib;  // elements of the next k-block's scales
-    int kb, t;    // the next k-block and its tile
-
-    __device__ __forceinline__ void tile(const E4Args &p, int num_n, int tm, int bn, int row, int col)
-    {
-        const int m = (t / num_n) * tm + row, n = (t % num_n) * bn + col;
-        ia = (long)min(m, p.M - 1) * p.ldsa;
-        ib = (long)(min(n, p.N - 1) / kScaleBlock) * p.ldsb;
-    }
-};
-
-template <bool FULL>
-__device__ __forceinline__ void add_bias(const float *bias, int n, int N, uint64_t (&acc)[64])
+// Scales [k .. k + 3] of a row (of `n` it has), as stored: one load where the row
+// is aligned for it.
+__device__ __forceinline__ void load_scales(const void *p, int dt, bool vec, long row, int k, int n,
+                                            uint32_t (&v)[kChunk])
 {
-#pragma unroll
-    for (int j = 0; j < 64; j += 2) {
-        if (FULL) {
-            const float4 v = __ldg(reinterpret_cast<const float4 *>(bias + n + 2 * j));
-            acc[j] = add2(acc[j], f2_make(v.x, v.y));
-            acc[j + 1] = add2(acc[j + 1], f2_make(v.z, v.w));
+    if (vec && k + kChunk <= n) {
+        if (dt == K_E8M0) {
+            const uint32_t w = __ldg(reinterpret_cast<const uint32_t *>(reinterpret_cast<const uint8_t *>(p) + row + k));
+            v[0] = w;  // taken apart by scale_at
         }
         else {
-            float v[4];
+            const uint4 w = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(p) + row + k));
+            v[0] = w.x;
+            v[1] = w.y;
+            v[2] = w.z;
+            v[3] = w.w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kChunk; i++)
+        v[i] = k + i < n ? scale_raw(p, dt, row + k + i) : 0u;
+}
+__device__ __forceinline__ float scale_at(const uint32_t (&v)[kChunk], int dt, bool vec, int k, int n, int i)
+{
+    if (dt == K_E8M0 && vec && k + kChunk <= n)
+        return scale_of(v[0] >> (8 * i) & 255u, dt);
+    return scale_of(v[i], dt);
+}
+
+// The products of both scales for the rows and the column block of one group's
+// tiles, four k-blocks at a time, by a warp that runs ahead of the group: the
+// loads of a chunk are in flight while the last one is handed over.
+__device__ __forceinline__ void feed_scales(const E4Args &p, float *ring, uint64_t *sfull, uint64_t *sempty, int t0,
+                                            int tstep, int num_tiles, int num_n, int tm, int bn, int row0, int col,
+                                            int kblocks, int lane, volatile int *abort_flag)
+{
+    constexpr int R = BM / 32;  // rows of a lane
+    uint32_t va[R][kChunk], vb[kChunk], wa[R][kChunk], wb[kChunk];
+    int t = t0, k = 0;
+    auto fetch = [&](uint32_t(&a)[R][kChunk], uint32_t(&b)[kChunk]) {
+        const int m = (t / num_n) * tm + row0 + lane, n = (t % num_n) * bn + col;
+        load_scales(p.sb, p.sbdt, p.sbvec, (long)(min(n, p.N - 1) / kScaleBlock) * p.ldsb, k, kblocks, b);
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            load_scales(p.sa, p.sadt, p.savec, (long)min(m + 32 * i, p.M - 1) * p.ldsa, k, kblocks, a[i]);
+    };
+    uint32_t c = 0;  // chunks handed over
+    auto give = [&](const uint32_t(&a)[R][kChunk], const uint32_t(&b)[kChunk], int k0) {
+        const uint32_t slot = c & 1, parity = (c >> 1 & 1) ^ 1;
+        if (!__all_sync(0xffffffffu, mbar_wait_brief(&sempty[slot], parity, p.err, abort_flag)))
+            return false;
+        float *dst = ring + slot * (kChunk * BM) + lane;
+#pragma unroll
+        for (int j = 0; j < kChunk; j++) {
+            const float sb = scale_at(b, p.sbdt, p.sbvec, k0, kblocks, j);
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                dst[j * BM + 32 * i] = scale_at(a[i], p.sadt, p.savec, k0, kblocks, j) * sb;
+        }
+        __syncwarp();
+        if (lane == 0)
+            mbar_arrive(&sfull[slot]);
+        c++;
+        return true;
+    };
+    auto advance = [&]() {
+        k += kChunk;
+        if (k >= kblocks) {
+            k = 0;
+            t += tstep;
+        }
+        return t < num_tiles;
+    };
+    bool more = t < num_tiles;
+    if (more)
+        fetch(va, vb);
+    while (more) {
+        const int k0 = k;
+        more = advance();
+        if (more)
+            fetch(wa, wb);
+        if (!give(va, vb, k0))
+            return;
+        if (!more)
+            return;
+        const int k1 = k;
+        more = advance();
+        if (more)
+            fetch(va, vb);
+        if (!give(wa, wb, k1))
+            return;
+    }
+}
+
+template <bool FULL>
+__device__ __forceinline__ void add_bias(const float *bias, int n, int N, float (&acc)[128])
+{
+#pragma unroll
+    for (int j = 0; j < 128; j += 4) {
+        if (FULL) {
+            const float4 v = __ldg(reinterpret_cast<const float4 *>(bias + n + j));
+            acc[j] += v.x;
+            acc[j + 1] += v.y;
+            acc[j + 2] += v.z;
+            acc[j + 3] += v.w;
+        }
+        else {
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                v[e] = n + 2 * j + e < N ? __ldg(bias + n + 2 * j + e) : 0.0f;
-            acc[j] = add2(acc[j], f2_make(v[0], v[1]));
-            acc[j + 1] = add2(acc[j + 1], f2_make(v[2], v[3]));
+                if (n + j + e < N)
+                    acc[j + e] += __ldg(bias + n + j + e);
         }
     }
 }
@@ -152,7 +236,7 @@ __device__ __forceinline__ void store_chunk(const E4Args &p, const CUtensorMap *
 // the warp's staging tile.
 template <bool GELU>
 __device__ __forceinline__ void finish(const E4Args &p, const CUtensorMap *tmC, uint32_t tile, int lane, int m0, int n,
-                                       uint64_t (&acc)[64])
+                                       float (&acc)[128])
 {
     const bool full = n + 128 <= p.N;
     if (p.bias) {
@@ -163,22 +247,13 @@ __device__ __forceinline__ void finish(const E4Args &p, const CUtensorMap *tmC, 
     }
     if (p.act == K_ACT_RELU) {
 #pragma unroll
-        for (int j = 0; j < 64; j++) {
-            float a, b;
-            f2_split(acc[j], a, b);
-            asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(0.0f));
-            asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(0.0f));
-            acc[j] = f2_make(a, b);
-        }
+        for (int j = 0; j < 128; j++)
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(acc[j]) : "f"(0.0f));
     }
     if (GELU && p.cdt != K_F32) {
 #pragma unroll
-        for (int j = 0; j < 64; j++) {
-            float a, b;
-            f2_split(acc[j], a, b);
-            gelu_pair_rel(a, b);
-            acc[j] = f2_make(a, b);
-        }
+        for (int j = 0; j < 128; j += 2)
+            gelu_pair_rel(acc[j], acc[j + 1]);
     }
     auto wait_tile = [&]() {  // the store issued from this tile before has read it
         if (p.tma && lane == 0)
@@ -192,10 +267,9 @@ __device__ __forceinline__ void finish(const E4Args &p, const CUtensorMap *tmC, 
                 break;
             wait_tile();
 #pragma unroll
-            for (int q = 0; q < 8; q++) {
-                const uint64_t u = acc[16 * c + 2 * q], v = acc[16 * c + 2 * q + 1];
-                stage_piece(tile, lane, q, (uint32_t)u, (uint32_t)(u >> 32), (uint32_t)v, (uint32_t)(v >> 32));
-            }
+            for (int q = 0; q < 8; q++)
+                stage_piece(tile, lane, q, __float_as_uint(acc[32 * c + 4 * q]), __float_as_uint(acc[32 * c + 4 * q + 1]),
+                            __float_as_uint(acc[32 * c + 4 * q + 2]), __float_as_uint(acc[32 * c + 4 * q + 3]));
             if (GELU) {
                 // the thread's own row again, so that the loop is not unrolled over the sums
 #pragma unroll 1
@@ -217,12 +291,17 @@ __device__ __forceinline__ void finish(const E4Args &p, const CUtensorMap *tmC, 
         }
     }
     else if (p.cdt == K_E4M3) {
-        uint32_t most = 0;
+        float most = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 64; j++) {
-            // columns behind N hold 0: B's rows there read as zero, the bias is not added
-            most = max(most, max(finite_bits(__uint_as_float((uint32_t)acc[j])),
-                                 finite_bits(__uint_as_float((uint32_t)(acc[j] >> 32)))));
+        for (int j = 0; j < 128; j++)  // (0 behind N: B's rows there read as zero, the bias is not added)
+            most = larger(most, acc[j]);
+        if (infinite(most)) {
+            most = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 128; j++) {
+                most = larger_finite(most, acc[j]);
+                acc[j] = fmaf(acc[j], 0.0f, acc[j]);  // NaN for an infinity
+            }
         }
         const uint32_t byte = scale_byte(most);
         const float inv = scale_inverse(byte);
@@ -232,10 +311,8 @@ __device__ __forceinline__ void finish(const E4Args &p, const CUtensorMap *tmC, 
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                float v0, v1, v2, v3;
-                f2_split(acc[8 * q + 2 * e], v0, v1);
-                f2_split(acc[8 * q + 2 * e + 1], v2, v3);
-                w[e] = pack_e4m3(v0, v1, v2, v3, inv);
+                const int j = 16 * q + 4 * e;
+                w[e] = pack_e4m3<false>(acc[j], acc[j + 1], acc[j + 2], acc[j + 3], inv);
             }
             stage_piece(tile, lane, q, w[0], w[1], w[2], w[3]);
         }
@@ -254,8 +331,7 @@ __device__ __forceinline__ void finish(const E4Args &p, const CUtensorMap *tmC, 
                 uint32_t w[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    float v0, v1;
-                    f2_split(acc[32 * c + 4 * q + e], v0, v1);
+                    const float v0 = acc[64 * c + 8 * q + 2 * e], v1 = acc[64 * c + 8 * q + 2 * e + 1];
                     w[e] = p.cdt == K_BF16 ? pack_bf16x2(v0, v1) : pack_f16x2(v0, v1);
                 }
                 stage_piece(tile, lane, q, w[0], w[1], w[2], w[3]);
@@ -281,7 +357,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t *empty = full + STAGES;
     uint64_t *tfull = empty + STAGES;
     uint64_t *tempty = tfull + 4;
-    uint64_t *drain = tempty + 4;
+    uint64_t *sfull = tempty + 4, *sempty = sfull + 4;  // [group][chunk]
+    uint64_t *drain = sempty + 4;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
@@ -297,6 +374,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < NBUF; i++) {
             mbar_init(&tfull[i], 1);
             mbar_init(&tempty[i], (PING ? 4 : 8) * (PAIR ? 2 : 1));
+        }
+        for (int i = 0; i < 4; i++) {
+            mbar_init(&sfull[i], 1);
+            mbar_init(&sempty[i], 4);
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
@@ -327,10 +408,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int num_n = (p.N + BN - 1) / BN;
     const int num_tiles = (p.M + TM - 1) / TM * num_n;
     const int kblocks = (p.K + BK - 1) / BK;
+    const int tstep = PING ? 2 * step : step;  // of a group's tiles
 
-    // The warpgroups start with 168 registers a thread: 128 x 40 + 256 x 224 <= 384 x 168.
+    // The warpgroups start with 168 registers a thread: 128 x 72 + 256 x 216 <= 384 x 168.
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 0) {
             if (elect_one()) {
                 prefetch_tmap(&tmA);
@@ -341,8 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int t = first; t < num_tiles && ok; t += step) {
                     const int m0 = (t / num_n) * TM + (int)rank * BM, n0 = (t % num_n) * BN;
                     for (int kb = 0; kb < kblocks; kb++) {
-                        if (!(PAIR ? mbar_wait_cluster(&empty[stage], phase ^ 1, p.err, abort_flag)
-                                   : mbar_wait(&empty[stage], phase ^ 1, p.err, abort_flag))) {
+                        if (!mbar_wait_brief<PAIR>(&empty[stage], phase ^ 1, p.err, abort_flag)) {
                             ok = false;
                             break;
                         }
@@ -388,9 +469,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         uint32_t c = done[g];
                         for (int kb = 0; kb < kblocks; kb++) {
                             const uint32_t buf = 2 * g + (c & 1), parity = (c >> 1 & 1) ^ 1;
-                            if (!(PAIR ? mbar_wait_cluster(&tempty[buf], parity, p.err, abort_flag)
-                                       : mbar_wait(&tempty[buf], parity, p.err, abort_flag)) ||
-                                !mbar_wait(&full[stage], phase, p.err, abort_flag)) {
+                            if (!mbar_wait_brief<PAIR>(&tempty[buf], parity, p.err, abort_flag) ||
+                                !mbar_wait_brief(&full[stage], phase, p.err, abort_flag)) {
                                 ok = false;
                                 break;
                             }
@@ -436,65 +516,43 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_wait(drain, 0, p.err, &no_abort);
             }
         }
+        else {
+            const int g = warp - 2;
+            feed_scales(p, reinterpret_cast<float *>(smem + L::SCALE_OFF + g * kScaleRing), sfull + 2 * g, sempty + 2 * g,
+                        first + (PING ? g * step : 0), tstep, num_tiles, num_n, TM, BN, (int)rank * BM,
+                        PING ? 0 : g * 128, kblocks, lane, abort_flag);
+        }
     }
     else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int group = (warp - 4) >> 2;
         const int quarter = warp & 3;  // the TMEM lanes this warp may read
         const int row = (int)rank * BM + quarter * 32, col = PING ? 0 : group * 128;
         const uint32_t stage_tile = smem_addr(smem + L::EPI_OFF + (warp - 4) * kStageTile);
-        const int tstep = PING ? 2 * step : step;
         const int t0 = first + (PING ? group * step : 0);
+        const float *ring = reinterpret_cast<const float *>(smem + L::SCALE_OFF + group * kScaleRing) + quarter * 32 + lane;
         if (lane == 0)
             prefetch_tmap(&tmC);
-        Scales sc;
-        sc.t = t0;
-        sc.kb = 0;
-        sc.tile(p, num_n, TM, BN, row + lane, col);
-        auto next_scales = [&]() {
-            sc.a[Scales::D - 1] = scale_raw(p.sa, p.sadt, sc.ia + sc.kb);
-            sc.b[Scales::D - 1] = scale_raw(p.sb, p.sbdt, sc.ib + sc.kb);
-            if (++sc.kb == kblocks) {
-                sc.kb = 0;
-                if (sc.t + tstep < num_tiles)
-                    sc.t += tstep;
-                sc.tile(p, num_n, TM, BN, row + lane, col);
-            }
-        };
-        auto shift_scales = [&]() {
-#pragma unroll
-            for (int i = 0; i + 1 < Scales::D; i++) {
-                sc.a[i] = sc.a[i + 1];
-                sc.b[i] = sc.b[i + 1];
-            }
-        };
-        if (t0 < num_tiles) {
-#pragma unroll
-            for (int i = 0; i < Scales::D; i++) {
-                shift_scales();
-                next_scales();
-            }
-        }
         // A barrier's parity tells neighbouring phases apart only: each group has
         // buffers of its own (PING), whose every phase it waits for.
-        uint32_t c = 0;
+        uint32_t c = 0, chunk = 0;
         bool ok = true;
         for (int t = t0; t < num_tiles && ok; t += tstep) {
-            uint64_t acc[64];
+            float acc[128];
 #pragma unroll
-            for (int j = 0; j < 64; j++)
-                acc[j] = 0;
+            for (int j = 0; j < 128; j++)
+                acc[j] = 0.0f;
             for (int kb = 0; kb < kblocks; kb++, c++) {
                 const uint32_t buf = (PING ? 2 * group : 0) + (c & 1), parity = c >> 1 & 1;
-                ok = PAIR ? mbar_wait_cluster(&tfull[buf], parity, p.err, abort_flag)
-                          : mbar_wait(&tfull[buf], parity, p.err, abort_flag);
+                const uint32_t slot = 2 * group + (chunk & 1);
+                ok = kb % kChunk || mbar_wait_brief(&sfull[slot], chunk >> 1 & 1, p.err, abort_flag);
+                ok = ok && mbar_wait_brief<PAIR>(&tfull[buf], parity, p.err, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok)
                     break;
                 tc_fence_after();
                 const uint32_t src = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * BN + col;
-                const float s = scale_of(sc.a[0], p.sadt) * scale_of(sc.b[0], p.sbdt);
-                const uint64_t s2 = f2_make(s, s);
+                const float s = ring[((chunk & 1) * kChunk + kb % kChunk) * BM];
                 uint32_t r[2][32];
                 tmem_ld32(src, r[0]);
                 tmem_wait_ld(r[0]);
@@ -503,9 +561,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (q < 3)
                         tmem_ld32(src + 32 * (q + 1), r[(q + 1) & 1]);
 #pragma unroll
-                    for (int j = 0; j < 16; j++)
-                        acc[16 * q + j] = fma2(f2_make(__uint_as_float(r[q & 1][2 * j]), __uint_as_float(r[q & 1][2 * j + 1])),
-                                               s2, acc[16 * q + j]);
+                    for (int j = 0; j < 32; j++)  // (packed pairs cost two moves each)
+                        acc[32 * q + j] = fmaf(__uint_as_float(r[q & 1][j]), s, acc[32 * q + j]);
                     if (q < 3)
                         tmem_wait_ld(r[(q + 1) & 1]);
                     if (q == 2) {  // the buffer has been read
@@ -513,14 +570,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                         __syncwarp();
                         if (lane == 0) {
                             if constexpr (PAIR)
-                                mbar_arrive_cluster(mapa_shared(smem_addr(&tempty[buf]), 0));
+                                mbar_arrive_cluster_relaxed(mapa_shared(smem_addr(&tempty[buf]), 0));
                             else
-                                mbar_arrive(&tempty[buf]);
+                                mbar_arrive_relaxed(&tempty[buf]);
                         }
                     }
                 }
-                shift_scales();
-                next_scales();
+                if (kb % kChunk == kChunk - 1 || kb + 1 == kblocks) {
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive(&sempty[slot]);
+                    chunk++;
+                }
             }
             if (!ok)
                 break;
@@ -635,6 +696,11 @@ extern "C" int k_gemm_e4m3(int M, int N, int K, const struct k_rows *A, const st
     p.ldsb = SB->ld;
     p.sadt = SA->dt;
     p.sbdt = SB->dt;
+    auto aligned = [](const struct k_rows *r) {
+        return r->ld % 4 == 0 && reinterpret_cast<uintptr_t>(r->p) % (r->dt == K_E8M0 ? 4 : 16) == 0;
+    };
+    p.savec = aligned(SA);
+    p.sbvec = aligned(SB);
     p.bias = bias;
     p.c = C->p;
     p.ldc = C->ld;
@@ -657,12 +723,9 @@ extern "C" int k_gemm_e4m3(int M, int N, int K, const struct k_rows *A, const st
                                 M > 1 ? (uint64_t)A->ld : ((uint64_t)K + 15) / 16 * 16, 128, 32))
         return K_ETMAP;  // (a map for the argument that is not used)
     cudaStream_t st = reinterpret_cast<cudaStream_t>(s);
-    // Pairs where their tiles of 256 x 128 fill the device.
-    const long pairs = (long)((M + 255) / 256) * ((N + 127) / 128);
-    if (pairs >= device_sms() / 2) {
-        const int rc = launch_act<128, true>(p, A, B, tc, st);
-        if (rc != K_EARG)
-            return rc;
-    }
+    // Tiles of 128 x 256 where they fill the device (41472 x 1024 x 4096: 191 us, 271
+    // with 128 columns; 603 x 520 x 588: 10.7 and 9.3).
+    if ((long)((M + 127) / 128) * ((N + 255) / 256) >= device_sms())
+        return launch_act<256, false>(p, A, B, tc, st);
     return launch_act<128, false>(p, A, B, tc, st);
 }

@@ -191,6 +191,46 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity
     }
 }
 
+// An arrival that orders no memory accesses: enough after tcgen05 loads, which
+// tcgen05.wait::ld and tcgen05.fence::before_thread_sync order. A release at cluster
+// scope takes about 1000 cycles.
+__device__ __forceinline__ void mbar_arrive_relaxed(uint64_t *bar)
+{
+    asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr)
+{
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+                 : "memory");
+}
+
+// The same waits (CLUSTER: acquire at cluster scope) for pipelines that wait often
+// and briefly: the timer, whose reading takes longer than such a wait, is first
+// read after 64 failed tries.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool mbar_wait_brief(uint64_t *bar, uint32_t parity, int *err,
+                                                volatile int *abort_flag)
+{
+    const uint32_t a = smem_addr(bar);
+    uint64_t t0 = 0;
+    for (uint32_t it = 1;; it++) {
+        if (CLUSTER ? mbar_try_wait_cluster(a, parity) : mbar_try_wait(a, parity))
+            return true;
+        if ((it & 63) == 0) {
+            if (*abort_flag)
+                return false;
+            const uint64_t t = globaltimer();
+            if (!t0)
+                t0 = t;
+            else if (t - t0 > kWaitLimitNs) {
+                atomicCAS(err, kErrNone, kErrWaitTimeout);
+                *abort_flag = 1;
+                return false;
+            }
+        }
+    }
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_load_2d(void *smem_dst, const CUtensorMap *map, uint64_t *bar,
                                             int32_t x, int32_t y)

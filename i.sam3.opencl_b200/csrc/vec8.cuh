@@ -58,19 +58,11 @@ __device__ __forceinline__ Raw8 load8(const void *p, int dt, long i, int n)
     return r;
 }
 
-__device__ __forceinline__ void unpack8(const Raw8 &r, int dt, float (&v)[8])
+// Eight 16-bit values.
+__device__ __forceinline__ void unpack8_16(const uint4 &a, int dt, float (&v)[8])
 {
-    const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
-    if (dt == K_F32) {
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            v[e] = __uint_as_float(w[e]);
-        v[4] = __uint_as_float(r.b.x);
-        v[5] = __uint_as_float(r.b.y);
-        v[6] = __uint_as_float(r.b.z);
-        v[7] = __uint_as_float(r.b.w);
-    }
-    else if (dt == K_BF16) {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    if (dt == K_BF16) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             v[2 * e] = __uint_as_float(w[e] << 16);
@@ -87,10 +79,36 @@ __device__ __forceinline__ void unpack8(const Raw8 &r, int dt, float (&v)[8])
     }
 }
 
+__device__ __forceinline__ void unpack8(const Raw8 &r, int dt, float (&v)[8])
+{
+    if (dt != K_F32) {
+        unpack8_16(r.a, dt, v);
+        return;
+    }
+    v[0] = __uint_as_float(r.a.x);
+    v[1] = __uint_as_float(r.a.y);
+    v[2] = __uint_as_float(r.a.z);
+    v[3] = __uint_as_float(r.a.w);
+    v[4] = __uint_as_float(r.b.x);
+    v[5] = __uint_as_float(r.b.y);
+    v[6] = __uint_as_float(r.b.z);
+    v[7] = __uint_as_float(r.b.w);
+}
+
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
 {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ void store1(void *p, int dt, long i, float v)
+{
+    if (dt == K_F32)
+        reinterpret_cast<float *>(p)[i] = v;
+    else if (dt == K_BF16)
+        reinterpret_cast<__nv_bfloat16 *>(p)[i] = from_f<__nv_bfloat16>(v);
+    else
+        reinterpret_cast<__half *>(p)[i] = from_f<__half>(v);
 }
 
 template <bool VEC>
@@ -126,17 +144,17 @@ __device__ __forceinline__ void store8(void *p, int dt, long i, int n, const flo
 
 // Eight E4M3 values, packed.
 template <bool VEC>
-__device__ __forceinline__ void store8_e4m3(void *p, long i, int n, uint32_t lo, uint32_t hi)
+__device__ __forceinline__ void store8_e4m3(void *p, long i, int n, uint2 v)
 {
     uint8_t *q = reinterpret_cast<uint8_t *>(p) + i;
     if (VEC && n >= 8) {
-        *reinterpret_cast<uint2 *>(q) = make_uint2(lo, hi);
+        *reinterpret_cast<uint2 *>(q) = v;
         return;
     }
 #pragma unroll
     for (int e = 0; e < 8; e++)
         if (e < n)
-            q[e] = (uint8_t)((e < 4 ? lo : hi) >> (8 * (e & 3)));
+            q[e] = (uint8_t)((e < 4 ? v.x : v.y) >> (8 * (e & 3)));
 }
 
 // Whether rows of the operand start at vectors of eight values (16 bytes; 8 of E4M3).

@@ -328,6 +328,17 @@ CASES = [
     (2, 700, 1024, "bf16", "bf16", "bf16", 0, 1, "sample", True, True, True, 1.0, 0),
     (3, 1801, 1000, "f32", "f32", "e4m3", 2, 2, "none", False, False, False, 1.0, 0),
     (2, 5184, 256, "bf16", "bf16", "e4m3", 1, 2, "sample", True, True, False, 1.0, 0),
+    (1, 13, 64, "bf16", "bf16", "e4m3", 1, 1, "row", True, True, True, 1.0, 8),        # parts of a warp
+    (3, 5001, 40, "f16", "f16", "e4m3", 1, 2, "sample", True, True, True, 1.0, 0),
+    (7, 1003, 128, "f32", "bf16", "f16", 2, 1, "row", False, True, True, 1.0, 0),
+    (2, 3003, 96, "bf16", "bf16", "bf16", 0, 1, "sample", True, True, True, 1.0, 8),
+    (2, 3003, 77, "bf16", "bf16", "e4m3", 1, 1, "sample", True, True, True, 1.0, 0),   # rows that are not aligned
+    (1, 3100, 333, "f32", "f16", "e4m3", 1, 2, "row", True, False, True, 1.0, 1),
+    (2, 700, 1021, "f16", "f16", "e4m3", 2, 1, "sample", True, True, True, 1.0, 2),
+    (1, 1300, 2047, "f32", "f32", "e4m3", 1, 1, "none", True, True, True, 1.0, 0),
+    (2, 400, 5001, "bf16", "bf16", "bf16", 1, 1, "sample", True, True, True, 1.0, 0),
+    (1, 20000, 1024, "bf16", "bf16", "e4m3", 2, 2, "row", True, False, False, 1.0, 0),
+    (3, 300, 8192, "f16", "f16", "f16", 1, 1, "sample", True, True, True, 1.0, 0),
 ]
 
 
