@@ -79,9 +79,8 @@ __device__ __forceinline__ float scale_of(uint32_t raw, int dt)
 {
     if (dt != K_E8M0)
         return __uint_as_float(raw);
-    // 2^-127 is below the normal numbers, 255 stands for NaN
-    return raw == 0 ? __uint_as_float(0x00400000u)
-                    : __uint_as_float(raw == 255 ? 0x7fffffffu : raw << 23);
+    // 0 is 2^-127, below the normal numbers, and 255 NaN: both have one more bit
+    return __uint_as_float(raw << 23 | (((raw + 1) & 255u) <= 1u ? 0x00400000u : 0u));
 }
 __device__ __forceinline__ void put_scale(void *p, int dt, long i, uint32_t byte)
 {

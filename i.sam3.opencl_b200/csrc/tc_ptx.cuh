@@ -191,6 +191,20 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity
     }
 }
 
+// Whether the phase has completed, without waiting for it.
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, P;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // An arrival that orders no memory accesses: enough after tcgen05 loads, which
 // tcgen05.wait::ld and tcgen05.fence::before_thread_sync order. A release at cluster
 // scope takes about 1000 cycles.
@@ -443,6 +457,40 @@ __device__ __forceinline__ void tc_mma_e4m3_pair(uint32_t d_tmem, uint64_t adesc
         : "memory");
 }
 
+// E4M3 operands with a power-of-two scale for each 32 columns of a row: the E8M0
+// byte of row r of a 128-row block lies at lane r % 32 (of every lane quarter),
+// column r / 32, byte `id` of the descriptor.
+__device__ __forceinline__ void tc_mma_mx(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t sfa, uint32_t sfb, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_mx_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t sfa, uint32_t sfb, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+
+// 32 lanes x 4 consecutive 32-bit columns from registers.
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c),
+                 "r"(d)
+                 : "memory");
+}
+
 // D (+)= A * B with A read from tensor memory (M rows in TMEM lanes, each
 // 32-bit column holding two consecutive K elements, K = 16 per instruction
 // in 8 columns from a_tmem) and B from a shared-memory descriptor.
@@ -615,6 +663,13 @@ __host__ __device__ constexpr uint32_t idesc_bf16_f32(int M, int N, int a_mn_maj
 __host__ __device__ constexpr uint32_t idesc_e4m3_f32(int M, int N)
 {
     return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// The same for kind::mxf8f6f4: E8M0 scales (bit 23), byte `id` of their words.
+__host__ __device__ constexpr uint32_t idesc_mx_e4m3(int M, int N, int id)
+{
+    return ((uint32_t)id << 4) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24) |
+           ((uint32_t)id << 29);
 }
 
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi)

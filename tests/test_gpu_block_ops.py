@@ -253,6 +253,13 @@ def run_gemm(be, sb, M, N, K, dsa, dsb, out, act, use_bias, seed=0, ldc=None, of
     (5185, 1111, 640, "e8m0", "e8m0", "bf16", "gelu", True),
     (2500, 4096, 1024, "e8m0", "e8m0", "e4m3", "gelu", True),
     (20000, 300, 4096, "e8m0", "e8m0", "bf16", "none", False),
+    (250, 100, 1000, "f32", "f32", "f16", "gelu", True),     # few rows, in groups of 32
+    (77, 2000, 33, "f32", "e8m0", "f32", "none", True),
+    (250, 1500, 4096, "f32", "f32", "bf16", "none", True),   # the groups take k-blocks in turn
+    (300, 1500, 700, "f32", "f32", "e4m3", "gelu", True),
+    (20000, 140, 128, "f32", "f32", "f32", "none", True),
+    (9000, 700, 1030, "e8m0", "f32", "e4m3", "relu", False),
+    (128, 128, 1, "f32", "f32", "e4m3", "none", False),
 ])
 def test_gemm(be, sb, M, N, K, dsa, dsb, out, act, use_bias):
     run_gemm(be, sb, M, N, K, dsa, dsb, out, act, use_bias)
