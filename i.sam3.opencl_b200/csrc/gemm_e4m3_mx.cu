@@ -1,10 +1,9 @@
 // SPDX-License-Identifier: Unlicense
 // Product of E4M3 matrices whose block scales are both powers of two (E8M0), into
-// 16-bit or E4M3 results: the matrix unit applies the scales itself
+// 16-bit, E4M3 or (over short rows) 32-bit results: the matrix unit applies the scales itself
 // (tcgen05.mma kind::mxf8f6f4, a scale for each 32 columns, the same for the four of a
 // block), so that a tile's products add up in tensor memory over all of K and
-// the epilogue runs once a tile. (32-bit results take the other form: the matrix
-// unit truncates its sums.)
+// the epilogue runs once a tile.
 //
 // Four warpgroups: a TMA producer and an MMA issuer; four warps that read the scales
 // of four k-blocks at a time and write them to tensor memory, each its own lane

@@ -18,8 +18,8 @@ __device__ __forceinline__ float elem(const void *p, int dt, long i)
 {
     if (dt == K_F32)
         return __ldg(reinterpret_cast<const float *>(p) + i);
-    return dt == K_BF16 ? to_f(reinterpret_cast<const __nv_bfloat16 *>(p)[i])
-                        : to_f(reinterpret_cast<const __half *>(p)[i]);
+    const uint16_t v = __ldg(reinterpret_cast<const uint16_t *>(p) + i);
+    return dt == K_BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
 }
 
 // n of the eight values at element i; VEC: i is vector aligned.
