@@ -569,9 +569,12 @@ int cb_quantize_e4m3(cb_backend *b, int nb, int N, int K, int brows,
  * values, each its own type; a product of two scales stays within 32 bits);
  * bias F32 [N] or NULL; C F32, BF16 or F16, rounded once, or E4M3, then SC [M,
  * ceil(N / 128)] (E8M0 or F32) receives the scales cb_quantize_e4m3 (brows 1)
- * would give act(...) in 32 bits. Sums in 32 bits. Rows of A and B start at
- * multiples of 16 bytes (off and ld; what lies behind column K of a row is not
- * used); C takes any ld. s0 is of no account. GELU as cb_groupnorm's. */
+ * would give act(...) in 32 bits. Sums in 32 bits; where both scales are E8M0 and C is
+ * not F32 or K at most 1024 by the matrix unit, which truncates (3e-7 of the result over
+ * 4096 columns), else a block's. Rows of A and B start at multiples of 16 bytes (off
+ * and ld; what lies behind column K of a row is not used); C takes any ld. s0 is of no
+ * account. GELU is 0.5 z (1 + erf(z / sqrt 2)) for F32 results; for others its part
+ * beside max(z, 0) is off by at most 1.2e-5 of itself up to |z| = 8, by 6e-15 beyond. */
 int cb_gemm_e4m3(cb_backend *b, int M, int N, int K, struct cb_opnd A,
                  struct cb_opnd SA, struct cb_opnd B, struct cb_opnd SB,
                  struct cb_opnd C, const struct cb_opnd *SC, cb_mem bias, int act);
@@ -592,7 +595,8 @@ struct cb_norm {
  *   r = X + alpha ls[c] gate[b, n, c] h        residual scale and gate (H NULL: r = X)
  *   R = r                                      the residual stream (R NULL: not kept)
  *   Y = pre(r) (1 + scale[b, n, c]) + shift[b, n, c]   norm before the next block
- * in 32 bits, r not rounded before pre. ls F32 [C] or NULL (1); gate, scale, shift
+ * in 32 bits (squares of a row's values, LAYER: of their distances from the mean, within
+ * them), r not rounded before pre. ls F32 [C] or NULL (1); gate, scale, shift
  * F32, BF16 or F16 operands, NULL for 1, 0, 0 (ld 0: one row for a sample, s0 0: for
  * all). X F32, BF16 or F16; H and R of X's type, H also BF16 or F16 beside an F32
  * X; Y of X's type, BF16 or F16 of an F32 X, or E4M3 with the scales S
