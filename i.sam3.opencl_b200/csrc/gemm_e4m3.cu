@@ -360,7 +360,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int j = 0; j < 32; j++)
                         join[j * BM] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
                 }
-                asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");  // the two warps of the rows
+                // the two warps of the rows, which go on or give up together
+                uint32_t both;
+                asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                             "bar.red.and.pred p, %2, 64, q;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+                             : "=r"(both)
+                             : "r"((uint32_t)ok), "r"(1 + quarter)
+                             : "memory");
+                ok = both != 0;
                 if (group == 0) {
 #pragma unroll
                     for (int j = 0; j < 32; j++) {

@@ -134,19 +134,20 @@ __device__ __forceinline__ void param8(const float *p, const Cols<T, V, VEC> &c,
         v[e] = none;
     if (!p)
         return;
-    if (VEC) {
+    if constexpr (VEC) {
         if (!c.in(j, 0, C))
             return;
         const float4 a = __ldg(reinterpret_cast<const float4 *>(p + c.at(j, 0)));
         const float4 b = __ldg(reinterpret_cast<const float4 *>(p + c.at(j, 4)));
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
         v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        return;
     }
+    else {
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-        if (c.in(j, e, C))
-            v[e] = __ldg(p + c.at(j, e));
+        for (int e = 0; e < 8; e++)
+            if (c.in(j, e, C))
+                v[e] = __ldg(p + c.at(j, e));
+    }
 }
 
 // Eight values of an operand's row.
