@@ -448,10 +448,10 @@ extern "C" int k_gemm_e4m3(int M, int N, int K, const struct k_rows *A, const st
     p.err = err;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(s);
     // Of the forms that take the call, the one whose time, from measured ones, is the
-    // smallest (in 1/100 us, without the launch). Tiles of the form below: 0.40 us a k-block
-    // and 2 a wave for 128 columns, 0.55 and 2.5 for 256 (256 x 4096 x 4096: 17.8 and 22.6
-    // us, 41472 x 1024 x 4096: 245 and 182); 32 rows of the form for few: 0.5 us for 2^20
-    // weights (32 x 4096 x 4096: 13.1 us, 10.4 by gemm_e4m3_mx.cu; 32 x 4096 x 1024: 4.8 and 6.1).
+    // smallest (in 1/100 us). Tiles of the form below: 0.40 us a k-block and 2 a wave for 128
+    // columns, 0.55 and 2.5 for 256 (256 x 4096 x 4096: 17.8 and 22.6 us, 41472 x 1024 x 4096:
+    // 245 and 182); 32 rows of the form for few: 0.62 us for 2^20 weights (32 x 4096 x 4096: 13.1
+    // us, 10.4 by gemm_e4m3_mx.cu; 32 x 4096 x 1024: 4.8 and 6.1).
     const long sms = device_sms(), kb = (K + BK - 1) / BK;
     const long t1 = (long)((M + 127) / 128) * ((N + 127) / 128), t2 = (long)((M + 127) / 128) * ((N + 255) / 256);
     const long c1 = (t1 + sms - 1) / sms * (40 * kb + 200), c2 = (t2 + sms - 1) / sms * (55 * kb + 250);
@@ -459,8 +459,8 @@ extern "C" int k_gemm_e4m3(int M, int N, int K, const struct k_rows *A, const st
     // against 64 bits 7e-8 of 32-bit results over 1024 columns (4e-8 by the form below), 2.8e-7
     // over 4096 (7e-8).
     const bool mx = p.sadt == K_E8M0 && p.sbdt == K_E8M0 && (p.cdt != K_F32 || kb <= 8);
-    const long tiles = mx ? cost_mx(p) : (c1 < c2 ? c1 : c2);
-    if (C->dt != K_E4M3 && M <= 256 && (long)((M + 31) / 32) * N * K / 20972 < tiles)
+    const long tiles = mx ? cost_mx(p) : 270 + (c1 < c2 ? c1 : c2);
+    if (C->dt != K_E4M3 && M <= 256 && 250 + (long)((M + 31) / 32) * N * K / 16900 < tiles)
         return launch_few(p, A, B, st);
     CUtensorMap tc;
     const int es = C->dt == K_F32 ? 4 : (C->dt == K_E4M3 ? 1 : 2);

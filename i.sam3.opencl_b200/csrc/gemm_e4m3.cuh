@@ -308,8 +308,7 @@ inline int launch_tiles(const E4Args &p, const struct k_rows *A, const struct k_
 // The form for few rows of A and results that are not E4M3 (gemm_e4m3_few.cu).
 int launch_few(const E4Args &p, const struct k_rows *A, const struct k_rows *B, cudaStream_t s);
 
-// The form for E8M0 scales and results of at most 16 bits (gemm_e4m3_mx.cu), and its
-// time without the launch in 1/100 us.
+// The form for E8M0 scales (gemm_e4m3_mx.cu), and its time in 1/100 us.
 long cost_mx(const E4Args &p);
 int launch_mx(const E4Args &p, const struct k_rows *A, const struct k_rows *B, const CUtensorMap &tc, cudaStream_t s);
 

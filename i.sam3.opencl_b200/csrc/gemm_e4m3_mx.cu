@@ -376,8 +376,11 @@ static long large_tiles(const E4Args &p)
 
 long cost_mx(const E4Args &p)
 {
-    const long a = small_tiles(p), b = large_tiles(p);
-    return (a < b ? a : b) / 19;
+    const long a = small_tiles(p), b = large_tiles(p), kb = (p.K + BK - 1) / BK;
+    // a wave of its own: 0.17 us a k-block (8 x 4096 x 1024 6.0 us, 256 x 4096 x 4096 11.5)
+    if ((long)((p.M + 127) / 128) * ((p.N + 127) / 128) <= device_sms())
+        return 460 + 17 * kb;
+    return 400 + (a < b ? a : b) / 19;
 }
 
 int launch_mx(const E4Args &p, const struct k_rows *A, const struct k_rows *B, const CUtensorMap &tc, cudaStream_t s)
