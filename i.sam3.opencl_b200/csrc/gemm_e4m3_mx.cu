@@ -12,6 +12,9 @@
 //           of B's tile; one accumulator, read into registers by both groups before
 //           the next tile's products start;
 //   BN 128: two accumulators of 128, a group each.
+// 41472 x 1024 x 4096 131 us (2.66 PFLOP/s), 41472 x 4096 x 1024 150 us; with GELU and E4M3
+// results 182 us, 215 under the power cap, where the epilogue counts: four instructions a
+// value for GELU's polynomial (in pairs), two for the scale and its product, one to round.
 #include "gemm_e4m3.cuh"
 
 namespace sam3 {

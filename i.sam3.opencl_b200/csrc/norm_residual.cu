@@ -15,6 +15,8 @@
 #include "tmap.cuh"
 #include "vec8.cuh"
 
+#include <type_traits>
+
 namespace sam3 {
 namespace {
 
@@ -75,6 +77,18 @@ struct Cols {
     }
 };
 
+// go(element type as a constant): one branch for a loop over elements.
+template <typename F>
+__device__ __forceinline__ void typed(int dt, const F &go)
+{
+    if (dt == K_F32)
+        go(std::integral_constant<int, K_F32>{});
+    else if (dt == K_BF16)
+        go(std::integral_constant<int, K_BF16>{});
+    else
+        go(std::integral_constant<int, K_F16>{});
+}
+
 // The values of an operand's row, as stored where they are vectors. DT: its type,
 // or kAnyType for the type that the operand names.
 constexpr int kAnyType = -1;
@@ -98,11 +112,13 @@ struct Row {
             }
         }
         else {
+            typed(dt, [&](auto t) {
 #pragma unroll
-            for (int j = 0; j < V; j++)
+                for (int j = 0; j < V; j++)
 #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    f[j][e] = c.in(j, e, C) ? elem(k.p, dt, base + c.at(j, e)) : 0.0f;
+                    for (int e = 0; e < 8; e++)
+                        f[j][e] = c.in(j, e, C) ? elem(k.p, decltype(t)::value, base + c.at(j, e)) : 0.0f;
+            });
         }
     }
     __device__ __forceinline__ void get(int any, int j, float (&v)[8]) const
@@ -156,16 +172,17 @@ __device__ __forceinline__ void operand8(const k_rows &k, long base, const Cols<
 {
     if constexpr (VEC)
         unpack8(c.in(j, 0, C) ? load8<true>(k.p, k.dt, base + c.at(j, 0), 8) : Raw8{}, k.dt, v);
-    else {
+    else
+        typed(k.dt, [&](auto t) {
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-            v[e] = c.in(j, e, C) ? elem(k.p, k.dt, base + c.at(j, e)) : 0.0f;
-    }
+            for (int e = 0; e < 8; e++)
+                v[e] = c.in(j, e, C) ? elem(k.p, decltype(t)::value, base + c.at(j, e)) : 0.0f;
+        });
 }
 
 // What multiplies and is added to a normalised row: one vector each, kept in shared
-// memory for the rows of a sample (SHARED) in two halves of four columns of every
-// eight, so that a warp's 16-byte reads meet no bank twice.
+// memory for the rows of a sample (SHARED); VEC: in two halves of four columns of
+// every eight, so that a warp's 16-byte reads meet no bank twice.
 template <int T, int V, bool VEC>
 __device__ __forceinline__ void shared8(const float *s, const Cols<T, V, VEC> &c, int j, int half, float (&v)[8])
 {
@@ -177,10 +194,8 @@ __device__ __forceinline__ void shared8(const float *s, const Cols<T, V, VEC> &c
     }
     else {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int at = c.at(j, e);
-            v[e] = s[(at & 4 ? half : 0) + (at >> 3) * 4 + (at & 3)];
-        }
+        for (int e = 0; e < 8; e++)
+            v[e] = s[c.at(j, e)];
     }
 }
 
@@ -240,12 +255,13 @@ __device__ __forceinline__ void put8(const k_norm_args &p, long y, long s, const
             if (write && c.in(j, 0, p.C))
                 store8<true>(p.Y.p, dt, y + c.at(j, 0), 8, v);
         }
-        else {
+        else if (write)
+            typed(dt, [&](auto t) {
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (c.in(j, e, p.C))
-                    store1(p.Y.p, dt, y + c.at(j, e), v[e]);
-        }
+                for (int e = 0; e < 8; e++)
+                    if (c.in(j, e, p.C))
+                        store1(p.Y.p, decltype(t)::value, y + c.at(j, e), v[e]);
+            });
         return;
     }
     // a half-warp holds a block of 128 columns (VEC), else four values of each lane
@@ -323,7 +339,7 @@ __global__ void __launch_bounds__(cta_threads(T)) norm_rows_kernel(const __grid_
             step = kRows;
             __syncthreads();  // the last sample's rows are done with the vectors
             for (int i = threadIdx.x; i < p.C; i += blockDim.x) {
-                const int at = (i & 4 ? kHalf : 0) + (i >> 3) * 4 + (i & 3);
+                const int at = VEC ? (i & 4 ? kHalf : 0) + (i >> 3) * 4 + (i & 3) : i;
                 float f = p.alpha;
                 if (p.ls)
                     f *= __ldg(p.ls + i);
@@ -432,12 +448,13 @@ __global__ void __launch_bounds__(cta_threads(T)) norm_rows_kernel(const __grid_
                         if (c.in(j, 0, p.C))
                             store8<true>(p.R.p, dt, at + c.at(j, 0), 8, r[j]);
                     }
-                    else {
+                    else
+                        typed(dt, [&](auto t) {
 #pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            if (c.in(j, e, p.C))
-                                store1(p.R.p, dt, at + c.at(j, e), r[j][e]);
-                    }
+                            for (int e = 0; e < 8; e++)
+                                if (c.in(j, e, p.C))
+                                    store1(p.R.p, decltype(t)::value, at + c.at(j, e), r[j][e]);
+                        });
                 }
             }
             if (!p.Y.p)
