@@ -304,13 +304,13 @@ __device__ __forceinline__ void put8(const k_norm_args &p, long y, long s, const
 
 __host__ __device__ constexpr int cta_threads(int T) { return T < 256 ? (T > 32 ? T : 256) : T; }
 
-// CTAs an SM is to hold. Of wide rows without the shared vectors as many as 64
+// CTAs an SM is to hold (0: left to the compiler). Of wide rows without the shared vectors as many as 64
 // registers a thread allow (4000 rows of 6000 fp32: 159 us with one CTA, 113 with two); with
 // them the next row's loads would be spilled (20000 rows of 2048 fp32: 107 and 160).
 template <int T, int V, bool VEC, bool SHARED>
 __host__ __device__ constexpr int ctas_wanted()
 {
-    return VEC && !SHARED && T > 32 && V == 2 ? 1024 / T : 1;
+    return VEC && !SHARED && T > 32 && V == 2 ? 1024 / T : 0;
 }
 
 // T threads to a row. SHARED: a CTA takes a range of rows and keeps the vectors of
