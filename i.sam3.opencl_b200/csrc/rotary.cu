@@ -124,8 +124,8 @@ __device__ __forceinline__ TO copied(TI v)
 // (cos, sin) pairs are read once for all of them. W columns are 16 bytes of
 // input, or 1 (a pair of columns 2 j, 2 j + 1 without HALVES) for rows that
 // are not 16-byte aligned. Memory bound: X read and Y written once, the
-// table rows from L2; 41472 rows of 24 heads of 64 bf16 columns 48 us, 5.3 TB/s
-// (81 % of a copy). Indexes without divisions (56 us with 64-bit ones).
+// table rows from L2; 41472 rows of 24 heads of 64 bf16 columns 42.7 us, 6.0 TB/s
+// (91 % of a copy). Indexes without divisions (64-bit ones: 56 us where 32-bit ones took 48).
 // AX = RotAxes: each pair takes the table row of its own axis; pairs of one axis
 // as a vector where a chunk has no others.
 template <typename TI, typename TO, int W, bool HALVES, typename AX>
@@ -155,16 +155,24 @@ __global__ void __launch_bounds__(256) rope_rotate_kernel(const __grid_constant_
         const int col = c < a.nrot ? (HALVES ? c * W : c * CW)
                                    : 2 * a.half + (c - a.nrot) * W;
         const int col2 = HALVES ? col + a.half : col + 1;
-        // all heads' loads before the first store, which may be to X
-        VI us[kHeads], ws[kHeads];
-#pragma unroll
-        for (int k = 0; k < kHeads; k++) {
+        // 32 bits: all heads' loads before the first store, which may be to X and which the
+        // compiler moves no load past (9003 rows of 7 heads of 80: 10.7 us, 12.4 otherwise;
+        // 16 bits: the registers cost more than that gains, 41472 rows of 24 heads of 64:
+        // 42.7 us, 51.9 with it; with three axes 47.7 and 53).
+        constexpr bool AHEAD = sizeof(TI) == 4;
+        VI us[AHEAD ? kHeads : 1], ws[AHEAD ? kHeads : 1];
+        auto fetch = [&](int k, int slot) {
             const int h = hg + k * a.nhg.d;
             if (h < a.heads) {
-                us[k] = *reinterpret_cast<const VI *>(x + h * a.sx1 + col);
+                us[slot] = *reinterpret_cast<const VI *>(x + h * a.sx1 + col);
                 if (two)
-                    ws[k] = *reinterpret_cast<const VI *>(x + h * a.sx1 + col2);
+                    ws[slot] = *reinterpret_cast<const VI *>(x + h * a.sx1 + col2);
             }
+        };
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int k = 0; k < kHeads; k++)
+                fetch(k, k);
         }
         float2 cs[NP];
         if constexpr (MANY) {
@@ -235,7 +243,9 @@ __global__ void __launch_bounds__(256) rope_rotate_kernel(const __grid_constant_
             if (h >= a.heads)
                 break;
             TO *yh = y + h * a.sy1;
-            const VI u = us[k], w = two ? ws[k] : us[k];
+            if constexpr (!AHEAD)
+                fetch(k, 0);
+            const VI u = us[AHEAD ? k : 0], w = two ? ws[AHEAD ? k : 0] : u;
             VO ou, ow;
 #pragma unroll
             for (int e = 0; e < W; e++) {
@@ -278,7 +288,8 @@ int launch(RotArgs &a, const AX &ax, long rows, int N, int hd, bool in_place, cu
     a.nrot = HALVES ? a.half / W : (W > 1 ? rot / W : a.half);
     const int nch = a.nrot + (in_place ? 0 : (hd - rot) / W);
     // Heads per thread: as many as leave a wave of threads (24 heads x 41472
-    // rows of 64 columns: 58 us with 1, 49.5 with 2, 48.0 with 4, 51.1 with 8).
+    // rows of 64 columns: 58 us with 1, 49.5 with 2, 48.0 with 4, 51.1 with 8,
+    // in a form of the loop that took 48 us where it takes 42.7 now).
     const double one = (double)rows * a.heads * nch;
     const double fill = (double)device_sms() * 2048 * 2;
     const int hpt = one >= 2 * fill ? kHeads : (one >= fill ? 2 : 1);
