@@ -26,7 +26,7 @@ struct NormArgs {
     long rows;
     long chunk;   // rows of a CTA (SHARED)
     float share;  // 1 / C
-    int gaterow, scalerow, shiftrow;  // the operand differs from row to row of a sample
+    int gaterow, scalerow, shiftrow;  // the operand is read with each row, not kept with a sample's vectors
 };
 
 // Sum over the T threads of a row in a fixed order; every thread gets it. A row of
@@ -758,7 +758,8 @@ extern "C" int k_norm_residual(const struct k_norm_args *p, k_stream s)
     auto by_row = [&](const struct k_rows &r) { return r.p && r.ld != 0 && p->N > 1; };
     a.gaterow = by_row(p->gate);
     a.scalerow = by_row(p->scale);
-    a.shiftrow = by_row(p->shift);
+    // (a sample's shift beside a scale of the rows' own is added behind that scale)
+    a.shiftrow = by_row(p->shift) || (p->shift.p && a.scalerow);
     auto whole = [](const float *v) { return reinterpret_cast<uintptr_t>(v) % 16 == 0; };
     const bool vec = p->C % 8 == 0 && rows_vec8(p->X) && rows_vec8(p->H) && rows_vec8(p->gate) && rows_vec8(p->R) &&
                      rows_vec8(p->scale) && rows_vec8(p->shift) && rows_vec8(p->Y) && whole(p->ls) &&
