@@ -89,8 +89,8 @@ __device__ __forceinline__ void typed(int dt, const F &go)
         go(std::integral_constant<int, K_F16>{});
 }
 
-// The values of an operand's row, as stored where they are vectors. DT: its type,
-// or kAnyType for the type that the operand names.
+// The values of a row of X or H (either may be R or Y too), as stored where they are
+// vectors. DT: its type, or kAnyType for the type that the operand names.
 constexpr int kAnyType = -1;
 template <int V, bool VEC, int DT>
 struct Row {
@@ -117,7 +117,7 @@ struct Row {
                 for (int j = 0; j < V; j++)
 #pragma unroll
                     for (int e = 0; e < 8; e++)
-                        f[j][e] = c.in(j, e, C) ? elem(k.p, decltype(t)::value, base + c.at(j, e)) : 0.0f;
+                        f[j][e] = c.in(j, e, C) ? elem<true>(k.p, decltype(t)::value, base + c.at(j, e)) : 0.0f;
             });
         }
     }

@@ -14,11 +14,17 @@ struct Raw8 {
     uint4 a, b;  // b: 32-bit values 4 .. 7
 };
 
+// The value at element i. WRITTEN: of memory that the kernel may write too (an operand that
+// is also the result), which the read-only path is not defined for.
+template <bool WRITTEN = false>
 __device__ __forceinline__ float elem(const void *p, int dt, long i)
 {
-    if (dt == K_F32)
-        return __ldg(reinterpret_cast<const float *>(p) + i);
-    const uint16_t v = __ldg(reinterpret_cast<const uint16_t *>(p) + i);
+    if (dt == K_F32) {
+        const float *q = reinterpret_cast<const float *>(p) + i;
+        return WRITTEN ? *q : __ldg(q);
+    }
+    const uint16_t *q = reinterpret_cast<const uint16_t *>(p) + i;
+    const uint16_t v = WRITTEN ? *q : __ldg(q);
     return dt == K_BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
 }
 

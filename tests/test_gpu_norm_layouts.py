@@ -1,6 +1,7 @@
 """GPU tests of cb_norm_residual over the layouts of its operands: gate, scale and
 shift for all rows, for a sample's or row by row, each on its own, in every form of the
-kernel on both sides of the row count where rows begin to share their sample's vectors.
+kernel on both sides of the row count where rows begin to share their sample's vectors;
+and over memory that is read and written, there too.
 
 Against norm_ref, in 64 bits; its tolerances.
 """
@@ -99,3 +100,14 @@ def test_scale_or_shift_alone(be, sb, form, many):
     for i, a in enumerate(LAYOUTS):
         call(be, sb, g, nb, N, C, dt, pad, scale=(a, "f32"), pre=1 + i % 2)
         call(be, sb, g, nb, N, C, dt, pad, shift=(a, "f16"), pre=i % 3, gate=(a, dt))
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("form", FORMS, ids=lambda f: f"{f[0]}-{f[1]}-{f[2]}")
+@pytest.mark.parametrize("place", [("X", None), ("H", None), (None, "X"), (None, "H"), ("X", "H"), ("H", "X")], ids=lambda p: f"R={p[0]},Y={p[1]}")
+def test_in_place(be, sb, place, form, many):
+    """Every row is read as it was before the call."""
+    C, dt, pad, few, lot = form
+    nb, N = lot if many else few
+    g = gen(C + N + 2)
+    call(be, sb, g, nb, N, C, dt, pad, gate=("sample", "f32"), scale=("sample", "f32"), shift=("sample", "f32"), post=2, place=place)
