@@ -26,7 +26,7 @@ CU = ["gemm_tc.cu", "attn_tc.cu", "attn_simt.cu", "attn_decoder.cu", "elementwis
       "quantize.cu", "norm_residual.cu", "gemm_e4m3.cu", "gemm_e4m3_mx.cu", "gemm_e4m3_few.cu"]
 C = ["cuda_backend.c", "sam3_ops.c", "sam3_encoder.c", "sam3_decoder.c", "sam3_neck.c", "sam3_input.c",
      "sam3_prompt.c", "sam3_block.c", "synth.c"]
-HEADERS = ["tc_ptx.cuh", "tmap.cuh", "pdl.cuh", "attn_cross.cuh", "cluster.cuh", "div.cuh", "vec.cuh", "vec8.cuh", "act.cuh", "e4m3.cuh", "gemm_e4m3.cuh", "kernels.h",
+HEADERS = ["tc_ptx.cuh", "tmap.cuh", "per_device.h", "pdl.cuh", "attn_cross.cuh", "cluster.cuh", "div.cuh", "vec.cuh", "vec8.cuh", "act.cuh", "e4m3.cuh", "gemm_e4m3.cuh", "kernels.h",
            "backend_internal.h", "operand.h"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -1001,23 +1001,11 @@ __global__ void __launch_bounds__(kThreads, HDP <= 64 ? 4 : 3) attn_few_kernel(c
     griddep_launch();
 }
 
-// CTAs of a kernel that run at the same time, asked once per device.
+// CTAs of a kernel that run at the same time.
 template <auto Kern>
 long resident(int smem)
 {
-    static int known[64];
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 && known[dev])
-        n = known[dev];
-    else {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kern, kThreads, smem) != cudaSuccess || n < 1) {
-            (void)cudaGetLastError();
-            n = 1;
-        }
-        if (dev >= 0 && dev < 64)
-            known[dev] = n;
-    }
-    return (long)n * device_sms();
+    return (long)ctas_of_sm<Kern>(kThreads, smem) * device_sms();
 }
 
 template <typename T, int HDP, int KT>

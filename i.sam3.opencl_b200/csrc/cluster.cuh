@@ -2,6 +2,8 @@
 // Host helpers of kernels launched in thread-block clusters.
 #pragma once
 
+#include "tmap.cuh"
+
 #include <cuda_runtime.h>
 
 namespace sam3 {
@@ -30,30 +32,21 @@ inline cudaError_t cluster_prepare_once(int smem)
 template <auto Kern>
 inline long clusters_at_once(int c, int threads, int smem)
 {
-    static int known[64][kMaxClusterCtas + 1];
-    int dev = 0;
-    if (c < 1 || c > kMaxClusterCtas || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
+    static PerDevice known[kMaxClusterCtas + 1];
+    if (c < 1 || c > kMaxClusterCtas)
         return 0;
-    if (!known[dev][c]) {
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = c;
-        attr[0].val.clusterDim.y = 1;
-        attr[0].val.clusterDim.z = 1;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(c);
-        cfg.blockDim = dim3(threads);
-        cfg.dynamicSmemBytes = smem;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, Kern, &cfg) != cudaSuccess) {
-            (void)cudaGetLastError();
-            return 0;
-        }
-        known[dev][c] = n + 1;
-    }
-    return known[dev][c] - 1;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = c;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(c);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return clusters_of<Kern>(known[c], cfg);
 }
 
 }  // namespace sam3

@@ -242,25 +242,6 @@ __device__ __forceinline__ void finish(const E4Args &p, const CUtensorMap *tmC, 
     }
 }
 
-// Clusters of two CTAs of a kernel that run at once (0: none), per device.
-template <auto Kern>
-inline int pairs_at_once(cudaLaunchConfig_t &cfg)
-{
-    static int known[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
-        return 0;
-    if (!known[dev]) {
-        int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, Kern, &cfg) != cudaSuccess) {
-            (void)cudaGetLastError();
-            n = 0;
-        }
-        known[dev] = n + 1;
-    }
-    return known[dev] - 1;
-}
-
 // A kernel over tiles of 128 (PAIR: 256) x BN, one CTA or pair to an SM or two;
 // K_EARG: pairs cannot be launched here.
 template <auto Kern, int BN, bool PAIR, int B_ROWS, int THREADS, int SMEM>
@@ -297,7 +278,8 @@ inline int launch_tiles(const E4Args &p, const struct k_rows *A, const struct k_
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const int most = pairs_at_once<Kern>(cfg);
+    static PerDevice pairs;
+    const int most = clusters_of<Kern>(pairs, cfg);
     if (most <= 0)
         return K_EARG;
     cfg.gridDim = dim3(2 * (tiles < most ? tiles : most));

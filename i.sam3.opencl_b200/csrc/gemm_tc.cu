@@ -930,10 +930,6 @@ int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tc,
     return launch_pdl(kern, dim3(grid), dim3(gemm_threads(EPI)), L::BYTES, s, ta, tb, tc, p, cg);
 }
 
-// Co-resident clusters of two CTAs of the pair kernel, per device (0: not
-// known yet; -1: none).
-static int g_pair_clusters[64];
-
 // The pair kernel over 256 x 256 tiles: a persistent grid of as many CTA
 // pairs as can be resident at once (each cluster on the two SMs of a TPC).
 // Returns 1 when pairs cannot be launched here (the caller uses single CTAs).
@@ -944,10 +940,8 @@ int launch_pair(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap 
 {
     constexpr int BN = 256;
     using L = GemmSmem<BN, true>;
-    auto kern = gemm_bf16_tc_kernel<BN, OUT_BF16, true, ROPE_PF, CONV3, true>;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
-        return 1;
+    constexpr auto kern = gemm_bf16_tc_kernel<BN, OUT_BF16, true, ROPE_PF, CONV3, true>;
+    static PerDevice known;
     cudaError_t e =
         smem_limit_once<gemm_bf16_tc_kernel<BN, OUT_BF16, true, ROPE_PF, CONV3, true>>(L::BYTES);
     if (e != cudaSuccess)
@@ -964,19 +958,12 @@ int launch_pair(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap 
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (g_pair_clusters[dev] == 0) {
-        int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
-            cudaGetLastError();
-            n = -1;
-        }
-        g_pair_clusters[dev] = n;
-    }
-    if (g_pair_clusters[dev] < 0)
+    const int most = clusters_of<kern>(known, cfg);
+    if (most <= 0)
         return 1;
     const int tiles = (CONV3 ? cg.cimg * cg.cyb * cg.cxb : (p.M + 2 * BM - 1) / (2 * BM)) *
                       ((p.N + BN - 1) / BN);
-    const int pairs = tiles < g_pair_clusters[dev] ? tiles : g_pair_clusters[dev];
+    const int pairs = tiles < most ? tiles : most;
     cfg.gridDim = dim3(2 * pairs);
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;

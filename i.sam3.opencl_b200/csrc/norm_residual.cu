@@ -677,24 +677,6 @@ __global__ void __launch_bounds__(T) norm_wide_kernel(const __grid_constant__ No
     }
 }
 
-// CTAs of a kernel that an SM holds, asked once per kernel and device.
-template <auto Kern>
-int ctas_of_sm(int threads, int smem)
-{
-    static int known[64];
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
-        return 1;
-    if (!known[dev]) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kern, threads, smem) != cudaSuccess || n < 1) {
-            (void)cudaGetLastError();
-            n = 1;
-        }
-        known[dev] = n;
-    }
-    return known[dev];
-}
-
 // The device's CTAs share the rows evenly, in one wave.
 template <int T, int V, bool VEC, int XT, int HT>
 int launch_shared(NormArgs &a, cudaStream_t st)

@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "per_device.h"
+
 namespace sam3 {
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
@@ -146,6 +148,44 @@ inline int device_sms()
         cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
         return 148;
     return sms[dev];
+}
+
+// The current device, -1 where the runtime does not say.
+inline int current_device()
+{
+    int dev = -1;
+    return cudaGetDevice(&dev) == cudaSuccess ? dev : -1;
+}
+
+// CTAs of a kernel that an SM holds (1 where the runtime does not say), asked once
+// per kernel and device.
+template <auto Kern>
+inline int ctas_of_sm(int threads, int smem)
+{
+    static PerDevice known;
+    int n = 0;
+    const bool ok = known.get(current_device(), n, [&](int &v) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v, Kern, threads, smem) == cudaSuccess && v >= 1)
+            return true;
+        (void)cudaGetLastError();
+        return false;
+    });
+    return ok ? n : 1;
+}
+
+// Clusters of a launch that run at the same time (0: none, or the runtime does not say),
+// asked once per device; known: of the kernel and the cluster size.
+template <auto Kern>
+inline int clusters_of(PerDevice &known, const cudaLaunchConfig_t &cfg)
+{
+    int n = 0;
+    const bool ok = known.get(current_device(), n, [&](int &v) {
+        if (cudaOccupancyMaxActiveClusters(&v, Kern, &cfg) == cudaSuccess)
+            return true;
+        (void)cudaGetLastError();
+        return false;
+    });
+    return ok ? n : 0;
 }
 
 }  // namespace sam3
