@@ -14,16 +14,15 @@ constexpr int kMaxClusterCtas = 16;
 template <auto Kern>
 inline cudaError_t cluster_prepare_once(int smem)
 {
-    static int done[64];
-    int dev = 0;
-    const bool known = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
-    if (known && done[dev])
-        return cudaSuccess;
-    cudaError_t e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(Kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess && known)
-        done[dev] = 1;
+    static PerDevice done;
+    int n = 0;
+    cudaError_t e = cudaSuccess;
+    done.get(current_device(), n, [&](int &) {
+        e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(Kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        return e == cudaSuccess;
+    });
     return e;
 }
 

@@ -19,7 +19,8 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t
 
 inline EncodeTiledFn encode_tiled_fn()
 {
-    static EncodeTiledFn fn = nullptr;
+    static std::atomic<EncodeTiledFn> known;
+    EncodeTiledFn fn = known.load(std::memory_order_relaxed);
     if (!fn) {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -27,6 +28,7 @@ inline EncodeTiledFn encode_tiled_fn()
                 cudaSuccess &&
             q == cudaDriverEntryPointSuccess)
             fn = reinterpret_cast<EncodeTiledFn>(p);
+        known.store(fn, std::memory_order_relaxed);
     }
     return fn;
 }
@@ -118,43 +120,39 @@ inline bool make_tmap_nhwc(CUtensorMap *map, CUtensorMapDataType dtype, uint32_t
            CUDA_SUCCESS;
 }
 
+// The current device, -1 where the runtime does not say.
+inline int current_device()
+{
+    int dev = -1;
+    return cudaGetDevice(&dev) == cudaSuccess ? dev : -1;
+}
+
 // Raises kernel Kern's dynamic shared-memory limit to `bytes` once per
 // device (the attribute persists; setting it before every launch costs host
 // time in front of short kernels).
 template <auto Kern>
 inline cudaError_t smem_limit_once(int bytes)
 {
-    static int set[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
-        return cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (set[dev] >= bytes)
-        return cudaSuccess;
-    const cudaError_t e =
-        cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess)
-        set[dev] = bytes;
+    static PerDeviceLimit limit;
+    cudaError_t e = cudaSuccess;
+    limit.raise(current_device(), bytes, [&](int n) {
+        e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, n);
+        return e == cudaSuccess;
+    });
     return e;
 }
 
-// Multiprocessor count of the current device, queried once per device.
+// Multiprocessor count of the current device, queried once per device (148 where the
+// runtime does not say).
 inline int device_sms()
 {
-    static int sms[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
-        return 148;
-    if (!sms[dev] &&
-        cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 148;
-    return sms[dev];
-}
-
-// The current device, -1 where the runtime does not say.
-inline int current_device()
-{
-    int dev = -1;
-    return cudaGetDevice(&dev) == cudaSuccess ? dev : -1;
+    static PerDevice known;
+    const int dev = current_device();
+    int n = 0;
+    const bool ok = dev >= 0 && known.get(dev, n, [&](int &v) {
+        return cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess;
+    });
+    return ok ? n : 148;
 }
 
 // CTAs of a kernel that an SM holds (1 where the runtime does not say), asked once
