@@ -872,8 +872,10 @@ __global__ void __launch_bounds__(gemm_threads(EPI), 1)
                                 tma_reduce_add_2d(&tmC, src, n, r0);
                             else
                                 tma_store_2d(&tmC, src, n, r0);
-                            bulk_commit();
                         }
+                        // (rows outside C: an empty group, so that the wait counts buffers)
+                        if (lane == 0)
+                            bulk_commit();
                         buf = (buf + 1) % kEpiBufs;
                     }
                     else
