@@ -469,7 +469,8 @@ extern "C" int k_gemm_e4m3(int M, int N, int K, const struct k_rows *A, const st
                                    : C->dt == K_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                                      : CU_TENSOR_MAP_DATA_TYPE_UINT16;
     const uint64_t pitch = M > 1 ? (uint64_t)C->ld : ((uint64_t)N + 15) / 16 * 16;
-    p.tma = make_tmap_2d(&tc, dt, es, C->p, (uint64_t)M, (uint64_t)N, pitch, 128 / es, 32);
+    p.ntma = N - N % (16 / es);
+    p.tma = p.ntma > 0 && make_tmap_2d(&tc, dt, es, C->p, (uint64_t)M, (uint64_t)p.ntma, pitch, 128 / es, 32);
     if (!p.tma && !make_tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, A->p, (uint64_t)M, (uint64_t)K,
                                 M > 1 ? (uint64_t)A->ld : ((uint64_t)K + 15) / 16 * 16, 128, 32))
         return K_ETMAP;  // (a map for the argument that is not used)

@@ -29,7 +29,8 @@ struct E4Args {
     long ldsc;
     int scdt;
     int act;
-    int tma;  // C is stored through its tensor map
+    int tma;   // C is stored through its tensor map:
+    int ntma;  // its columns up to here, the others by elements
     int *err;
 };
 
@@ -92,43 +93,55 @@ __device__ __forceinline__ void stage_piece(uint32_t tile, int r, int q, uint32_
     st_shared_v4(tile + r * 128 + ((q ^ (r & 7)) << 4), a, b, c, d);
 }
 
+// Element j of row r of the staged chunk to element i of C; es: bytes of an element.
+__device__ __forceinline__ void copy_staged(const E4Args &p, int es, uint32_t tile, int r, int j, long i)
+{
+    const int byte = j * es;
+    const uint32_t src = tile + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15);
+    if (es == 4) {
+        uint32_t v;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(src) : "memory");
+        reinterpret_cast<uint32_t *>(p.c)[i] = v;
+    }
+    else if (es == 2) {
+        uint16_t v;
+        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(src) : "memory");
+        reinterpret_cast<uint16_t *>(p.c)[i] = v;
+    }
+    else {
+        uint16_t v;
+        asm volatile("{.reg .b8 t; ld.shared.b8 t, [%1]; cvt.u16.u8 %0, t;}" : "=h"(v) : "r"(src) : "memory");
+        reinterpret_cast<uint8_t *>(p.c)[i] = (uint8_t)v;
+    }
+}
+
 // The staged chunk to C at rows m0 .., columns n ..: by TMA, or element by element
-// along the rows where C's rows are not 16-byte aligned.
+// along the rows where C's rows are not 16-byte aligned. TMA writes whole 16-byte
+// pieces, past the end of its map's rows too: the map ends with the row's last whole
+// piece, the elements behind it each lane copies from the row that it staged.
 __device__ __forceinline__ void store_chunk(const E4Args &p, const CUtensorMap *tmC, uint32_t tile, int lane, int m0,
                                             int n)
 {
+    const int es = p.cdt == K_F32 ? 4 : (p.cdt == K_E4M3 ? 1 : 2), per = 128 / es;
     if (p.tma) {
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) {
+        if (lane == 0 && n < p.ntma) {
             tma_store_2d(tmC, reinterpret_cast<const void *>(__cvta_shared_to_generic(tile)), n, m0);
             bulk_commit();
+        }
+        if (m0 + lane < p.M) {
+#pragma unroll 1
+            for (int j = max(p.ntma, n); j < min(p.N, n + per); j++)
+                copy_staged(p, es, tile, lane, j - n, (long)(m0 + lane) * p.ldc + j);
         }
         return;
     }
     __syncwarp();
-    const int es = p.cdt == K_F32 ? 4 : (p.cdt == K_E4M3 ? 1 : 2), per = 128 / es;
     for (int r = 0; r < 32 && m0 + r < p.M; r++) {
         const long row = (long)(m0 + r) * p.ldc + n;
-        for (int j = lane; j < per && n + j < p.N; j += 32) {
-            const int byte = j * es;
-            const uint32_t src = tile + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15);
-            if (es == 4) {
-                uint32_t v;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(src) : "memory");
-                reinterpret_cast<uint32_t *>(p.c)[row + j] = v;
-            }
-            else if (es == 2) {
-                uint16_t v;
-                asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(src) : "memory");
-                reinterpret_cast<uint16_t *>(p.c)[row + j] = v;
-            }
-            else {
-                uint16_t v;
-                asm volatile("{.reg .b8 t; ld.shared.b8 t, [%1]; cvt.u16.u8 %0, t;}" : "=h"(v) : "r"(src) : "memory");
-                reinterpret_cast<uint8_t *>(p.c)[row + j] = (uint8_t)v;
-            }
-        }
+        for (int j = lane; j < per && n + j < p.N; j += 32)
+            copy_staged(p, es, tile, r, j, row + j);
     }
     __syncwarp();
 }
