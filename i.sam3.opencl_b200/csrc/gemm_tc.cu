@@ -52,6 +52,7 @@ struct GemmEpi {
     k_rope rope;
     int *err;
     int red;  // fp32 C updated in place: C += epilogue result by TMA reduce-add
+    int ntma;  // columns of C that TMA stores, in whole 16-byte pieces
 };
 
 // CONV3 geometry: 3x3 / pad-1 convolution of cimg maps cH x cW x (K / 9)
@@ -224,6 +225,32 @@ __device__ __forceinline__ void stage_row(uint32_t tile, int r, const uint32_t (
     for (int q = 0; q < 8; q++)
         st_shared_v4(row + ((q ^ (r & 7)) << 4), pk[4 * q], pk[4 * q + 1], pk[4 * q + 2],
                      pk[4 * q + 3]);
+}
+
+// Columns from p.ntma on of a chunk of CW columns at n, which TMA does not store
+// (tma_store_2d): each lane those of the row that it staged.
+template <int CW, bool OUT_BF16>
+__device__ __forceinline__ void store_tail(const GemmEpi &p, uint32_t tile, int lane, int m, int n)
+{
+    if (m >= p.M)
+        return;
+#pragma unroll 1
+    for (int j = max(p.ntma, n); j < min(p.N, n + CW); j++) {
+        const int byte = (j - n) * (OUT_BF16 ? 2 : 4);
+        const uint32_t src = tile + lane * 128 + (((byte >> 4) ^ (lane & 7)) << 4) + (byte & 15);
+        const long i = (long)m * p.ldc + j;
+        if (OUT_BF16) {
+            uint16_t v;
+            asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(src) : "memory");
+            reinterpret_cast<uint16_t *>(p.C)[i] = v;
+        }
+        else {
+            float v;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(src) : "memory");
+            float *c = reinterpret_cast<float *>(p.C) + i;
+            *c = p.red ? *c + v : v;
+        }
+    }
 }
 
 // LOGITS epilogue: the last output-upscaling stage of the mask decoder fused
@@ -863,7 +890,7 @@ __global__ void __launch_bounds__(gemm_threads(EPI), 1)
                         stage_row(tile, lane, pk);
                         fence_proxy_async_smem();
                         __syncwarp();
-                        if (lane == 0 && r0 < p.M) {
+                        if (lane == 0 && r0 < p.M && n < p.ntma) {
                             const void *src = smem + L::EPI_OFF + ew * kEpiBufs * kStageTile +
                                               buf * kStageTile;
                             if constexpr (CONV3)
@@ -873,9 +900,11 @@ __global__ void __launch_bounds__(gemm_threads(EPI), 1)
                             else
                                 tma_store_2d(&tmC, src, n, r0);
                         }
-                        // (rows outside C: an empty group, so that the wait counts buffers)
+                        // (nothing to store: an empty group, so that the wait counts buffers)
                         if (lane == 0)
                             bulk_commit();
+                        if (!CONV3 && n + CW > p.ntma)
+                            store_tail<CW, OUT_BF16>(p, tile, lane, m, n);
                         buf = (buf + 1) % kEpiBufs;
                     }
                     else
@@ -1013,15 +1042,17 @@ extern "C" int k_gemm_bf16_tc(int M, int N, int K, const void *A, int lda, const
         !make_tmap_bf16(&tb, B, (uint64_t)N, (uint64_t)K, (uint64_t)ldb, (uint32_t)BN))
         return K_ETMAP;
     // TMA stores need a 16-byte aligned base and row pitch; else direct stores.
+    const int ntma = N - N % (c_bf16 ? 8 : 4);
     const bool tma = c_bf16 ? make_tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, C,
-                                           (uint64_t)M, (uint64_t)N, (uint64_t)ldc, 64, 32)
+                                           (uint64_t)M, (uint64_t)ntma, (uint64_t)ldc, 64, 32)
                             : make_tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, C,
-                                           (uint64_t)M, (uint64_t)N, (uint64_t)ldc, 32, 32);
+                                           (uint64_t)M, (uint64_t)ntma, (uint64_t)ldc, 32, 32);
     if (!tma)
         tc = ta;  // unused by the direct-store kernels
     GemmEpi p;
     p.M = M;
     p.N = N;
+    p.ntma = ntma;
     p.K = K;
     p.C = C;
     p.ldc = ldc;
@@ -1091,6 +1122,7 @@ extern "C" int k_conv3x3_bf16_tc(const void *X, int nimg, int H, int W, int C, c
     GemmEpi p;
     p.M = nimg * H * W;
     p.N = N;
+    p.ntma = N;
     p.K = K;
     p.C = out;
     p.ldc = N;
@@ -1147,7 +1179,7 @@ extern "C" int k_dec_convt_logits(const void *X, int P, int H, int W, const void
         return K_ETMAP;
     GemmEpi p;
     p.M = M;
-    p.N = 128;
+    p.N = p.ntma = 128;
     p.K = 64;
     p.C = out;
     p.ldc = 0;
@@ -1183,7 +1215,7 @@ extern "C" int k_dec_convt_ln2d(const void *X, int P, int H, int W, const void *
         return K_ETMAP;
     GemmEpi p;
     p.M = M;
-    p.N = 256;
+    p.N = p.ntma = 256;
     p.K = 256;
     p.C = out;
     p.ldc = 0;
@@ -1218,6 +1250,7 @@ extern "C" int k_convt2x2_bf16_tc(const void *X, int nimg, int H, int W, int cin
     GemmEpi p;
     p.M = M;
     p.N = N;
+    p.ntma = N;
     p.K = cin;
     p.C = out;
     p.ldc = 0;

@@ -1,6 +1,10 @@
 """GPU tests of products whose result is part of a wider matrix: rows that start at
 multiples of 16 bytes and end anywhere. What lies behind a row's last column, and behind the last
-row, keeps its bits, at every width and in every form of cb_gemm_e4m3.
+row, keeps its bits, at every width and in every form of cb_gemm and cb_gemm_e4m3.
+
+Tolerance of cb_gemm on bf16 operands: products are exact in 32 bits, their sum is off by
+at most K 2^-23 of sum |a b| (the matrix unit may truncate each addition), bias and residual
+add 2^-24 of theirs; the result is rounded once.
 """
 import pytest
 
@@ -91,3 +95,36 @@ def test_gemm_e4m3_pairs_inside_a_matrix(be, sb):
             check_quantised(got, sc, z, tol)
         else:
             check_rounded(got, z, tol, DT[out])
+
+
+@pytest.mark.parametrize("how", ["bf16", "f32", "in place", "residual"])
+@pytest.mark.parametrize("N", WIDTHS)
+@pytest.mark.parametrize("M,K", [(1, 64), (300, 64), (20000, 136)])
+def test_gemm_inside_a_matrix(be, sb, M, N, K, how):
+    run_gemm(be, sb, M, N, K, how)
+
+
+@pytest.mark.parametrize("how", ["bf16", "in place", "f32"])
+def test_gemm_pairs_inside_a_matrix(be, sb, how):
+    run_gemm(be, sb, 20000, 1021, 1032, how)
+
+
+def run_gemm(be, sb, M, N, K, how):
+    g = gen(M + N)
+    dt = torch.bfloat16 if how == "bf16" else torch.float32
+    a, b, bias = randn(g, M, K).bfloat16(), randn(g, N, K).bfloat16(), randn(g, N)
+    c = Matrix(be, M, N, dt, 1, 1)
+    other = Matrix(be, M, N, dt, 1, 1, 1) if how == "residual" else c
+    if how in ("residual", "in place"):
+        other.rows[:, :N] = randn(g, M, N)
+    c.start()
+    was = other.rows[:, :N].to(f64) if how in ("residual", "in place") else 0.0
+    d = c.op
+    be.gemm(M, N, K, (be.wrap(a), 0, K), (be.wrap(b), 0, K), 1, (be.wrap(c.given), d.off, d.ld), bias=be.wrap(bias),
+            R=be.wrap(other.given) if how in ("residual", "in place") else None, roff=d.off)
+    be.sync()
+    av, bv = a.to(f64), b.to(f64)
+    z = av @ bv.t() + bias.to(f64)
+    tol = (K * 2.0 ** -23 + 2.0 ** -24) * (av.abs() @ bv.abs().t()) + 2.0 ** -24 * (z.abs() + bias.abs().to(f64))
+    z = z + was
+    check_rounded(c.result(), z, tol + 2.0 ** -24 * z.abs(), dt)
