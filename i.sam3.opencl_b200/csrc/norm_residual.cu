@@ -695,23 +695,42 @@ int launch_shared(NormArgs &a, cudaStream_t st)
     return launch_pdl(kern, grid, dim3(threads), smem, st, (const NormArgs)a);
 }
 
+// Rows an SM from which a CTA's share of them pays for keeping its sample's vectors in
+// shared memory (0: never). Measured in us with and without them, on 148 SMs:
+//   64 columns: 20000 rows 7.3 and 8.3, 12000 6.2 and 6.1;   128: 9472 rows 5.6 and 7.1, 5000 6.7 and 6.3;
+//   256: 9472 rows 7.5 and 8.7, 4800 6.6 and 5.6;            512: 4000 rows 12.6 and 15.1, 2400 9.3 and 6.3;
+//   1024 by warps: 12000 rows 38 and 55;                     1024 by CTAs: 80000 rows 250 and 283, 40000 147 and 144;
+//   2048: 33000 rows 236 and 262, 20000 183 and 164;         4096: 20000 rows 314 and 331, 12000 233 and 210;
+//   8192: 12000 rows 274 and 294, 8200 331 and 303;
+// rows that are not aligned: 1001 columns as 1024 (80000 rows 210 and 232, 20000 100 and
+// 79), others never (77 columns: 75 and 57 at 80000 rows; 2047: 857 and 621; 7001: 1161 and 1152 at 20000).
+// A sample needs rows too, two steps of the CTA's and at least 32 (20480 x 4096 in samples of 32 rows:
+// 217 and 252, of 16 255 and 253, of 2 949 and 277).
+template <int T, int V, bool VEC>
+__host__ __device__ constexpr int shared_rows()
+{
+    if (!VEC)
+        return T == 128 && V == 1 ? 448 : 0;
+    if (T <= 32)
+        return T == 8 ? 128 : (V == 1 ? 64 : 32);
+    return T == 128 ? (V == 1 ? 448 : 224) : (T == 256 ? 112 : 84);
+}
+
 template <int T, int V, bool VEC>
 int launch(NormArgs &a, cudaStream_t st)
 {
     constexpr int kRows = cta_threads(T) / T;
     const int sms = device_sms(), xt = a.p.X.dt, ht = a.p.H.p ? a.p.H.dt : xt;
-    // Shared vectors pay where CTAs (two to an SM) have two steps of rows of a sample;
-    // where a CTA has one aligned row at a time only from many rows on (5403 rows of 1000
-    // fp32: 27.5 us with, 18.2 without; 20736 x 512 bf16, warps: 21.3 and 25.9).
-    constexpr int kSteps = VEC && T > 32 ? 64 : 2;
-    if (a.rows >= (long)sms * 2 * kSteps * kRows && a.p.N >= 2 * kRows) {
-        if (xt == K_BF16)
-            return launch_shared<T, V, VEC, K_BF16, K_BF16>(a, st);
-        if (xt == K_F16)
-            return launch_shared<T, V, VEC, K_F16, K_F16>(a, st);
-        if (ht == K_F32)
-            return launch_shared<T, V, VEC, K_F32, K_F32>(a, st);
-        return launch_shared<T, V, VEC, K_F32, kAnyType>(a, st);
+    if constexpr (shared_rows<T, V, VEC>() > 0) {
+        if (a.rows >= (long)sms * shared_rows<T, V, VEC>() && a.p.N >= (kRows > 16 ? 2 * kRows : 32)) {
+            if (xt == K_BF16)
+                return launch_shared<T, V, VEC, K_BF16, K_BF16>(a, st);
+            if (xt == K_F16)
+                return launch_shared<T, V, VEC, K_F16, K_F16>(a, st);
+            if (ht == K_F32)
+                return launch_shared<T, V, VEC, K_F32, K_F32>(a, st);
+            return launch_shared<T, V, VEC, K_F32, kAnyType>(a, st);
+        }
     }
     const long need = (a.rows + kRows - 1) / kRows, most = (long)sms * 16;
     return launch_pdl(norm_rows_kernel<T, V, VEC, kAnyType, kAnyType, false>, dim3((unsigned)(need < most ? need : most)),

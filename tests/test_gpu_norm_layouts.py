@@ -17,15 +17,16 @@ LAYOUTS = ("all", "sample", "row")
 FORMS = [
     (64, "bf16", 0, (3, 5), (2, 10001)),        # parts of a warp
     (128, "f16", 0, (3, 7), (3, 3301)),
-    (256, "bf16", 0, (2, 301), (5, 1003)),      # a warp, aligned
+    (256, "bf16", 0, (2, 301), (5, 2003)),      # a warp, aligned
     (512, "f32", 0, (2, 301), (5, 1003)),
     (1024, "bf16", 0, (2, 301), (2, 5001)),
-    (1024, "f32", 0, (2, 301), (2, 9601)),      # a CTA, aligned
-    (2048, "f16", 0, (2, 33), (2, 9601)),
-    (4096, "bf16", 0, (2, 33), (3, 6401)),
+    (1024, "f32", 0, (2, 301), (2, 33301)),     # a CTA, aligned
+    (2048, "f16", 0, (2, 33), (2, 16601)),
+    (4096, "bf16", 0, (2, 33), (2, 8301)),
+    (8192, "f32", 0, (2, 33), (2, 6301)),
     (77, "bf16", 0, (2, 301), (5, 1003)),       # a warp, not aligned
     (333, "f32", 0, (2, 301), (5, 1003)),
-    (1024, "bf16", 1, (2, 101), (2, 701)),      # a CTA, not aligned
+    (1024, "bf16", 1, (2, 101), (2, 33301)),     # a CTA, not aligned
     (2047, "f16", 0, (2, 33), (2, 701)),
     (5001, "bf16", 0, (2, 33), (3, 301)),
     (9001, "f16", 0, (2, 3), (3, 301)),         # rows of any width
@@ -111,3 +112,11 @@ def test_in_place(be, sb, place, form, many):
     nb, N = lot if many else few
     g = gen(C + N + 2)
     call(be, sb, g, nb, N, C, dt, pad, gate=("sample", "f32"), scale=("sample", "f32"), shift=("sample", "f32"), post=2, place=place)
+
+
+@pytest.mark.parametrize("C,dt,nb,N", [(512, "bf16", 700, 31), (512, "bf16", 700, 32), (4096, "f16", 600, 31), (4096, "f16", 600, 32), (64, "f32", 400, 63),
+                                       (64, "f32", 400, 64)])
+def test_many_samples_of_few_rows(be, sb, C, dt, nb, N):
+    """Around the rows of a sample from which they share its vectors."""
+    g = gen(C + N + 3)
+    call(be, sb, g, nb, N, C, dt, 0, gate=("sample", "f32"), scale=("sample", "f32"), shift=("row", dt), post=1)
