@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 tc_fence_after();
                 if (quarter == 0 && (TURNS || group == 0) && lane == 0)
-                    mbar_arrive_relaxed(&empty[(before + kb) % STAGES]);  // the MMAs have read the stage
+                    mbar_arrive(&empty[(before + kb) % STAGES]);  // the MMAs have read the stage
                 const uint32_t src = tmem_base + ((uint32_t)row << 16) + buf * BN + col;
                 const float s = ring[(chunk % kChunks * kChunk + i % kChunk) * BM];
                 const bool last = i % kChunk == kChunk - 1 || kb + KS >= kblocks;
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (lane == 0) {
                             mbar_arrive_relaxed(&tempty[buf]);
                             if (last)  // the chunk's scales are in registers
-                                mbar_arrive_relaxed(&sempty[slot]);
+                                mbar_arrive(&sempty[slot]);
                         }
                         // the next block's barriers, asked beside the last sums
                         const uint32_t cn = c + 1, chn = chunk + last;

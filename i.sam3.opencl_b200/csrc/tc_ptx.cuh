@@ -205,9 +205,9 @@ __device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity)
     return ok != 0;
 }
 
-// An arrival that orders no memory accesses: enough after tcgen05 loads, which
-// tcgen05.wait::ld and tcgen05.fence::before_thread_sync order. A release at cluster
-// scope takes about 1000 cycles.
+// An arrival that orders no memory accesses: enough after tcgen05 loads and stores, which
+// tcgen05.wait and tcgen05.fence::before_thread_sync order; what was read from shared memory
+// is given back by mbar_arrive, a release. A release at cluster scope takes about 1000 cycles.
 __device__ __forceinline__ void mbar_arrive_relaxed(uint64_t *bar)
 {
     asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
