@@ -695,25 +695,29 @@ int launch_shared(NormArgs &a, cudaStream_t st)
     return launch_pdl(kern, grid, dim3(threads), smem, st, (const NormArgs)a);
 }
 
-// Rows an SM from which a CTA's share of them pays for keeping its sample's vectors in
-// shared memory (0: never). Measured in us with and without them, on 148 SMs:
-//   64 columns: 20000 rows 7.3 and 8.3, 12000 6.2 and 6.1;   128: 9472 rows 5.6 and 7.1, 5000 6.7 and 6.3;
-//   256: 9472 rows 7.5 and 8.7, 4800 6.6 and 5.6;            512: 4000 rows 12.6 and 15.1, 2400 9.3 and 6.3;
-//   1024 by warps: 12000 rows 38 and 55;                     1024 by CTAs: 80000 rows 250 and 283, 40000 147 and 144;
-//   2048: 33000 rows 236 and 262, 20000 183 and 164;         4096: 20000 rows 314 and 331, 12000 233 and 210;
-//   8192: 12000 rows 274 and 294, 8200 331 and 303;
-// rows that are not aligned: 1001 columns as 1024 (80000 rows 210 and 232, 20000 100 and
-// 79), others never (77 columns: 75 and 57 at 80000 rows; 2047: 857 and 621; 7001: 1161 and 1152 at 20000).
-// A sample needs rows too, two steps of the CTA's and at least 32 (20480 x 4096 in samples of 32 rows:
-// 217 and 252, of 16 255 and 253, of 2 949 and 277).
+// Rows an SM from which it pays that CTAs keep their sample's vectors in shared memory.
+// Measured on 148 SMs, us with and without them, below and above the border (residual scale,
+// gate, LayerNorm, shift and scale; fewer vectors move a border by up to a half either way):
+//   aligned rows, bf16 to E4M3 (1024 columns by CTAs fp32)   not aligned, fp32
+//     64: 15000 rows 8.4, 7.2     20000 8.5, 9.4              77: 20000 rows 15.6, 14.9   60000 36, 41
+//    128:  5000      7.8, 6.7     10000 9.3, 9.6             500: 2500       13.0, 11.8   10000 26, 37
+//    256: 10000     11.6, 11.0    20000 16.0, 18.6           601: 10000      41, 34       60000 130, 161
+//    512:  5000     14.0, 12.2    15000 24, 32
+//   1024: 30000     116, 115      60000 193, 227
+//   2048: 30000     174, 161      60000 272, 316            2047: 10000      133, 101     60000 385, 456
+//   4096: 10000     140, 119      20000 198, 225            3001: 5000       103, 91      10000 149, 165
+//   8192: 10000     274, 253      15000 360, 377            5001: 1000       64, 45       5000 154, 192
+// Rows that are not aligned with 16-bit X or H never (60000 x 77 bf16 66 and 50, 20000 x 2047 287
+// and 202, 10000 x 7001 587 and 545). A sample needs rows too, two steps of the CTA's and
+// at least 32 (20480 x 4096 bf16 in samples of 32 rows 217 and 252, of 16 255 and 253, of 2 949 and 277).
 template <int T, int V, bool VEC>
 __host__ __device__ constexpr int shared_rows()
 {
-    if (!VEC)
-        return T == 128 && V == 1 ? 448 : 0;
     if (T <= 32)
-        return T == 8 ? 128 : (V == 1 ? 64 : 32);
-    return T == 128 ? (V == 1 ? 448 : 224) : (T == 256 ? 112 : 84);
+        return VEC ? (T == 8 ? 128 : (T == 32 ? (V == 1 ? 80 : 48) : 64)) : (V == 1 ? 256 : 32);
+    if (T == 128)
+        return VEC ? (V == 1 ? 288 : 256) : (V == 1 ? 224 : 128);
+    return VEC ? (T == 256 ? 112 : 84) : (T == 256 ? 48 : 14);
 }
 
 template <int T, int V, bool VEC>
@@ -721,14 +725,14 @@ int launch(NormArgs &a, cudaStream_t st)
 {
     constexpr int kRows = cta_threads(T) / T;
     const int sms = device_sms(), xt = a.p.X.dt, ht = a.p.H.p ? a.p.H.dt : xt;
-    if constexpr (shared_rows<T, V, VEC>() > 0) {
-        if (a.rows >= (long)sms * shared_rows<T, V, VEC>() && a.p.N >= (kRows > 16 ? 2 * kRows : 32)) {
+    if (a.rows >= (long)sms * shared_rows<T, V, VEC>() && a.p.N >= (kRows > 16 ? 2 * kRows : 32)) {
+        if (xt == K_F32 && ht == K_F32)
+            return launch_shared<T, V, VEC, K_F32, K_F32>(a, st);
+        if constexpr (VEC) {
             if (xt == K_BF16)
                 return launch_shared<T, V, VEC, K_BF16, K_BF16>(a, st);
             if (xt == K_F16)
                 return launch_shared<T, V, VEC, K_F16, K_F16>(a, st);
-            if (ht == K_F32)
-                return launch_shared<T, V, VEC, K_F32, K_F32>(a, st);
             return launch_shared<T, V, VEC, K_F32, kAnyType>(a, st);
         }
     }

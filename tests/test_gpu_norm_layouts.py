@@ -17,16 +17,21 @@ LAYOUTS = ("all", "sample", "row")
 FORMS = [
     (64, "bf16", 0, (3, 5), (2, 10001)),        # parts of a warp
     (128, "f16", 0, (3, 7), (3, 3301)),
-    (256, "bf16", 0, (2, 301), (5, 2003)),      # a warp, aligned
-    (512, "f32", 0, (2, 301), (5, 1003)),
+    (256, "bf16", 0, (2, 301), (5, 3003)),      # a warp, aligned
+    (512, "f32", 0, (2, 301), (5, 2003)),
     (1024, "bf16", 0, (2, 301), (2, 5001)),
-    (1024, "f32", 0, (2, 301), (2, 33301)),     # a CTA, aligned
-    (2048, "f16", 0, (2, 33), (2, 16601)),
+    (1024, "f32", 0, (2, 301), (2, 21501)),     # a CTA, aligned
+    (2048, "f16", 0, (2, 33), (2, 19001)),
     (4096, "bf16", 0, (2, 33), (2, 8301)),
     (8192, "f32", 0, (2, 33), (2, 6301)),
-    (77, "bf16", 0, (2, 301), (5, 1003)),       # a warp, not aligned
-    (333, "f32", 0, (2, 301), (5, 1003)),
-    (1024, "bf16", 1, (2, 101), (2, 33301)),     # a CTA, not aligned
+    (77, "f32", 0, (2, 301), (2, 19001)),       # a warp, not aligned
+    (333, "f32", 0, (2, 301), (3, 2403)),
+    (1024, "f32", 1, (2, 101), (2, 16601)),     # a CTA, not aligned
+    (2047, "f32", 0, (2, 33), (2, 10701)),
+    (3001, "f32", 0, (2, 33), (2, 3601)),
+    (5001, "f32", 0, (2, 33), (2, 1503)),
+    (77, "bf16", 0, (2, 301), (2, 19001)),      # not aligned, 16 bits: one form
+    (1024, "bf16", 1, (2, 101), (2, 4001)),
     (2047, "f16", 0, (2, 33), (2, 701)),
     (5001, "bf16", 0, (2, 33), (3, 301)),
     (9001, "f16", 0, (2, 3), (3, 301)),         # rows of any width
