@@ -569,11 +569,15 @@ int cb_quantize_e4m3(cb_backend *b, int nb, int N, int K, int brows,
  * values, each its own type; a product of two scales stays within 32 bits);
  * bias F32 [N] or NULL; C F32, BF16 or F16, rounded once, or E4M3, then SC [M,
  * ceil(N / 128)] (E8M0 or F32) receives the scales cb_quantize_e4m3 (brows 1)
- * would give act(...) in 32 bits. Sums in 32 bits; where both scales are E8M0 and C is
- * not F32 or K at most 1024 by the matrix unit, which truncates (3e-7 of the result over
- * 4096 columns), else a block's. Rows of A and B start at multiples of 16 bytes (off
- * and ld; what lies behind column K of a row is not used); C takes any ld. s0 is of no
- * account. GELU is 0.5 z (1 + erf(z / sqrt 2)) for F32 results; for others its part
+ * would give act(...) in 32 bits. Rows of A and B start at multiples of 16 bytes (off and
+ * ld; what lies behind column K of a row is not used); C takes any ld, and what lies behind
+ * column N of its rows is left as it was. s0 is of no account.
+ *
+ * Sums in 32 bits: those of a block by the matrix unit, which truncates, their sum rounded
+ * to nearest. Where both scales are E8M0, and C is not F32 or K at most 1024, the matrix unit
+ * sums all of K: against 64 bits F32 results are off by 7e-8 (rms) over 1024 columns, where
+ * they are by 4e-8 with a scale given as F32, which always rounds; others by 3e-7 over 4096
+ * before their rounding. GELU is 0.5 z (1 + erf(z / sqrt 2)) for F32 results; for others its part
  * beside max(z, 0) is off by at most 1.2e-5 of itself up to |z| = 8, by 6e-15 beyond. */
 int cb_gemm_e4m3(cb_backend *b, int M, int N, int K, struct cb_opnd A,
                  struct cb_opnd SA, struct cb_opnd B, struct cb_opnd SB,
