@@ -16,8 +16,8 @@
 //           under way, for problems of few tiles) and join their sums at the end.
 // What bounds a tile is the way of a k-block through its buffer: about 900 cycles from
 // the issue of its MMAs to the epilogue's first load, 250 for loads and sums, 250
-// until the buffer is given back (41472 x 1024 x 4096: 182 us, 217 under the power cap; two
-// buffers of 256 columns or four of 128 make no difference).
+// until the buffer is given back (41472 x 1024 x 4096: 187 us in a burst, 218 at the 1511 MHz that
+// the power cap leaves; two buffers of 256 columns or four of 128 make no difference).
 // A 128-column block of a row lies in one thread, so an E4M3 result is scaled and
 // rounded there.
 #include "gemm_e4m3.cuh"

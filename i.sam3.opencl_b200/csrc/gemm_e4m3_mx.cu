@@ -12,9 +12,10 @@
 //           of B's tile; one accumulator, read into registers by both groups before
 //           the next tile's products start;
 //   BN 128: two accumulators of 128, a group each.
-// 41472 x 1024 x 4096 131 us (2.66 PFLOP/s), 41472 x 4096 x 1024 150 us; with GELU and E4M3
-// results 182 us, 215 under the power cap, where the epilogue counts: four instructions a
-// value for GELU's polynomial (in pairs), two for the scale and its product, one to round.
+// 41472 x 1024 x 4096 131 us (2.66 PFLOP/s), 41472 x 4096 x 1024 149 us; with GELU and E4M3
+// results 184 us, where the epilogue counts: four instructions a value for GELU's polynomial
+// (in pairs), two for the scale and its product, one to round. Under the power cap 161, 183 and
+// 214 us at 1136, 1237 and 1545 MHz: 183, 227 and 331 thousand cycles.
 #include "gemm_e4m3.cuh"
 
 namespace sam3 {
