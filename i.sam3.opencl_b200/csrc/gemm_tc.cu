@@ -52,7 +52,6 @@ struct GemmEpi {
     k_rope rope;
     int *err;
     int red;  // fp32 C updated in place: C += epilogue result by TMA reduce-add
-    int ntma;  // columns of C that TMA stores, in whole 16-byte pieces
 };
 
 // CONV3 geometry: 3x3 / pad-1 convolution of cimg maps cH x cW x (K / 9)
@@ -225,32 +224,6 @@ __device__ __forceinline__ void stage_row(uint32_t tile, int r, const uint32_t (
     for (int q = 0; q < 8; q++)
         st_shared_v4(row + ((q ^ (r & 7)) << 4), pk[4 * q], pk[4 * q + 1], pk[4 * q + 2],
                      pk[4 * q + 3]);
-}
-
-// Columns from p.ntma on of a chunk of CW columns at n, which TMA does not store
-// (tma_store_2d): each lane those of the row that it staged.
-template <int CW, bool OUT_BF16>
-__device__ __forceinline__ void store_tail(const GemmEpi &p, uint32_t tile, int lane, int m, int n)
-{
-    if (m >= p.M)
-        return;
-#pragma unroll 1
-    for (int j = max(p.ntma, n); j < min(p.N, n + CW); j++) {
-        const int byte = (j - n) * (OUT_BF16 ? 2 : 4);
-        const uint32_t src = tile + lane * 128 + (((byte >> 4) ^ (lane & 7)) << 4) + (byte & 15);
-        const long i = (long)m * p.ldc + j;
-        if (OUT_BF16) {
-            uint16_t v;
-            asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(src) : "memory");
-            reinterpret_cast<uint16_t *>(p.C)[i] = v;
-        }
-        else {
-            float v;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(src) : "memory");
-            float *c = reinterpret_cast<float *>(p.C) + i;
-            *c = p.red ? *c + v : v;
-        }
-    }
 }
 
 // LOGITS epilogue: the last output-upscaling stage of the mask decoder fused
@@ -890,21 +863,21 @@ __global__ void __launch_bounds__(gemm_threads(EPI), 1)
                         stage_row(tile, lane, pk);
                         fence_proxy_async_smem();
                         __syncwarp();
-                        if (lane == 0 && r0 < p.M && n < p.ntma) {
+                        // (a pixel block's rows outside the map, with others behind it: an
+                        // empty group, so that the wait counts buffers)
+                        if (lane == 0 && (CONV3 || r0 < p.M)) {
                             const void *src = smem + L::EPI_OFF + ew * kEpiBufs * kStageTile +
                                               buf * kStageTile;
-                            if constexpr (CONV3)
-                                tma_store_4d(&tmC, src, n, cx0, cy, cimg);
+                            if constexpr (CONV3) {
+                                if (r0 < p.M)
+                                    tma_store_4d(&tmC, src, n, cx0, cy, cimg);
+                            }
                             else if (!OUT_BF16 && p.red)
                                 tma_reduce_add_2d(&tmC, src, n, r0);
                             else
                                 tma_store_2d(&tmC, src, n, r0);
-                        }
-                        // (nothing to store: an empty group, so that the wait counts buffers)
-                        if (lane == 0)
                             bulk_commit();
-                        if (!CONV3 && n + CW > p.ntma)
-                            store_tail<CW, OUT_BF16>(p, tile, lane, m, n);
+                        }
                         buf = (buf + 1) % kEpiBufs;
                     }
                     else
@@ -1031,6 +1004,23 @@ extern "C" int k_gemm_bf16_tc(int M, int N, int K, const void *A, int lda, const
         return K_EARG;
     if (bias && (reinterpret_cast<uintptr_t>(bias) & 15))
         return K_EARG;
+    // Rows that end inside a 16-byte piece, in a pitch that TMA can store: it would write
+    // that piece to its end (tma_store_2d), so the columns behind the last whole piece
+    // are a product of their own with direct stores (41472 x 1020 x 1024 bf16 in rows of 1024:
+    // 138 us, 616 with direct stores for all columns).
+    const int piece = c_bf16 ? 8 : 4, rest = N % piece;
+    const bool whole = rest == 0;
+    if (!whole && N > piece && ldc % piece == 0 && !(reinterpret_cast<uintptr_t>(C) & 15)) {
+        const int n = N - rest;
+        const int rc = k_gemm_bf16_tc(M, n, K, A, lda, B, ldb, C, ldc, c_bf16, bias, R, ldr, rmod, alpha, act,
+                                      rope, err, num_sms, s);
+        if (rc)
+            return rc;
+        return k_gemm_bf16_tc(M, rest, K, A, lda, reinterpret_cast<const uint16_t *>(B) + (long)n * ldb, ldb,
+                              reinterpret_cast<char *>(C) + (long)n * (c_bf16 ? 2 : 4), ldc, c_bf16,
+                              bias ? bias + n : nullptr, R ? R + n : nullptr, ldr, rmod, alpha, act, nullptr, err,
+                              num_sms, s);
+    }
     // 128-wide tiles for N <= 128, and where 256-wide ones would leave more
     // than half of the SMs without a tile (the decoder's token stream: 512
     // rows, 4 tiles at N = 256): twice the CTAs, half the serial MMA work
@@ -1041,18 +1031,17 @@ extern "C" int k_gemm_bf16_tc(int M, int N, int K, const void *A, int lda, const
     if (!make_tmap_bf16(&ta, A, (uint64_t)M, (uint64_t)K, (uint64_t)lda, BM) ||
         !make_tmap_bf16(&tb, B, (uint64_t)N, (uint64_t)K, (uint64_t)ldb, (uint32_t)BN))
         return K_ETMAP;
-    // TMA stores need a 16-byte aligned base and row pitch; else direct stores.
-    const int ntma = N - N % (c_bf16 ? 8 : 4);
-    const bool tma = c_bf16 ? make_tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, C,
-                                           (uint64_t)M, (uint64_t)ntma, (uint64_t)ldc, 64, 32)
-                            : make_tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, C,
-                                           (uint64_t)M, (uint64_t)ntma, (uint64_t)ldc, 32, 32);
+    // TMA stores need a 16-byte aligned base and row pitch, and rows of whole 16-byte
+    // pieces; else direct stores.
+    const bool tma = whole && (c_bf16 ? make_tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, C,
+                                                     (uint64_t)M, (uint64_t)N, (uint64_t)ldc, 64, 32)
+                                      : make_tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, C,
+                                                     (uint64_t)M, (uint64_t)N, (uint64_t)ldc, 32, 32));
     if (!tma)
         tc = ta;  // unused by the direct-store kernels
     GemmEpi p;
     p.M = M;
     p.N = N;
-    p.ntma = ntma;
     p.K = K;
     p.C = C;
     p.ldc = ldc;
@@ -1122,7 +1111,6 @@ extern "C" int k_conv3x3_bf16_tc(const void *X, int nimg, int H, int W, int C, c
     GemmEpi p;
     p.M = nimg * H * W;
     p.N = N;
-    p.ntma = N;
     p.K = K;
     p.C = out;
     p.ldc = N;
@@ -1179,7 +1167,7 @@ extern "C" int k_dec_convt_logits(const void *X, int P, int H, int W, const void
         return K_ETMAP;
     GemmEpi p;
     p.M = M;
-    p.N = p.ntma = 128;
+    p.N = 128;
     p.K = 64;
     p.C = out;
     p.ldc = 0;
@@ -1215,7 +1203,7 @@ extern "C" int k_dec_convt_ln2d(const void *X, int P, int H, int W, const void *
         return K_ETMAP;
     GemmEpi p;
     p.M = M;
-    p.N = p.ntma = 256;
+    p.N = 256;
     p.K = 256;
     p.C = out;
     p.ldc = 0;
@@ -1250,7 +1238,6 @@ extern "C" int k_convt2x2_bf16_tc(const void *X, int nimg, int H, int W, int cin
     GemmEpi p;
     p.M = M;
     p.N = N;
-    p.ntma = N;
     p.K = cin;
     p.C = out;
     p.ldc = 0;
