@@ -26,9 +26,10 @@ inline EncodeTiledFn encode_tiled_fn()
         cudaDriverEntryPointQueryResult q;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
                 cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
+            q == cudaDriverEntryPointSuccess) {
             fn = reinterpret_cast<EncodeTiledFn>(p);
-        known.store(fn, std::memory_order_relaxed);
+            known.store(fn, std::memory_order_relaxed);
+        }
     }
     return fn;
 }
